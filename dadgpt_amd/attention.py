@@ -46,6 +46,17 @@ C_SYMBOLS = (
     "dadgpt_decode_attention_bf16",
     "dadgpt_decode_attention_bf16_noalloc",
     "dadgpt_decode_attention_f32",
+    "dadgpt_flash_attention_window_workspace_bytes",
+    "dadgpt_flash_attention_window_forward",
+    "dadgpt_flash_attention_window_backward",
+    "dadgpt_flash_attention_window_forward_bf16",
+    "dadgpt_flash_attention_window_backward_bf16",
+    "dadgpt_flash_attention_window_forward_bf16_strided",
+    "dadgpt_flash_attention_window_backward_bf16_strided",
+    "dadgpt_flash_attention_window_forward_bf16_tokens",
+    "dadgpt_flash_attention_window_backward_bf16_tokens",
+    "dadgpt_decode_attention_window_bf16",
+    "dadgpt_decode_attention_window_f32",
     "dadgpt_softmax",
     "dadgpt_softmax_backward",
     "dadgpt_causal_mask",
@@ -143,6 +154,25 @@ def lib():
     L.dadgpt_decode_attention_bf16.argtypes = [vp] * 5 + [i, i, i, i, f, vp, sz, vp]
     L.dadgpt_decode_attention_f32.argtypes = [vp] * 5 + [i, i, i, i, f, vp, sz, vp]
     L.dadgpt_decode_attention_bf16_noalloc.argtypes = [vp] * 5 + [i, i, i, i, f, vp]
+    win, ws = [i, i], [vp, sz]  # window and sinks, workspace and its size
+    L.dadgpt_flash_attention_window_workspace_bytes.restype = sz
+    L.dadgpt_flash_attention_window_workspace_bytes.argtypes = [i] * 5
+    for name in ("window_forward", "window_forward_bf16"):
+        getattr(L, "dadgpt_flash_attention_" + name).argtypes = [vp] * 5 + [i, i, i, f] + win + [vp]
+    for name in ("window_backward", "window_backward_bf16"):
+        getattr(L, "dadgpt_flash_attention_" + name).argtypes = ([vp] * 10 + [i, i, i, f] + win +
+                                                                 ws + [vp])
+    L.dadgpt_flash_attention_window_forward_bf16_strided.argtypes = (
+        [vp] * 5 + [i, i, i, i, f] + win + [hs, vp])
+    L.dadgpt_flash_attention_window_backward_bf16_strided.argtypes = (
+        [vp] * 10 + [i, i, i, i, f] + win + [hs] + ws + [vp])
+    L.dadgpt_flash_attention_window_forward_bf16_tokens.argtypes = (
+        [vp, i64, vp, vp, vp, vp, i64, i, i, i, i, f] + win + [vp])
+    L.dadgpt_flash_attention_window_backward_bf16_tokens.argtypes = (
+        [vp, vp, vp, i64, vp, vp, vp, i64, vp, vp, vp, vp, i64, i, i, i, i, f] + win + ws + [vp])
+    for name in ("bf16", "f32"):
+        getattr(L, "dadgpt_decode_attention_window_" + name).argtypes = (
+            [vp] * 5 + [i, i, i, i, f] + win + ws + [vp])
     L.dadgpt_softmax.argtypes = [vp, vp, i, i, vp]
     L.dadgpt_softmax_backward.argtypes = [vp, vp, vp, i, i, vp]
     L.dadgpt_causal_mask.argtypes = [vp, i, i, vp]
@@ -427,6 +457,149 @@ def decode_attention(out, q, k_cache, v_cache, lens, n_seq, n_heads, max_len, d_
           else lib().dadgpt_decode_attention_f32)
     _check(fn(po, pq, pk, pv, pl, n_seq, n_heads, max_len, d_head, scale, _ptr(workspace),
               ws_bytes, _stream_ptr(stream)))
+
+
+# --------------------------------------------------- sliding window with sinks
+
+# The most sinks and the longest sequence of a windowed call (the header's DADGPT_WINDOW_*).
+WINDOW_MAX_SINKS, WINDOW_MAX_SEQ = 1024, 1 << 19
+
+
+def _same_device(tensors) -> None:
+    """Every tensor on the current device, whose stream the call runs on (plain tensors that are
+    not there would fault; None passes)."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{device}")
+
+
+def _workspace(workspace):
+    """A caller's workspace -> (address, bytes)."""
+    if workspace is None:
+        return None, 0
+    if not workspace.is_cuda or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous device tensor")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def window_workspace_bytes(BH: int, S: int, d_head: int, window: int, sinks: int) -> int:
+    return int(lib().dadgpt_flash_attention_window_workspace_bytes(BH, S, d_head, window, sinks))
+
+
+def window_workspace(BH: int, S: int, d_head: int, window: int, sinks: int, device="cuda"):
+    """The workspace that a windowed backward of this shape needs, or None when it needs none. It
+    holds nothing between calls; calls that overlap in time need one each."""
+    nbytes = window_workspace_bytes(BH, S, d_head, window, sinks)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def flash_attention_window_forward(out, lse, q, k, v, BH: int, S: int, d_head: int, scale: float,
+                                   window: int, sinks: int = 0, stream=None) -> None:
+    """fp32 forward in which query i sees key j when j <= i and (j > i - window or j < sinks)."""
+    ptrs = _forward_ptrs(torch.float32, out, lse, q, k, v, BH, S, d_head)
+    _same_device((out, lse, q, k, v))
+    _check(lib().dadgpt_flash_attention_window_forward(
+        *ptrs, BH, S, d_head, scale, window, sinks, _stream_ptr(stream)))
+
+
+def flash_attention_window_backward(dq, dk, dv, delta, dout, out, lse, q, k, v, BH: int, S: int,
+                                    d_head: int, scale: float, window: int, sinks: int = 0,
+                                    workspace=None, stream=None) -> None:
+    """Its backward, with the same window and sinks; workspace: window_workspace(...)."""
+    ptrs = _backward_ptrs(torch.float32, dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S, d_head)
+    _same_device((dq, dk, dv, delta, dout, out, lse, q, k, v, workspace))
+    _check(lib().dadgpt_flash_attention_window_backward(
+        *ptrs, BH, S, d_head, scale, window, sinks, *_workspace(workspace), _stream_ptr(stream)))
+
+
+def flash_attention_window_forward_bf16(out, lse, q, k, v, BH: int, S: int, d_head: int,
+                                        scale: float, window: int, sinks: int = 0,
+                                        stream=None) -> None:
+    ptrs = _forward_ptrs(torch.bfloat16, out, lse, q, k, v, BH, S, d_head)
+    _same_device((out, lse, q, k, v))
+    _check(lib().dadgpt_flash_attention_window_forward_bf16(
+        *ptrs, BH, S, d_head, scale, window, sinks, _stream_ptr(stream)))
+
+
+def flash_attention_window_backward_bf16(dq, dk, dv, delta, dout, out, lse, q, k, v, BH: int,
+                                         S: int, d_head: int, scale: float, window: int,
+                                         sinks: int = 0, workspace=None, stream=None) -> None:
+    ptrs = _backward_ptrs(torch.bfloat16, dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S,
+                          d_head)
+    _same_device((dq, dk, dv, delta, dout, out, lse, q, k, v, workspace))
+    _check(lib().dadgpt_flash_attention_window_backward_bf16(
+        *ptrs, BH, S, d_head, scale, window, sinks, *_workspace(workspace), _stream_ptr(stream)))
+
+
+def flash_attention_window_forward_bf16_strided(out, lse, q, k, v, scale: float, window: int,
+                                                sinks: int = 0, stream=None) -> None:
+    """The windowed forward over [B, H, S, d_head] views of any row placement."""
+    shape = B, H, S, D = q.shape
+    st = _Strides4(_head_view(q, "q", shape), _head_view(k, "k", shape),
+                   _head_view(v, "v", shape), _head_view(out, "out", shape))
+    _require(lse, "lse", torch.float32, B * H * S)
+    _same_device((out, lse, q, k, v))
+    _check(lib().dadgpt_flash_attention_window_forward_bf16_strided(
+        _ptr(out), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), B, H, S, D, scale, window, sinks, st,
+        _stream_ptr(stream)))
+
+
+def flash_attention_window_backward_bf16_strided(dq, dk, dv, delta, dout, out, lse, q, k, v,
+                                                 scale: float, window: int, sinks: int = 0,
+                                                 workspace=None, stream=None) -> None:
+    """Its backward over [B, H, S, d_head] views."""
+    shape = B, H, S, D = q.shape
+    st = _Strides8(_head_view(q, "q", shape), _head_view(k, "k", shape),
+                   _head_view(v, "v", shape), _head_view(out, "out", shape),
+                   _head_view(dout, "dout", shape), _head_view(dq, "dq", shape),
+                   _head_view(dk, "dk", shape), _head_view(dv, "dv", shape))
+    _require(delta, "delta", torch.float32, B * H * S)
+    _require(lse, "lse", torch.float32, B * H * S)
+    _same_device((dq, dk, dv, delta, dout, out, lse, q, k, v, workspace))
+    _check(lib().dadgpt_flash_attention_window_backward_bf16_strided(
+        _ptr(dq), _ptr(dk), _ptr(dv), _ptr(delta), _ptr(dout), _ptr(out), _ptr(lse), _ptr(q),
+        _ptr(k), _ptr(v), B, H, S, D, scale, window, sinks, st, *_workspace(workspace),
+        _stream_ptr(stream)))
+
+
+def flash_attention_window_forward_bf16_tokens(out, ld_out: int, lse, q, k, v, ld_qkv: int,
+                                               B: int, H: int, S: int, d_head: int, scale: float,
+                                               window: int, sinks: int = 0, stream=None) -> None:
+    """Token-major windowed forward (see flash_attention_forward_bf16_tokens)."""
+    _check(lib().dadgpt_flash_attention_window_forward_bf16_tokens(
+        _ptr(out), ld_out, _ptr(lse), _ptr(q), _ptr(k), _ptr(v), ld_qkv, B, H, S, d_head, scale,
+        window, sinks, _stream_ptr(stream)))
+
+
+def flash_attention_window_backward_bf16_tokens(dq, dk, dv, ld_dqkv: int, delta, dout, out,
+                                                ld_out: int, lse, q, k, v, ld_qkv: int, B: int,
+                                                H: int, S: int, d_head: int, scale: float,
+                                                window: int, sinks: int = 0, workspace=None,
+                                                stream=None) -> None:
+    """Token-major windowed backward (see flash_attention_backward_bf16_tokens)."""
+    _check(lib().dadgpt_flash_attention_window_backward_bf16_tokens(
+        _ptr(dq), _ptr(dk), _ptr(dv), ld_dqkv, _ptr(delta), _ptr(dout), _ptr(out), ld_out,
+        _ptr(lse), _ptr(q), _ptr(k), _ptr(v), ld_qkv, B, H, S, d_head, scale, window, sinks,
+        *_workspace(workspace), _stream_ptr(stream)))
+
+
+def decode_attention_window(out, q, k_cache, v_cache, lens, n_seq, n_heads, max_len, d_head, scale,
+                            window, sinks, workspace, stream=None) -> None:
+    """decode_attention under the mask of each cache's last row: keys [0, sinks) and
+    [len - window, len). The workspace is decode_workspace's."""
+    dt = q.dtype
+    if dt not in (torch.bfloat16, torch.float32):
+        raise TypeError("decode_attention_window: q must be bfloat16 or float32")
+    rows = n_seq * n_heads
+    pq, po = _ptrs(dt, rows * d_head, (q, out), ("q", "out"))
+    pk, pv = _ptrs(dt, rows * max_len * d_head, (k_cache, v_cache), ("k_cache", "v_cache"))
+    pl, = _ptrs(torch.int32, n_seq, (lens,), ("lens",))
+    _same_device((out, q, k_cache, v_cache, lens, workspace))
+    fn = (lib().dadgpt_decode_attention_window_bf16 if dt == torch.bfloat16
+          else lib().dadgpt_decode_attention_window_f32)
+    _check(fn(po, pq, pk, pv, pl, n_seq, n_heads, max_len, d_head, scale, window, sinks,
+              *_workspace(workspace), _stream_ptr(stream)))
 
 
 # --------------------------------------------------------------- allocating conveniences

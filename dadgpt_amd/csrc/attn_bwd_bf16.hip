@@ -29,6 +29,7 @@
 #include "kernels.hpp"
 #include "lanes.hpp"
 #include "tiles.hpp"
+#include "window.hpp"
 
 namespace dadgpt {
 namespace {
@@ -103,8 +104,9 @@ constexpr int kKW = 32;  // keys per wave
 //   s  = -lse/scale + Q K^T         so P = exp2(c s) with c = scale log2(e)
 //   dp = -delta + dO V^T            so P dp = P (dP - delta) = dS
 // which leaves two multiplies and an exp2 per score on the VALU. slc holds the tile's
-// -lse/scale, sdl its -delta. `mask` zeroes P for keys after the query and for tile rows past
-// S (rows_left = S - r0; those rows hold copies of row S-1). It is a runtime flag, not a
+// -lse/scale, sdl its -delta. `mask` zeroes P for keys after the query and for tile rows at or past
+// rows_left (S - r0: those rows hold copies of row S-1; with a window, the lane's key's last query
+// if that comes first). It is a runtime flag, not a
 // template parameter, and guards only the few instructions that zero P: with two inlined copies
 // of the block the compiler gave their MFMAs different accumulator registers and copied all 64
 // accumulator values back after every block.
@@ -249,6 +251,16 @@ struct BwdArgs {
   AttnLayout L;
   DropParams dr;
 };
+// The windowed backward's arguments: query tiles of a piece of a sink block (piece_tiles), and
+// the fp32 partials of the sink rows, [BH][piece][dK, dV][sink rows, whole 32s][D].
+struct WindowBwdArgs : Window {
+  int piece_tiles, pieces;
+  float* partial;
+};
+template <bool WIN>
+struct WindowBwdArg {};
+template <>
+struct WindowBwdArg<true> : WindowBwdArgs {};
 
 // LDS of a workgroup: two streamed tiles (Q and dO, or K and V), double-buffered (constant
 // buffer indices in the unrolled loop; see the forward kernel).
@@ -292,12 +304,30 @@ __device__ __forceinline__ void delta_rows(float* delta, const Slice<D, STRIDED>
   }
 }
 
+// A wave's 32 x D fp32 accumulators (accumulator layout, as store_rows_staged) as rows of a
+// partial.
+template <int D>
+__device__ __forceinline__ void store_partial(float* dst, const f32x16 (&acc)[D / 32], int lane) {
+  const int l32 = lane & 31, hi = lane >> 5;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(dst + l32 * D + 32 * db + 8 * g + 4 * hi) =
+          f32x4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+}
+
 // One workgroup's dK and dV. OWN_DELTA: delta is computed here, into own_delta (one float for
 // each row from the first tile on); otherwise it is read from a.delta.
-template <int D, bool STRIDED, bool DROP, int KS, bool OWN_DELTA>
+// WIN: the queries of a key block end with its last key's window; a block with sink keys instead
+// has every later query, in pieces of win.piece_tiles tiles. The first piece is at least as long
+// as a block's window, so later ones have the sink keys alone: they leave them as partials, and
+// the first piece leaves its sink keys' partial next to the block's final rows.
+template <int D, bool STRIDED, bool DROP, int KS, bool OWN_DELTA, bool WIN = false>
 __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kblk,
                                                BwdTiles<D>& tiles, BwdStats& stats,
-                                               float* own_delta) {
+                                               float* own_delta,
+                                               const WindowBwdArg<WIN>& win = {}, int piece = 0) {
   constexpr int kGroups = kWaves / KS, KB = kKW * kGroups;  // key groups, keys
   constexpr int DS = D / 16, DB = D / 32;
   auto& sq = tiles.a;
@@ -321,8 +351,19 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
 
   const int kw0 = kblk * KB + grp * kKW;
   const int key = kw0 + l32;
-  const int t_first = (kblk * KB) / kTileRows;
-  const int t_end = (S - 1) / kTileRows + 1;
+  int t_first = (kblk * KB) / kTileRows;
+  int t_end = (S - 1) / kTileRows + 1;
+  bool split = false;  // the sink keys' sums go on in other pieces
+  if constexpr (WIN) {
+    if (kblk * KB < win.sinks) {
+      split = t_end - t_first > win.piece_tiles;
+      t_first += piece * win.piece_tiles;
+      if (t_first >= t_end) return;
+      t_end = min(t_end, t_first + win.piece_tiles);
+    } else {
+      t_end = min(t_end, (kblk * KB + KB + win.window - 2) / kTileRows + 1);
+    }
+  }
 
   // B operands (K^T, V^T along D): lane holds key row `key`, columns 16*ds + 8*hi + 0..7.
   bf16x8 kop[DS], vop[DS];
@@ -361,7 +402,8 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
   // compiler, which does not see the direct loads, then has nothing left to wait for).
   issue(t_first, sq[0], sdo[0], 0);
   if constexpr (OWN_DELTA)
-    delta_rows<D, STRIDED>(own_delta, sl, dout, a.out, t_first * kTileRows, S);
+    delta_rows<D, STRIDED>(own_delta, sl, dout, a.out, t_first * kTileRows,
+                           WIN ? min(S, t_end * kTileRows) : S);
   wait_vm_lds<0>();
   __builtin_amdgcn_s_barrier();
 
@@ -382,12 +424,17 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
       for (int i = 0; i < 2 / KS; ++i) {
         const int qb = KS == 1 ? i : sub, qlo = r0 + 32 * qb;  // first query of the block
         if (qlo + 31 < kw0) continue;   // every key of the wave is after every query
+        bool mask = edge || qlo < kw0 + kKW - 1;  // some key after some query, or rows past S
+        int rows_left = S - r0;
+        if constexpr (WIN) {
+          if (!chunk_visible(kw0, qlo, win)) continue;
+          mask = edge || !chunk_whole(kw0, qlo, win);
+          if (key >= win.sinks) rows_left = min(rows_left, key - r0 + win.window);
+        }
         uint32_t keep = 0;
         if constexpr (DROP) keep = keep_col16(dr, (uint64_t)bh * S + qlo, kw0, lane);
-        // some key after some query, or rows past S: mask
-        dkdv_block<D, DROP, XA>(edge || qlo < kw0 + kKW - 1, dkacc, dvacc, kop, vop, cq, cdo,
-                                st[cb][0], st[cb][1], qb, key - r0, S - r0, lane, a.c, keep,
-                                dr.scale, lo);
+        dkdv_block<D, DROP, XA>(mask, dkacc, dvacc, kop, vop, cq, cdo, st[cb][0], st[cb][1], qb,
+                                key - r0, rows_left, lane, a.c, keep, dr.scale, lo);
       }
     }
     wait_vm_lds<0>();
@@ -398,10 +445,24 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
     if (t + 1 < t_end) tile(t + 1, sq[1], sdo[1], 1, sq[0], sdo[0], 0);
   }
 
+  // (where the wave's partials of dK and dV go, if it has any)
+  float* part = nullptr;
+  int part_dv = 0;
+  if constexpr (WIN) {
+    if (split && kw0 < win.sinks) {
+      part_dv = (win.sinks + 31) / 32 * 32 * D;
+      part = win.partial + ((size_t)bh * win.pieces + piece) * 2 * part_dv + kw0 * D;
+    }
+  }
+  const bool rows_out = !WIN || piece == 0;
   // the tiles are free after the last barrier
   if constexpr (KS == 1) {
+    if (WIN && part != nullptr) {
+      store_partial<D>(part, dkacc, lane);
+      store_partial<D>(part + part_dv, dvacc, lane);
+    }
     // each wave stages its 32 rows in its quarter of sq (dK) and sdo (dV)
-    if (kw0 < S) {
+    if (kw0 < S && rows_out) {
       store_rows_staged<D>(sl.row(dk, kTDK, kw0), sl.pitch(kTDK), S - kw0, dkacc, a.scale,
                            &sq[0][0] + wave * kKW * D, lane);
       store_rows_staged<D>(sl.row(dv, kTDV, kw0), sl.pitch(kTDV), S - kw0, dvacc, 1.0f,
@@ -421,12 +482,16 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
     if (kw0 >= S) return;
     if (sub == 0) {
       add_acc(dkacc, slot_k, lane);
-      store_rows_staged<D>(sl.row(dk, kTDK, kw0), sl.pitch(kTDK), S - kw0, dkacc, a.scale,
-                           reinterpret_cast<bf16*>(slot_k), lane);
+      if (WIN && part != nullptr) store_partial<D>(part, dkacc, lane);
+      if (rows_out)
+        store_rows_staged<D>(sl.row(dk, kTDK, kw0), sl.pitch(kTDK), S - kw0, dkacc, a.scale,
+                             reinterpret_cast<bf16*>(slot_k), lane);
     } else {
       add_acc(dvacc, slot_v, lane);
-      store_rows_staged<D>(sl.row(dv, kTDV, kw0), sl.pitch(kTDV), S - kw0, dvacc, 1.0f,
-                           reinterpret_cast<bf16*>(slot_v), lane);
+      if (WIN && part != nullptr) store_partial<D>(part + part_dv, dvacc, lane);
+      if (rows_out)
+        store_rows_staged<D>(sl.row(dv, kTDV, kw0), sl.pitch(kTDV), S - kw0, dvacc, 1.0f,
+                             reinterpret_cast<bf16*>(slot_v), lane);
     }
   }
 }
@@ -452,13 +517,15 @@ constexpr int kQW = 32;  // queries per wave
 // loop must not cost a wave per SIMD, though (see dq_bf16_kernel). With dropout (DROP), dS =
 // P (dP * f - delta), f = keep/(1-p) from register 8j+e's uniform in `keep`: dP from zero, as
 // those registers cost that kernel more too (96 x 1024: backward 88 -> 92.5).
-template <int D, bool DROP, bool FROM_DELTA>
+// WIN: a masked chunk hides what `hidden` says, keys counted from the chunk's first of the lane.
+template <int D, bool DROP, bool FROM_DELTA, bool WIN = false>
 __device__ __forceinline__ void dq_chunk(bool diag, f32x16 (&dqacc)[D / 32],
                                          const bf16x8 (&qop)[D / 16],
                                          const bf16x8 (&doop)[D / 16], const bf16* sk,
                                          const bf16* sv, int kb, int qrow_minus_k0, float lse2,
                                          const f32x16& ndl, int lane, float scale_log2,
-                                         const KeepWords16& keep, const DropParams& dr) {
+                                         const KeepWords16& keep, const DropParams& dr,
+                                         const HiddenKeys& hidden = {}) {
   constexpr int DS = D / 16, DB = D / 32;
   const int l32 = lane & 31, hi = lane >> 5;
   f32x16 s = f32x16{}, dp = f32x16{};
@@ -483,8 +550,12 @@ __device__ __forceinline__ void dq_chunk(bool diag, f32x16 (&dqacc)[D / 32],
   }
   if (diag) {  // runtime flag around the zeroing only (see dkdv_block)
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      pr[i] = 32 * kb + 16 * (i / 8) + 8 * hi + i % 8 > qrow_minus_k0 ? 0.f : pr[i];
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (WIN)
+        pr[i] = hidden(16 * (i / 8) + i % 8) ? 0.f : pr[i];
+      else
+        pr[i] = 32 * kb + 16 * (i / 8) + 8 * hi + i % 8 > qrow_minus_k0 ? 0.f : pr[i];
+    }
   }
   bf16x8 dsb[2];
 #pragma unroll
@@ -517,9 +588,10 @@ __device__ __forceinline__ void dq_chunk(bool diag, f32x16 (&dqacc)[D / 32],
 // dQ for one query block per wave; the kernel also computes delta = rowsum(dO * O) of its
 // rows (from the dO operands it holds and one load of O) and writes it for the dK/dV kernel,
 // so the backward needs no separate delta pass.
-template <int D, bool STRIDED, bool DROP, int KS, bool WRITE_DELTA, bool FROM_DELTA>
+template <int D, bool STRIDED, bool DROP, int KS, bool WRITE_DELTA, bool FROM_DELTA,
+          bool WIN = false>
 __device__ __forceinline__ void dq_workgroup(const BwdArgs& a, int bh, int qblk,
-                                             BwdTiles<D>& tiles) {
+                                             BwdTiles<D>& tiles, const WindowArg<WIN>& win = {}) {
   constexpr int kGroups = kWaves / KS, QB = kQW * kGroups;  // query groups, queries
   constexpr int DS = D / 16, DB = D / 32;
   auto& sk = tiles.a;
@@ -545,7 +617,8 @@ __device__ __forceinline__ void dq_workgroup(const BwdArgs& a, int bh, int qblk,
   const int q0 = qblk * QB + grp * kQW;
   const int qrow = q0 + l32;
   const int wg_last = min(S, (qblk + 1) * QB) - 1;
-  const int n_tiles = wg_last / kTileRows + 1;
+  const KeyTiles<WIN> keys(qblk * QB, wg_last, win);
+  const int n_tiles = keys.count();
 
   // lane holds row qrow, columns 16*ds + 8*hi + 0..7 of Q, dO and O (zeros past S)
   bf16x8 qop[DS], doop[DS], oop[DS];
@@ -571,8 +644,8 @@ __device__ __forceinline__ void dq_workgroup(const BwdArgs& a, int bh, int qblk,
   uint32_t koff[Dma::PER_WAVE], voff[Dma::PER_WAVE];
   Dma::offsets(koff, wave, lane, kp);
   Dma::offsets(voff, wave, lane, vp);
-  Dma::load_any(sk[0], kg, 0, S, koff, wave, lane, kp);
-  Dma::load_any(sv[0], vg, 0, S, voff, wave, lane, vp);
+  Dma::load_any(sk[0], kg, keys.row(0), S, koff, wave, lane, kp);
+  Dma::load_any(sv[0], vg, keys.row(0), S, voff, wave, lane, vp);
   wait_vm_lds<0>();
   __builtin_amdgcn_s_barrier();
   // Use the loaded values only from here on, so their loads share the wait above.
@@ -595,10 +668,11 @@ __device__ __forceinline__ void dq_workgroup(const BwdArgs& a, int bh, int qblk,
   if (WRITE_DELTA && hi == 0 && qrow < S && sub == 0) delta[(size_t)bh * S + qrow] = dlt;
 
   auto tile = [&](int t, const bf16* ck, const bf16* cv, bf16* nk, bf16* nv) {
-    const int k0 = t * kTileRows;
+    const int k0 = keys.row(t);
     if (t + 1 < n_tiles) {
-      Dma::load_any(nk, kg, k0 + kTileRows, S, koff, wave, lane, kp);
-      Dma::load_any(nv, vg, k0 + kTileRows, S, voff, wave, lane, vp);
+      const int kn = WIN ? keys.row(t + 1) : k0 + kTileRows;
+      Dma::load_any(nk, kg, kn, S, koff, wave, lane, kp);
+      Dma::load_any(nv, vg, kn, S, voff, wave, lane, vp);
     }
     if (q0 < S) {
 #pragma unroll
@@ -607,9 +681,16 @@ __device__ __forceinline__ void dq_workgroup(const BwdArgs& a, int bh, int qblk,
         if (klo > q0 + kQW - 1) continue;    // every key after every query of the wave
         KeepWords16 keep = {};
         if constexpr (DROP) keep = keep_words16(dr, (uint64_t)bh * S + qrow, klo, hi);
-        // some key after some query: mask
-        dq_chunk<D, DROP, FROM_DELTA>(klo + 31 > q0, dqacc, qop, doop, ck, cv, kb, qrow - k0,
-                                      lse2, ndl, lane, scale_log2, keep, dr);
+        if constexpr (WIN) {
+          if (!chunk_visible(klo, q0, win)) continue;
+          dq_chunk<D, DROP, FROM_DELTA, true>(!chunk_whole(klo, q0, win), dqacc, qop, doop, ck, cv,
+                                              kb, qrow - k0, lse2, ndl, lane, scale_log2, keep,
+                                              dr, HiddenKeys(klo + 8 * hi, qrow, win));
+        } else {
+          // some key after some query: mask
+          dq_chunk<D, DROP, FROM_DELTA>(klo + 31 > q0, dqacc, qop, doop, ck, cv, kb, qrow - k0,
+                                        lse2, ndl, lane, scale_log2, keep, dr);
+        }
       }
     }
     wait_vm_lds<0>();
@@ -662,6 +743,76 @@ __global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(DROP)) void bwd_bf16_k
   else
     dq_workgroup<D, STRIDED, DROP, KS, OWN_DELTA, !DROP>(a, blockIdx.x,
                                                          gridDim.y - 1 - blockIdx.y, tiles);
+}
+
+// ---------------------------------------------------------------- sliding window
+// The windowed kernels' grids: dQ as above; dK/dV has `blocks` key blocks and then the later pieces
+// of the sink blocks, piece by piece.
+template <int D, bool STRIDED, int KS, bool OWN_DELTA>
+__device__ __forceinline__ void window_dkdv(const BwdArgs& a, const WindowBwdArg<true>& win,
+                                            int blocks, int y, BwdTiles<D>& tiles,
+                                            BwdStats& stats, float* own_delta) {
+  int kblk = y, piece = 0;
+  if (y >= blocks) {
+    constexpr int KB = kKW * kWaves / KS;
+    const int sink_blocks = min(blocks, (win.sinks + KB - 1) / KB);
+    piece = (y - blocks) / sink_blocks + 1;
+    kblk = (y - blocks) % sink_blocks;
+  }
+  dkdv_workgroup<D, STRIDED, false, KS, OWN_DELTA, true>(a, blockIdx.x, kblk, tiles, stats,
+                                                         own_delta, win, piece);
+}
+template <int D, bool STRIDED, int KS>
+__global__ __launch_bounds__(64 * kWaves, kDqMinBlocks) void window_dq_bf16_kernel(
+    const BwdArgs a, const WindowArg<true> win) {
+  __shared__ BwdTiles<D> tiles;
+  constexpr bool kFromDelta = D == 64 || KS == 2;  // as dq_bf16_kernel
+  dq_workgroup<D, STRIDED, false, KS, true, kFromDelta, true>(a, blockIdx.x, blockIdx.y, tiles,
+                                                              win);
+}
+template <int D, bool STRIDED, int KS>
+__global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(false)) void window_dkdv_bf16_kernel(
+    const BwdArgs a, const WindowBwdArg<true> win, int blocks) {
+  __shared__ BwdTiles<D> tiles;
+  __shared__ BwdStats stats;
+  window_dkdv<D, STRIDED, KS, false>(a, win, blocks, blockIdx.y, tiles, stats, nullptr);
+}
+// Both in one launch, delta where it is needed (at most kOwnDeltaMaxS rows a dK/dV workgroup): the
+// dK/dV workgroups first.
+template <int D, bool STRIDED, int KS>
+__global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(false)) void window_bwd_bf16_kernel(
+    const BwdArgs a, const WindowBwdArg<true> win, int blocks, int dkdv_blocks) {
+  __shared__ BwdTiles<D> tiles;
+  __shared__ BwdStats stats;
+  __shared__ float own_delta[kOwnDeltaMaxS];
+  const int y = blockIdx.y;
+  if (y < dkdv_blocks)
+    window_dkdv<D, STRIDED, KS, true>(a, win, blocks, y, tiles, stats, own_delta);
+  else
+    dq_workgroup<D, STRIDED, false, KS, true, true, true>(a, blockIdx.x, y - dkdv_blocks, tiles,
+                                                          {win});
+}
+
+// The sink rows of dK and dV from their pieces' partials, summed in the pieces' order: a thread
+// for four columns.
+template <int D>
+__global__ __launch_bounds__(256) void window_join_bf16_kernel(const BwdArgs a,
+                                                               const WindowBwdArgs win, int KB) {
+  const int i = blockIdx.y * 256 + threadIdx.x, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
+  const int which = i / (D / 4) / win.sinks, bh = blockIdx.x;
+  if (which > 1 || row >= a.S) return;
+  const int rows = (win.sinks + 31) / 32 * 32;
+  const int tiles = (a.S - 1) / kTileRows + 1 - row / KB * KB / kTileRows;  // of the row's block
+  const int pieces = (tiles + win.piece_tiles - 1) / win.piece_tiles;
+  if (pieces < 2) return;  // its workgroup has written the final row
+  const float* p = win.partial + ((size_t)bh * win.pieces * 2 + which) * rows * D +
+                   (size_t)row * D + col;
+  f32x4 sum = f32x4{};
+  for (int j = 0; j < pieces; ++j) sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * rows * D);
+  const Slice<D, true> sl(a.L, bh, a.S);
+  const float mul = which == 0 ? a.scale : 1.0f;
+  st_g64((which == 0 ? sl.row(a.dk, kTDK, row) : sl.row(a.dv, kTDV, row)) + col,
+         u32x2{pack_bf16x2(sum[0] * mul, sum[1] * mul), pack_bf16x2(sum[2] * mul, sum[3] * mul)});
 }
 
 // How a backward is launched: dQ, then dK/dV (kSeparate); both in one launch with delta
@@ -781,7 +932,80 @@ hipError_t launch_bwd_bf16_t(bf16* dq, bf16* dk, bf16* dv, float* delta, const b
   return e;
 }
 
+// Query tiles of a piece of a sink block: a key block's window (of KB keys), so that the pieces
+// take as long as the other workgroups, and at least eight.
+int window_piece_tiles(const Window& w, int KB) {
+  const long long tiles = ((long long)KB + w.window - 2) / kTileRows + 1;
+  return (int)(tiles > 8 ? tiles : 8);
+}
+int window_pieces(int S, const Window& w, int KB) {
+  if (w.sinks == 0) return 1;
+  const int tiles = (S - 1) / kTileRows + 1, of = window_piece_tiles(w, KB);
+  return (tiles + of - 1) / of;
+}
+
+template <int D>
+hipError_t launch_window_bwd_bf16_t(const BwdArgs& args, int BH, const Window& w, float* partial,
+                                    hipStream_t stream) {
+  const int S = args.S, ks = waves_per_group(BH, S, D, false);
+  const int KB = 32 * kWaves / ks, blocks = (S + KB - 1) / KB;
+  WindowBwdArg<true> win;
+  static_cast<Window&>(win) = w;
+  win.piece_tiles = window_piece_tiles(w, KB);
+  win.pieces = window_pieces(S, w, KB);
+  win.partial = partial;
+  const int sink_blocks = (w.sinks + KB - 1) / KB < blocks ? (w.sinks + KB - 1) / KB : blocks;
+  const int dkdv_blocks = blocks + (win.pieces - 1) * sink_blocks;
+  const bool one = win.piece_tiles * kTileRows <= kOwnDeltaMaxS;
+  hipError_t e = hipSuccess;
+  with_shape(ks, false, !is_contiguous(args.L, S, D), [&](auto strided, auto, auto kw) {
+    if (one) {
+      window_bwd_bf16_kernel<D, strided(), kw()>
+          <<<dim3(BH, dkdv_blocks + blocks), 64 * kWaves, 0, stream>>>(args, win, blocks,
+                                                                       dkdv_blocks);
+      e = hipGetLastError();
+      return;
+    }
+    window_dq_bf16_kernel<D, strided(), kw()>
+        <<<dim3(BH, blocks), 64 * kWaves, 0, stream>>>(args, {w});
+    if ((e = hipGetLastError()) != hipSuccess) return;
+    window_dkdv_bf16_kernel<D, strided(), kw()>
+        <<<dim3(BH, dkdv_blocks), 64 * kWaves, 0, stream>>>(args, win, blocks);
+    e = hipGetLastError();
+  });
+  if (e != hipSuccess || win.pieces == 1) return e;
+  window_join_bf16_kernel<D>
+      <<<dim3(BH, (w.sinks * (D / 4) * 2 + 255) / 256), 256, 0, stream>>>(args, win, KB);
+  return hipGetLastError();
+}
+
 }  // namespace
+
+// Of the two element types' and both wave counts' largest.
+size_t window_workspace_bytes(int BH, int S, int D, const Window& w) {
+  if (w.window >= S || w.sinks == 0) return 0;
+  const int pieces = window_pieces(S, w, 32 * kWaves / 2);
+  const size_t rows = (size_t)(w.sinks < S ? w.sinks + 31 : S + 31) / 32 * 32;
+  return pieces == 1 ? 0 : sizeof(float) * BH * pieces * 2 * rows * D;
+}
+
+hipError_t launch_window_bwd_bf16(bf16* dq, bf16* dk, bf16* dv, float* delta, const bf16* dout,
+                                  const bf16* out, const float* lse, const bf16* q, const bf16* k,
+                                  const bf16* v, int BH, int S, int D, float scale,
+                                  const AttnLayout& layout, const Window& window,
+                                  void* workspace, hipStream_t stream) {
+  if (window.window >= S)
+    return launch_bwd_bf16(dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S, D, scale, layout,
+                           stream);
+  const float se = scale != 0.f ? scale : 1e-30f;  // as launch_bwd_bf16_t
+  const BwdArgs args{dq,  dk,  dv, delta, q,     k,     v,          dout,
+                     out, lse, S,  scale, scale * kLog2e, se * kLog2e, -1.0f / se, layout, {}};
+  const Window w{window.window, window.sinks < S ? window.sinks : S};
+  float* partial = static_cast<float*>(workspace);
+  if (D == 64) return launch_window_bwd_bf16_t<64>(args, BH, w, partial, stream);
+  if (D == 32) return launch_window_bwd_bf16_t<32>(args, BH, w, partial, stream);
+  return hipErrorInvalidValue;
+}
 
 hipError_t launch_bwd_bf16(bf16* dq, bf16* dk, bf16* dv, float* delta, const bf16* dout,
                            const bf16* out, const float* lse, const bf16* q, const bf16* k,

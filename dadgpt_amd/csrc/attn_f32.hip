@@ -42,6 +42,7 @@
 #include "kernels.hpp"
 #include "lanes.hpp"
 #include "tiles.hpp"
+#include "window.hpp"
 
 namespace dadgpt {
 namespace {
@@ -349,11 +350,12 @@ __device__ __forceinline__ void store_rows_t(float* dst, int row0, int S,
 // ------------------------------------------------------------------------------ forward
 
 // ONCE: the conversions of Q's and the weights' splits forced to happen once (pack_once).
-template <int D, bool DROP, int KS, bool ONCE>
+// WIN: sliding window and sinks, as in the bf16 forward.
+template <int D, bool DROP, int KS, bool ONCE, bool WIN = false>
 __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_kernel(
     float* __restrict__ out, float* __restrict__ lse, const float* __restrict__ q,
     const float* __restrict__ k, const float* __restrict__ v, int S, float scale,
-    const DropParams dr) {
+    const DropParams dr, const WindowArg<WIN> win) {
   constexpr int NT = 64 * kGroups * KS, TR = 64, CPT = 2 / KS;  // chunks per tile and wave
   // K and V tiles as three bf16 planes each; after the tile loop they hold the second waves'
   // partial results, then the epilogue's fp32 staging rows. With two waves per group there are
@@ -373,7 +375,8 @@ __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_ker
   const int q0 = blk * kRows + 32 * grp;  // the wave's first query
   const int qi = q0 + l32;                // this lane's query
   const int last = min(S, (blk + 1) * kRows) - 1;  // the workgroup's last query
-  const int n_tiles = last / TR + 1;
+  const KeyTiles<WIN, TR> keys(blk * kRows, last, win);
+  const int n_tiles = keys.count();
 
   X3 qb[D / 16];  // the lane's query row, split
   load_split_row<D, ONCE>(qb, q + base + (size_t)min(qi, S - 1) * D, h);
@@ -383,15 +386,15 @@ __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_ker
   float m = neg_inf(), lh = 0.f;  // running maximum; this lane half's sum of weights
 
   Tile<D, TR, NT> tk, tv;
-  tk.load(k + base, 0, S);
-  tv.load(v + base, 0, S);
+  tk.load(k + base, keys.row(0), S);
+  tv.load(v + base, keys.row(0), S);
   // Splits the loaded tile t into `to` and loads tile t + 1.
   auto stage = [&](int t, bf16* to) {
     store_x3<D, TR>(tk, to);
     store_x3<D, TR>(tv, to + kPlane);
     if (t + 1 < n_tiles) {
-      tk.load(k + base, (t + 1) * TR, S);
-      tv.load(v + base, (t + 1) * TR, S);
+      tk.load(k + base, keys.row(t + 1), S);
+      tv.load(v + base, keys.row(t + 1), S);
     }
   };
   auto compute = [&](int t, const bf16* skp) {
@@ -399,12 +402,21 @@ __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_ker
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
       const int c = KS == 1 ? i : sub;
-      const int key0 = t * TR + 32 * c;
+      const int key0 = keys.row(t) + 32 * c;
       if (key0 > q0 + 31) continue;  // wave-uniform: the whole chunk is in the future
+      if constexpr (WIN)
+        if (!chunk_visible(key0, q0, win)) continue;
       f32x16 s = score_tile_p<D, TR>(skp, 32 * c, qb, lane);
       // only the chunk whose first key is the wave's first query holds keys after a query
       // (or past S); waves are 32-query aligned, so it is the one with key0 == q0
-      const bool diag = key0 == q0;
+      bool diag = key0 == q0;
+      if constexpr (WIN) diag = !chunk_whole(key0, q0, win);
+      auto hidden = [&](int u) {
+        if constexpr (WIN)
+          return HiddenKeys(key0 + 8 * h, qi, win)(reg_row(u, 0));
+        else
+          return key0 + reg_row(u, h) > qi;
+      };
       // weights against the running maximum m as it stands (natural-log units)
       float w[16], ps;
       auto weights = [&](float mref) {
@@ -413,7 +425,7 @@ __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_ker
         if (diag) {
 #pragma unroll
           for (int u = 0; u < 16; ++u)
-            if (key0 + reg_row(u, h) > qi) w[u] = 0.f;
+            if (hidden(u)) w[u] = 0.f;
         }
         ps = w[0];  // (0 + w[0] could not be folded: it maps -0 to +0)
 #pragma unroll
@@ -430,8 +442,8 @@ __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_ker
         float cm = neg_inf();
 #pragma unroll
         for (int u = 0; u < 16; ++u)
-          if (!(diag && key0 + reg_row(u, h) > qi)) cm = fmaxf(cm, s[u] * scale);
-        // every row of a chunk the wave computes has a visible key: the row maximum is finite
+          if (!(diag && hidden(u))) cm = fmaxf(cm, s[u] * scale);
+        // a row that needs it has a visible key in the chunk: its maximum is finite
         const float mn = or_halves(need) ? fmaxf(m, max_halves(cm)) : m;
         // 0 on a row's first chunk (exp_acc has no -inf input path)
         const float alpha = m == neg_inf() ? 0.f : exp_acc(m - mn);
@@ -584,11 +596,26 @@ __device__ __forceinline__ void delta_rows(float* delta, const float* dout, cons
   }
 }
 
+// The windowed backward's arguments: rows of a piece of a sink block (a multiple of 64), and the
+// partials of the sink rows, [BH][piece][dK, dV][sink rows, whole 32s][D].
+struct F32WindowBwdArgs : Window {
+  int piece_rows, pieces;
+  float* partial;
+};
+template <bool WIN>
+struct F32WindowBwdArg {};
+template <>
+struct F32WindowBwdArg<true> : F32WindowBwdArgs {};
+
 // One workgroup's dK and dV. OWN_DELTA: delta is computed here, into own_delta (a float for each
-// row from the first tile on); otherwise it is read from a.delta.
-template <int D, bool DROP, int KS, bool OWN_DELTA>
+// row from the first tile on); otherwise it is read from a.delta. WIN: as in the bf16 kernel, the
+// queries of a key block end with its last key's window, and a block with sink keys has every
+// later query, in pieces; the first is at least as long as a block's window.
+template <int D, bool DROP, int KS, bool OWN_DELTA, bool WIN = false>
 __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, int blk,
-                                                   F32BwdShared<D, KS>& sm, float* own_delta) {
+                                                   F32BwdShared<D, KS>& sm, float* own_delta,
+                                                   const F32WindowBwdArg<WIN>& win = {},
+                                                   int piece = 0) {
   // Q and dO tiles: planes and raw
   using Lds = BwdLds<D, KS>;
   constexpr int TR = Lds::TR, NT = 64 * kGroups * KS;
@@ -609,8 +636,20 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
   const size_t base = (size_t)bh * S * D;
   const int k0 = blk * kRows + 32 * grp;  // the wave's first key
   const int kj = k0 + l32;                // this lane's key
-  const int t0 = (blk * kRows) / TR;  // first query tile with a query >= the first key
-  const int n_tiles = (S + TR - 1) / TR;
+  int t0 = (blk * kRows) / TR;  // first query tile with a query >= the first key
+  int n_tiles = (S + TR - 1) / TR;
+  bool split = false;  // the sink keys' sums go on in other pieces
+  if constexpr (WIN) {
+    if (blk * kRows < win.sinks) {
+      const int of = win.piece_rows / TR;
+      split = n_tiles - t0 > of;
+      t0 += piece * of;
+      if (t0 >= n_tiles) return;
+      n_tiles = min(n_tiles, t0 + of);
+    } else {
+      n_tiles = min(n_tiles, (blk * kRows + kRows + win.window - 2) / TR + 1);
+    }
+  }
 
   // The lane's K and V rows (score-product B layout), split. At D = 64 V's lower planes go to LDS,
   // which the two waves of a group share (published by the first barrier): with all six planes
@@ -658,7 +697,8 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
   tg.issue(t0 * TR);
   load_stats(t0 * TR);
   if constexpr (OWN_DELTA)
-    delta_rows<D, NT>(own_delta, dout + base, a.out + base, t0 * TR, S);
+    delta_rows<D, NT>(own_delta, dout + base, a.out + base, t0 * TR,
+                      WIN ? min(S, n_tiles * TR) : S);
   for (int t = t0; t < n_tiles; ++t) {
     wait_vm_lds<0>();  // this wave's pieces of the tile
     __syncthreads();   // every wave is done with the previous tile's planes
@@ -677,6 +717,8 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
     const int qrow0 = t * TR + 32 * sub;
     // wave-uniform: every query of the chunk precedes every key, or lies past S
     if (qrow0 + 31 < k0 || (KS > 1 && qrow0 >= S)) continue;
+    if constexpr (WIN)
+      if (!chunk_visible(k0, qrow0, win)) continue;
     const bf16 *qc = sqp + 32 * sub * D, *gc = sgp + 32 * sub * D;
     // lane (l32, h), register u: query qrow0 + reg_row(u, h), key kj
     f32x16 s = score_tile_px<D, TR>(qc, kb, lo);   // Q K^T
@@ -698,11 +740,17 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
     }
     // keys after a query, or rows past S, only where the chunk reaches the wave's first
     // keys or S (wave-uniform)
-    if (qrow0 < k0 + 31 || qrow0 + 31 >= S) {
+    bool mask = qrow0 < k0 + 31 || qrow0 + 31 >= S;
+    int end = S;
+    if constexpr (WIN) {
+      mask = qrow0 + 31 >= S || !chunk_whole(k0, qrow0, win);
+      if (kj >= win.sinks) end = min(S, kj + win.window);
+    }
+    if (mask) {
 #pragma unroll
       for (int u = 0; u < 16; ++u) {
         const int qrow = qrow0 + reg_row(u, h);
-        s[u] = kj <= qrow && qrow < S ? s[u] : 0.f;
+        s[u] = kj <= qrow && qrow < end ? s[u] : 0.f;
       }
     }
 #pragma unroll
@@ -734,14 +782,24 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
     add_acc(da, reinterpret_cast<const AccLds*>(slot), lane);
     __builtin_amdgcn_wave_barrier();
   }
+  if constexpr (WIN) {
+    if (split && k0 < win.sinks) {
+      const int rows = (win.sinks + 31) / 32 * 32;
+      float* part = win.partial + ((size_t)bh * win.pieces + piece) * 2 * rows * D;
+      store_rows_t<D>(part, k0, rows, dka, 1.0f, slot, lane);
+      store_rows_t<D>(part + rows * D, k0, rows, dva, 1.0f, slot, lane);
+    }
+    if (piece > 0) return;
+  }
   store_rows_t<D>(dk + base, k0, S, dka, 1.0f, slot, lane);
   store_rows_t<D>(dv + base, k0, S, dva, 1.0f, slot, lane);  // after the wave's dK reads
 }
 
 // One workgroup's dQ. OWN_DELTA: delta of its rows is computed here and written; otherwise read.
-template <int D, bool DROP, int KS, bool OWN_DELTA>
+template <int D, bool DROP, int KS, bool OWN_DELTA, bool WIN = false>
 __device__ __forceinline__ void dq_f32_workgroup(const F32BwdArgs& a, int bh, int blk,
-                                                 F32BwdShared<D, KS>& sm) {
+                                                 F32BwdShared<D, KS>& sm,
+                                                 const WindowArg<WIN>& win = {}) {
   // K and V tiles: planes and raw
   using Lds = BwdLds<D, KS>;
   constexpr int TR = Lds::TR, NT = 64 * kGroups * KS;
@@ -763,7 +821,8 @@ __device__ __forceinline__ void dq_f32_workgroup(const F32BwdArgs& a, int bh, in
   const int qi = q0 + l32;
   const int qc = min(qi, S - 1);
   const int last = min(S, (blk + 1) * kRows) - 1;
-  const int n_tiles = last / TR + 1;
+  const KeyTiles<WIN, TR> keys(blk * kRows, last, win);
+  const int n_tiles = keys.count();
 
   X3 qb[D / 16], gb[D / 16];  // the lane's Q and dO rows (score-product B layout), split
   load_split_row<D>(qb, q + base + (size_t)qc * D, h);
@@ -794,8 +853,8 @@ __device__ __forceinline__ void dq_f32_workgroup(const F32BwdArgs& a, int bh, in
 
   const RawTile<D, TR, NT> tk{k + base, raw, S, wave, lane},
       tv{v + base, raw + TR * D, S, wave, lane};
-  tk.issue(0);
-  tv.issue(0);
+  tk.issue(keys.row(0));
+  tv.issue(keys.row(0));
   for (int t = 0; t < n_tiles; ++t) {
     wait_vm_lds<0>();  // this wave's pieces of the tile
     __syncthreads();   // every wave is done with the previous tile's planes
@@ -803,11 +862,13 @@ __device__ __forceinline__ void dq_f32_workgroup(const F32BwdArgs& a, int bh, in
     store_x3<D, TR>(tv, svp);
     __syncthreads();
     if (t + 1 < n_tiles) {
-      tk.issue((t + 1) * TR);
-      tv.issue((t + 1) * TR);
+      tk.issue(keys.row(t + 1));
+      tv.issue(keys.row(t + 1));
     }
-    const int key0 = t * TR + 32 * sub;
+    const int key0 = keys.row(t) + 32 * sub;
     if (key0 > q0 + 31) continue;  // wave-uniform: the whole chunk is in the future
+    if constexpr (WIN)
+      if (!chunk_visible(key0, q0, win)) continue;
     // lane (l32, h), register u: query qi, key key0 + reg_row(u, h)
     f32x16 s = score_tile_p<D, TR>(skp, 32 * sub, qb, lane);   // K Q^T
     f32x16 dp = score_tile_p<D, TR>(svp, 32 * sub, gb, lane);  // V dO^T
@@ -818,7 +879,13 @@ __device__ __forceinline__ void dq_f32_workgroup(const F32BwdArgs& a, int bh, in
     const bool diag = key0 == q0;
 #pragma unroll
     for (int u = 0; u < 16; ++u) s[u] = exp_acc(fmaf(s[u], scale, -my_lse));  // P
-    if (diag) {
+    if constexpr (WIN) {
+      if (!chunk_whole(key0, q0, win)) {
+        const HiddenKeys hidden(key0 + 8 * h, qi, win);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) s[u] = hidden(reg_row(u, 0)) ? 0.f : s[u];
+      }
+    } else if (diag) {
 #pragma unroll
       for (int u = 0; u < 16; ++u)
         if (key0 + reg_row(u, h) > qi) s[u] = 0.f;
@@ -877,6 +944,48 @@ __global__ __launch_bounds__(64 * kGroups, wgs_per_cu(1)) void dq_f32_kernel(con
   dq_f32_workgroup<D, DROP, 1, false>(a, blockIdx.x, gridDim.y - 1 - blockIdx.y, sm);
 }
 
+// The windowed backward: dK/dV workgroups (`blocks` key blocks, then the later pieces of the sink
+// blocks, piece by piece), then the dQ ones, with delta computed where it is needed (pieces and
+// windows up to kWindowDeltaRows rows) or by a pass before.
+constexpr int kWindowDeltaRows = 1024;
+template <int D, int KS, bool OWN_DELTA>
+__global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void window_bwd_f32_kernel(
+    const F32BwdArgs a, const F32WindowBwdArg<true> win, int blocks, int dkdv_blocks) {
+  __shared__ F32BwdShared<D, KS> sm;
+  __shared__ float own_delta[OWN_DELTA ? kWindowDeltaRows : 1];
+  const int y = blockIdx.y;
+  if (y < dkdv_blocks) {
+    int blk = y, piece = 0;
+    if (y >= blocks) {
+      const int sink_blocks = min(blocks, (win.sinks + kRows - 1) / kRows);
+      piece = (y - blocks) / sink_blocks + 1;
+      blk = (y - blocks) % sink_blocks;
+    }
+    dkdv_f32_workgroup<D, false, KS, OWN_DELTA, true>(a, blockIdx.x, blk, sm, own_delta, win,
+                                                      piece);
+  } else {
+    dq_f32_workgroup<D, false, KS, OWN_DELTA, true>(a, blockIdx.x, y - dkdv_blocks, sm, {win});
+  }
+}
+
+// The sink rows of dK and dV from their pieces' partials, summed in the pieces' order: a thread
+// for four columns.
+template <int D>
+__global__ __launch_bounds__(256) void window_join_f32_kernel(const F32BwdArgs a,
+                                                              const F32WindowBwdArgs win) {
+  const int i = blockIdx.y * 256 + threadIdx.x, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
+  const int which = i / (D / 4) / win.sinks, bh = blockIdx.x;
+  if (which > 1 || row >= a.S) return;
+  const int rows = (win.sinks + 31) / 32 * 32, left = a.S - row / kRows * kRows;
+  const int pieces = (left + win.piece_rows - 1) / win.piece_rows;  // of the row's block
+  if (pieces < 2) return;  // its workgroup has written the final row
+  const float* p = win.partial + ((size_t)bh * win.pieces * 2 + which) * rows * D +
+                   (size_t)row * D + col;
+  f32x4 sum = f32x4{};
+  for (int j = 0; j < pieces; ++j) sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * rows * D);
+  *reinterpret_cast<f32x4*>((which == 0 ? a.dk : a.dv) + ((size_t)bh * a.S + row) * D + col) = sum;
+}
+
 // Waves per row group. With one, a workgroup walks its chunks four waves wide, two workgroups
 // to a CU; a grid of no more workgroups than that (all of them start at once) lasts as long as
 // the longest one's chain, so each group then gets a second wave and the chain is half as long.
@@ -916,13 +1025,21 @@ void with_f32_shape(int waves_per_group, bool drop, F f) {
 
 template <int D>
 hipError_t fwd_f32_t(float* out, float* lse, const float* q, const float* k, const float* v,
-                     int BH, int S, float scale, hipStream_t stream, const Dropout* drop) {
+                     int BH, int S, float scale, hipStream_t stream, const Dropout* drop,
+                     const Window* window) {
   const dim3 grid(BH, (S + kRows - 1) / kRows);
   const DropParams dr = drop_params(drop);
+  if (window != nullptr) {
+    with_f32_shape(fwd_waves_per_group(BH, S), false, [&](auto, auto ks) {
+      fwd_f32_kernel<D, false, ks(), true, true>
+          <<<grid, 64 * kGroups * ks(), 0, stream>>>(out, lse, q, k, v, S, scale, dr, {*window});
+    });
+    return hipGetLastError();
+  }
   with_f32_shape(fwd_waves_per_group(BH, S), drop != nullptr, [&](auto drop_c, auto ks) {
     auto launch = [&](auto once) {
       fwd_f32_kernel<D, drop_c(), ks(), once()>
-          <<<grid, 64 * kGroups * ks(), 0, stream>>>(out, lse, q, k, v, S, scale, dr);
+          <<<grid, 64 * kGroups * ks(), 0, stream>>>(out, lse, q, k, v, S, scale, dr, {});
     };
     // At d_head 64 with one wave per group, up to two rounds of workgroups (two per CU), the last
     // of which run a wave per SIMD: a lone wave is faster if the conversions need not wait for
@@ -971,13 +1088,66 @@ hipError_t bwd_f32_t(float* dq, float* dk, float* dv, float* delta, const float*
   return e;
 }
 
+template <int D>
+hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, float* partial,
+                            hipStream_t stream) {
+  const int S = args.S, blocks = (S + kRows - 1) / kRows;
+  F32WindowBwdArg<true> win;
+  static_cast<Window&>(win) = w;
+  // pieces as long as a key block's window, and at least 512 rows
+  const long long span = ((long long)kRows + w.window + 63) / 64 * 64;
+  win.piece_rows = (int)(span > 512 ? span : 512);
+  win.pieces = w.sinks == 0 ? 1 : (S + win.piece_rows - 1) / win.piece_rows;
+  win.partial = partial;
+  const int of = (w.sinks + kRows - 1) / kRows, sink_blocks = of < blocks ? of : blocks;
+  const int dkdv_blocks = blocks + (win.pieces - 1) * sink_blocks;
+  const bool own = win.piece_rows <= kWindowDeltaRows;
+  hipError_t e = hipSuccess;
+  if (!own) {
+    const long long rows = (long long)BH * S, n = (rows * (D / 4) + 255) / 256;
+    delta_f32_kernel<D><<<(unsigned)(n < 16384 ? n : 16384), 256, 0, stream>>>(
+        args.delta, args.dout, args.out, rows);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  const dim3 grid(BH, dkdv_blocks + blocks);
+  with_f32_shape(bwd_waves_per_group(BH, S), false, [&](auto, auto ks) {
+    if (own)
+      window_bwd_f32_kernel<D, ks(), true>
+          <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, dkdv_blocks);
+    else
+      window_bwd_f32_kernel<D, ks(), false>
+          <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, dkdv_blocks);
+    e = hipGetLastError();
+  });
+  if (e != hipSuccess || win.pieces == 1) return e;
+  window_join_f32_kernel<D>
+      <<<dim3(BH, (w.sinks * (D / 4) * 2 + 255) / 256), 256, 0, stream>>>(args, win);
+  return hipGetLastError();
+}
+
 }  // namespace
+
+hipError_t launch_window_bwd_f32(float* dq, float* dk, float* dv, float* delta,
+                                 const float* dout, const float* out, const float* lse,
+                                 const float* q, const float* k, const float* v, int BH, int S,
+                                 int D, float scale, const Window& window, void* workspace,
+                                 hipStream_t stream) {
+  if (window.window >= S)
+    return launch_bwd_f32(dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S, D, scale, stream);
+  const F32BwdArgs args{dq, dk, dv, delta, q, k, v, dout, out, lse, S, scale, drop_params(nullptr)};
+  const Window w{window.window, window.sinks < S ? window.sinks : S};
+  float* partial = static_cast<float*>(workspace);
+  if (D == 64) return window_bwd_f32_t<64>(args, BH, w, partial, stream);
+  if (D == 32) return window_bwd_f32_t<32>(args, BH, w, partial, stream);
+  return hipErrorInvalidValue;
+}
 
 hipError_t launch_fwd_f32(float* out, float* lse, const float* q, const float* k,
                           const float* v, int BH, int S, int D, float scale,
-                          hipStream_t stream, const Dropout* drop) {
-  if (D == 64) return fwd_f32_t<64>(out, lse, q, k, v, BH, S, scale, stream, drop);
-  if (D == 32) return fwd_f32_t<32>(out, lse, q, k, v, BH, S, scale, stream, drop);
+                          hipStream_t stream, const Dropout* drop, const Window* window) {
+  if (window != nullptr && window->window >= S) window = nullptr;  // every earlier key is seen
+  if (D == 64) return fwd_f32_t<64>(out, lse, q, k, v, BH, S, scale, stream, drop, window);
+  if (D == 32) return fwd_f32_t<32>(out, lse, q, k, v, BH, S, scale, stream, drop, window);
   return hipErrorInvalidValue;
 }
 

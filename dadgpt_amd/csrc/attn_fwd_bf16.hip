@@ -41,6 +41,7 @@
 #include "dropout.hpp"
 #include "kernels.hpp"
 #include "tiles.hpp"
+#include "window.hpp"
 
 namespace dadgpt {
 namespace {
@@ -232,12 +233,16 @@ __device__ __forceinline__ void fwd_softmax_pv(f32x16 (&s)[NQB], f32x16 (&oacc)[
 }
 
 // FRESH: V's tile-edge correction computed at each issue (DmaTile::load_any).
-template <int D, bool STRIDED, bool DROP, int KS, bool FRESH = false>
+// WIN: sliding window and sinks (window.hpp): the tile list leaves out the tiles between the sinks
+// and the workgroup's first visible key, waves leave out chunks none of their queries sees, and
+// chunks that some of them see in part are masked by comparison. A query may see nothing of its
+// wave's first chunks; its maximum stays -inf until it does (finite_max).
+template <int D, bool STRIDED, bool DROP, int KS, bool FRESH = false, bool WIN = false>
 __global__ __launch_bounds__(64 * kWaves, kMinBlocks)
 __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_kernel(
     bf16* __restrict__ out, float* __restrict__ lse, const bf16* __restrict__ q,
     const bf16* __restrict__ k, const bf16* __restrict__ v, int S, float scale_log2,
-    int negate_q, int snake, const AttnLayout L, const DropParams dr) {
+    int negate_q, int snake, const AttnLayout L, const DropParams dr, const WindowArg<WIN> win) {
   // scale_log2 = |scale| * log2(e); a negative scale is applied by negating Q (exact in bf16),
   // so the row max of the raw scores is the row max of the scaled ones.
   constexpr int kGroups = kWaves / KS, QB = kQW * kGroups;  // query groups, queries
@@ -279,7 +284,8 @@ __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_
 
   const int q0 = qblk * QB + grp * kQW;
   const int wg_last = min(S, (qblk + 1) * QB) - 1;
-  const int n_tiles = wg_last / kTileRows + 1;
+  const KeyTiles<WIN> tiles(qblk * QB, wg_last, win);
+  const int n_tiles = tiles.count();
 
   // B operands of S^T: lane holds query q0 + 32i + l32, columns 16*ds + 8*hi + 0..7.
   // (rows past S read row S-1: finite scores for rows that are never stored)
@@ -301,7 +307,7 @@ __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_
     lrun[i] = 0.f;
   }
 
-  if (wave == 0) write_mask_table(smask, lane);  // published by the first barrier
+  if (!WIN && wave == 0) write_mask_table(smask, lane);  // published by the first barrier
 
   // The first tile loads alongside Q, under one wait; Q is touched only after it (the
   // compiler, which does not see the direct loads, then has nothing left to wait for).
@@ -309,8 +315,8 @@ __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_
   uint32_t koff[Dma::PER_WAVE], voff[Dma::PER_WAVE];
   Dma::offsets(koff, wave, lane, kp);
   Dma::offsets(voff, wave, lane, vp);
-  Dma::load_any(sk[0], kg, 0, S, koff, wave, lane, kp);
-  Dma::load_any(sv[0], vg, 0, S, voff, wave, lane, vp);
+  Dma::load_any(sk[0], kg, tiles.row(0), S, koff, wave, lane, kp);
+  Dma::load_any(sv[0], vg, tiles.row(0), S, voff, wave, lane, vp);
   wait_vm_lds<0>();
   __builtin_amdgcn_s_barrier();
 #pragma unroll
@@ -325,11 +331,12 @@ __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_
   // barrier), compute tile t from (ck, cv), then wait for tile t+1 and barrier, which also
   // ends every wave's reads of tile t.
   auto tile = [&](int t, const bf16* ck, const bf16* cv, bf16* nk, bf16* nv) {
-    const int k0 = t * kTileRows;
+    const int k0 = tiles.row(t);
     const bool prefetch = t + 1 < n_tiles;
     if (prefetch) {
-      Dma::load_any(nk, kg, k0 + kTileRows, S, koff, wave, lane, kp);
-      Dma::template load_any<FRESH>(nv, vg, k0 + kTileRows, S, voff, wave, lane, vp);
+      const int kn = WIN ? tiles.row(t + 1) : k0 + kTileRows;
+      Dma::load_any(nk, kg, kn, S, koff, wave, lane, kp);
+      Dma::template load_any<FRESH>(nv, vg, kn, S, voff, wave, lane, vp);
     }
     if (q0 < S && k0 <= q0 + kQW - 1) {  // some key of the tile at or before a query
       // One 32-key chunk at a time (holding both chunks' scores at once measured no faster
@@ -338,6 +345,8 @@ __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_
       for (int i = 0; i < 2 / KS; ++i) {
         const int kb = KS == 1 ? i : sub, c0 = k0 + 32 * kb;
         if (c0 > q0 + kQW - 1) break;  // every key of the chunk after every query
+        if constexpr (WIN)
+          if (!chunk_visible(c0, q0, win)) continue;
         bf16x8 ka[DS], va[DB][2];
         f32x16 sc[kNQB];
         KeepWords16 keep[kNQB] = {};
@@ -347,8 +356,15 @@ __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_
             keep[n] = keep_words16(dr, (uint64_t)bh * S + q0 + 32 * n + l32, c0, hi);
         }
         fwd_k_ops<D>(ka, ck, kb, lane);
-        // the chunk whose first key is the wave's first query is the one to mask
-        if (c0 == q0)
+        if constexpr (WIN) {
+          fwd_scores<D, kNQB>(sc, qop, ka, f32x16{});
+          if (!chunk_whole(c0, q0, win)) {
+            const HiddenKeys hidden(c0 + 8 * hi, q0 + l32, win);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              sc[0][r] = hidden(16 * (r >> 3) + (r & 7)) ? neg_inf() : sc[0][r];
+          }
+        } else if (c0 == q0)  // the chunk whose first key is the wave's first query: the masked one
           fwd_scores<D, kNQB>(sc, qop, ka, read_mask_table(smask, lane));
         else
           fwd_scores<D, kNQB>(sc, qop, ka, f32x16{});
@@ -407,7 +423,7 @@ __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_
 template <int D>
 hipError_t launch_fwd_bf16_t(bf16* out, float* lse, const bf16* q, const bf16* k, const bf16* v,
                              int BH, int S, float scale, const AttnLayout& L,
-                             const Dropout* drop, hipStream_t stream) {
+                             const Dropout* drop, const Window* window, hipStream_t stream) {
   const int cus = device_cus();
   // Masked scores are -inf and exponentiate as exp2(-inf * c - m), so c must be positive: a
   // zero scale (uniform attention) runs with c = 1e-30: every score below 1e22 in magnitude
@@ -424,8 +440,15 @@ hipError_t launch_fwd_bf16_t(bf16* out, float* lse, const bf16* q, const bf16* k
         cus > 0 && (long long)grid.x * grid.y <= (long long)cus * kMinBlocks ? cus : 0;
     auto run = [&](auto fresh) {
       fwd_bf16_kernel<D, strided(), dropped(), ks(), fresh()><<<grid, 64 * kWaves, 0, stream>>>(
-          out, lse, q, k, v, S, c, scale < 0.f, snake, L, dr);
+          out, lse, q, k, v, S, c, scale < 0.f, snake, L, dr, {});
     };
+    if constexpr (!dropped())
+      if (window != nullptr) {
+        fwd_bf16_kernel<D, strided(), false, ks(), false, true>
+            <<<grid, 64 * kWaves, 0, stream>>>(out, lse, q, k, v, S, c, scale < 0.f, snake, L, dr,
+                                               {*window});
+        return;
+      }
     // With K's and V's edge corrections held, the two-wave strided kernel takes 129 registers,
     // three workgroups per CU; where the grid has more, V's is computed at each issue (125, four):
     // 96 x 600 token-major 13.2 -> 11.4 us, 120 x 467 12.3 -> 10.5, 64 x 900 16.2 -> 13.8, 48 x
@@ -460,12 +483,13 @@ int device_cus() {
 
 hipError_t launch_fwd_bf16(bf16* out, float* lse, const bf16* q, const bf16* k, const bf16* v,
                            int BH, int S, int D, float scale, const AttnLayout& layout,
-                           hipStream_t stream, const Dropout* drop) {
+                           hipStream_t stream, const Dropout* drop, const Window* window) {
   if (drop != nullptr && drop->p == 0.f) drop = nullptr;  // the plain kernel's bits, undrawn
+  if (window != nullptr && window->window >= S) window = nullptr;  // every earlier key is seen
   if (D == 64)
-    return launch_fwd_bf16_t<64>(out, lse, q, k, v, BH, S, scale, layout, drop, stream);
+    return launch_fwd_bf16_t<64>(out, lse, q, k, v, BH, S, scale, layout, drop, window, stream);
   if (D == 32)
-    return launch_fwd_bf16_t<32>(out, lse, q, k, v, BH, S, scale, layout, drop, stream);
+    return launch_fwd_bf16_t<32>(out, lse, q, k, v, BH, S, scale, layout, drop, window, stream);
   return hipErrorInvalidValue;
 }
 

@@ -185,6 +185,54 @@ dadgpt_head_strides tokens(int64_t ld, int S, int d_head) {
   return dadgpt_head_strides{ld * S, d_head, ld};
 }
 
+// Window and sinks of a windowed call on sequences of S rows: the split of the sink keys' sums
+// makes up to pieces x sink blocks workgroups along grid.y, which the two limits keep below 2^16.
+int check_window(const char* fn, long long S, int window, int sinks) {
+  if (window < 1)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: window=%d must be at least 1", fn, window);
+  if (sinks < 0 || sinks > DADGPT_WINDOW_MAX_SINKS)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: sinks=%d must be in [0, %d]", fn, sinks,
+                DADGPT_WINDOW_MAX_SINKS);
+  if (S > DADGPT_WINDOW_MAX_SEQ)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: S=%lld exceeds %d", fn, S,
+                DADGPT_WINDOW_MAX_SEQ);
+  return DADGPT_OK;
+}
+
+int check_decode_window(const char* fn, int n_seq, int H, int max_len, int d_head, float scale,
+                        int window, int sinks, const void* ws, size_t ws_bytes,
+                        std::initializer_list<const void*> ptrs) {
+  if (int st = check_decode_shape(fn, n_seq, H, max_len, d_head, scale, ptrs)) return st;
+  if (int st = check_window(fn, 0, window, sinks)) return st;
+  const long long most = (long long)window + sinks;
+  return check_decode(fn, n_seq, H, most < max_len ? (int)most : max_len, d_head, scale, ws,
+                      ws_bytes, ptrs);
+}
+
+// The windowed backward's workspace, and that no gradient shares memory with an input or it: the
+// sink keys' pieces read K and V, and the join writes dK and dV, long after a workgroup has
+// written its own rows. `size` is a tensor's extent in bytes by its index in AttnTensor.
+int check_window_backward(const char* fn, int BH, int S, int d_head, const dadgpt::Window& w,
+                          const void* ws, size_t ws_bytes, const void* const (&tensor)[8],
+                          const size_t (&size)[8]) {
+  const size_t need = dadgpt::window_workspace_bytes(BH, S, d_head, w);
+  if (need > 0 && (ws == nullptr || ws_bytes < need))
+    return fail(DADGPT_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", fn,
+                ws == nullptr ? 0 : ws_bytes, need);
+  if (need > 0 && reinterpret_cast<uintptr_t>(ws) % 16 != 0)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: workspace is not 16-byte aligned", fn);
+  static const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv"};
+  for (int g = dadgpt::kTDQ; g <= dadgpt::kTDV; ++g) {
+    const dadgpt::Span grad{tensor[g], size[g]};
+    for (int t = dadgpt::kTQ; t <= dadgpt::kTDO; ++t)
+      if (dadgpt::overlap(grad, dadgpt::Span{tensor[t], size[t]}))
+        return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: %s overlaps %s", fn, names[g], names[t]);
+    if (need > 0 && dadgpt::overlap(grad, dadgpt::Span{ws, need}))
+      return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: %s overlaps the workspace", fn, names[g]);
+  }
+  return DADGPT_OK;
+}
+
 static_assert(DADGPT_DECODE_NOALLOC_SCRATCH_BYTES == dadgpt::kDecodeScratchBytes,
               "the header's scratch limit must be the kernels' own");
 
@@ -456,6 +504,185 @@ int dadgpt_decode_attention_bf16(uint16_t* out, const uint16_t* q, const uint16_
   return from_hip(dadgpt::launch_decode_bf16(B(out), B(q), B(k_cache), B(v_cache), lens, n_seq,
                                              n_heads, max_len, d_head, scale, workspace,
                                              workspace_bytes, as_stream(stream)),
+                  fn);
+}
+
+// ---- sliding window with sinks ----
+
+size_t dadgpt_flash_attention_window_workspace_bytes(int BH, int S, int d_head, int window,
+                                                     int sinks) {
+  if (BH < 1 || S < 1 || S > DADGPT_WINDOW_MAX_SEQ || !supported(d_head) || window < 1 ||
+      sinks < 0 || sinks > DADGPT_WINDOW_MAX_SINKS)
+    return 0;
+  return dadgpt::window_workspace_bytes(BH, S, d_head, {window, sinks});
+}
+
+int dadgpt_flash_attention_window_forward(float* out, float* lse, const float* q, const float* k,
+                                          const float* v, int BH, int S, int d_head, float scale,
+                                          int window, int sinks, void* stream) {
+  const char* fn = "dadgpt_flash_attention_window_forward";
+  if (int st = check_attn(fn, BH, S, d_head, scale, {out, lse, q, k, v})) return st;
+  if (int st = check_window(fn, S, window, sinks)) return st;
+  const dadgpt::Window w{window, sinks};
+  return from_hip(dadgpt::launch_fwd_f32(out, lse, q, k, v, BH, S, d_head, scale,
+                                         as_stream(stream), nullptr, &w),
+                  fn);
+}
+
+int dadgpt_flash_attention_window_backward(float* dq, float* dk, float* dv, float* delta,
+                                           const float* dout, const float* out, const float* lse,
+                                           const float* q, const float* k, const float* v, int BH,
+                                           int S, int d_head, float scale, int window, int sinks,
+                                           void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "dadgpt_flash_attention_window_backward";
+  if (int st = check_attn(fn, BH, S, d_head, scale, {dq, dk, dv, delta, dout, out, lse, q, k, v}))
+    return st;
+  if (int st = check_window(fn, S, window, sinks)) return st;
+  const dadgpt::Window w{window, sinks};
+  const size_t n = sizeof(float) * BH * S * d_head;
+  if (int st = check_window_backward(fn, BH, S, d_head, w, workspace, workspace_bytes,
+                                     {q, k, v, out, dout, dq, dk, dv}, {n, n, n, n, n, n, n, n}))
+    return st;
+  return from_hip(dadgpt::launch_window_bwd_f32(dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S,
+                                                d_head, scale, w, workspace, as_stream(stream)),
+                  fn);
+}
+
+int dadgpt_flash_attention_window_forward_bf16(uint16_t* out, float* lse, const uint16_t* q,
+                                               const uint16_t* k, const uint16_t* v, int BH, int S,
+                                               int d_head, float scale, int window, int sinks,
+                                               void* stream) {
+  const char* fn = "dadgpt_flash_attention_window_forward_bf16";
+  if (int st = check_attn(fn, BH, S, d_head, scale, {out, lse, q, k, v})) return st;
+  if (int st = check_window(fn, S, window, sinks)) return st;
+  const dadgpt::Window w{window, sinks};
+  return from_hip(dadgpt::launch_fwd_bf16(B(out), lse, B(q), B(k), B(v), BH, S, d_head, scale,
+                                          dadgpt::contiguous_layout(S, d_head),
+                                          as_stream(stream), nullptr, &w),
+                  fn);
+}
+
+int dadgpt_flash_attention_window_backward_bf16(uint16_t* dq, uint16_t* dk, uint16_t* dv,
+                                                float* delta, const uint16_t* dout,
+                                                const uint16_t* out, const float* lse,
+                                                const uint16_t* q, const uint16_t* k,
+                                                const uint16_t* v, int BH, int S, int d_head,
+                                                float scale, int window, int sinks,
+                                                void* workspace, size_t workspace_bytes,
+                                                void* stream) {
+  const char* fn = "dadgpt_flash_attention_window_backward_bf16";
+  if (int st = check_attn(fn, BH, S, d_head, scale, {dq, dk, dv, delta, dout, out, lse, q, k, v}))
+    return st;
+  if (int st = check_window(fn, S, window, sinks)) return st;
+  const dadgpt::Window w{window, sinks};
+  const size_t n = sizeof(uint16_t) * BH * S * d_head;
+  if (int st = check_window_backward(fn, BH, S, d_head, w, workspace, workspace_bytes,
+                                     {q, k, v, out, dout, dq, dk, dv}, {n, n, n, n, n, n, n, n}))
+    return st;
+  return from_hip(dadgpt::launch_window_bwd_bf16(B(dq), B(dk), B(dv), delta, B(dout), B(out), lse,
+                                                 B(q), B(k), B(v), BH, S, d_head, scale,
+                                                 dadgpt::contiguous_layout(S, d_head), w,
+                                                 workspace, as_stream(stream)),
+                  fn);
+}
+
+int dadgpt_flash_attention_window_forward_bf16_strided(
+    uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int batch,
+    int H, int S, int d_head, float scale, int window, int sinks,
+    const dadgpt_head_strides* strides, void* stream) {
+  const char* fn = "dadgpt_flash_attention_window_forward_bf16_strided";
+  dadgpt::AttnLayout L;
+  if (int st = check_strides(fn, batch, H, S, d_head, strides, 4, &L)) return st;
+  if (int st = check_attn(fn, batch * H, S, d_head, scale, {out, lse, q, k, v})) return st;
+  if (int st = check_window(fn, S, window, sinks)) return st;
+  const dadgpt::Window w{window, sinks};
+  return from_hip(dadgpt::launch_fwd_bf16(B(out), lse, B(q), B(k), B(v), batch * H, S, d_head,
+                                          scale, L, as_stream(stream), nullptr, &w),
+                  fn);
+}
+
+int dadgpt_flash_attention_window_backward_bf16_strided(
+    uint16_t* dq, uint16_t* dk, uint16_t* dv, float* delta, const uint16_t* dout,
+    const uint16_t* out, const float* lse, const uint16_t* q, const uint16_t* k,
+    const uint16_t* v, int batch, int H, int S, int d_head, float scale, int window, int sinks,
+    const dadgpt_head_strides* strides, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "dadgpt_flash_attention_window_backward_bf16_strided";
+  dadgpt::AttnLayout L;
+  if (int st = check_strides(fn, batch, H, S, d_head, strides, 8, &L)) return st;
+  if (int st = check_attn(fn, batch * H, S, d_head, scale,
+                          {dq, dk, dv, delta, dout, out, lse, q, k, v}))
+    return st;
+  if (int st = check_window(fn, S, window, sinks)) return st;
+  const dadgpt::Window w{window, sinks};
+  size_t n[8];
+  for (int t = 0; t < 8; ++t)
+    n[t] = sizeof(uint16_t) * ((size_t)(batch - 1) * L.t[t].batch + (size_t)(H - 1) * L.t[t].head +
+                               (size_t)(S - 1) * L.t[t].row + d_head);
+  if (int st = check_window_backward(fn, batch * H, S, d_head, w, workspace, workspace_bytes,
+                                     {q, k, v, out, dout, dq, dk, dv}, n))
+    return st;
+  return from_hip(dadgpt::launch_window_bwd_bf16(B(dq), B(dk), B(dv), delta, B(dout), B(out), lse,
+                                                 B(q), B(k), B(v), batch * H, S, d_head, scale, L,
+                                                 w, workspace, as_stream(stream)),
+                  fn);
+}
+
+int dadgpt_flash_attention_window_forward_bf16_tokens(
+    uint16_t* out, int64_t ld_out, float* lse, const uint16_t* q, const uint16_t* k,
+    const uint16_t* v, int64_t ld_qkv, int batch, int H, int S, int d_head, float scale,
+    int window, int sinks, void* stream) {
+  const char* fn = "dadgpt_flash_attention_window_forward_bf16_tokens";
+  if (int st = check_ld(fn, H, d_head, {ld_qkv, ld_out})) return st;
+  const dadgpt_head_strides in = tokens(ld_qkv, S, d_head), o = tokens(ld_out, S, d_head);
+  const dadgpt_head_strides st[4] = {in, in, in, o};
+  return dadgpt_flash_attention_window_forward_bf16_strided(out, lse, q, k, v, batch, H, S, d_head,
+                                                            scale, window, sinks, st, stream);
+}
+
+int dadgpt_flash_attention_window_backward_bf16_tokens(
+    uint16_t* dq, uint16_t* dk, uint16_t* dv, int64_t ld_dqkv, float* delta, const uint16_t* dout,
+    const uint16_t* out, int64_t ld_out, const float* lse, const uint16_t* q, const uint16_t* k,
+    const uint16_t* v, int64_t ld_qkv, int batch, int H, int S, int d_head, float scale,
+    int window, int sinks, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "dadgpt_flash_attention_window_backward_bf16_tokens";
+  if (int st = check_ld(fn, H, d_head, {ld_qkv, ld_out, ld_dqkv})) return st;
+  const dadgpt_head_strides in = tokens(ld_qkv, S, d_head), o = tokens(ld_out, S, d_head),
+                            g = tokens(ld_dqkv, S, d_head);
+  const dadgpt_head_strides st[8] = {in, in, in, o, o, g, g, g};
+  return dadgpt_flash_attention_window_backward_bf16_strided(
+      dq, dk, dv, delta, dout, out, lse, q, k, v, batch, H, S, d_head, scale, window, sinks, st,
+      workspace, workspace_bytes, stream);
+}
+
+int dadgpt_decode_attention_window_bf16(uint16_t* out, const uint16_t* q, const uint16_t* k_cache,
+                                        const uint16_t* v_cache, const int32_t* lens, int n_seq,
+                                        int n_heads, int max_len, int d_head, float scale,
+                                        int window, int sinks, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  const char* fn = "dadgpt_decode_attention_window_bf16";
+  if (int st = check_decode_window(fn, n_seq, n_heads, max_len, d_head, scale, window, sinks,
+                                   workspace, workspace_bytes, {out, q, k_cache, v_cache, lens}))
+    return st;
+  const dadgpt::Window w{window, sinks};
+  return from_hip(dadgpt::launch_decode_bf16(B(out), B(q), B(k_cache), B(v_cache), lens, n_seq,
+                                             n_heads, max_len, d_head, scale, workspace,
+                                             workspace_bytes, as_stream(stream), &w),
+                  fn);
+}
+
+int dadgpt_decode_attention_window_f32(float* out, const float* q, const float* k_cache,
+                                       const float* v_cache, const int32_t* lens, int n_seq,
+                                       int n_heads, int max_len, int d_head, float scale,
+                                       int window, int sinks, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  const char* fn = "dadgpt_decode_attention_window_f32";
+  if (int st = check_decode_window(fn, n_seq, n_heads, max_len, d_head, scale, window, sinks,
+                                   workspace, workspace_bytes, {out, q, k_cache, v_cache, lens}))
+    return st;
+  const dadgpt::Window w{window, sinks};
+  return from_hip(dadgpt::launch_decode_f32(out, q, k_cache, v_cache, lens, n_seq, n_heads,
+                                            max_len, d_head, scale, workspace, workspace_bytes,
+                                            as_stream(stream), &w),
                   fn);
 }
 

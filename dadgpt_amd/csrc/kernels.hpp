@@ -76,6 +76,17 @@ struct Dropout {
   uint64_t seed;
 };
 
+// Sliding window of a call: query i sees key j iff j <= i and (j > i - window or j < sinks).
+// window >= 1, sinks >= 0. A window of S keys or more is plain causal attention, and runs as it.
+struct Window {
+  int window, sinks;
+};
+// A kernel's Window argument: nothing in the kernels without one.
+template <bool WIN>
+struct WindowArg {};
+template <>
+struct WindowArg<true> : Window {};
+
 // Compute units of the current device (cached per device; 0 if unknown).
 int device_cus();
 
@@ -116,7 +127,8 @@ inline int waves_per_group(int BH, int S, int D, bool drop) {
 // probabilities multiplying V are dropped (the logsumexp is that of the undropped scores).
 hipError_t launch_fwd_bf16(bf16* out, float* lse, const bf16* q, const bf16* k, const bf16* v,
                            int BH, int S, int D, float scale, const AttnLayout& layout,
-                           hipStream_t stream, const Dropout* drop = nullptr);
+                           hipStream_t stream, const Dropout* drop = nullptr,
+                           const Window* window = nullptr);
 
 // Causal flash backward, bf16 in/out. delta [BH,S] fp32 is written (scratch, as the
 // reference's). dq/dk/dv are overwritten. `phases` selects the kernels launched, in order:
@@ -130,10 +142,27 @@ hipError_t launch_bwd_bf16(bf16* dq, bf16* dk, bf16* dv, float* delta, const bf1
                            const AttnLayout& layout, hipStream_t stream, int phases = kBwdAll,
                            const Dropout* drop = nullptr);
 
+// The windowed backward (window < S). A sink key is seen by every later query, so its dK and dV
+// are sums over the whole sequence where another key's run over `window` rows: they are split
+// over query ranges, whose fp32 partials pass through `workspace` (window_workspace_bytes, 0
+// where one range holds the sequence) and are joined in a fixed order by a last small kernel.
+// No gradient shares memory with an input.
+size_t window_workspace_bytes(int BH, int S, int D, const Window& window);
+hipError_t launch_window_bwd_bf16(bf16* dq, bf16* dk, bf16* dv, float* delta, const bf16* dout,
+                                  const bf16* out, const float* lse, const bf16* q, const bf16* k,
+                                  const bf16* v, int BH, int S, int D, float scale,
+                                  const AttnLayout& layout, const Window& window,
+                                  void* workspace, hipStream_t stream);
+hipError_t launch_window_bwd_f32(float* dq, float* dk, float* dv, float* delta,
+                                 const float* dout, const float* out, const float* lse,
+                                 const float* q, const float* k, const float* v, int BH, int S,
+                                 int D, float scale, const Window& window, void* workspace,
+                                 hipStream_t stream);
+
 // fp32 flash forward/backward (the reference's own precision), optionally with dropout.
 hipError_t launch_fwd_f32(float* out, float* lse, const float* q, const float* k,
                           const float* v, int BH, int S, int D, float scale, hipStream_t stream,
-                          const Dropout* drop = nullptr);
+                          const Dropout* drop = nullptr, const Window* window = nullptr);
 hipError_t launch_bwd_f32(float* dq, float* dk, float* dv, float* delta, const float* dout,
                           const float* out, const float* lse, const float* q, const float* k,
                           const float* v, int BH, int S, int D, float scale,
@@ -147,11 +176,13 @@ size_t decode_workspace_bytes(int n_seq, int H, int max_len, int D);
 hipError_t launch_decode_bf16(bf16* out, const bf16* q, const bf16* k_cache,
                               const bf16* v_cache, const int* lens, int n_seq, int H,
                               int max_len, int D, float scale, void* workspace,
-                              size_t workspace_bytes, hipStream_t stream);
+                              size_t workspace_bytes, hipStream_t stream,
+                              const Window* window = nullptr);
 hipError_t launch_decode_f32(float* out, const float* q, const float* k_cache,
                              const float* v_cache, const int* lens, int n_seq, int H,
                              int max_len, int D, float scale, void* workspace,
-                             size_t workspace_bytes, hipStream_t stream);
+                             size_t workspace_bytes, hipStream_t stream,
+                             const Window* window = nullptr);
 
 // Row kernels of the materialized attention path (materialized.hip), fp32 [rows, cols]:
 // the reference's softmax (out may be in), softmax backward (din += p (dout - rowsum(dout p))),

@@ -253,6 +253,81 @@ int dadgpt_decode_attention_f32(float* out, const float* q, const float* k_cache
                                 int n_heads, int max_len, int d_head, float scale,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Sliding-window attention with sinks (no reference counterpart: the reference attends to
+ * the whole context). Query i sees key j iff j <= i and (j > i - window or j < sinks): the last
+ * `window` keys, itself among them, and the first `sinks` of the sequence. window >= 1 and
+ * 0 <= sinks <= DADGPT_WINDOW_MAX_SINKS (checked), S <= DADGPT_WINDOW_MAX_SEQ. A window of S or
+ * more is the causal call and gives its bits. Arguments, layouts, alignment and the lse as in the
+ * calls without a window; work and time are in proportion to window + sinks, not to S.
+ *
+ * The backward takes a workspace of dadgpt_flash_attention_window_workspace_bytes() (0, and NULL
+ * allowed, for sinks = 0 or a sequence of about a window's length): a sink key's dK and dV are
+ * sums over all later queries, which are split and joined through it in a fixed order, so a call
+ * repeats bit for bit. The workspace needs no initial contents and holds nothing between calls;
+ * calls that overlap in time (two streams, two captured graphs replayed at once) need one each.
+ * No output of a windowed backward may overlap another output, an input or the workspace
+ * (gradients over an input are refused). */
+#define DADGPT_WINDOW_MAX_SINKS 1024
+#define DADGPT_WINDOW_MAX_SEQ (1 << 19)
+size_t dadgpt_flash_attention_window_workspace_bytes(int BH, int S, int d_head, int window,
+                                                     int sinks);
+int dadgpt_flash_attention_window_forward(float* out, float* lse, const float* q, const float* k,
+                                          const float* v, int BH, int S, int d_head, float scale,
+                                          int window, int sinks, void* stream);
+int dadgpt_flash_attention_window_backward(float* dq, float* dk, float* dv, float* delta,
+                                           const float* dout, const float* out, const float* lse,
+                                           const float* q, const float* k, const float* v, int BH,
+                                           int S, int d_head, float scale, int window, int sinks,
+                                           void* workspace, size_t workspace_bytes, void* stream);
+int dadgpt_flash_attention_window_forward_bf16(uint16_t* out, float* lse, const uint16_t* q,
+                                               const uint16_t* k, const uint16_t* v, int BH, int S,
+                                               int d_head, float scale, int window, int sinks,
+                                               void* stream);
+int dadgpt_flash_attention_window_backward_bf16(uint16_t* dq, uint16_t* dk, uint16_t* dv,
+                                                float* delta, const uint16_t* dout,
+                                                const uint16_t* out, const float* lse,
+                                                const uint16_t* q, const uint16_t* k,
+                                                const uint16_t* v, int BH, int S, int d_head,
+                                                float scale, int window, int sinks,
+                                                void* workspace, size_t workspace_bytes,
+                                                void* stream);
+/* The strided and token-major forms (strides and leading dimensions as above). dq, dk and dv may
+ * share one buffer as long as their rows do not overlap. */
+int dadgpt_flash_attention_window_forward_bf16_strided(
+    uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int B,
+    int H, int S, int d_head, float scale, int window, int sinks,
+    const dadgpt_head_strides* strides, void* stream);
+int dadgpt_flash_attention_window_backward_bf16_strided(
+    uint16_t* dq, uint16_t* dk, uint16_t* dv, float* delta, const uint16_t* dout,
+    const uint16_t* out, const float* lse, const uint16_t* q, const uint16_t* k,
+    const uint16_t* v, int B, int H, int S, int d_head, float scale, int window, int sinks,
+    const dadgpt_head_strides* strides, void* workspace, size_t workspace_bytes, void* stream);
+int dadgpt_flash_attention_window_forward_bf16_tokens(
+    uint16_t* out, int64_t ld_out, float* lse, const uint16_t* q, const uint16_t* k,
+    const uint16_t* v, int64_t ld_qkv, int B, int H, int S, int d_head, float scale, int window,
+    int sinks, void* stream);
+int dadgpt_flash_attention_window_backward_bf16_tokens(
+    uint16_t* dq, uint16_t* dk, uint16_t* dv, int64_t ld_dqkv, float* delta, const uint16_t* dout,
+    const uint16_t* out, int64_t ld_out, const float* lse, const uint16_t* q, const uint16_t* k,
+    const uint16_t* v, int64_t ld_qkv, int B, int H, int S, int d_head, float scale, int window,
+    int sinks, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The form for one token: the decode calls above under the mask of each cache's last row, at
+ * lens[s] - 1: its keys are rows [0, sinks) and [lens[s] - window, lens[s]). Other rows of the
+ * cache are not read. The workspace is the decode's (its contract, and the same buffer may serve
+ * both); it may be smaller by what window + sinks keys need:
+ * dadgpt_decode_workspace_bytes(n_seq, n_heads, min(max_len, window + sinks), d_head). */
+int dadgpt_decode_attention_window_bf16(uint16_t* out, const uint16_t* q, const uint16_t* k_cache,
+                                        const uint16_t* v_cache, const int32_t* lens, int n_seq,
+                                        int n_heads, int max_len, int d_head, float scale,
+                                        int window, int sinks, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+int dadgpt_decode_attention_window_f32(float* out, const float* q, const float* k_cache,
+                                       const float* v_cache, const int32_t* lens, int n_seq,
+                                       int n_heads, int max_len, int d_head, float scale,
+                                       int window, int sinks, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
 /* ---- Materialized attention (the reference's second attention path, src/model.cpp:395-420
  * forward and :575-616 backward, with the [BH, S, S] probabilities in memory). Its batched
  * GEMMs are in <dadgpt/gpu_matmul.h> (libdadgpt_gen.so), which also composes the whole path
