@@ -8,12 +8,15 @@
 #include <cstdarg>
 #include <cstdio>
 
+#include "capi_util.hpp"
 #include "dadgpt/gpu_attention.h"
 #include "kernels.hpp"
 
 namespace {
-
 thread_local char g_last_error[512] = "";
+}
+
+namespace dadgpt::capi {
 
 int fail(int status, const char* fmt, ...) {
   va_list ap;
@@ -51,6 +54,45 @@ int check_ptrs(const char* fn, std::initializer_list<const void*> ptrs) {
   return DADGPT_OK;
 }
 
+// Decode shape: grid (n_seq * H, chunks) of 512-lane workgroups, so n_seq * H * 512 < 2^32
+// work-items and at most 65535 chunks of the shortest chunk (256 keys, fp32 at d_head 64).
+int check_decode_shape(const char* fn, int n_seq, int H, int max_len, int d_head, float scale,
+                       std::initializer_list<const void*> ptrs) {
+  if (int st = check_ptrs(fn, ptrs)) return st;
+  if (n_seq < 1 || H < 1 || max_len < 1)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT,
+                "%s: n_seq=%d, n_heads=%d, max_len=%d must be positive", fn, n_seq, H, max_len);
+  if ((long long)n_seq * H >= (1LL << 23) || max_len > 65535L * 256)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT,
+                "%s: n_seq=%d x n_heads=%d or max_len=%d exceeds the launch limits", fn, n_seq,
+                H, max_len);
+  if (!supported(d_head))
+    return fail(DADGPT_ERR_UNSUPPORTED, "decode attention: unsupported d_head %d", d_head);
+  if (!std::isfinite(scale))
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: scale must be finite", fn);
+  return DADGPT_OK;
+}
+
+// Window and sinks of a windowed call on sequences of S rows: the split of the sink keys' sums
+// makes up to pieces x sink blocks workgroups along grid.y, which the two limits keep below 2^16.
+int check_window(const char* fn, long long S, int window, int sinks) {
+  if (window < 1)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: window=%d must be at least 1", fn, window);
+  if (sinks < 0 || sinks > DADGPT_WINDOW_MAX_SINKS)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: sinks=%d must be in [0, %d]", fn, sinks,
+                DADGPT_WINDOW_MAX_SINKS);
+  if (S > DADGPT_WINDOW_MAX_SEQ)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: S=%lld exceeds %d", fn, S,
+                DADGPT_WINDOW_MAX_SEQ);
+  return DADGPT_OK;
+}
+
+}  // namespace dadgpt::capi
+
+namespace {
+
+using namespace dadgpt::capi;
+
 // Launch limits. Row and stride arithmetic in the kernels is 32-bit (row counts up to 2^24);
 // every attention grid is (BH, ceil(S / tile)) with tiles of at least 64 rows and
 // grid.y <= 65535; a dispatch counts its work-items along x in 32 bits (BH workgroups of at
@@ -69,25 +111,6 @@ int check_attn(const char* fn, int BH, int S, int d_head, float scale,
     return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: BH=%d x S=%d too large", fn, BH, S);
   if (!supported(d_head))
     return fail(DADGPT_ERR_UNSUPPORTED, "flash attention: unsupported d_head %d", d_head);
-  if (!std::isfinite(scale))
-    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: scale must be finite", fn);
-  return DADGPT_OK;
-}
-
-// Decode shape: grid (n_seq * H, chunks) of 512-lane workgroups, so n_seq * H * 512 < 2^32
-// work-items and at most 65535 chunks of the shortest chunk (256 keys, fp32 at d_head 64).
-int check_decode_shape(const char* fn, int n_seq, int H, int max_len, int d_head, float scale,
-                       std::initializer_list<const void*> ptrs) {
-  if (int st = check_ptrs(fn, ptrs)) return st;
-  if (n_seq < 1 || H < 1 || max_len < 1)
-    return fail(DADGPT_ERR_INVALID_ARGUMENT,
-                "%s: n_seq=%d, n_heads=%d, max_len=%d must be positive", fn, n_seq, H, max_len);
-  if ((long long)n_seq * H >= (1LL << 23) || max_len > 65535L * 256)
-    return fail(DADGPT_ERR_INVALID_ARGUMENT,
-                "%s: n_seq=%d x n_heads=%d or max_len=%d exceeds the launch limits", fn, n_seq,
-                H, max_len);
-  if (!supported(d_head))
-    return fail(DADGPT_ERR_UNSUPPORTED, "decode attention: unsupported d_head %d", d_head);
   if (!std::isfinite(scale))
     return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: scale must be finite", fn);
   return DADGPT_OK;
@@ -132,8 +155,6 @@ int check_blocks(const char* fn, int n_blocks, int S, const void* p) {
                 n_blocks, S);
   return check_rows(fn, (long long)n_blocks * S, S, {p});
 }
-
-hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
 
 int check_dropout(const char* fn, float p) {
   if (!(p >= 0.0f && p < 1.0f))
@@ -185,28 +206,13 @@ dadgpt_head_strides tokens(int64_t ld, int S, int d_head) {
   return dadgpt_head_strides{ld * S, d_head, ld};
 }
 
-// Window and sinks of a windowed call on sequences of S rows: the split of the sink keys' sums
-// makes up to pieces x sink blocks workgroups along grid.y, which the two limits keep below 2^16.
-int check_window(const char* fn, long long S, int window, int sinks) {
-  if (window < 1)
-    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: window=%d must be at least 1", fn, window);
-  if (sinks < 0 || sinks > DADGPT_WINDOW_MAX_SINKS)
-    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: sinks=%d must be in [0, %d]", fn, sinks,
-                DADGPT_WINDOW_MAX_SINKS);
-  if (S > DADGPT_WINDOW_MAX_SEQ)
-    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: S=%lld exceeds %d", fn, S,
-                DADGPT_WINDOW_MAX_SEQ);
-  return DADGPT_OK;
-}
-
 int check_decode_window(const char* fn, int n_seq, int H, int max_len, int d_head, float scale,
                         int window, int sinks, const void* ws, size_t ws_bytes,
                         std::initializer_list<const void*> ptrs) {
   if (int st = check_decode_shape(fn, n_seq, H, max_len, d_head, scale, ptrs)) return st;
   if (int st = check_window(fn, 0, window, sinks)) return st;
-  const long long most = (long long)window + sinks;
-  return check_decode(fn, n_seq, H, most < max_len ? (int)most : max_len, d_head, scale, ws,
-                      ws_bytes, ptrs);
+  return check_decode(fn, n_seq, H, dadgpt::visible_keys(max_len, {window, sinks}), d_head, scale,
+                      ws, ws_bytes, ptrs);
 }
 
 // The windowed backward's workspace, and that no gradient shares memory with an input or it: the

@@ -102,12 +102,6 @@ struct VisibleKeys {
   }
   __device__ __forceinline__ int row(int i) const { return WIN && i >= sinks ? i + gap : i; }
 };
-// Keys seen of a full cache.
-inline int visible_keys(int max_len, const Window& w) {
-  const long long most = (long long)w.window + w.sinks;
-  return most < max_len ? (int)most : max_len;
-}
-
 template <int D, int WAVES>
 struct MergeLds {
   float o[WAVES][D];

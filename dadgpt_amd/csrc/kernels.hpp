@@ -81,6 +81,12 @@ struct Dropout {
 struct Window {
   int window, sinks;
 };
+// Keys that the last row of a full cache sees.
+inline int visible_keys(int max_len, const Window& w) {
+  const long long most = (long long)w.window + w.sinks;
+  return most < max_len ? (int)most : max_len;
+}
+
 // A kernel's Window argument: nothing in the kernels without one.
 template <bool WIN>
 struct WindowArg {};
@@ -216,6 +222,59 @@ hipError_t launch_split_heads(float* out, const float* in, int B, int S, int H, 
                               hipStream_t stream);
 hipError_t launch_merge_heads(float* out, const float* in, int B, int S, int H, int dh,
                               hipStream_t stream);
+
+// Bounded KV caches (kv_cache.hip). Where the rows of new keys or values lie: row t of head h of
+// sequence s starts at element s * batch + h * head + t * row.
+struct HeadStrides64 {
+  long long batch, head, row;
+};
+// Blocks of `block` tokens that `rows` new ones can touch.
+inline int kv8_touched_blocks(int rows, int block) {
+  return (int)(((long long)rows + block - 2) / block + 1);
+}
+// Appends rows lens[s] .. of every sequence (counts[s] of them, `rows` where counts is null; those
+// past max_len are dropped) to a cache of e4m3 codes [n_seq, H, max_len, D] with a power-of-two
+// scale per block of `block` tokens (16, 32, 64 or 128) and head.
+hipError_t launch_kv8_append_bf16(uint8_t* k8, uint8_t* v8, float* k_scale, float* v_scale,
+                                  const bf16* k, const bf16* v, const HeadStrides64& ks,
+                                  const HeadStrides64& vs, const int* lens, const int* counts,
+                                  int n_seq, int H, int rows, int max_len, int D, int block,
+                                  hipStream_t stream);
+hipError_t launch_kv8_append_f32(uint8_t* k8, uint8_t* v8, float* k_scale, float* v_scale,
+                                 const float* k, const float* v, const HeadStrides64& ks,
+                                 const HeadStrides64& vs, const int* lens, const int* counts,
+                                 int n_seq, int H, int rows, int max_len, int D, int block,
+                                 hipStream_t stream);
+// Decode over such a cache, whole or (window != null) windowed; workspace as decode's.
+size_t kv8_decode_workspace_bytes(int n_seq, int H, int max_len, int D);
+hipError_t launch_kv8_decode_bf16(bf16* out, const bf16* q, const uint8_t* k8, const uint8_t* v8,
+                                  const float* k_scale, const float* v_scale, const int* lens,
+                                  int n_seq, int H, int max_len, int D, int block, float scale,
+                                  const Window* window, void* workspace, size_t workspace_bytes,
+                                  hipStream_t stream);
+hipError_t launch_kv8_decode_f32(float* out, const float* q, const uint8_t* k8, const uint8_t* v8,
+                                 const float* k_scale, const float* v_scale, const int* lens,
+                                 int n_seq, int H, int max_len, int D, int block, float scale,
+                                 const Window* window, void* workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
+// Decode that also writes wout = win + p for every key's probability p (win itself from the
+// length on; [n_seq, H, max_len] fp32, wout may be win). The workspace needs no initial contents.
+size_t weights_decode_workspace_bytes(int n_seq, int H, int max_len, int D);
+hipError_t launch_weights_decode_bf16(bf16* out, float* wout, const bf16* q, const bf16* kc,
+                                      const bf16* vc, const float* win, const int* lens, int n_seq,
+                                      int H, int max_len, int D, float scale, void* workspace,
+                                      hipStream_t stream);
+hipError_t launch_weights_decode_f32(float* out, float* wout, const float* q, const float* kc,
+                                     const float* vc, const float* win, const int* lens, int n_seq,
+                                     int H, int max_len, int D, float scale, void* workspace,
+                                     hipStream_t stream);
+// Keeps `budget` rows of every (sequence, head): the first sinks, the last recent, and those of the
+// largest weights between. Rows are row_bytes wide (64, 128 or 256); k_out and v_out are k and v
+// (max_out = max_len), or neither.
+hipError_t launch_kv_evict(void* k_out, void* v_out, float* wout, int* kept, int* lens_out,
+                           const void* k, const void* v, const float* weights, const int* lens,
+                           int n_seq, int H, int max_len, int max_out, int row_bytes, int budget,
+                           int sinks, int recent, hipStream_t stream);
 
 // Device scratch that stands in for the decode workspace in the allocation-free entry point:
 // kDecodeScratchBytes per device, held until the process ends. decode_scratch returns the

@@ -17,6 +17,8 @@ constexpr int kQuadXor1 = 0xB1;    // quad_perm [1, 0, 3, 2]
 constexpr int kQuadXor2 = 0x4E;    // quad_perm [2, 3, 0, 1]
 constexpr int kHalfMirror = 0x141;
 constexpr int kMirror = 0x140;
+constexpr int kRor2 = 0x122;      // row_ror:n rotates each row by n
+constexpr int kRor4 = 0x124;
 constexpr int kRor8 = 0x128;
 
 template <int CTRL>
