@@ -251,11 +251,24 @@ struct BwdArgs {
   AttnLayout L;
   DropParams dr;
 };
-// The windowed backward's arguments: query tiles of a piece of a sink block (piece_tiles), and
-// the fp32 partials of the sink rows, [BH][piece][dK, dV][sink rows, whole 32s][D].
+// The windowed backward's arguments. A dK/dV workgroup walks the query tiles of its key block's
+// window (block_end); a sink key's later queries are `pieces` pieces at most of piece_tiles tiles,
+// whose sums lie in `partial`, fp32 [BH][piece][dK, dV][sink rows, whole 32s][D]. Without pieces
+// (piece_tiles 0) a block with sink keys walks them too.
 struct WindowBwdArgs : Window {
-  int piece_tiles, pieces;
+  int block_keys, piece_tiles, pieces;
   float* partial;
+  __device__ __forceinline__ int block_end(int kblk, int S) const {
+    const int last = (S - 1) / kTileRows;
+    if (piece_tiles == 0 && kblk * block_keys < sinks) return last + 1;
+    return min(last, ((kblk + 1) * block_keys + window - 2) / kTileRows) + 1;
+  }
+  // the partials of sink keys 32 * group .. of one piece: dK, and dV sink_rows() * D further on
+  __device__ __forceinline__ int sink_rows() const { return (sinks + 31) / 32 * 32; }
+  template <int D>
+  __device__ __forceinline__ float* partials(int bh, int piece, int group) const {
+    return partial + (((size_t)bh * pieces + piece) * 2 * sink_rows() + 32 * group) * D;
+  }
 };
 template <bool WIN>
 struct WindowBwdArg {};
@@ -305,10 +318,12 @@ __device__ __forceinline__ void delta_rows(float* delta, const Slice<D, STRIDED>
 }
 
 // A wave's 32 x D fp32 accumulators (accumulator layout, as store_rows_staged) as rows of a
-// partial.
+// partial, of the lanes that `mine`.
 template <int D>
-__device__ __forceinline__ void store_partial(float* dst, const f32x16 (&acc)[D / 32], int lane) {
+__device__ __forceinline__ void store_partial(float* dst, const f32x16 (&acc)[D / 32], bool mine,
+                                              int lane) {
   const int l32 = lane & 31, hi = lane >> 5;
+  if (!mine) return;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -317,17 +332,34 @@ __device__ __forceinline__ void store_partial(float* dst, const f32x16 (&acc)[D 
           f32x4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
 }
 
+// Adds the pieces' partials (dst of store_partial, `stride` floats apart) to the accumulators, in
+// their order, for the lanes that `mine`.
+template <int D>
+__device__ __forceinline__ void add_partials(f32x16 (&acc)[D / 32], const float* p, size_t stride,
+                                             int pieces, bool mine, int lane) {
+  const int l32 = lane & 31, hi = lane >> 5;
+  if (!mine) return;
+  p += l32 * D + 4 * hi;
+  for (int j = 0; j < pieces; ++j, p += stride)
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p + 32 * db + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[db][4 * g + e] += x[e];
+      }
+}
+
 // One workgroup's dK and dV. OWN_DELTA: delta is computed here, into own_delta (one float for
 // each row from the first tile on); otherwise it is read from a.delta.
-// WIN: the queries of a key block end with its last key's window; a block with sink keys instead
-// has every later query, in pieces of win.piece_tiles tiles. The first piece is at least as long
-// as a block's window, so later ones have the sink keys alone: they leave them as partials, and
-// the first piece leaves its sink keys' partial next to the block's final rows.
+// WIN: the queries of a key block end with its last key's window; what later queries add to sink
+// keys is in the partials that an earlier launch left (sink_workgroup).
 template <int D, bool STRIDED, bool DROP, int KS, bool OWN_DELTA, bool WIN = false>
 __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kblk,
                                                BwdTiles<D>& tiles, BwdStats& stats,
                                                float* own_delta,
-                                               const WindowBwdArg<WIN>& win = {}, int piece = 0) {
+                                               const WindowBwdArg<WIN>& win = {}) {
   constexpr int kGroups = kWaves / KS, KB = kKW * kGroups;  // key groups, keys
   constexpr int DS = D / 16, DB = D / 32;
   auto& sq = tiles.a;
@@ -351,19 +383,9 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
 
   const int kw0 = kblk * KB + grp * kKW;
   const int key = kw0 + l32;
-  int t_first = (kblk * KB) / kTileRows;
+  const int t_first = (kblk * KB) / kTileRows;
   int t_end = (S - 1) / kTileRows + 1;
-  bool split = false;  // the sink keys' sums go on in other pieces
-  if constexpr (WIN) {
-    if (kblk * KB < win.sinks) {
-      split = t_end - t_first > win.piece_tiles;
-      t_first += piece * win.piece_tiles;
-      if (t_first >= t_end) return;
-      t_end = min(t_end, t_first + win.piece_tiles);
-    } else {
-      t_end = min(t_end, (kblk * KB + KB + win.window - 2) / kTileRows + 1);
-    }
-  }
+  if constexpr (WIN) t_end = win.block_end(kblk, S);
 
   // B operands (K^T, V^T along D): lane holds key row `key`, columns 16*ds + 8*hi + 0..7.
   bf16x8 kop[DS], vop[DS];
@@ -410,6 +432,9 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
   // One query tile: prefetch tile t+1 (into the buffers of tile t-1, released by the last
   // barrier), convert this wave's statistics rows, compute tile t, wait for tile t+1 and
   // barrier.
+  // (with a window, the two blocks as a loop: one after the other in one scope, their conditions made
+  // the compiler keep 150 bytes a lane of the operands in scratch)
+  constexpr int kUnroll = WIN ? 1 : 2;
   auto tile = [&](int t, const bf16* cq, const bf16* cdo, int cb, bf16* nq, bf16* ndo,
                   int nb) {
     const int r0 = t * kTileRows;
@@ -420,7 +445,7 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
       st[cb][1][lane] = OWN_DELTA ? -own_delta[min(r0 + lane, S - 1) - t_first * kTileRows]
                                   : -st[cb][1][lane];
       const bool edge = r0 + kTileRows > S;
-#pragma unroll
+#pragma unroll kUnroll
       for (int i = 0; i < 2 / KS; ++i) {
         const int qb = KS == 1 ? i : sub, qlo = r0 + 32 * qb;  // first query of the block
         if (qlo + 31 < kw0) continue;   // every key of the wave is after every query
@@ -445,24 +470,23 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
     if (t + 1 < t_end) tile(t + 1, sq[1], sdo[1], 1, sq[0], sdo[0], 0);
   }
 
-  // (where the wave's partials of dK and dV go, if it has any)
-  float* part = nullptr;
-  int part_dv = 0;
-  if constexpr (WIN) {
-    if (split && kw0 < win.sinks) {
-      part_dv = (win.sinks + 31) / 32 * 32 * D;
-      part = win.partial + ((size_t)bh * win.pieces + piece) * 2 * part_dv + kw0 * D;
+  // (the sink keys' later queries)
+  auto add_far = [&](f32x16(&acc)[DB], int which) {
+    if constexpr (WIN) {
+      const int far = (S - 1) / kTileRows + 1 - t_end;  // tiles
+      if (far > 0 && kw0 < win.sinks) {
+        const size_t stride = (size_t)2 * win.sink_rows() * D;
+        add_partials<D>(acc, win.template partials<D>(bh, 0, kw0 / 32) + which * (stride / 2), stride,
+                        (far + win.piece_tiles - 1) / win.piece_tiles, key < win.sinks, lane);
+      }
     }
-  }
-  const bool rows_out = !WIN || piece == 0;
+  };
   // the tiles are free after the last barrier
   if constexpr (KS == 1) {
-    if (WIN && part != nullptr) {
-      store_partial<D>(part, dkacc, lane);
-      store_partial<D>(part + part_dv, dvacc, lane);
-    }
     // each wave stages its 32 rows in its quarter of sq (dK) and sdo (dV)
-    if (kw0 < S && rows_out) {
+    if (kw0 < S) {
+      add_far(dkacc, 0);
+      add_far(dvacc, 1);
       store_rows_staged<D>(sl.row(dk, kTDK, kw0), sl.pitch(kTDK), S - kw0, dkacc, a.scale,
                            &sq[0][0] + wave * kKW * D, lane);
       store_rows_staged<D>(sl.row(dv, kTDV, kw0), sl.pitch(kTDV), S - kw0, dvacc, 1.0f,
@@ -482,16 +506,14 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
     if (kw0 >= S) return;
     if (sub == 0) {
       add_acc(dkacc, slot_k, lane);
-      if (WIN && part != nullptr) store_partial<D>(part, dkacc, lane);
-      if (rows_out)
-        store_rows_staged<D>(sl.row(dk, kTDK, kw0), sl.pitch(kTDK), S - kw0, dkacc, a.scale,
-                             reinterpret_cast<bf16*>(slot_k), lane);
+      add_far(dkacc, 0);
+      store_rows_staged<D>(sl.row(dk, kTDK, kw0), sl.pitch(kTDK), S - kw0, dkacc, a.scale,
+                           reinterpret_cast<bf16*>(slot_k), lane);
     } else {
       add_acc(dvacc, slot_v, lane);
-      if (WIN && part != nullptr) store_partial<D>(part + part_dv, dvacc, lane);
-      if (rows_out)
-        store_rows_staged<D>(sl.row(dv, kTDV, kw0), sl.pitch(kTDV), S - kw0, dvacc, 1.0f,
-                             reinterpret_cast<bf16*>(slot_v), lane);
+      add_far(dvacc, 1);
+      store_rows_staged<D>(sl.row(dv, kTDV, kw0), sl.pitch(kTDV), S - kw0, dvacc, 1.0f,
+                           reinterpret_cast<bf16*>(slot_v), lane);
     }
   }
 }
@@ -746,73 +768,135 @@ __global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(DROP)) void bwd_bf16_k
 }
 
 // ---------------------------------------------------------------- sliding window
-// The windowed kernels' grids: dQ as above; dK/dV has `blocks` key blocks and then the later pieces
-// of the sink blocks, piece by piece.
-template <int D, bool STRIDED, int KS, bool OWN_DELTA>
-__device__ __forceinline__ void window_dkdv(const BwdArgs& a, const WindowBwdArg<true>& win,
-                                            int blocks, int y, BwdTiles<D>& tiles,
-                                            BwdStats& stats, float* own_delta) {
-  int kblk = y, piece = 0;
-  if (y >= blocks) {
-    constexpr int KB = kKW * kWaves / KS;
-    const int sink_blocks = min(blocks, (win.sinks + KB - 1) / KB);
-    piece = (y - blocks) / sink_blocks + 1;
-    kblk = (y - blocks) % sink_blocks;
+// A piece of the sum that 32 sink keys have over the queries past their block's window: all of
+// these queries see all of these keys. The four waves share the keys; a round takes two tiles, one
+// 32-query chunk a wave (in dK/dV's arrangement, each wave its own keys, three of four would have
+// none that is a sink), and the waves' sums are added at the end.
+template <int D, bool STRIDED>
+__device__ __forceinline__ void sink_workgroup(const BwdArgs& a, int bh, int group, int piece,
+                                               BwdTiles<D>& tiles, BwdStats& stats,
+                                               float* own_delta, const WindowBwdArgs& win) {
+  constexpr int DS = D / 16, DB = D / 32;
+  const int S = a.S, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hi = lane >> 5;
+  const int t0 = win.block_end(32 * group / win.block_keys, S) + piece * win.piece_tiles;
+  const int t1 = min((S - 1) / kTileRows + 1, t0 + win.piece_tiles);
+  if (t0 >= t1) return;  // (a later block's far queries start later: it has fewer pieces)
+  const Slice<D, STRIDED> sl(a.L, bh, S);
+  const bf16* qg = sl.base(a.q, kTQ);
+  const bf16* dog = sl.base(a.dout, kTDO);
+  const int qp = sl.pitch(kTQ), dop = sl.pitch(kTDO);
+  const int key = min(32 * group + l32, S - 1);
+  bf16x8 kop[DS], vop[DS];
+#pragma unroll
+  for (int ds = 0; ds < DS; ++ds) {
+    kop[ds] = ld_g128(sl.row(a.k, kTK, key) + 16 * ds + 8 * hi);
+    vop[ds] = ld_g128(sl.row(a.v, kTV, key) + 16 * ds + 8 * hi);
   }
-  dkdv_workgroup<D, STRIDED, false, KS, OWN_DELTA, true>(a, blockIdx.x, kblk, tiles, stats,
-                                                         own_delta, win, piece);
+  f32x16 dkacc[DB], dvacc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    dkacc[db] = f32x16{};
+    dvacc[db] = f32x16{};
+  }
+  const LaneLds lo = lane_lds<D>(lane);
+  using Dma = DmaTile<D, kWaves>;
+  uint32_t qoff[Dma::PER_WAVE], dooff[Dma::PER_WAVE];
+  Dma::offsets(qoff, wave, lane, qp);
+  Dma::offsets(dooff, wave, lane, dop);
+  const int at = wave >> 1, qb = wave & 1;  // the wave's tile and chunk of a round
+  float(*st)[kTileRows] = stats.row[wave][0];
+  delta_rows<D, STRIDED>(own_delta, sl, a.dout, a.out, t0 * kTileRows, min(S, t1 * kTileRows));
+  for (int t = t0; t < t1; t += 2) {
+    __syncthreads();  // the last round's reads are done (and, at first, own_delta is written)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (t + i < t1) {
+        Dma::template load_any<true>(tiles.a[i], qg, (t + i) * kTileRows, S, qoff, wave, lane, qp);
+        Dma::template load_any<true>(tiles.b[i], dog, (t + i) * kTileRows, S, dooff, wave, lane,
+                                     dop);
+      }
+    const int r0 = (t + at) * kTileRows;
+    const bool mine = t + at < t1 && r0 + 32 * qb < S;
+    if (mine) dma_row64(st[0], a.lse + (size_t)bh * S, r0, S, lane);
+    wait_vm_lds<0>();
+    __syncthreads();
+    if (!mine) continue;
+    st[0][lane] *= a.lse_mul;
+    st[1][lane] = -own_delta[min(r0 + lane, S - 1) - t0 * kTileRows];
+    dkdv_block<D, false, true>(r0 + kTileRows > S, dkacc, dvacc, kop, vop, tiles.a[at],
+                               tiles.b[at], st[0], st[1], qb, -1, S - r0, lane, a.c, 0, 0.f, lo);
+  }
+  // waves 2 and 3 to 0 and 1, then dK to wave 0 and dV to wave 1
+  AccLds* slot[2] = {reinterpret_cast<AccLds*>(&tiles.a[0][0]),
+                     reinterpret_cast<AccLds*>(&tiles.b[0][0])};
+  static_assert(sizeof(tiles.a) >= 2 * DB * sizeof(AccLds), "a wave's sums fit");
+  __syncthreads();
+  if (wave >= 2) {
+    put_acc(dkacc, slot[wave - 2], lane);
+    put_acc(dvacc, slot[wave - 2] + DB, lane);
+  }
+  __syncthreads();
+  if (wave < 2) {
+    add_acc(dkacc, slot[wave], lane);
+    add_acc(dvacc, slot[wave] + DB, lane);
+  }
+  __syncthreads();
+  if (wave == 1) put_acc(dkacc, slot[0], lane);
+  if (wave == 0) put_acc(dvacc, slot[1], lane);
+  __syncthreads();
+  float* dst = win.template partials<D>(bh, piece, group);
+  const bool mine = 32 * group + l32 < win.sinks;  // (what others hold is in their block's own sum)
+  if (wave == 0) {
+    add_acc(dkacc, slot[0], lane);
+    store_partial<D>(dst, dkacc, mine, lane);
+  } else if (wave == 1) {
+    add_acc(dvacc, slot[1], lane);
+    store_partial<D>(dst + win.sink_rows() * D, dvacc, mine, lane);
+  }
 }
+
+// dQ (which writes delta), the sink keys' pieces in front: they are short, and the dQ workgroups
+// fill in behind them.
+constexpr int kMaxPieceTiles = 16;
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, kDqMinBlocks) void window_dq_bf16_kernel(
-    const BwdArgs a, const WindowArg<true> win) {
+    const BwdArgs a, const WindowBwdArg<true> win, int sink_groups) {
   __shared__ BwdTiles<D> tiles;
+  __shared__ BwdStats stats;
+  __shared__ float own_delta[kMaxPieceTiles * kTileRows];
+  const int y = blockIdx.y, n = sink_groups * win.pieces;
+  if (y < n) {
+    const int piece = y / sink_groups;
+    sink_workgroup<D, STRIDED>(a, blockIdx.x, y - piece * sink_groups, piece, tiles, stats,
+                               own_delta, win);
+    return;
+  }
   constexpr bool kFromDelta = D == 64 || KS == 2;  // as dq_bf16_kernel
-  dq_workgroup<D, STRIDED, false, KS, true, kFromDelta, true>(a, blockIdx.x, blockIdx.y, tiles,
-                                                              win);
+  dq_workgroup<D, STRIDED, false, KS, true, kFromDelta, true>(a, blockIdx.x, y - n, tiles, {win});
 }
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(false)) void window_dkdv_bf16_kernel(
-    const BwdArgs a, const WindowBwdArg<true> win, int blocks) {
+    const BwdArgs a, const WindowBwdArg<true> win) {
   __shared__ BwdTiles<D> tiles;
   __shared__ BwdStats stats;
-  window_dkdv<D, STRIDED, KS, false>(a, win, blocks, blockIdx.y, tiles, stats, nullptr);
+  dkdv_workgroup<D, STRIDED, false, KS, false, true>(a, blockIdx.x, blockIdx.y, tiles, stats,
+                                                     nullptr, win);
 }
-// Both in one launch, delta where it is needed (at most kOwnDeltaMaxS rows a dK/dV workgroup): the
-// dK/dV workgroups first.
+// Both in one launch where there are no pieces, delta where it is needed (a block's window of at
+// most kOwnDeltaMaxS rows): the dK/dV workgroups first.
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(false)) void window_bwd_bf16_kernel(
-    const BwdArgs a, const WindowBwdArg<true> win, int blocks, int dkdv_blocks) {
+    const BwdArgs a, const WindowBwdArg<true> win) {
   __shared__ BwdTiles<D> tiles;
   __shared__ BwdStats stats;
   __shared__ float own_delta[kOwnDeltaMaxS];
-  const int y = blockIdx.y;
-  if (y < dkdv_blocks)
-    window_dkdv<D, STRIDED, KS, true>(a, win, blocks, y, tiles, stats, own_delta);
+  if (blockIdx.z == 0)
+    dkdv_workgroup<D, STRIDED, false, KS, true, true>(a, blockIdx.x, blockIdx.y, tiles, stats,
+                                                      own_delta, win);
   else
-    dq_workgroup<D, STRIDED, false, KS, true, true, true>(a, blockIdx.x, y - dkdv_blocks, tiles,
-                                                          {win});
-}
-
-// The sink rows of dK and dV from their pieces' partials, summed in the pieces' order: a thread
-// for four columns.
-template <int D>
-__global__ __launch_bounds__(256) void window_join_bf16_kernel(const BwdArgs a,
-                                                               const WindowBwdArgs win, int KB) {
-  const int i = blockIdx.y * 256 + threadIdx.x, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
-  const int which = i / (D / 4) / win.sinks, bh = blockIdx.x;
-  if (which > 1 || row >= a.S) return;
-  const int rows = (win.sinks + 31) / 32 * 32;
-  const int tiles = (a.S - 1) / kTileRows + 1 - row / KB * KB / kTileRows;  // of the row's block
-  const int pieces = (tiles + win.piece_tiles - 1) / win.piece_tiles;
-  if (pieces < 2) return;  // its workgroup has written the final row
-  const float* p = win.partial + ((size_t)bh * win.pieces * 2 + which) * rows * D +
-                   (size_t)row * D + col;
-  f32x4 sum = f32x4{};
-  for (int j = 0; j < pieces; ++j) sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * rows * D);
-  const Slice<D, true> sl(a.L, bh, a.S);
-  const float mul = which == 0 ? a.scale : 1.0f;
-  st_g64((which == 0 ? sl.row(a.dk, kTDK, row) : sl.row(a.dv, kTDV, row)) + col,
-         u32x2{pack_bf16x2(sum[0] * mul, sum[1] * mul), pack_bf16x2(sum[2] * mul, sum[3] * mul)});
+    dq_workgroup<D, STRIDED, false, KS, true, true, true>(a, blockIdx.x, blockIdx.y, tiles, {win});
 }
 
 // How a backward is launched: dQ, then dK/dV (kSeparate); both in one launch with delta
@@ -932,68 +1016,90 @@ hipError_t launch_bwd_bf16_t(bf16* dq, bf16* dk, bf16* dv, float* delta, const b
   return e;
 }
 
-// Query tiles of a piece of a sink block: a key block's window (of KB keys), so that the pieces
-// take as long as the other workgroups, and at least eight.
-int window_piece_tiles(const Window& w, int KB) {
-  const long long tiles = ((long long)KB + w.window - 2) / kTileRows + 1;
-  return (int)(tiles > 8 ? tiles : 8);
-}
-int window_pieces(int S, const Window& w, int KB) {
-  if (w.sinks == 0) return 1;
-  const int tiles = (S - 1) / kTileRows + 1, of = window_piece_tiles(w, KB);
-  return (tiles + of - 1) / of;
+// How a windowed backward is launched: in one launch or as dQ and then dK/dV, the waves of a row
+// group, the pieces of its sink keys' later queries (in query tiles) and the bytes of their
+// partials.
+struct WindowPlan {
+  bool one;
+  int waves_per_group, piece_tiles, pieces;
+  size_t workspace;
+};
+WindowPlan window_plan(int BH, int S, int D, const Window& w) {
+  WindowPlan p{};
+  const long long tiles = (S - 1) / kTileRows + 1;
+  auto end = [&](int block_keys) {  // of the first block, in tiles
+    return ((long long)block_keys + w.window - 2) / kTileRows + 1;
+  };
+  // One launch, as the plain backward, where a workgroup's rows are few enough for its own delta: a
+  // window's without sinks; with sinks, a sequence whose sink blocks need no pieces, as their
+  // later queries are few next to the window or in all (pieces in a launch of their own -> whole,
+  // us: 4 x 300, window 64 20.7 -> 17.5, 192 x 256, 64 33.1 -> 24.6, 96 x 1024, 512 90.6 -> 80.4;
+  // but 12 x 1024, 256 30.5 -> 34.9, 48 x 1024, 128 38.2 -> 53.2).
+  const long long end128 = end(128), far128 = tiles - end128;
+  const bool whole = w.sinks == 0 || far128 <= 6 || far128 <= end128;
+  const bool short_rows = w.window <= kOwnDeltaMaxS - 3 * kTileRows;
+  p.one = bwd_in_one_launch(BH, S, D, false) && whole &&
+          (S <= kOwnDeltaMaxS || (short_rows && w.sinks == 0));
+  p.waves_per_group = window_waves_per_group(BH, S, p.one ? 2 : 1);
+  const long long far = tiles - end(32 * kWaves / p.waves_per_group);
+  if (p.one || w.sinks == 0 || far <= 0) return p;
+  // of 8 tiles (four rounds; of four, B16 H12 T1024 with a window of 256 takes dQ 56 for 52 us), up
+  // to 16 where that still makes 64 pieces
+  const long long of = (far + 63) / 64;
+  p.piece_tiles = (int)(of < 8 ? 8 : of > kMaxPieceTiles ? kMaxPieceTiles : of);
+  p.pieces = (int)((far + p.piece_tiles - 1) / p.piece_tiles);
+  p.workspace = sizeof(float) * BH * (size_t)p.pieces * 2 * ((w.sinks + 31) / 32 * 32) * D;
+  return p;
 }
 
 template <int D>
 hipError_t launch_window_bwd_bf16_t(const BwdArgs& args, int BH, const Window& w, float* partial,
-                                    hipStream_t stream) {
-  const int S = args.S, ks = waves_per_group(BH, S, D, false);
-  const int KB = 32 * kWaves / ks, blocks = (S + KB - 1) / KB;
+                                    size_t workspace_bytes, hipStream_t stream) {
+  const int S = args.S;
+  const WindowPlan plan = window_plan(BH, S, D, w);
+  if (plan.workspace > workspace_bytes) return hipErrorInvalidValue;
   WindowBwdArg<true> win;
   static_cast<Window&>(win) = w;
-  win.piece_tiles = window_piece_tiles(w, KB);
-  win.pieces = window_pieces(S, w, KB);
+  win.block_keys = 32 * kWaves / plan.waves_per_group;
+  win.piece_tiles = plan.piece_tiles;
+  win.pieces = plan.pieces;
   win.partial = partial;
-  const int sink_blocks = (w.sinks + KB - 1) / KB < blocks ? (w.sinks + KB - 1) / KB : blocks;
-  const int dkdv_blocks = blocks + (win.pieces - 1) * sink_blocks;
-  const bool one = win.piece_tiles * kTileRows <= kOwnDeltaMaxS;
+  const int blocks = (S + win.block_keys - 1) / win.block_keys, sink_groups = (w.sinks + 31) / 32;
   hipError_t e = hipSuccess;
-  with_shape(ks, false, !is_contiguous(args.L, S, D), [&](auto strided, auto, auto kw) {
-    if (one) {
+  with_shape(plan.waves_per_group, false, !is_contiguous(args.L, S, D),
+             [&](auto strided, auto, auto kw) {
+    if (plan.one) {
       window_bwd_bf16_kernel<D, strided(), kw()>
-          <<<dim3(BH, dkdv_blocks + blocks), 64 * kWaves, 0, stream>>>(args, win, blocks,
-                                                                       dkdv_blocks);
+          <<<dim3(BH, blocks, 2), 64 * kWaves, 0, stream>>>(args, win);
       e = hipGetLastError();
       return;
     }
     window_dq_bf16_kernel<D, strided(), kw()>
-        <<<dim3(BH, blocks), 64 * kWaves, 0, stream>>>(args, {w});
+        <<<dim3(BH, sink_groups * win.pieces + blocks), 64 * kWaves, 0, stream>>>(args, win,
+                                                                                  sink_groups);
     if ((e = hipGetLastError()) != hipSuccess) return;
     window_dkdv_bf16_kernel<D, strided(), kw()>
-        <<<dim3(BH, dkdv_blocks), 64 * kWaves, 0, stream>>>(args, win, blocks);
+        <<<dim3(BH, blocks), 64 * kWaves, 0, stream>>>(args, win);
     e = hipGetLastError();
   });
-  if (e != hipSuccess || win.pieces == 1) return e;
-  window_join_bf16_kernel<D>
-      <<<dim3(BH, (w.sinks * (D / 4) * 2 + 255) / 256), 256, 0, stream>>>(args, win, KB);
-  return hipGetLastError();
+  return e;
 }
 
 }  // namespace
 
-// Of the two element types' and both wave counts' largest.
 size_t window_workspace_bytes(int BH, int S, int D, const Window& w) {
-  if (w.window >= S || w.sinks == 0) return 0;
-  const int pieces = window_pieces(S, w, 32 * kWaves / 2);
-  const size_t rows = (size_t)(w.sinks < S ? w.sinks + 31 : S + 31) / 32 * 32;
-  return pieces == 1 ? 0 : sizeof(float) * BH * pieces * 2 * rows * D;
+  if (w.window >= S) return 0;
+  const size_t bf16_bytes =
+      window_plan(BH, S, D, {w.window, w.sinks < S ? w.sinks : S}).workspace;
+  const size_t f32_bytes = window_f32_workspace_bytes(BH, S, D, w);
+  return bf16_bytes > f32_bytes ? bf16_bytes : f32_bytes;
 }
 
 hipError_t launch_window_bwd_bf16(bf16* dq, bf16* dk, bf16* dv, float* delta, const bf16* dout,
                                   const bf16* out, const float* lse, const bf16* q, const bf16* k,
                                   const bf16* v, int BH, int S, int D, float scale,
                                   const AttnLayout& layout, const Window& window,
-                                  void* workspace, hipStream_t stream) {
+                                  void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (window.window >= S)
     return launch_bwd_bf16(dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S, D, scale, layout,
                            stream);
@@ -1002,8 +1108,8 @@ hipError_t launch_window_bwd_bf16(bf16* dq, bf16* dk, bf16* dv, float* delta, co
                      out, lse, S,  scale, scale * kLog2e, se * kLog2e, -1.0f / se, layout, {}};
   const Window w{window.window, window.sinks < S ? window.sinks : S};
   float* partial = static_cast<float*>(workspace);
-  if (D == 64) return launch_window_bwd_bf16_t<64>(args, BH, w, partial, stream);
-  if (D == 32) return launch_window_bwd_bf16_t<32>(args, BH, w, partial, stream);
+  if (D == 64) return launch_window_bwd_bf16_t<64>(args, BH, w, partial, workspace_bytes, stream);
+  if (D == 32) return launch_window_bwd_bf16_t<32>(args, BH, w, partial, workspace_bytes, stream);
   return hipErrorInvalidValue;
 }
 

@@ -596,11 +596,21 @@ __device__ __forceinline__ void delta_rows(float* delta, const float* dout, cons
   }
 }
 
-// The windowed backward's arguments: rows of a piece of a sink block (a multiple of 64), and the
-// partials of the sink rows, [BH][piece][dK, dV][sink rows, whole 32s][D].
+// The windowed backward's arguments. A dK/dV workgroup walks the queries up to its key block's
+// window (block_end, in rows); a sink key's later queries are up to `pieces` pieces of piece_rows
+// rows, and the sums of all lie in `partial`, [BH][block's own, piece 1, ..][dK, dV][sink rows,
+// whole 32s][D]. Without pieces a block with sink keys walks all of them.
 struct F32WindowBwdArgs : Window {
   int piece_rows, pieces;
   float* partial;
+  __device__ __forceinline__ int block_end(int blk, int S) const {
+    if (pieces == 0 && blk * kRows < sinks) return S;
+    return min(S, ((blk + 1) * kRows + window - 2) / 64 * 64 + 64);
+  }
+  // pieces of a block's later queries
+  __device__ __forceinline__ int far_pieces(int blk, int S) const {
+    return (S - block_end(blk, S) + piece_rows - 1) / max(piece_rows, 1);
+  }
 };
 template <bool WIN>
 struct F32WindowBwdArg {};
@@ -608,9 +618,10 @@ template <>
 struct F32WindowBwdArg<true> : F32WindowBwdArgs {};
 
 // One workgroup's dK and dV. OWN_DELTA: delta is computed here, into own_delta (a float for each
-// row from the first tile on); otherwise it is read from a.delta. WIN: as in the bf16 kernel, the
-// queries of a key block end with its last key's window, and a block with sink keys has every
-// later query, in pieces; the first is at least as long as a block's window.
+// row from the first tile on); otherwise it is read from a.delta. WIN: the queries of a key block
+// end with its last key's window (piece 0), and what later ones add to a block's sink keys is other
+// workgroups' (piece 1, 2, ..): their sums and the block's own sink rows go to the partials, which
+// window_join_f32_kernel adds up.
 template <int D, bool DROP, int KS, bool OWN_DELTA, bool WIN = false>
 __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, int blk,
                                                    F32BwdShared<D, KS>& sm, float* own_delta,
@@ -638,17 +649,11 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
   const int kj = k0 + l32;                // this lane's key
   int t0 = (blk * kRows) / TR;  // first query tile with a query >= the first key
   int n_tiles = (S + TR - 1) / TR;
-  bool split = false;  // the sink keys' sums go on in other pieces
   if constexpr (WIN) {
-    if (blk * kRows < win.sinks) {
-      const int of = win.piece_rows / TR;
-      split = n_tiles - t0 > of;
-      t0 += piece * of;
-      if (t0 >= n_tiles) return;
-      n_tiles = min(n_tiles, t0 + of);
-    } else {
-      n_tiles = min(n_tiles, (blk * kRows + kRows + win.window - 2) / TR + 1);
-    }
+    const int end = win.block_end(blk, S);
+    if (piece > 0) t0 = (end + (piece - 1) * win.piece_rows) / TR;
+    n_tiles = (min(S, piece > 0 ? t0 * TR + win.piece_rows : end) + TR - 1) / TR;
+    if (t0 >= n_tiles) return;
   }
 
   // The lane's K and V rows (score-product B layout), split. At D = 64 V's lower planes go to LDS,
@@ -783,9 +788,9 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
     __builtin_amdgcn_wave_barrier();
   }
   if constexpr (WIN) {
-    if (split && k0 < win.sinks) {
+    if (k0 < win.sinks && win.block_end(blk, S) < S) {
       const int rows = (win.sinks + 31) / 32 * 32;
-      float* part = win.partial + ((size_t)bh * win.pieces + piece) * 2 * rows * D;
+      float* part = win.partial + ((size_t)bh * (win.pieces + 1) + piece) * 2 * rows * D;
       store_rows_t<D>(part, k0, rows, dka, 1.0f, slot, lane);
       store_rows_t<D>(part + rows * D, k0, rows, dva, 1.0f, slot, lane);
     }
@@ -944,45 +949,41 @@ __global__ __launch_bounds__(64 * kGroups, wgs_per_cu(1)) void dq_f32_kernel(con
   dq_f32_workgroup<D, DROP, 1, false>(a, blockIdx.x, gridDim.y - 1 - blockIdx.y, sm);
 }
 
-// The windowed backward: dK/dV workgroups (`blocks` key blocks, then the later pieces of the sink
-// blocks, piece by piece), then the dQ ones, with delta computed where it is needed (pieces and
-// windows up to kWindowDeltaRows rows) or by a pass before.
-constexpr int kWindowDeltaRows = 1024;
+// The windowed backward: the pieces of the sink blocks' later queries first (`far` workgroups, piece
+// by piece: they are short), then dK/dV (`blocks` key blocks), then dQ, with delta computed where
+// it is needed (block windows up to kWindowDeltaRows rows) or by a pass before.
+constexpr int kWindowDeltaRows = 1024, kPieceRows = 256;
 template <int D, int KS, bool OWN_DELTA>
 __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void window_bwd_f32_kernel(
-    const F32BwdArgs a, const F32WindowBwdArg<true> win, int blocks, int dkdv_blocks) {
+    const F32BwdArgs a, const F32WindowBwdArg<true> win, int blocks, int sink_blocks) {
   __shared__ F32BwdShared<D, KS> sm;
   __shared__ float own_delta[OWN_DELTA ? kWindowDeltaRows : 1];
-  const int y = blockIdx.y;
-  if (y < dkdv_blocks) {
-    int blk = y, piece = 0;
-    if (y >= blocks) {
-      const int sink_blocks = min(blocks, (win.sinks + kRows - 1) / kRows);
-      piece = (y - blocks) / sink_blocks + 1;
-      blk = (y - blocks) % sink_blocks;
-    }
+  const int y = blockIdx.y, far = win.pieces * sink_blocks;
+  if (y < far + blocks) {
+    const int piece = y < far ? y / sink_blocks + 1 : 0;
+    const int blk = y < far ? y - (piece - 1) * sink_blocks : y - far;
     dkdv_f32_workgroup<D, false, KS, OWN_DELTA, true>(a, blockIdx.x, blk, sm, own_delta, win,
                                                       piece);
   } else {
-    dq_f32_workgroup<D, false, KS, OWN_DELTA, true>(a, blockIdx.x, y - dkdv_blocks, sm, {win});
+    dq_f32_workgroup<D, false, KS, OWN_DELTA, true>(a, blockIdx.x, y - far - blocks, sm, {win});
   }
 }
 
-// The sink rows of dK and dV from their pieces' partials, summed in the pieces' order: a thread
-// for four columns.
+// The sink rows of dK and dV of blocks with pieces, from the partials, summed in their order: a
+// thread for four columns.
 template <int D>
 __global__ __launch_bounds__(256) void window_join_f32_kernel(const F32BwdArgs a,
                                                               const F32WindowBwdArgs win) {
   const int i = blockIdx.y * 256 + threadIdx.x, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
   const int which = i / (D / 4) / win.sinks, bh = blockIdx.x;
-  if (which > 1 || row >= a.S) return;
-  const int rows = (win.sinks + 31) / 32 * 32, left = a.S - row / kRows * kRows;
-  const int pieces = (left + win.piece_rows - 1) / win.piece_rows;  // of the row's block
-  if (pieces < 2) return;  // its workgroup has written the final row
-  const float* p = win.partial + ((size_t)bh * win.pieces * 2 + which) * rows * D +
+  if (which > 1) return;
+  const int rows = (win.sinks + 31) / 32 * 32, far = win.far_pieces(row / kRows, a.S);
+  if (far == 0) return;  // its workgroup has written the final row
+  const float* p = win.partial + ((size_t)bh * (win.pieces + 1) * 2 + which) * rows * D +
                    (size_t)row * D + col;
-  f32x4 sum = f32x4{};
-  for (int j = 0; j < pieces; ++j) sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * rows * D);
+  f32x4 sum = *reinterpret_cast<const f32x4*>(p);
+  for (int j = 1; j <= far; ++j)
+    sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * rows * D);
   *reinterpret_cast<f32x4*>((which == 0 ? a.dk : a.dv) + ((size_t)bh * a.S + row) * D + col) = sum;
 }
 
@@ -1088,20 +1089,37 @@ hipError_t bwd_f32_t(float* dq, float* dk, float* dv, float* delta, const float*
   return e;
 }
 
+// How a windowed backward is launched: the pieces of its sink keys' later queries, and the bytes
+// of their partials.
+struct F32WindowPlan {
+  int pieces;
+  size_t workspace;
+};
+F32WindowPlan window_f32_plan(int BH, int S, int D, const Window& w) {
+  const long long end = ((long long)kRows + w.window - 2) / 64 * 64 + 64;  // of block 0
+  F32WindowPlan p{0, 0};
+  if (w.sinks > 0 && S > end) p.pieces = (int)((S - end + kPieceRows - 1) / kPieceRows);
+  const size_t rows = (size_t)(w.sinks + 31) / 32 * 32;
+  if (p.pieces > 0) p.workspace = sizeof(float) * BH * (size_t)(p.pieces + 1) * 2 * rows * D;
+  return p;
+}
+
 template <int D>
 hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, float* partial,
-                            hipStream_t stream) {
+                            size_t workspace_bytes, hipStream_t stream) {
   const int S = args.S, blocks = (S + kRows - 1) / kRows;
+  const F32WindowPlan plan = window_f32_plan(BH, S, D, w);
+  if (plan.workspace > workspace_bytes) return hipErrorInvalidValue;
   F32WindowBwdArg<true> win;
   static_cast<Window&>(win) = w;
-  // pieces as long as a key block's window, and at least 512 rows
-  const long long span = ((long long)kRows + w.window + 63) / 64 * 64;
-  win.piece_rows = (int)(span > 512 ? span : 512);
-  win.pieces = w.sinks == 0 ? 1 : (S + win.piece_rows - 1) / win.piece_rows;
+  win.piece_rows = kPieceRows;
+  win.pieces = plan.pieces;
   win.partial = partial;
   const int of = (w.sinks + kRows - 1) / kRows, sink_blocks = of < blocks ? of : blocks;
-  const int dkdv_blocks = blocks + (win.pieces - 1) * sink_blocks;
-  const bool own = win.piece_rows <= kWindowDeltaRows;
+  // rows that a dK/dV workgroup may walk: all, or a block's window in whole 64s
+  const bool own =
+      S <= kWindowDeltaRows ||
+      (kRows + w.window + 64 <= kWindowDeltaRows && (w.sinks == 0 || plan.pieces > 0));
   hipError_t e = hipSuccess;
   if (!own) {
     const long long rows = (long long)BH * S, n = (rows * (D / 4) + 255) / 256;
@@ -1109,17 +1127,17 @@ hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, flo
         args.delta, args.dout, args.out, rows);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  const dim3 grid(BH, dkdv_blocks + blocks);
+  const dim3 grid(BH, plan.pieces * sink_blocks + 2 * blocks);
   with_f32_shape(bwd_waves_per_group(BH, S), false, [&](auto, auto ks) {
     if (own)
       window_bwd_f32_kernel<D, ks(), true>
-          <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, dkdv_blocks);
+          <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, sink_blocks);
     else
       window_bwd_f32_kernel<D, ks(), false>
-          <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, dkdv_blocks);
+          <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, sink_blocks);
     e = hipGetLastError();
   });
-  if (e != hipSuccess || win.pieces == 1) return e;
+  if (e != hipSuccess || plan.pieces == 0) return e;
   window_join_f32_kernel<D>
       <<<dim3(BH, (w.sinks * (D / 4) * 2 + 255) / 256), 256, 0, stream>>>(args, win);
   return hipGetLastError();
@@ -1127,18 +1145,22 @@ hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, flo
 
 }  // namespace
 
+size_t window_f32_workspace_bytes(int BH, int S, int D, const Window& w) {
+  return w.window >= S ? 0 : window_f32_plan(BH, S, D, {w.window, w.sinks < S ? w.sinks : S}).workspace;
+}
+
 hipError_t launch_window_bwd_f32(float* dq, float* dk, float* dv, float* delta,
                                  const float* dout, const float* out, const float* lse,
                                  const float* q, const float* k, const float* v, int BH, int S,
                                  int D, float scale, const Window& window, void* workspace,
-                                 hipStream_t stream) {
+                                 size_t workspace_bytes, hipStream_t stream) {
   if (window.window >= S)
     return launch_bwd_f32(dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S, D, scale, stream);
   const F32BwdArgs args{dq, dk, dv, delta, q, k, v, dout, out, lse, S, scale, drop_params(nullptr)};
   const Window w{window.window, window.sinks < S ? window.sinks : S};
   float* partial = static_cast<float*>(workspace);
-  if (D == 64) return window_bwd_f32_t<64>(args, BH, w, partial, stream);
-  if (D == 32) return window_bwd_f32_t<32>(args, BH, w, partial, stream);
+  if (D == 64) return window_bwd_f32_t<64>(args, BH, w, partial, workspace_bytes, stream);
+  if (D == 32) return window_bwd_f32_t<32>(args, BH, w, partial, workspace_bytes, stream);
   return hipErrorInvalidValue;
 }
 

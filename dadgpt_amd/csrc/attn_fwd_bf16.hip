@@ -435,9 +435,11 @@ hipError_t launch_fwd_bf16_t(bf16* out, float* lse, const bf16* q, const bf16* k
     const dim3 grid(BH, (S + QB - 1) / QB);
     // Snake order only for grids of at most kMinBlocks workgroups per CU (all resident at once,
     // the dispatcher dealing each CU the same number): measured 2% faster at B8 H12 T1024 (768
-    // workgroups, 3 per CU) and 6% slower at B16 (1,536).
-    const int snake =
-        cus > 0 && (long long)grid.x * grid.y <= (long long)cus * kMinBlocks ? cus : 0;
+    // workgroups, 3 per CU) and 6% slower at B16 (1,536). With a window all blocks are as long.
+    const int snake = cus > 0 && window == nullptr &&
+                              (long long)grid.x * grid.y <= (long long)cus * kMinBlocks
+                          ? cus
+                          : 0;
     auto run = [&](auto fresh) {
       fwd_bf16_kernel<D, strided(), dropped(), ks(), fresh()><<<grid, 64 * kWaves, 0, stream>>>(
           out, lse, q, k, v, S, c, scale < 0.f, snake, L, dr, {});

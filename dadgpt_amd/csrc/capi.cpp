@@ -550,7 +550,8 @@ int dadgpt_flash_attention_window_backward(float* dq, float* dk, float* dv, floa
                                      {q, k, v, out, dout, dq, dk, dv}, {n, n, n, n, n, n, n, n}))
     return st;
   return from_hip(dadgpt::launch_window_bwd_f32(dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S,
-                                                d_head, scale, w, workspace, as_stream(stream)),
+                                                d_head, scale, w, workspace, workspace_bytes,
+                                                as_stream(stream)),
                   fn);
 }
 
@@ -588,7 +589,7 @@ int dadgpt_flash_attention_window_backward_bf16(uint16_t* dq, uint16_t* dk, uint
   return from_hip(dadgpt::launch_window_bwd_bf16(B(dq), B(dk), B(dv), delta, B(dout), B(out), lse,
                                                  B(q), B(k), B(v), BH, S, d_head, scale,
                                                  dadgpt::contiguous_layout(S, d_head), w,
-                                                 workspace, as_stream(stream)),
+                                                 workspace, workspace_bytes, as_stream(stream)),
                   fn);
 }
 
@@ -629,7 +630,7 @@ int dadgpt_flash_attention_window_backward_bf16_strided(
     return st;
   return from_hip(dadgpt::launch_window_bwd_bf16(B(dq), B(dk), B(dv), delta, B(dout), B(out), lse,
                                                  B(q), B(k), B(v), batch * H, S, d_head, scale, L,
-                                                 w, workspace, as_stream(stream)),
+                                                 w, workspace, workspace_bytes, as_stream(stream)),
                   fn);
 }
 

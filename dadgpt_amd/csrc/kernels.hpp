@@ -128,6 +128,14 @@ inline int waves_per_group(int BH, int S, int D, bool drop) {
   return two ? 2 : 1;
 }
 
+// The same with a sliding window, where every workgroup's chain is about as long: two waves per
+// group while the grid (`kinds` kinds of 64-row workgroups) is resident at once.
+inline int window_waves_per_group(int BH, int S, int kinds) {
+  if (S <= 64) return 1;
+  const long long cus = device_cus(), wgs = (long long)BH * ((S + 63) / 64) * kinds;
+  return wgs <= (S <= 256 ? cus : 3 * cus) ? 2 : 1;
+}
+
 // Causal flash forward, bf16 in/out, fp32 logsumexp (natural log) [BH, S]. q, k, v, out as
 // `layout` places them (tensors kTQ, kTK, kTV, kTO), D in {32,64}. With `drop`, the
 // probabilities multiplying V are dropped (the logsumexp is that of the undropped scores).
@@ -151,19 +159,22 @@ hipError_t launch_bwd_bf16(bf16* dq, bf16* dk, bf16* dv, float* delta, const bf1
 // The windowed backward (window < S). A sink key is seen by every later query, so its dK and dV
 // are sums over the whole sequence where another key's run over `window` rows: they are split
 // over query ranges, whose fp32 partials pass through `workspace` (window_workspace_bytes, 0
-// where one range holds the sequence) and are joined in a fixed order by a last small kernel.
+// where one range holds the sequence) and are added in a fixed order.
 // No gradient shares memory with an input.
+// (The size is the larger of the two element types' plans, so that one serves both; a launch refuses
+// a workspace smaller than its own plan's.)
 size_t window_workspace_bytes(int BH, int S, int D, const Window& window);
+size_t window_f32_workspace_bytes(int BH, int S, int D, const Window& window);
 hipError_t launch_window_bwd_bf16(bf16* dq, bf16* dk, bf16* dv, float* delta, const bf16* dout,
                                   const bf16* out, const float* lse, const bf16* q, const bf16* k,
                                   const bf16* v, int BH, int S, int D, float scale,
                                   const AttnLayout& layout, const Window& window,
-                                  void* workspace, hipStream_t stream);
+                                  void* workspace, size_t workspace_bytes, hipStream_t stream);
 hipError_t launch_window_bwd_f32(float* dq, float* dk, float* dv, float* delta,
                                  const float* dout, const float* out, const float* lse,
                                  const float* q, const float* k, const float* v, int BH, int S,
                                  int D, float scale, const Window& window, void* workspace,
-                                 hipStream_t stream);
+                                 size_t workspace_bytes, hipStream_t stream);
 
 // fp32 flash forward/backward (the reference's own precision), optionally with dropout.
 hipError_t launch_fwd_f32(float* out, float* lse, const float* q, const float* k,

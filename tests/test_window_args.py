@@ -71,9 +71,9 @@ def test_window_backward_workspace(name):
     assert _bwd(name, S=2000, ws=FAKE + 20 * STEP, wsb=need - 1) == 4
     assert "needed" in A.last_error()
     assert _bwd(name, S=2000, ws=FAKE + 20 * STEP + 8, wsb=need) == 1
-    # none where every sum is whole: no sinks, or a sequence no longer than a piece or a window
+    # none where every sum is whole: no sinks, or no query past a sink block's window
     assert A.window_workspace_bytes(4, 2000, 64, 16, 0) == 0
-    assert A.window_workspace_bytes(4, 512, 64, 16, 2) == 0
+    assert A.window_workspace_bytes(4, 128, 64, 16, 2) == 0
     assert A.window_workspace_bytes(4, 2000, 64, 2000, 2) == 0
     # and for what the calls refuse
     for bad in ((0, 2000, 64, 16, 2), (4, 0, 64, 16, 2), (4, 2000, 48, 16, 2), (4, 2000, 64, 0, 2),
@@ -81,22 +81,24 @@ def test_window_backward_workspace(name):
         assert A.window_workspace_bytes(*bad) == 0
 
 
-def test_window_workspace_covers_every_plan():
-    """fp32 partials [BH][piece][2][sink rows in whole 32s][D] of pieces of at least eight 64-row
-    tiles, or as many as hold a window and a key block of 64 rows (the smaller of the two block
-    sizes has the more pieces)."""
-    for S in (513, 1024, 5000, 1 << 19):
-        for window in (1, 100, 500, 4000):
+def test_window_workspace_covers_both_types_plans():
+    """fp32 partials [BH][piece][2][sink rows in whole 32s][D]. The fp32 backward has pieces of 256
+    rows past a 128-key block's window and one for the block itself; the bf16 one pieces of 8 to 16
+    64-row tiles (fewer than the fp32 one's)."""
+    for S in (513, 530, 1024, 5000, 1 << 19):
+        for window in (1, 40, 100, 500, 4000):
             for sinks in (1, 32, 33, 700, 1024):
                 if window >= S:
                     continue
-                span = max(8, (64 + window - 2) // 64 + 1) * 64
-                pieces = (S + span - 1) // span
+                end = (128 + window - 2) // 64 * 64 + 64
+                pieces = max(0, (S - end + 255) // 256)
                 rows = (min(sinks, S) + 31) // 32 * 32
-                want = 0 if pieces == 1 else 4 * 3 * pieces * 2 * rows * 32
+                want = 4 * 3 * (pieces + 1) * 2 * rows * 32 if pieces else 0
                 assert A.window_workspace_bytes(3, S, 32, window, sinks) >= want
-                span32 = max(512, (128 + window + 63) // 64 * 64)  # the fp32 kernels' pieces
-                assert (S + span32 - 1) // span32 <= max(1, pieces)
+                end = (64 + window - 2) // 64 + 1  # the smaller key block of the bf16 kernels
+                tiles = max(0, (S + 63) // 64 - end)
+                of = min(16, max(8, (tiles + 63) // 64))
+                assert (tiles + of - 1) // of <= pieces + 1
 
 
 def test_window_strided_validation():
