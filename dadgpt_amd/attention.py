@@ -465,9 +465,17 @@ def decode_attention(out, q, k_cache, v_cache, lens, n_seq, n_heads, max_len, d_
 WINDOW_MAX_SINKS, WINDOW_MAX_SEQ = 1024, 1 << 19
 
 
+_devices = None
+
+
 def _same_device(tensors) -> None:
-    """Every tensor on the current device, whose stream the call runs on (plain tensors that are
-    not there would fault; None passes)."""
+    """Every tensor on the current device, whose stream the call runs on (None passes). Where the
+    process sees one device only, there is no other to be on."""
+    global _devices
+    if _devices is None:
+        _devices = torch.cuda.device_count()
+    if _devices == 1:
+        return
     device = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != device:
@@ -480,7 +488,7 @@ def _workspace(workspace):
         return None, 0
     if not workspace.is_cuda or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous device tensor")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.nbytes
 
 
 def window_workspace_bytes(BH: int, S: int, d_head: int, window: int, sinks: int) -> int:

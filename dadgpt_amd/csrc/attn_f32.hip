@@ -1008,6 +1008,14 @@ int bwd_waves_per_group(int BH, int S) {
   return wgs <= (S > 96 ? cus : cus / 4) ? 2 : 1;
 }
 
+// With a window every workgroup's chain is about as long, so two waves per group pay only while
+// the workgroups, one per CU then, all start at once. One -> two, us: forward 24 x 777 (168
+// workgroups) 20.7 -> 17.8, 12 x 2048 (192) 48 -> 35, 48 x 1024 (384) 35 -> 48; backward 12 x 1024
+// (228) 48 -> 39, 24 x 777 (336) 22.6 -> 25.4, 12 x 2048 (384) 80 -> 95.
+int window_f32_waves_per_group(int S, long long wgs) {
+  return S > 96 && wgs <= device_cus() ? 2 : 1;
+}
+
 // f(whether to drop, waves per row group) as compile-time constants.
 template <typename F>
 void with_f32_shape(int waves_per_group, bool drop, F f) {
@@ -1031,7 +1039,8 @@ hipError_t fwd_f32_t(float* out, float* lse, const float* q, const float* k, con
   const dim3 grid(BH, (S + kRows - 1) / kRows);
   const DropParams dr = drop_params(drop);
   if (window != nullptr) {
-    with_f32_shape(fwd_waves_per_group(BH, S), false, [&](auto, auto ks) {
+    with_f32_shape(window_f32_waves_per_group(S, (long long)grid.x * grid.y), false,
+                   [&](auto, auto ks) {
       fwd_f32_kernel<D, false, ks(), true, true>
           <<<grid, 64 * kGroups * ks(), 0, stream>>>(out, lse, q, k, v, S, scale, dr, {*window});
     });
@@ -1090,15 +1099,18 @@ hipError_t bwd_f32_t(float* dq, float* dk, float* dv, float* delta, const float*
 }
 
 // How a windowed backward is launched: the pieces of its sink keys' later queries, and the bytes
-// of their partials.
+// of their partials. No pieces where the later queries are few next to the window or in all
+// (short sequences: pieces and their join cost more than the sink blocks' longer chain).
 struct F32WindowPlan {
   int pieces;
   size_t workspace;
 };
 F32WindowPlan window_f32_plan(int BH, int S, int D, const Window& w) {
   const long long end = ((long long)kRows + w.window - 2) / 64 * 64 + 64;  // of block 0
+  const long long far = S - end;
   F32WindowPlan p{0, 0};
-  if (w.sinks > 0 && S > end) p.pieces = (int)((S - end + kPieceRows - 1) / kPieceRows);
+  if (w.sinks > 0 && far > 0 && (far > end || S > kWindowDeltaRows) && far > 384)
+    p.pieces = (int)((far + kPieceRows - 1) / kPieceRows);
   const size_t rows = (size_t)(w.sinks + 31) / 32 * 32;
   if (p.pieces > 0) p.workspace = sizeof(float) * BH * (size_t)(p.pieces + 1) * 2 * rows * D;
   return p;
@@ -1128,7 +1140,8 @@ hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, flo
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   const dim3 grid(BH, plan.pieces * sink_blocks + 2 * blocks);
-  with_f32_shape(bwd_waves_per_group(BH, S), false, [&](auto, auto ks) {
+  with_f32_shape(window_f32_waves_per_group(S, (long long)grid.x * grid.y), false,
+                 [&](auto, auto ks) {
     if (own)
       window_bwd_f32_kernel<D, ks(), true>
           <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, sink_blocks);

@@ -87,8 +87,8 @@ int append(const char* fn, uint8_t* k8, uint8_t* v8, float* k_scale, float* v_sc
   if (int st = check_new_rows(fn, "v", v_strides, &vs)) return st;
   if (rows < 1)
     return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: rows=%d must be positive", fn, rows);
-  // one wave per touched block, head, sequence and tensor: their lanes count in 32 bits
-  if (2LL * n_seq * H * dadgpt::kv8_touched_blocks(rows, block) >= (1LL << 26))
+  // grid (heads, touched blocks, sequences)
+  if (n_seq > 65535 || dadgpt::kv8_touched_blocks(rows, block) > 65535)
     return fail(DADGPT_ERR_INVALID_ARGUMENT,
                 "%s: n_seq=%d x n_heads=%d x rows=%d exceeds the launch limits", fn, n_seq, H,
                 rows);

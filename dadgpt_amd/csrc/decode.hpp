@@ -112,8 +112,9 @@ struct MergeLds {
 // Merges the workgroup's waves (running maximum mx in log2 units, sum lsum, unnormalised o of
 // EPL columns from `col`, given by the lanes with `holds`) and writes the cache's output row, or,
 // where the cache has nch > 1 chunks, publishes the chunk's partial; the last chunk to arrive
-// merges all of them.
-template <typename T, int D, int WAVES, int EPL>
+// merges all of them. An empty cache (nch 0) gives zeros; NAN_ZERO also where the sum of an unsplit
+// cache is NaN (the plain decode's behaviour; the others pass NaN on).
+template <bool NAN_ZERO, typename T, int D, int WAVES, int EPL>
 __device__ __forceinline__ void merge_chunks(MergeLds<D, WAVES>& sm, T* out, const float (&o)[EPL],
                                              float mx, float lsum, int wave, int lane, bool holds,
                                              int col, int chunk, int nch, float* part,
@@ -142,7 +143,7 @@ __device__ __forceinline__ void merge_chunks(MergeLds<D, WAVES>& sm, T* out, con
     }
   }
   if (nch <= 1) {  // the whole cache is this chunk
-    if (tid < D) out[tid] = Elem<T>::from(wl > 0.f ? wo / wl : 0.f);
+    if (tid < D) out[tid] = Elem<T>::from((NAN_ZERO ? wl > 0.f : nch == 1) ? wo / wl : 0.f);
     return;
   }
 

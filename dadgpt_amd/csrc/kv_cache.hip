@@ -65,23 +65,20 @@ __device__ __forceinline__ float e4m3_scale(uint32_t a) {
 }
 
 // One wave for each touched block of a (sequence, head) and tensor: D/8 lanes a row, NI rows a
-// lane. Waves run over the heads of a block, then blocks, then sequences, so that neighbours read
-// one stretch of the projection's token-major rows.
+// lane. Grid (heads, K and V: 4 waves a workgroup; touched blocks; sequences), heads fastest, so that
+// neighbours read one stretch of the projection's token-major rows.
 template <typename T, int D, int NI>
 __global__ __launch_bounds__(64 * kAppendWaves) void kv8_append_kernel(
     uint8_t* __restrict__ k8, uint8_t* __restrict__ v8, float* __restrict__ k_scale,
     float* __restrict__ v_scale, const T* __restrict__ k, const T* __restrict__ v,
     const HeadStrides64 ks, const HeadStrides64 vs, const int* __restrict__ lens,
-    const int* __restrict__ counts, int n_seq, int H, int rows, int max_len, int touched) {
+    const int* __restrict__ counts, int H, int rows, int max_len) {
   constexpr int LPR = D / 8, RPI = 64 / LPR, BLOCK = NI * RPI;
   const int lane = threadIdx.x & 63, sub = lane % LPR, grp = lane / LPR;
-  unsigned u = blockIdx.x * kAppendWaves + (threadIdx.x >> 6);
-  const bool is_v = u & 1;
-  u >>= 1;
-  const int head = u % H;
-  u /= H;
-  const int seq = u / touched, at = u % touched;
-  if (seq >= n_seq) return;
+  const int unit = blockIdx.x * kAppendWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool is_v = unit & 1;
+  const int head = unit >> 1, seq = blockIdx.z, at = blockIdx.y;
+  if (head >= H) return;
   const int begin = clamp_len(lens[seq], max_len);
   const int count = counts == nullptr ? rows : clamp_len(counts[seq], rows);
   const int end = begin + min(count, max_len - begin);
@@ -145,12 +142,10 @@ hipError_t launch_kv8_append_d(uint8_t* k8, uint8_t* v8, float* k_scale, float* 
                                const HeadStrides64& vs, const int* lens, const int* counts,
                                int n_seq, int H, int rows, int max_len, int block,
                                hipStream_t stream) {
-  const int touched = kv8_touched_blocks(rows, block);
-  const long long waves = 2LL * n_seq * H * touched;
-  const unsigned grid = (unsigned)((waves + kAppendWaves - 1) / kAppendWaves);
+  const dim3 grid((2 * H + kAppendWaves - 1) / kAppendWaves, kv8_touched_blocks(rows, block), n_seq);
   auto launch = [&](auto ni) {
     kv8_append_kernel<T, D, ni()><<<grid, 64 * kAppendWaves, 0, stream>>>(
-        k8, v8, k_scale, v_scale, k, v, ks, vs, lens, counts, n_seq, H, rows, max_len, touched);
+        k8, v8, k_scale, v_scale, k, v, ks, vs, lens, counts, H, rows, max_len);
   };
   switch (block * D / 512) {
     case 1:  // 16 tokens of 32 columns
@@ -194,7 +189,7 @@ hipError_t launch_kv8_append_t(uint8_t* k8, uint8_t* v8, float* k_scale, float* 
 // key rows (16 codes a lane: 4 lanes a row at D = 64), all of a wave's loads issued before any
 // arithmetic, chunks of one cache merged by the last to arrive.
 constexpr int kKv8Waves = 8;
-constexpr int kKv8Loads = 4;  // 16-byte loads per lane and tensor
+constexpr int kKv8Loads = 8;  // 16-byte loads per lane and tensor
 template <int D>
 __host__ __device__ constexpr int kv8_chunk_keys() {
   return kKv8Waves * kKv8Loads * 64 / (D / 16);
@@ -276,7 +271,8 @@ __global__ __launch_bounds__(64 * kKv8Waves) void kv8_decode_kernel(
   // Chunks past the length do nothing; chunk 0 of an empty cache still writes the zero output.
   if (chunk >= (nch > 1 ? nch : 1)) return;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform: scalar
   const int sub = lane % LPR, grp = lane / LPR;
   const size_t hrow = (size_t)seq * H + head;
   const uint8_t* kh = k8 + hrow * max_len * D + sub * 16;
@@ -294,19 +290,21 @@ __global__ __launch_bounds__(64 * kKv8Waves) void kv8_decode_kernel(
     Query16<T> qv;
     qv.load(q + hrow * D + sub * 16);
     // Keys past the length load key L-1 instead (valid, since key0 < L) and are masked out below.
+    // Without a window the KPL = 16 rows of a load at D = 64 lie in one block: scalar scales.
+    constexpr bool kUniform = !WIN && KPL == 16;
     u32x4 kr[NLD], vr[NLD];
     float ks[NLD], vs[NLD];
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
       const int row = keys.row(min(key0 + i * KPL + grp, L - 1));
       kr[i] = ld_stream(kh + (size_t)row * D);
-      ks[i] = ksh[row >> block_log2];
+      ks[i] = ksh[(kUniform ? min(key0 + i * KPL, L - 1) : row) >> block_log2];
     }
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
       const int row = keys.row(min(key0 + i * KPL + grp, L - 1));
       vr[i] = ld_stream(vh + (size_t)row * D);
-      vs[i] = vsh[row >> block_log2];
+      vs[i] = vsh[(kUniform ? min(key0 + i * KPL, L - 1) : row) >> block_log2];
     }
     // Keep the scheduler from sinking loads towards their uses: all of them stay in flight.
     __builtin_amdgcn_sched_barrier(0);
@@ -336,8 +334,9 @@ __global__ __launch_bounds__(64 * kKv8Waves) void kv8_decode_kernel(
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e] = sum_modulo<LPR>(o[e]);
   }
-  merge_chunks<T, D, kKv8Waves>(sm, out + hrow * D, o, mx, lsum, wave, lane, grp == 0, sub * 16,
-                                chunk, nch, part + hrow * n_chunk * (D + 2), counter + hrow);
+  merge_chunks<false, T, D, kKv8Waves>(sm, out + hrow * D, o, mx, lsum, wave, lane, grp == 0,
+                                       sub * 16, chunk, nch, part + hrow * n_chunk * (D + 2),
+                                       counter + hrow);
 }
 
 template <typename T, int D>
@@ -374,27 +373,30 @@ hipError_t launch_kv8_decode_d(T* out, const T* q, const uint8_t* k8, const uint
 // decode_kernel's split, with each key's score kept: the probability needs the cache's final
 // maximum and sum. A cache of one chunk has them in the workgroup; longer ones leave scores and
 // partials in the workspace for weights_kernel.
+// A workgroup has 8 waves, or 16 where those hold the whole cache (ONE): the second launch then
+// costs more than the uneven ends of longer chunks.
 constexpr int kWWaves = 8, kWLoads = 8;
 template <typename T, int D>
-__host__ __device__ constexpr int weights_chunk_keys() {
-  return kWWaves * kWLoads * 64 / (D / Elem<T>::kPer16B);
+__host__ __device__ constexpr int weights_chunk_keys(int waves = kWWaves) {
+  return waves * kWLoads * 64 / (D / Elem<T>::kPer16B);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kWWaves) void weights_decode_kernel(
+template <typename T, int D, bool ONE>
+__global__ __launch_bounds__(64 * kWWaves * (ONE ? 2 : 1)) void weights_decode_kernel(
     T* __restrict__ out, float* wout, const T* __restrict__ q, const T* __restrict__ kc,
     const T* __restrict__ vc, const float* win, const int* __restrict__ lens, int H, int max_len,
     float scale_log2, float* __restrict__ part, float* __restrict__ scores, int n_chunk) {
   constexpr int EPL = Elem<T>::kPer16B, LPR = D / EPL, KPL = 64 / LPR, NLD = kWLoads;
-  constexpr int KW = NLD * KPL, C = weights_chunk_keys<T, D>(), NT = 64 * kWWaves;
-  __shared__ float sm_o[kWWaves][D];
-  __shared__ float sm_m[kWWaves], sm_l[kWWaves];
+  constexpr int WAVES = kWWaves * (ONE ? 2 : 1), NT = 64 * WAVES;
+  constexpr int KW = NLD * KPL, C = weights_chunk_keys<T, D>(WAVES);
+  __shared__ float sm_o[WAVES][D];
+  __shared__ float sm_m[WAVES], sm_l[WAVES];
   __shared__ float sm_s[C];
 
   const int seq = blockIdx.x / H, head = blockIdx.x % H, chunk = blockIdx.y;
   const int L = clamp_len(lens[seq], max_len);
   const int nch = (L + C - 1) / C;
-  if (n_chunk > 1 && chunk >= (nch > 1 ? nch : 1)) return;
+  if (!ONE && chunk >= (nch > 1 ? nch : 1)) return;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int sub = lane % LPR, grp = lane / LPR;
@@ -456,15 +458,15 @@ __global__ __launch_bounds__(64 * kWWaves) void weights_decode_kernel(
   __syncthreads();
   float wm = neg_inf(), wl = 0.f, wo = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWWaves; ++w) wm = fmaxf(wm, sm_m[w]);
+  for (int w = 0; w < WAVES; ++w) wm = fmaxf(wm, sm_m[w]);
 #pragma unroll
-  for (int w = 0; w < kWWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     const float f = sm_m[w] == neg_inf() ? 0.f : fast_exp2(sm_m[w] - wm);
     wl += sm_l[w] * f;
     if (tid < D) wo += sm_o[w][tid] * f;
   }
-  if (n_chunk == 1) {
-    if (tid < D) out[hrow * D + tid] = Elem<T>::from(wl > 0.f ? wo / wl : 0.f);
+  if constexpr (ONE) {
+    if (tid < D) out[hrow * D + tid] = Elem<T>::from(L > 0 ? wo / wl : 0.f);
     const float inv = 1.0f / wl;
     for (int key = tid; key < max_len; key += NT) {
       const float w = win[hrow * max_len + key];
@@ -530,14 +532,18 @@ hipError_t launch_weights_decode_d(T* out, float* wout, const T* q, const T* kc,
                                    const float* win, const int* lens, int n_seq, int H,
                                    int max_len, float scale, void* workspace,
                                    hipStream_t stream) {
+  if (max_len <= weights_chunk_keys<T, D>(2 * kWWaves)) {
+    weights_decode_kernel<T, D, true><<<dim3(n_seq * H), 128 * kWWaves, 0, stream>>>(
+        out, wout, q, kc, vc, win, lens, H, max_len, scale * kLog2e, nullptr, nullptr, 1);
+    return hipGetLastError();
+  }
   constexpr int C = weights_chunk_keys<T, D>();
   const int nc = (max_len + C - 1) / C;
   float* part = static_cast<float*>(workspace);
-  float* scores = part + (nc > 1 ? (size_t)n_seq * H * nc * (D + 2) : 0);
-  weights_decode_kernel<T, D><<<dim3(n_seq * H, nc), 64 * kWWaves, 0, stream>>>(
+  float* scores = part + (size_t)n_seq * H * nc * (D + 2);
+  weights_decode_kernel<T, D, false><<<dim3(n_seq * H, nc), 64 * kWWaves, 0, stream>>>(
       out, wout, q, kc, vc, win, lens, H, max_len, scale * kLog2e, part, scores, nc);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || nc == 1) return e;
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   constexpr int per = kWeightsThreads * kWeightsPer;
   weights_kernel<T, D><<<dim3(n_seq * H, (max_len + per - 1) / per), kWeightsThreads, 0, stream>>>(
       out, wout, win, lens, H, max_len, part, scores, nc);
@@ -546,7 +552,11 @@ hipError_t launch_weights_decode_d(T* out, float* wout, const T* q, const T* kc,
 
 // ------------------------------------------------------------------------ eviction
 
-constexpr int kSelThreads = 512, kSelPer = 4;  // keys per thread and tile
+constexpr int kSelThreads = 512, kSelWaves = kSelThreads / 64;
+constexpr int kSelHeld = 8;  // keys a thread holds; longer rows are read again for each pass
+constexpr int kSelRanked = kSelThreads;  // candidates ranked against each other: one a thread at most
+// Radix passes from the top: 11, 11 and 10 bits.
+constexpr int kSelBins = 2048;
 
 // Floats as unsigned words in their order: -0 as +0, NaN below everything.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -556,39 +566,46 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive prefix sum of x over the workgroup's threads; `total` is the sum. Each call needs its
-// own `scratch` until the next barrier after it.
-__device__ __forceinline__ int block_scan(int x, int* scratch, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int inc = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(inc, d, 64);
-    if (lane >= d) inc += y;
-  }
-  if (lane == 63) scratch[wave] = inc;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kSelThreads / 64; ++w) {
-    before += w < wave ? scratch[w] : 0;
-    total += scratch[w];
-  }
-  return before + inc - x;
+// Inclusive prefix sum over the wave's lanes: DPP shifts within rows of 16, then the last lane of a
+// row broadcast to the next one (rows 1 and 3), and of the first half to the second.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
 }
 
+// The wave's loads are in. A workgroup barrier alone does not wait for loads in flight, which a
+// store by another wave after it must not overtake.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+struct SelectLds {
+  int hist[kSelBins];
+  uint32_t cand_key[kSelRanked];  // a bin's keys, and their rows
+  int cand_row[kSelRanked], cand_rank[kSelRanked];
+  int wave_sum[2][kSelWaves];
+  int n_cand, digit, left, in_bin;  // the pass's digit, the rank left below it, its bin's size
+  uint32_t edge_key;
+  int edge_row;
+};
+
 // One workgroup per (sequence, head): which rows stay. The first `sinks` and the last `recent` do,
-// and of the others the `most` of largest weight, found by a radix search for the weight of rank
-// `most` (four passes of eight bits over the row, which the caches hold after the first); of rows
-// with that very weight the first ones. Then their indices in order, and their weights.
+// and of the others (first .. last - 1) the `most` of largest weight, of equal ones the lowest rows.
+// That is: the rows before an edge in the order (weight down, row up), and the edge, the row of
+// rank `most`, is found by a radix search from the top bits: as soon as its bin holds no more than
+// kSelRanked rows (mostly after one pass), these are ranked against each other; if the bits run out
+// first, the edge is among rows of one weight, and its row is found by counting them in order.
+// Then the indices that stay, in order, and their weights. HELD: a thread holds its keys (row
+// e * kSelThreads + t); else each pass reads the row again (from the caches).
+template <bool HELD>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     int* __restrict__ kept, float* wout, const float* weights, const int* __restrict__ lens, int H,
     int max_len, int max_out, int budget, int sinks, int recent) {
-  __shared__ int hist[256];
-  __shared__ int pick[2];  // the digit found, and what is left to find below it
-  __shared__ int scratch[2][kSelThreads / 64];
-  const int tid = threadIdx.x, seq = blockIdx.x / H;
+  __shared__ SelectLds sm;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.x / H;
   const long long hrow = blockIdx.x;
   const int L = clamp_len(lens[seq], max_len);
   const float* w = weights + hrow * max_len;
@@ -598,85 +615,190 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   for (int i = keep + tid; i < budget; i += kSelThreads) kp[i] = -1;
 
   const int first = min(sinks, L), last = max(first, L - recent);
-  uint32_t edge = 0;  // keys above it stay
-  int ties = 0;       // and so many of those that equal it
+  float held[HELD ? kSelHeld : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int e = 0; e < kSelHeld; ++e) {
+      const int i = e * kSelThreads + tid;
+      held[e] = i < L ? w[i] : 0.f;
+    }
+  }
+  // f(row, weight) for the thread's rows
+  auto rows = [&](auto f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int e = 0; e < kSelHeld; ++e) {
+        const int i = e * kSelThreads + tid;
+        if (i < L) f(i, held[e]);
+      }
+    } else {
+      for (int i = tid; i < L; i += kSelThreads) f(i, w[i]);
+    }
+  };
+
+  uint32_t edge_key = 0;
+  int edge_row = -1;  // (no row is at the edge or past it)
   if (L > budget) {
-    ties = budget - first - (L - last);  // >= 0, and fewer than last - first
+    int rank = budget - first - (L - last);  // >= 0, and less than last - first
     uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+    int shift = 32;
+    while (true) {
+      const int bits = shift == 10 ? 10 : 11;
+      shift -= bits;
+      for (int i = tid; i < kSelBins; i += kSelThreads) sm.hist[i] = 0;
+      if (tid == 0) sm.n_cand = 0;
       __syncthreads();
-      for (int i = first + tid; i < last; i += kSelThreads) {
-        const uint32_t k = order_key(w[i]);
-        if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      rows([&](int i, float x) {
+        const uint32_t k = order_key(x);
+        if (i >= first && i < last && (shift + bits == 32 || (k >> (shift + bits)) == prefix))
+          atomicAdd(&sm.hist[(k >> shift) & ((1u << bits) - 1)], 1);
+      });
+      __syncthreads();
+      // the digit whose rows, counted from the largest down, hold the row of that rank: four bins
+      // a thread, the highest first
+      int c[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += c[e] = sm.hist[kSelBins - 1 - (4 * tid + e)];
+      const int inc = wave_scan(sum);
+      if (lane == 63) sm.wave_sum[0][wave] = inc;
+      __syncthreads();
+      int above = inc - sum;
+#pragma unroll
+      for (int v = 0; v < kSelWaves; ++v) above += v < wave ? sm.wave_sum[0][v] : 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (above <= rank && rank < above + c[e]) {  // one thread, one bin
+          sm.digit = kSelBins - 1 - (4 * tid + e);
+          sm.left = rank - above;
+          sm.in_bin = c[e];
+        }
+        above += c[e];
       }
       __syncthreads();
-      // the digit whose rows, counted from the largest down, hold the row of rank `ties`
-      if (tid < 64) {
-        int c[4], sum = 0;
+      prefix = prefix << bits | (uint32_t)sm.digit;
+      rank = sm.left;
+      const int in_bin = sm.in_bin;
+      if (in_bin <= kSelRanked) {
+        rows([&](int i, float x) {
+          const uint32_t k = order_key(x);
+          if (i >= first && i < last && (k >> shift) == prefix) {
+            const int at = atomicAdd(&sm.n_cand, 1);
+            sm.cand_key[at] = k;
+            sm.cand_row[at] = i;
+          }
+        });
+        __syncthreads();
+        // a wave takes every kSelWaves-th candidate, a lane compares it with one of 64 others (a
+        // lane a candidate, walking the others in LDS, took 7k cycles for 30 of them: 18.5 us for
+        // the 32 x 12 rows of 2048 that take EVICT_US now)
+        for (int j0 = 0, most = (in_bin + 63) / 64 * 64; j0 < most; j0 += 64) {
+          const int j = j0 + lane;
+          const uint32_t kj = j < in_bin ? sm.cand_key[j] : 0u;
+          const int rj = j < in_bin ? sm.cand_row[j] : max_len;
+          constexpr int N = 4;  // candidates whose LDS reads are in flight together
+          for (int i = wave; i < in_bin; i += N * kSelWaves) {
+            uint32_t k[N];
+            int row[N];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += c[e] = hist[255 - (4 * tid + e)];
-        int inc = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const int y = __shfl_up(inc, d, 64);
-          if (tid >= d) inc += y;
-        }
-        int above = inc - sum;
-        if (above <= ties && ties < inc) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (above <= ties && ties < above + c[e]) {
-              pick[0] = 255 - (4 * tid + e);
-              pick[1] = ties - above;
+            for (int u = 0; u < N; ++u) {
+              const int at = min(i + u * kSelWaves, in_bin - 1);
+              k[u] = sm.cand_key[at];
+              row[u] = sm.cand_row[at];
             }
-            above += c[e];
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+              const int at = i + u * kSelWaves;
+              const int before = __popcll(__ballot(kj > k[u] || (kj == k[u] && rj < row[u])));
+              if (lane == 0 && at < in_bin)
+                sm.cand_rank[at] = j0 == 0 ? before : sm.cand_rank[at] + before;
+            }
           }
         }
+        __syncthreads();
+        if (tid < in_bin && sm.cand_rank[tid] == rank) {
+          sm.edge_key = sm.cand_key[tid];
+          sm.edge_row = sm.cand_row[tid];
+        }
+        __syncthreads();
+        edge_key = sm.edge_key;
+        edge_row = sm.edge_row;
+        break;
       }
-      __syncthreads();
-      prefix = prefix << 8 | (uint32_t)pick[0];
-      ties = pick[1];
+      if (shift == 0) {  // more than kSelRanked rows of one weight: the one of that rank, in order
+        edge_key = prefix;
+        int seen = 0;
+        for (int t0 = 0; t0 < L; t0 += kSelThreads) {  // (every thread sees the same counts)
+          const int i = t0 + tid;
+          const bool tie = i >= first && i < last && order_key(w[min(i, L - 1)]) == edge_key;
+          const unsigned long long m = __ballot(tie);
+          if (lane == 0) sm.wave_sum[(t0 / kSelThreads) & 1][wave] = __popcll(m);
+          __syncthreads();
+          int at = seen + __popcll(m & ((1ull << lane) - 1));
+#pragma unroll
+          for (int v = 0; v < kSelWaves; ++v) {
+            const int n = sm.wave_sum[(t0 / kSelThreads) & 1][v];
+            at += v < wave ? n : 0;
+            seen += n;
+          }
+          if (tie && at == rank) sm.edge_row = i;
+        }
+        __syncthreads();
+        edge_row = sm.edge_row;
+        break;
+      }
     }
-    edge = prefix;
   }
-  int tied = 0, at = 0;  // ties and kept rows before the tile
-  for (int t0 = 0; t0 < L; t0 += kSelThreads * kSelPer) {
-    const int i0 = t0 + tid * kSelPer;
-    float x[kSelPer];
-    bool stays[kSelPer], tie[kSelPer];
-    int n_tie = 0;
+  auto stays = [&](int i, float x) {
+    if (L <= budget || i < first || i >= last) return true;
+    const uint32_t k = order_key(x);
+    return k > edge_key || (k == edge_key && i < edge_row);
+  };
+  // in slabs of a row a thread: a row's place is the count of those that stay before it
+  if constexpr (HELD) {
+    unsigned long long m[kSelHeld];
+    __syncthreads();  // (hist holds the slabs' wave counts now)
 #pragma unroll
-    for (int e = 0; e < kSelPer; ++e) {
-      const int i = i0 + e;
-      x[e] = i < L ? w[i] : 0.f;
-      const uint32_t k = order_key(x[e]);
-      const bool middle = i >= first && i < last;
-      stays[e] = i < L && (L <= budget || !middle || k > edge);
-      tie[e] = i < L && L > budget && middle && k == edge;
-      n_tie += tie[e];
+    for (int e = 0; e < kSelHeld; ++e) {
+      const int i = e * kSelThreads + tid;
+      m[e] = __ballot(i < L && stays(i, held[e]));
+      if (lane == 0) sm.hist[e * kSelWaves + wave] = __popcll(m[e]);
     }
-    int total;
-    int rank = tied + block_scan(n_tie, scratch[0], total);
-    tied += total;
-    int n_stay = 0;
-#pragma unroll
-    for (int e = 0; e < kSelPer; ++e) {
-      if (tie[e]) stays[e] = rank++ < ties;
-      n_stay += stays[e];
-    }
-    // (the tile's weights have been read by every thread at the first scan's barrier: they may
-    // be written over)
-    int pos = at + block_scan(n_stay, scratch[1], total);
-    at += total;
-#pragma unroll
-    for (int e = 0; e < kSelPer; ++e)
-      if (stays[e]) {
-        kp[pos] = i0 + e;
-        wo[pos] = x[e];
-        ++pos;
-      }
+    wait_loads();  // in place, other waves write over rows that this one has loaded
     __syncthreads();
+    static_assert(kSelHeld * kSelWaves == 64, "a lane for each slab and wave");
+    const int n = sm.hist[lane], before = wave_scan(n) - n;
+#pragma unroll
+    for (int e = 0; e < kSelHeld; ++e) {
+      const int at = __shfl(before, e * kSelWaves + wave, 64) +
+                     __popcll(m[e] & ((1ull << lane) - 1));
+      if (((m[e] >> lane) & 1) && at < keep) {  // (never past it: `keep` rows stay)
+        kp[at] = e * kSelThreads + tid;
+        wo[at] = held[e];
+      }
+    }
+  } else {
+    int seen = 0;
+    for (int t0 = 0; t0 < L; t0 += kSelThreads) {
+      const int i = t0 + tid;
+      const float x = w[min(i, L - 1)];
+      const bool s = i < L && stays(i, x);
+      const unsigned long long m = __ballot(s);
+      int* sums = sm.wave_sum[(t0 / kSelThreads) & 1];
+      __syncthreads();
+      if (lane == 0) sums[wave] = __popcll(m);
+      wait_loads();  // as above: at most the slab's own rows are written over, at <= i
+      __syncthreads();
+      int at = seen + __popcll(m & ((1ull << lane) - 1));
+#pragma unroll
+      for (int v = 0; v < kSelWaves; ++v) {
+        at += v < wave ? sums[v] : 0;
+        seen += sums[v];
+      }
+      if (s && at < keep) {
+        kp[at] = i;
+        wo[at] = x;
+      }
+    }
   }
 }
 
@@ -736,9 +858,7 @@ __global__ __launch_bounds__(kInPlaceThreads) void evict_in_place_kernel(
     for (int i = 0; i < kInPlacePer; ++i)
       if (from[i] >= 0)
         x[i] = *reinterpret_cast<const u32x4*>(rows + ((long long)from[i] << row_log2) + 16 * lane);
-    // every thread's loads are in before any thread stores (the barrier alone does not wait for
-    // loads in flight)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wait_loads();
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kInPlacePer; ++i) {
@@ -808,7 +928,7 @@ size_t weights_decode_workspace_bytes(int n_seq, int H, int max_len, int D) {
   // fp32 chunks are the shorter ones: their count serves both element types
   const int c = D == 64 ? weights_chunk_keys<float, 64>() : weights_chunk_keys<float, 32>();
   const int nc = (max_len + c - 1) / c;
-  return nc == 1 ? 0 : sizeof(float) * (size_t)n_seq * H * ((size_t)nc * (D + 2) + max_len);
+  return nc <= 2 ? 0 : sizeof(float) * (size_t)n_seq * H * ((size_t)nc * (D + 2) + max_len);
 }
 template <typename T>
 static hipError_t launch_weights_decode_t(T* out, float* wout, const T* q, const T* kc, const T* vc,
@@ -844,8 +964,12 @@ hipError_t launch_kv_evict(void* k_out, void* v_out, float* wout, int* kept, int
                            int sinks, int recent, hipStream_t stream) {
   const unsigned rows = (unsigned)(n_seq * H);
   const int row_log2 = __builtin_ctz((unsigned)row_bytes);
-  evict_select_kernel<<<rows, kSelThreads, 0, stream>>>(kept, wout, weights, lens, H, max_len,
-                                                        max_out, budget, sinks, recent);
+  if (max_len <= kSelHeld * kSelThreads)
+    evict_select_kernel<true><<<rows, kSelThreads, 0, stream>>>(
+        kept, wout, weights, lens, H, max_len, max_out, budget, sinks, recent);
+  else
+    evict_select_kernel<false><<<rows, kSelThreads, 0, stream>>>(
+        kept, wout, weights, lens, H, max_len, max_out, budget, sinks, recent);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (k_out == k) {
     evict_in_place_kernel<<<dim3(rows, 1, 2), kInPlaceThreads, 0, stream>>>(

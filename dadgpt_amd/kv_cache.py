@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import attention as _attn
-from .attention import (HeadStrides, _check, _ptr, _ptrs, _same_device, _stream_ptr, _workspace)
+from .attention import _check, _ptrs, _same_device, _stream_ptr, _workspace
 
 # Symbols declared in include/dadgpt/kv_cache.h.
 CACHE_SYMBOLS = (
@@ -48,13 +48,11 @@ def lib():
         return _lib
     L = _attn.lib()
     vp, i, f, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
-    hs = ctypes.POINTER(HeadStrides)
     L.dadgpt_kv8_blocks.argtypes = [i, i]
     L.dadgpt_decode_kv8_workspace_bytes.argtypes = [i] * 4
     L.dadgpt_decode_weights_workspace_bytes.argtypes = [i] * 4
     for name in ("bf16", "f32"):
-        getattr(L, "dadgpt_kv8_append_" + name).argtypes = ([vp] * 6 + [hs, hs, vp, vp] + [i] * 6 +
-                                                            [vp])
+        getattr(L, "dadgpt_kv8_append_" + name).argtypes = ([vp] * 10 + [i] * 6 + [vp])
         getattr(L, "dadgpt_decode_attention_kv8_" + name).argtypes = (
             [vp] * 7 + [i] * 5 + [f, i, i, vp, sz, vp])
         getattr(L, "dadgpt_decode_attention_weights_" + name).argtypes = (
@@ -66,23 +64,27 @@ def lib():
     return L
 
 
+_entries = {}  # (name, element type) -> entry point
+
+
 def _by_dtype(name, dtype):
     """The entry point of `name` for bf16 or fp32 tensors."""
-    if dtype is torch.bfloat16:
-        return getattr(lib(), name + "_bf16")
-    if dtype is torch.float32:
-        return getattr(lib(), name + "_f32")
-    raise TypeError(f"{name}: tensors must be bfloat16 or float32, got {dtype}")
+    fn = _entries.get((name, dtype))
+    if fn is None:
+        suffix = {torch.bfloat16: "_bf16", torch.float32: "_f32"}.get(dtype)
+        if suffix is None:
+            raise TypeError(f"{name}: tensors must be bfloat16 or float32, got {dtype}")
+        fn = _entries[name, dtype] = getattr(lib(), name + suffix)
+    return fn
 
 
 # ------------------------------------------------------------------------ 8-bit cache
 
 def kv8_blocks(max_len: int, block: int) -> int:
     """Blocks of `block` tokens in a cache of max_len rows: the scales' last dimension."""
-    n = int(lib().dadgpt_kv8_blocks(max_len, block))
-    if n == 0:
+    if max_len < 1 or block not in KV8_BLOCKS:
         raise ValueError(f"max_len={max_len} must be positive, block={block} one of {KV8_BLOCKS}")
-    return n
+    return (max_len + block - 1) // block
 
 
 def kv8_cache(n_seq: int, n_heads: int, max_len: int, d_head: int, block: int, device="cuda"):
@@ -94,9 +96,19 @@ def kv8_cache(n_seq: int, n_heads: int, max_len: int, d_head: int, block: int, d
             *(torch.zeros(scales, dtype=torch.float32, device=device) for _ in range(2)))
 
 
-def _row_strides(t) -> HeadStrides:
-    """The strides of a [n_seq, n_heads, rows, d_head] view (a dimension of one needs none)."""
-    return HeadStrides(*(st if size > 1 else 0 for st, size in zip(t.stride()[:3], t.shape)))
+_Int64x6 = ctypes.c_int64 * 6
+
+
+def _new_rows(t, name, shape, dtype):
+    """Address and (batch, head, row) strides of a view of new rows; a dimension of one has no
+    stride."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not dtype:
+        raise TypeError(f"{name} must be a device tensor of {dtype}")
+    strides = t.stride()
+    if t.shape != shape or strides[3] != 1:
+        raise ValueError(f"{name} must be a [n_seq, n_heads, rows, d_head] view with contiguous "
+                         f"rows, got {tuple(t.shape)} with strides {strides}")
+    return t.data_ptr(), [st if size > 1 else 0 for st, size in zip(strides, shape[:3])]
 
 
 def kv8_append(k_cache, v_cache, k_scale, v_scale, k, v, lens, counts, n_seq: int, n_heads: int,
@@ -104,21 +116,19 @@ def kv8_append(k_cache, v_cache, k_scale, v_scale, k, v, lens, counts, n_seq: in
     """Appends k and v, [n_seq, n_heads, rows, d_head] views with contiguous rows (bf16 or fp32;
     the heads of a token-major projection will do), at cache rows lens[s] + t for t < counts[s]
     (counts None: all). lens, counts: device int32; the caller advances lens."""
-    for t, name in ((k, "k"), (v, "v")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not k.dtype:
-            raise TypeError(f"{name} must be a device tensor of k's type")
-        if t.shape != (n_seq, n_heads, rows, d_head) or t.stride(3) != 1:
-            raise ValueError(f"{name} must be a [n_seq, n_heads, rows, d_head] view with contiguous "
-                             f"rows, got {tuple(t.shape)} with strides {t.stride()}")
-    pk, pv = _ptrs(KV8_DTYPE, n_seq * n_heads * max_len * d_head, (k_cache, v_cache),
+    fn = _by_dtype("dadgpt_kv8_append", k.dtype)
+    shape = (n_seq, n_heads, rows, d_head)
+    pk, ks = _new_rows(k, "k", shape, k.dtype)
+    pv, vs = _new_rows(v, "v", shape, k.dtype)
+    c8, d8 = _ptrs(KV8_DTYPE, n_seq * n_heads * max_len * d_head, (k_cache, v_cache),
                    ("k_cache", "v_cache"))
-    ps, pt = _ptrs(torch.float32, n_seq * n_heads * kv8_blocks(max_len, block),
+    sc, sd = _ptrs(torch.float32, n_seq * n_heads * kv8_blocks(max_len, block),
                    (k_scale, v_scale), ("k_scale", "v_scale"))
     pl, pc = _ptrs(torch.int32, n_seq, (lens, counts), ("lens", "counts"))
     _same_device((k_cache, v_cache, k_scale, v_scale, k, v, lens, counts))
-    _check(_by_dtype("dadgpt_kv8_append", k.dtype)(
-        pk, pv, ps, pt, _ptr(k), _ptr(v), _row_strides(k), _row_strides(v), pl, pc, n_seq, n_heads, rows,
-        max_len, d_head, block, _stream_ptr(stream)))
+    strides = _Int64x6(*ks, *vs)  # two dadgpt_head_strides
+    _check(fn(c8, d8, sc, sd, pk, pv, ctypes.byref(strides), ctypes.byref(strides, 24), pl, pc,
+              n_seq, n_heads, rows, max_len, d_head, block, _stream_ptr(stream)))
 
 
 def decode_kv8_workspace_bytes(n_seq: int, n_heads: int, max_len: int, d_head: int) -> int:

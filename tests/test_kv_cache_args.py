@@ -1,5 +1,6 @@
 """CPU tests of the bounded caches' C ABI: header and binding agree, every check answers on the host
 before any HIP call."""
+import ctypes
 import os
 import re
 
@@ -24,10 +25,14 @@ def test_header_and_binding_agree():
 
 
 def test_blocks():
+    for block in C.KV8_BLOCKS:
+        for L in (1, 15, 16, 17, 127, 128, 129, 1024):
+            assert C.kv8_blocks(L, block) == C.lib().dadgpt_kv8_blocks(L, block)
     assert [C.kv8_blocks(L, 32) for L in (1, 32, 33, 1024)] == [1, 1, 2, 32]
     for L, block in ((0, 32), (10, 0), (10, 8), (10, 48), (10, 256)):
         with pytest.raises(ValueError):
             C.kv8_blocks(L, block)
+        assert C.lib().dadgpt_kv8_blocks(L, block) == 0
 
 
 def _st(batch=1 << 16, head=64, row=768):
@@ -40,7 +45,7 @@ def test_append_validation(name):
 
     def call(ptrs=None, ks=None, vs=None, lens=FAKE + 6 * STEP, counts=None, n=4, h=2, rows=3, L=100,
              d=64, block=32):
-        return f(*(ptrs or _ptrs(6)), ks or _st(), vs or _st(), lens, counts, n, h, rows, L, d, block,
+        return f(*(ptrs or _ptrs(6)), ctypes.byref(ks or _st()), ctypes.byref(vs or _st()), lens, counts, n, h, rows, L, d, block,
                  None)
 
     for i in range(6):
@@ -57,8 +62,9 @@ def test_append_validation(name):
     for kw in ({"batch": -8}, {"head": 4}, {"row": 12}, {"row": 1 << 41}):
         assert call(ks=_st(**kw)) == 1 and "strides of k" in A.last_error()
         assert call(vs=_st(**kw)) == 1 and "strides of v" in A.last_error()
-    assert f(*_ptrs(6), None, _st(), FAKE, None, 4, 2, 3, 100, 64, 32, None) == 1
-    assert call(n=1 << 15, h=64, rows=1024, block=16) == 1 and "launch limits" in A.last_error()
+    assert f(*_ptrs(6), None, ctypes.byref(_st()), FAKE, None, 4, 2, 3, 100, 64, 32, None) == 1
+    assert call(n=65536) == 1 and "launch limits" in A.last_error()
+    assert call(rows=16 * 65535 + 2, block=16) == 1 and "launch limits" in A.last_error()
     same = _ptrs(6)
     same[1] = same[0]
     assert call(same) == 1 and "k_cache overlaps v_cache" in A.last_error()
@@ -72,7 +78,7 @@ def test_append_validation(name):
 def test_kv8_decode_validation(name):
     f = getattr(C.lib(), "dadgpt_decode_attention_kv8_" + name)
 
-    def call(ptrs=None, n=4, h=2, L=2000, d=64, block=32, scale=0.125, window=0, sinks=0, ws=None,
+    def call(ptrs=None, n=4, h=2, L=5000, d=64, block=32, scale=0.125, window=0, sinks=0, ws=None,
              wsb=0):
         return f(*(ptrs or _ptrs(7)), n, h, L, d, block, scale, window, sinks, ws, wsb, None)
 
@@ -84,7 +90,7 @@ def test_kv8_decode_validation(name):
     assert call(scale=float("nan")) == 1
     assert call(sinks=3) == 1 and "without a window" in A.last_error()
     assert call(window=-1) == 1 and call(window=5, sinks=-1) == 1 and call(window=5, sinks=1025) == 1
-    need = C.decode_kv8_workspace_bytes(4, 2, 2000, 64)
+    need = C.decode_kv8_workspace_bytes(4, 2, 5000, 64)
     assert need > 0
     assert call() == 4 and call(ws=FAKE, wsb=need - 1) == 4 and call(ws=FAKE + 8, wsb=need) == 1
     # a window needs what its own keys need

@@ -83,22 +83,25 @@ def test_window_backward_workspace(name):
 
 def test_window_workspace_covers_both_types_plans():
     """fp32 partials [BH][piece][2][sink rows in whole 32s][D]. The fp32 backward has pieces of 256
-    rows past a 128-key block's window and one for the block itself; the bf16 one pieces of 8 to 16
-    64-row tiles (fewer than the fp32 one's)."""
+    rows past a 128-key block's window and one for the block itself, or none where the later queries are
+    few; the bf16 one pieces of 8 to 16 64-row tiles."""
     for S in (513, 530, 1024, 5000, 1 << 19):
         for window in (1, 40, 100, 500, 4000):
             for sinks in (1, 32, 33, 700, 1024):
                 if window >= S:
                     continue
                 end = (128 + window - 2) // 64 * 64 + 64
-                pieces = max(0, (S - end + 255) // 256)
+                far = S - end
+                split = far > 384 and (far > end or S > 1024)
+                pieces = (far + 255) // 256 if split else 0
                 rows = (min(sinks, S) + 31) // 32 * 32
                 want = 4 * 3 * (pieces + 1) * 2 * rows * 32 if pieces else 0
                 assert A.window_workspace_bytes(3, S, 32, window, sinks) >= want
-                end = (64 + window - 2) // 64 + 1  # the smaller key block of the bf16 kernels
-                tiles = max(0, (S + 63) // 64 - end)
+                # the bf16 plan without a GPU (no compute units known): separate launches, 128 keys
+                tiles = max(0, (S + 63) // 64 - ((128 + window - 2) // 64 + 1))
                 of = min(16, max(8, (tiles + 63) // 64))
-                assert (tiles + of - 1) // of <= pieces + 1
+                assert A.window_workspace_bytes(3, S, 32, window, sinks) >= (
+                    4 * 3 * ((tiles + of - 1) // of) * 2 * rows * 32)
 
 
 def test_window_strided_validation():
