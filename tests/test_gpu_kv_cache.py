@@ -378,3 +378,98 @@ def test_cache_calls_repeat_on_streams_and_in_graphs(gpu):
         torch.cuda.synchronize()
         assert all(torch.equal(a, x) for a, x in zip(flat(b), want))
         step(eager)
+
+
+@pytest.mark.gpu
+def test_kv8_past_32_bit_offsets(gpu):
+    """Five 8-bit caches of 16,776,960 rows (1.07 GB of codes each, so the last ones lie past 2^32
+    bytes): rows appended at the very end and read back through a window."""
+    n, H, L, D, block, window = 5, 1, 65535 * 256, 64, 64, 40
+    cache = C.kv8_cache(n, H, L, D, block)
+    x = _randn((n, H, window, D), seed=41, dtype=BF)
+    y = _randn((n, H, window, D), seed=42, dtype=BF)
+    q = _randn((n, H, D), seed=43, dtype=BF)
+    C.kv8_append(*cache, x, y, _int([L - window] * n), None, n, H, window, L, D, block)
+    want = torch.zeros((1, H, 2 * block, D), dtype=torch.uint8), torch.zeros((1, H, 2))
+    at = 2 * block - window
+    for i in (0, n - 1):
+        codes, scale = want[0].clone(), want[1].clone()
+        R.append(codes, scale, x[i:i + 1].float().cpu(), [at], [window], block)
+        assert torch.equal(_u8(cache[0])[i, :, L - window:].cpu(), codes[0, :, at:])
+        assert torch.equal(cache[2][i, :, -1].cpu(), scale[0, :, -1])
+    out = torch.empty_like(q)
+    C.decode_attention_kv8(out, q, *cache, _int([L] * n), n, H, L, D, block, 0.125, window, 0, None)
+    k, v = (R.values(_u8(c)[:, :, L - window:].contiguous()) * s[:, :, -1:, None].double()
+            for c, s in ((cache[0], cache[2]), (cache[1], cache[3])))
+    ref, bound, _, _ = R.decode(q, k, v, [window] * n, 0.125, out_half=2.0 ** -8)
+    assert ((out.double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L,budget,sinks,recent", [(6000, 700, 3, 50), (3000, 1500, 0, 0),
+                                                   (9000, 4000, 10, 10)])
+def test_evict_of_many_equal_weights(gpu, L, budget, sinks, recent):
+    """More rows of one weight than are ranked against each other: the edge is among them, and the
+    lowest rows of it stay."""
+    n, H, D = 3, 2, 32
+    k, v = (_randn((n, H, L, D), s) for s in (1, 2))
+    w = torch.zeros((n, H, L), device="cuda")
+    w[1] = (torch.arange(L, device="cuda") % 7 == 0).float()      # two weights
+    w[2] = -0.0
+    w[2, 1, ::3] = float("nan")
+    out = [torch.empty((n, H, budget, D), device="cuda") for _ in range(2)]
+    w_out = torch.empty((n, H, budget), device="cuda")
+    kept = torch.empty((n, H, budget), dtype=torch.int32, device="cuda")
+    lens_out = torch.empty(n, dtype=torch.int32, device="cuda")
+    C.kv_evict(*out, w_out, kept, lens_out, k, v, w, _int([L, L, L - 1]), n, H, L, budget, D, budget,
+               sinks, recent)
+    for i, end in enumerate((L, L, L - 1)):
+        for h in range(H):
+            assert kept[i, h].tolist() == R.evict(w[i, h].cpu(), end, budget, sinks, recent), (i, h)
+            assert torch.equal(out[0][i, h], k[i, h, kept[i, h].long()])
+
+
+@pytest.mark.gpu
+def test_kv8_append_of_rows_with_odd_strides(gpu):
+    """Rows read out of wider buffers, K and V with strides of their own, and a single head or row
+    whose stride torch leaves arbitrary."""
+    n, H, L, D, block, rows = 2, 3, 64, 32, 16, 9
+    big = _randn((rows, n, H, 48), seed=51)            # row-major in tokens, gaps after each head
+    k = big[..., 8:40].permute(1, 2, 0, 3)
+    v = _randn((H, n, rows, D), seed=52).permute(1, 0, 2, 3)
+    a, b = C.kv8_cache(n, H, L, D, block), C.kv8_cache(n, H, L, D, block)
+    C.kv8_append(*a, k, v, _int([3, 11]), None, n, H, rows, L, D, block)
+    C.kv8_append(*b, k.contiguous(), v.contiguous(), _int([3, 11]), None, n, H, rows, L, D, block)
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+    one = torch.as_strided(k.contiguous()[:1, :1, :1], (1, 1, 1, D), (5, 3, 1, 1))
+    c = C.kv8_cache(1, 1, L, D, block)
+    C.kv8_append(*c, one, one, _int([0]), None, 1, 1, 1, L, D, block)
+    want = torch.zeros((1, 1, L, D), dtype=torch.uint8), torch.zeros((1, 1, L // block))
+    R.append(*want, one.cpu(), [0], [1], block)
+    assert torch.equal(_u8(c[0]).cpu(), want[0]) and torch.equal(c[2].cpu(), want[1])
+
+
+@pytest.mark.gpu
+def test_cache_wrappers_refuse_what_does_not_fit(gpu):
+    n, H, L, D, block = 2, 2, 32, 32, 16
+    cache = C.kv8_cache(n, H, L, D, block)
+    x, lens = _randn((n, H, 3, D), seed=1), _int([0, 0])
+    with pytest.raises(ValueError, match="contiguous rows"):
+        C.kv8_append(*cache, x.transpose(2, 3), x, lens, None, n, H, 3, L, D, block)
+    with pytest.raises(TypeError, match="v must be"):
+        C.kv8_append(*cache, x, x.to(BF), lens, None, n, H, 3, L, D, block)
+    with pytest.raises(TypeError, match="bfloat16 or float32"):
+        C.kv8_append(*cache, x.half(), x.half(), lens, None, n, H, 3, L, D, block)
+    with pytest.raises(ValueError, match="k_cache has"):
+        C.kv8_append(cache[0][:1], *cache[1:], x, x, lens, None, n, H, 3, L, D, block)
+    with pytest.raises(TypeError, match="float8"):
+        C.kv8_append(_u8(cache[0]), *cache[1:], x, x, lens, None, n, H, 3, L, D, block)
+    with pytest.raises(ValueError, match="block"):
+        C.kv8_append(*cache, x, x, lens, None, n, H, 3, L, D, 24)
+    k = _randn((n, H, L, D), seed=2)
+    w = torch.zeros((n, H, L), device="cuda")
+    kept = torch.empty((n, H, 8), dtype=torch.int32, device="cuda")
+    with pytest.raises(A.AttentionError, match="in place"):
+        C.kv_evict(k, k.clone(), w, kept, lens, k, k.clone(), w, lens, n, H, L, L, D, 8, 0, 0)
+    with pytest.raises(ValueError, match="kept has"):
+        C.kv_evict(k, k, w, kept[:1], lens, k, k, w, lens, n, H, L, L, D, 8, 0, 0)

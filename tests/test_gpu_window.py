@@ -40,7 +40,8 @@ CASES = [
     (4, 300, 64, 16, 65), (2, 511, 32, 130, 64), (7, 600, 64, 1, 5), (3, 777, 32, 100, 3),
     (2, 777, 64, 100, 3), (2, 1024, 64, 256, 4), (40, 650, 64, 65, 33), (130, 530, 64, 40, 2),
     (300, 300, 32, 90, 4), (1, 1500, 64, 3, 130), (2, 2100, 64, 1000, 4), (1, 2300, 32, 900, 200),
-    (1, 1800, 64, 17, 1024),
+    (1, 1800, 64, 17, 1024), (240, 1100, 64, 80, 4), (240, 1100, 32, 80, 4), (240, 1100, 64, 80, 0),
+    (20, 2100, 64, 1000, 4), (20, 2100, 32, 1000, 0), (260, 200, 64, 33, 2), (24, 1024, 32, 200, 40),
 ]
 
 
@@ -94,7 +95,9 @@ def test_a_window_of_the_sequence_is_the_causal_call(gpu, dtype, S, window):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,H,S,D,window,sinks", [(2, 3, 777, 64, 100, 3), (1, 4, 1300, 32, 1100, 70),
-                                                  (16, 12, 300, 64, 64, 4), (3, 2, 63, 64, 9, 1)])
+                                                  (16, 12, 300, 64, 64, 4), (3, 2, 63, 64, 9, 1),
+                                                  (20, 12, 1100, 64, 80, 4), (20, 12, 1100, 32, 80, 0),
+                                                  (2, 4, 1300, 64, 200, 0)])
 def test_token_major_and_strided_give_the_contiguous_bits(gpu, B, H, S, D, window, sinks):
     d, scale = H * D, D ** -0.5
     gen = torch.Generator(device="cuda").manual_seed(B + S)
@@ -282,3 +285,53 @@ def test_window_decode_is_the_windowed_forward_of_the_last_row(gpu):
     ref = R.attention(q, k, v, g, 0.125, window, sinks, BF)["out"]
     o, e = ref[0][:, -1], ref[1][:, -1]
     assert ((out.view(B * H, D).double() - got).abs() <= 2 * e).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_window_over_a_long_sequence(gpu, dtype):
+    """30,000 tokens with a gradient in the first and the last 300 rows only: what those rows give is
+    what they give in two short sequences, of the first rows, and of the sinks and the last rows;
+    the sink keys' gradients are the sum of both."""
+    BH, S, D, window, sinks, n = 3, 30000, 64, 100, 5, 300
+    q, k, v, g = _inputs(BH, S, D, dtype, seed=23)
+    g[:, n:S - n] = 0
+    got = _run(q, k, v, g, 0.125, window, sinks)
+    first = [x[:, :n + 200] for x in (q, k, v, g)]
+    last = [torch.cat((x[:, :sinks], x[:, S - n - 200:]), 1) for x in (q, k, v, g)]
+    last[3] = last[3].clone()
+    last[3][:, :sinks] = 0
+    a = R.attention(*first, 0.125, window, sinks, dtype)
+    b = R.attention(*last, 0.125, window, sinks, dtype)
+    R.assert_within({m: got[m][:, :n] for m in ("out", "lse", "dq")},
+                    {m: (a[m][0][:, :n], a[m][1][:, :n]) for m in ("out", "lse", "dq")})
+    R.assert_within({m: got[m][:, S - n:] for m in got},
+                    {m: (b[m][0][:, -n:], b[m][1][:, -n:]) for m in got})
+    R.assert_within({m: got[m][:, sinks:n] for m in ("dk", "dv")},
+                    {m: (a[m][0][:, sinks:n], a[m][1][:, sinks:n]) for m in ("dk", "dv")})
+    # the sums over 30,000 rows: the rows between add nothing but their place in the order of the sum
+    slack = 2.0 ** -24 * (S / 16) * (1 if dtype == BF else 6)
+    for m in ("dk", "dv"):
+        y = a[m][0][:, :sinks] + b[m][0][:, :sinks]
+        e = a[m][1][:, :sinks] + b[m][1][:, :sinks] + slack * y.abs().amax()
+        assert ((got[m][:, :sinks].double() - y).abs() <= e).all(), m
+
+
+@pytest.mark.gpu
+def test_window_decode_past_32_bit_offsets(gpu):
+    """fp32 caches of 16,776,960 rows (the launch limit; 4.3 GB each, so the last rows lie past 2^32
+    bytes): the windowed rows only are read."""
+    n, H, L, D, window, sinks = 1, 1, 65535 * 256, 64, 700, 4
+    k, v = (torch.zeros((n, H, L, D), device="cuda") for _ in range(2))
+    rows = torch.cat((torch.arange(sinks), torch.arange(L - window, L))).cuda()
+    gen = torch.Generator(device="cuda").manual_seed(29)
+    q = torch.randn((n, H, D), generator=gen, device="cuda")
+    kk, vv = (torch.randn((len(rows), D), generator=gen, device="cuda") for _ in range(2))
+    k[0, 0, rows], v[0, 0, rows] = kk, vv
+    lens = torch.tensor([L], dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    ws = A.decode_workspace(n, H, window + sinks, D)
+    A.decode_attention_window(out, q, k, v, lens, n, H, L, D, 0.125, window, sinks, ws)
+    ref, bound = _decode_ref(q, kk[None, None], vv[None, None],
+                             torch.tensor([len(rows)]), len(rows), 0, 0.125)
+    assert ((out.double() - ref).abs() <= bound).all()

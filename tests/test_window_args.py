@@ -152,3 +152,23 @@ def test_window_decode_validation(name):
     assert call() == 4
     assert call(ws=FAKE, wsb=need - 1) == 4
     assert A.decode_workspace_bytes(4, 2, 104, 64) == 0
+
+
+def test_tensors_off_the_current_device_are_refused(monkeypatch):
+    """With more than one device, a tensor that is not on the current one would be read on its
+    stream: ValueError. None passes; with one device there is nothing to look at."""
+    class Fake:
+        def __init__(self, device):
+            self.device = f"cuda:{device}"
+            self._d = device
+
+        def get_device(self):
+            return self._d
+
+    monkeypatch.setattr(A, "_devices", 2)
+    monkeypatch.setattr(A.torch.cuda, "current_device", lambda: 0)
+    A._same_device((Fake(0), None, Fake(0)))
+    with pytest.raises(ValueError, match="cuda:1, but the current device is cuda:0"):
+        A._same_device((Fake(0), Fake(1)))
+    monkeypatch.setattr(A, "_devices", 1)
+    A._same_device((Fake(0),))
