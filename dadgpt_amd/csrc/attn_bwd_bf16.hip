@@ -859,7 +859,7 @@ __device__ __forceinline__ void sink_workgroup(const BwdArgs& a, int bh, int gro
 
 // dQ (which writes delta), the sink keys' pieces in front: they are short, and the dQ workgroups
 // fill in behind them.
-constexpr int kMaxPieceTiles = 16;
+constexpr int kMaxPieceTiles = 12;
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, kDqMinBlocks) void window_dq_bf16_kernel(
     const BwdArgs a, const WindowBwdArg<true> win, int sink_groups) {
@@ -1043,11 +1043,10 @@ WindowPlan window_plan(int BH, int S, int D, const Window& w) {
   p.waves_per_group = window_waves_per_group(BH, S, p.one ? 2 : 1);
   const long long far = tiles - end(32 * kWaves / p.waves_per_group);
   if (p.one || w.sinks == 0 || far <= 0) return p;
-  // of 8 tiles (four rounds; of four, B16 H12 T1024 with a window of 256 takes dQ 56 for 52 us), up
-  // to 16 where that still makes 64 pieces
-  const long long of = (far + 63) / 64;
-  p.piece_tiles = (int)(of < 8 ? 8 : of > kMaxPieceTiles ? kMaxPieceTiles : of);
-  p.pieces = (int)((far + p.piece_tiles - 1) / p.piece_tiles);
+  // pieces of even lengths up to 12 tiles (six rounds; of four tiles, B16 H12 T1024 with a window of
+  // 256 takes dQ 56 for 51 us)
+  p.pieces = (int)((far + kMaxPieceTiles - 1) / kMaxPieceTiles);
+  p.piece_tiles = (int)((far + p.pieces - 1) / p.pieces);
   p.workspace = sizeof(float) * BH * (size_t)p.pieces * 2 * ((w.sinks + 31) / 32 * 32) * D;
   return p;
 }
