@@ -147,8 +147,9 @@ __global__ __launch_bounds__(64 * kWaves) void decode_kernel(
 #pragma unroll
     for (int e = 0; e < EPL; ++e) o[e] = lanes::sum_across<K0>(o[e]);
   }
-  merge_chunks<!WIN, T, D, kWaves>(sm, out + hrow * D, o, mx, lsum, wave, lane, grp == 0, sub * EPL, chunk,
-                             nch, part + hrow * n_chunk * (D + 2), counter + hrow);
+  merge_chunks<!WIN, T, D, kWaves>(sm, out + hrow * D, o, mx, lsum, wave, lane, grp == 0,
+                                   sub * EPL, chunk, nch, part + hrow * n_chunk * (D + 2),
+                                   counter + hrow);
 }
 
 template <typename T, int D>

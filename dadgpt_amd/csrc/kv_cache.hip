@@ -373,25 +373,24 @@ hipError_t launch_kv8_decode_d(T* out, const T* q, const uint8_t* k8, const uint
 // decode_kernel's split, with each key's score kept: the probability needs the cache's final
 // maximum and sum. A cache of one chunk has them in the workgroup; longer ones leave scores and
 // partials in the workspace for weights_kernel.
-// A workgroup has 8 waves, or 16 where those hold the whole cache (ONE): the second launch then
-// costs more than the uneven ends of longer chunks.
-constexpr int kWWaves = 8, kWLoads = 8;
+// ONE: a workgroup runs through its cache's chunks, two at most, and needs neither.
+constexpr int kWWaves = 8, kWLoads = 8, kWChunks = 2;
 template <typename T, int D>
-__host__ __device__ constexpr int weights_chunk_keys(int waves = kWWaves) {
-  return waves * kWLoads * 64 / (D / Elem<T>::kPer16B);
+__host__ __device__ constexpr int weights_chunk_keys() {
+  return kWWaves * kWLoads * 64 / (D / Elem<T>::kPer16B);
 }
 
 template <typename T, int D, bool ONE>
-__global__ __launch_bounds__(64 * kWWaves * (ONE ? 2 : 1)) void weights_decode_kernel(
+__global__ __launch_bounds__(64 * kWWaves) void weights_decode_kernel(
     T* __restrict__ out, float* wout, const T* __restrict__ q, const T* __restrict__ kc,
     const T* __restrict__ vc, const float* win, const int* __restrict__ lens, int H, int max_len,
     float scale_log2, float* __restrict__ part, float* __restrict__ scores, int n_chunk) {
   constexpr int EPL = Elem<T>::kPer16B, LPR = D / EPL, KPL = 64 / LPR, NLD = kWLoads;
-  constexpr int WAVES = kWWaves * (ONE ? 2 : 1), NT = 64 * WAVES;
-  constexpr int KW = NLD * KPL, C = weights_chunk_keys<T, D>(WAVES);
+  constexpr int WAVES = kWWaves, NT = 64 * WAVES;
+  constexpr int KW = NLD * KPL, C = weights_chunk_keys<T, D>();
   __shared__ float sm_o[WAVES][D];
   __shared__ float sm_m[WAVES], sm_l[WAVES];
-  __shared__ float sm_s[C];
+  __shared__ float sm_s[C * (ONE ? kWChunks : 1)];
 
   const int seq = blockIdx.x / H, head = blockIdx.x % H, chunk = blockIdx.y;
   const int L = clamp_len(lens[seq], max_len);
@@ -403,14 +402,15 @@ __global__ __launch_bounds__(64 * kWWaves * (ONE ? 2 : 1)) void weights_decode_k
   const size_t hrow = (size_t)seq * H + head;
   const T* kh = kc + hrow * max_len * D + sub * EPL;
   const T* vh = vc + hrow * max_len * D + sub * EPL;
-  const int key0 = chunk * C + wave * KW;
 
   float mx = neg_inf(), lsum = 0.f;
   float o[EPL];
 #pragma unroll
   for (int e = 0; e < EPL; ++e) o[e] = 0.f;
-  if (key0 < L) {
-    const u32x4 qw = ld_g128u(q + hrow * D + sub * EPL);
+  const u32x4 qw = ld_g128u(q + hrow * D + sub * EPL);
+  const int local = wave * KW;
+  for (int at = 0; chunk * C + at + local < L; at += C) {  // once, unless ONE
+    const int key0 = chunk * C + at + local;
     u32x4 kr[NLD], vr[NLD];
 #pragma unroll
     for (int i = 0; i < NLD; ++i)
@@ -419,34 +419,44 @@ __global__ __launch_bounds__(64 * kWWaves * (ONE ? 2 : 1)) void weights_decode_k
     for (int i = 0; i < NLD; ++i)
       vr[i] = ld_stream(vh + (size_t)min(key0 + i * KPL + grp, L - 1) * D);
     __builtin_amdgcn_sched_barrier(0);
+    const float before = mx;
     float s[NLD];
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
       const float acc = lanes::group_sum<LPR>(Elem<T>::dot(qw, kr[i]));
       s[i] = key0 + i * KPL + grp < L ? acc * scale_log2 : neg_inf();
       mx = fmaxf(mx, s[i]);
-      if (sub == 0) sm_s[wave * KW + i * KPL + grp] = s[i];
+      if (sub == 0) sm_s[at + local + i * KPL + grp] = s[i];
     }
     mx = lanes::wave_max_of_groups<LPR>(mx);
+    // where every score so far is -inf, 0 stands in for the maximum: those keys' terms are 0
+    const float base = mx == neg_inf() ? 0.f : mx;
+    if (ONE && at > 0) {
+      const float f = fast_exp2(before - base);
+      lsum *= f;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[e] *= f;
+    }
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
-      const float p = fast_exp2(s[i] - mx);  // exactly 0 for masked rows
+      const float p = fast_exp2(s[i] - base);  // exactly 0 for masked rows
       lsum += p;
       float vf[EPL];
       Elem<T>::unpack(vr[i], vf);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) o[e] = fmaf(p, vf[e], o[e]);
     }
-    if constexpr (LPR < 8) {
-      lsum += __shfl_xor(lsum, LPR, 64);
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) o[e] += __shfl_xor(o[e], LPR, 64);
-    }
-    constexpr int K0 = LPR < 8 ? 8 : LPR;
-    lsum = lanes::sum_across<K0>(lsum);
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) o[e] = lanes::sum_across<K0>(o[e]);
+    if constexpr (!ONE) break;
   }
+  if constexpr (LPR < 8) {
+    lsum += __shfl_xor(lsum, LPR, 64);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[e] += __shfl_xor(o[e], LPR, 64);
+  }
+  constexpr int K0 = LPR < 8 ? 8 : LPR;
+  lsum = lanes::sum_across<K0>(lsum);
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) o[e] = lanes::sum_across<K0>(o[e]);
   if (grp == 0) {
 #pragma unroll
     for (int e = 0; e < EPL; ++e) sm_o[wave][sub * EPL + e] = o[e];
@@ -532,12 +542,16 @@ hipError_t launch_weights_decode_d(T* out, float* wout, const T* q, const T* kc,
                                    const float* win, const int* lens, int n_seq, int H,
                                    int max_len, float scale, void* workspace,
                                    hipStream_t stream) {
-  if (max_len <= weights_chunk_keys<T, D>(2 * kWWaves)) {
-    weights_decode_kernel<T, D, true><<<dim3(n_seq * H), 128 * kWWaves, 0, stream>>>(
+  constexpr int C = weights_chunk_keys<T, D>();
+  // Two chunks by one workgroup of 8 waves, of which a CU holds two: 16 x 12 caches of 2048 rows of
+  // 64 bf16 take 14.4 us over four chunks (15.4 split) where 8 x 12 take 12.6 (11.5 split), and 64
+  // of 4096 take 91 (84.5 split): past two chunks the split wins or is even. One workgroup of 16
+  // waves for two chunks fits a CU once: 32 x 12 caches of 1024 rows took 15.4 us for 13.9.
+  if (max_len <= kWChunks * C) {
+    weights_decode_kernel<T, D, true><<<dim3(n_seq * H), 64 * kWWaves, 0, stream>>>(
         out, wout, q, kc, vc, win, lens, H, max_len, scale * kLog2e, nullptr, nullptr, 1);
     return hipGetLastError();
   }
-  constexpr int C = weights_chunk_keys<T, D>();
   const int nc = (max_len + C - 1) / C;
   float* part = static_cast<float*>(workspace);
   float* scores = part + (size_t)n_seq * H * nc * (D + 2);
@@ -690,7 +704,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
         __syncthreads();
         // a wave takes every kSelWaves-th candidate, a lane compares it with one of 64 others (a
         // lane a candidate, walking the others in LDS, took 7k cycles for 30 of them: 18.5 us for
-        // the 32 x 12 rows of 2048 that take EVICT_US now)
+        // the 32 x 12 rows of 2048 that take 10 us now)
         for (int j0 = 0, most = (in_bin + 63) / 64 * 64; j0 < most; j0 += 64) {
           const int j = j0 + lane;
           const uint32_t kj = j < in_bin ? sm.cand_key[j] : 0u;

@@ -204,6 +204,30 @@ def test_weights_decode(gpu, dtype, n, H, L, D):
     assert torch.equal(acc.masked_select(hidden[:, None]), before.masked_select(hidden[:, None]))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("L,m", [(900, 300), (1000, 600), (2500, 1100)])
+def test_weights_decode_of_scores_of_minus_infinity(gpu, dtype, L, m):
+    """Keys whose score is -inf weigh 0, also where a wave, a chunk or the first of two chunks
+    holds nothing else: the answer is that of the other keys alone."""
+    n, H, D = 2, 2, 64
+    q, k, v = (_randn(s, seed, dtype) for s, seed in
+               (((n, H, D), 4), ((n, H, L, D), 5), ((n, H, L, D), 6)))
+    q[..., 0] = 1
+    lens, rest = _int([L, L - 5]), _int([L - m, L - 5 - m])
+    out_half = 2.0 ** -8 if dtype == BF else 2.0 ** -24
+    ref, bound, p, e_p = R.decode(q, k[:, :, m:].double(), v[:, :, m:].double(), rest, D ** -0.5,
+                                  out_half=out_half)
+    k[:, :, :m, 0] = -float("inf")
+    before = torch.zeros((n, H, L), device="cuda")
+    ws = C.decode_weights_workspace(n, H, L, D)
+    out, after = torch.empty_like(q), torch.empty_like(before)
+    C.decode_attention_weights(out, after, q, k, v, before, lens, n, H, L, D, D ** -0.5, ws)
+    assert ((out.double() - ref).abs() <= bound).all()
+    assert (after[..., :m] == 0).all()
+    assert ((after[..., m:].double() - p).abs() <= e_p + p * 2.0 ** -24).all()
+
+
 # ------------------------------------------------------------------------ eviction
 
 def _weights(n, H, L, seed):
