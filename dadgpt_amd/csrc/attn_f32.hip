@@ -55,6 +55,11 @@ constexpr int kGroups = 4;
 constexpr int kRows = 32 * kGroups;  // rows a workgroup owns
 // At most 256 registers a lane (two waves per SIMD; one runs the backward ~15% slower).
 constexpr int wgs_per_cu(int ks) { return 2 / ks; }
+// The windowed kernels also have KG = 2 with KS = 2, for grids that leave CUs idle: at D = 64 its
+// tiles leave a CU room for one such workgroup.
+constexpr int wgs_per_cu(int ks, int kg, int d) {
+  return kg == kGroups ? wgs_per_cu(ks) : d == 64 ? 1 : 2;
+}
 
 // Row (within a 32-row chunk) that score register u of lane half h stands for, when the A
 // operand rows were read through sigma32: 16 * (u / 8) + 8 * h + u % 8.
@@ -351,12 +356,12 @@ __device__ __forceinline__ void store_rows_t(float* dst, int row0, int S,
 
 // ONCE: the conversions of Q's and the weights' splits forced to happen once (pack_once).
 // WIN: sliding window and sinks, as in the bf16 forward.
-template <int D, bool DROP, int KS, bool ONCE, bool WIN = false>
-__global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_kernel(
+template <int D, bool DROP, int KS, bool ONCE, bool WIN = false, int KG = kGroups>
+__global__ __launch_bounds__(64 * KG * KS, wgs_per_cu(KS, KG, D)) void fwd_f32_kernel(
     float* __restrict__ out, float* __restrict__ lse, const float* __restrict__ q,
     const float* __restrict__ k, const float* __restrict__ v, int S, float scale,
     const DropParams dr, const WindowArg<WIN> win) {
-  constexpr int NT = 64 * kGroups * KS, TR = 64, CPT = 2 / KS;  // chunks per tile and wave
+  constexpr int NT = 64 * KG * KS, TR = 64, CPT = 2 / KS;  // chunks per tile and wave
   // K and V tiles as three bf16 planes each; after the tile loop they hold the second waves'
   // partial results, then the epilogue's fp32 staging rows. With two waves per group there are
   // two sets (one workgroup has the CU's LDS to itself), see the tile loop.
@@ -364,18 +369,19 @@ __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_ker
   __shared__ __attribute__((aligned(16))) bf16 planes[KS * 2 * kPlane];
   constexpr int kPart = (D / 32) * 1024 + 128;  // a partial: O, m and l (floats)
   constexpr int kStage = 32 * (D + kPitchPad);  // a wave's staged rows (floats)
-  static_assert(4 * kPlane >= 4 * kGroups * (KS > 1 && kPart > kStage ? kPart : kStage),
+  static_assert(4 * kPlane >= 4 * KG * (KS > 1 && kPart > kStage ? kPart : kStage),
                 "partials and staging fit");
   const int bh = blockIdx.x;
   const int blk = gridDim.y - 1 - blockIdx.y;  // longest query blocks first
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform: scalar
-  const int grp = wave % kGroups, sub = wave / kGroups;
+  const int grp = wave % KG, sub = wave / KG;
   const size_t base = (size_t)bh * S * D;
-  const int q0 = blk * kRows + 32 * grp;  // the wave's first query
+  const int row0 = blk * 32 * KG;          // the workgroup's first query
+  const int q0 = row0 + 32 * grp;           // the wave's first query
   const int qi = q0 + l32;                // this lane's query
-  const int last = min(S, (blk + 1) * kRows) - 1;  // the workgroup's last query
-  const KeyTiles<WIN, TR> keys(blk * kRows, last, win);
+  const int last = min(S, row0 + 32 * KG) - 1;  // the workgroup's last query
+  const KeyTiles<WIN, TR> keys(row0, last, win);
   const int n_tiles = keys.count();
 
   X3 qb[D / 16];  // the lane's query row, split
@@ -431,14 +437,12 @@ __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_ker
 #pragma unroll
         for (int u = 1; u < 16; ++u) ps += w[u];
       };
-      weights(m);
       // The maximum moves only when a row's weights would reach 2^64 (or are inf/NaN: m is
       // -inf before a row's first chunk), compared on the bits (ps is +0, positive or NaN).
       // Both lane halves of a row take the row's decision, and only the rows that need it
       // move: the others rescale by exp(0) = 1 and recompute the same weights, so no row's
       // bits depend on another row.
-      const bool need = __float_as_uint(ps) >= __float_as_uint(kMaxW);
-      if (__builtin_amdgcn_ballot_w64(need) != 0) {  // wave-uniform
+      auto move = [&](bool need) {
         float cm = neg_inf();
 #pragma unroll
         for (int u = 0; u < 16; ++u)
@@ -453,6 +457,16 @@ __global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void fwd_f32_ker
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+      };
+      if constexpr (WIN) {
+        // with few chunks a row, the first one's weights are not tried against -inf
+        const bool none = m == neg_inf();
+        if (__builtin_amdgcn_ballot_w64(none) != 0) move(none);  // (wave-uniform)
+      }
+      weights(m);
+      const bool need = __float_as_uint(ps) >= __float_as_uint(kMaxW);
+      if (__builtin_amdgcn_ballot_w64(need) != 0) {  // wave-uniform
+        move(need);
         weights(m);
       }
       lh += ps;
@@ -563,12 +577,12 @@ struct F32BwdArgs {
   DropParams dr;
 };
 // LDS of a workgroup: the tiles, and per query row of a dK/dV tile lse and delta * scale.
-template <int D, int KS>
+template <int D, int KS, int KG = kGroups>
 struct F32BwdShared {
   __attribute__((aligned(16))) char tiles[BwdLds<D, KS>::kBytes];
   __attribute__((aligned(16))) float sl[32 * KS], sd[32 * KS];
   // dK/dV at D = 64: the lower planes of the groups' V rows, by lane
-  bf16x8 vlo[kGroups][D == 64 ? D / 16 : 1][2][64];
+  bf16x8 vlo[KG][D == 64 ? D / 16 : 1][2][64];
 };
 
 // delta of rows row0 .. S-1 into LDS, by the whole workgroup: D/4 lanes per row, one 16-byte
@@ -603,13 +617,17 @@ __device__ __forceinline__ void delta_rows(float* delta, const float* dout, cons
 struct F32WindowBwdArgs : Window {
   int piece_rows, pieces;
   float* partial;
-  __device__ __forceinline__ int block_end(int blk, int S) const {
-    if (pieces == 0 && blk * kRows < sinks) return S;
-    return min(S, ((blk + 1) * kRows + window - 2) / 64 * 64 + 64);
+  // of the block of `rows` keys from row0 on; where it holds sink keys, of the 128 keys around it
+  __device__ __forceinline__ int block_end(int row0, int rows, int S) const {
+    if (row0 < sinks) {
+      if (pieces == 0) return S;
+      row0 = row0 / kRows * kRows, rows = kRows;
+    }
+    return min(S, (row0 + rows + window - 2) / 64 * 64 + 64);
   }
-  // pieces of a block's later queries
-  __device__ __forceinline__ int far_pieces(int blk, int S) const {
-    return (S - block_end(blk, S) + piece_rows - 1) / max(piece_rows, 1);
+  // pieces of a sink key's later queries
+  __device__ __forceinline__ int far_pieces(int key, int S) const {
+    return (S - block_end(key, 1, S) + piece_rows - 1) / max(piece_rows, 1);
   }
 };
 template <bool WIN>
@@ -622,19 +640,19 @@ struct F32WindowBwdArg<true> : F32WindowBwdArgs {};
 // end with its last key's window (piece 0), and what later ones add to a block's sink keys is other
 // workgroups' (piece 1, 2, ..): their sums and the block's own sink rows go to the partials, which
 // window_join_f32_kernel adds up.
-template <int D, bool DROP, int KS, bool OWN_DELTA, bool WIN = false>
+template <int D, bool DROP, int KS, bool OWN_DELTA, bool WIN = false, int KG = kGroups>
 __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, int blk,
-                                                   F32BwdShared<D, KS>& sm, float* own_delta,
+                                                   F32BwdShared<D, KS, KG>& sm, float* own_delta,
                                                    const F32WindowBwdArg<WIN>& win = {},
                                                    int piece = 0) {
   // Q and dO tiles: planes and raw
   using Lds = BwdLds<D, KS>;
-  constexpr int TR = Lds::TR, NT = 64 * kGroups * KS;
+  constexpr int TR = Lds::TR, NT = 64 * KG * KS;
   char* smem = sm.tiles;
   bf16 *sqp = reinterpret_cast<bf16*>(smem), *sgp = sqp + Lds::kPlane;
   float* raw = reinterpret_cast<float*>(sgp + Lds::kPlane);
   constexpr int kSlot = Lds::slot_floats(2 * (D / 32));
-  static_assert(kGroups * kSlot * 4 <= Lds::kBytes, "partials and staging fit");
+  static_assert(KG * kSlot * 4 <= Lds::kBytes, "partials and staging fit");
   float *sl = sm.sl, *sd = sm.sd;
   const float *q = a.q, *k = a.k, *v = a.v, *dout = a.dout, *lse = a.lse, *delta = a.delta;
   float *dk = a.dk, *dv = a.dv;
@@ -643,14 +661,15 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
   const DropParams& dr = a.dr;
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform: scalar
-  const int grp = wave % kGroups, sub = wave / kGroups;
+  const int grp = wave % KG, sub = wave / KG;
   const size_t base = (size_t)bh * S * D;
-  const int k0 = blk * kRows + 32 * grp;  // the wave's first key
+  const int row0 = blk * 32 * KG;         // the workgroup's first key
+  const int k0 = row0 + 32 * grp;         // the wave's first key
   const int kj = k0 + l32;                // this lane's key
-  int t0 = (blk * kRows) / TR;  // first query tile with a query >= the first key
+  int t0 = row0 / TR;  // first query tile with a query >= the first key
   int n_tiles = (S + TR - 1) / TR;
   if constexpr (WIN) {
-    const int end = win.block_end(blk, S);
+    const int end = win.block_end(row0, 32 * KG, S);
     if (piece > 0) t0 = (end + (piece - 1) * win.piece_rows) / TR;
     n_tiles = (min(S, piece > 0 ? t0 * TR + win.piece_rows : end) + TR - 1) / TR;
     if (t0 >= n_tiles) return;
@@ -788,7 +807,7 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
     __builtin_amdgcn_wave_barrier();
   }
   if constexpr (WIN) {
-    if (k0 < win.sinks && win.block_end(blk, S) < S) {
+    if (k0 < win.sinks && win.block_end(row0, 32 * KG, S) < S) {
       const int rows = (win.sinks + 31) / 32 * 32;
       float* part = win.partial + ((size_t)bh * (win.pieces + 1) + piece) * 2 * rows * D;
       store_rows_t<D>(part, k0, rows, dka, 1.0f, slot, lane);
@@ -801,18 +820,18 @@ __device__ __forceinline__ void dkdv_f32_workgroup(const F32BwdArgs& a, int bh, 
 }
 
 // One workgroup's dQ. OWN_DELTA: delta of its rows is computed here and written; otherwise read.
-template <int D, bool DROP, int KS, bool OWN_DELTA, bool WIN = false>
+template <int D, bool DROP, int KS, bool OWN_DELTA, bool WIN = false, int KG = kGroups>
 __device__ __forceinline__ void dq_f32_workgroup(const F32BwdArgs& a, int bh, int blk,
-                                                 F32BwdShared<D, KS>& sm,
+                                                 F32BwdShared<D, KS, KG>& sm,
                                                  const WindowArg<WIN>& win = {}) {
   // K and V tiles: planes and raw
   using Lds = BwdLds<D, KS>;
-  constexpr int TR = Lds::TR, NT = 64 * kGroups * KS;
+  constexpr int TR = Lds::TR, NT = 64 * KG * KS;
   char* smem = sm.tiles;
   bf16 *skp = reinterpret_cast<bf16*>(smem), *svp = skp + Lds::kPlane;
   float* raw = reinterpret_cast<float*>(svp + Lds::kPlane);
   constexpr int kSlot = Lds::slot_floats(D / 32);
-  static_assert(kGroups * kSlot * 4 <= Lds::kBytes, "partials and staging fit");
+  static_assert(KG * kSlot * 4 <= Lds::kBytes, "partials and staging fit");
   const float *q = a.q, *k = a.k, *v = a.v, *dout = a.dout, *lse = a.lse;
   float *dq = a.dq, *delta = a.delta;
   const int S = a.S;
@@ -820,13 +839,14 @@ __device__ __forceinline__ void dq_f32_workgroup(const F32BwdArgs& a, int bh, in
   const DropParams& dr = a.dr;
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform: scalar
-  const int grp = wave % kGroups, sub = wave / kGroups;
+  const int grp = wave % KG, sub = wave / KG;
   const size_t base = (size_t)bh * S * D;
-  const int q0 = blk * kRows + 32 * grp;
+  const int row0 = blk * 32 * KG;
+  const int q0 = row0 + 32 * grp;
   const int qi = q0 + l32;
   const int qc = min(qi, S - 1);
-  const int last = min(S, (blk + 1) * kRows) - 1;
-  const KeyTiles<WIN, TR> keys(blk * kRows, last, win);
+  const int last = min(S, row0 + 32 * KG) - 1;
+  const KeyTiles<WIN, TR> keys(row0, last, win);
   const int n_tiles = keys.count();
 
   X3 qb[D / 16], gb[D / 16];  // the lane's Q and dO rows (score-product B layout), split
@@ -953,19 +973,20 @@ __global__ __launch_bounds__(64 * kGroups, wgs_per_cu(1)) void dq_f32_kernel(con
 // by piece: they are short), then dK/dV (`blocks` key blocks), then dQ, with delta computed where
 // it is needed (block windows up to kWindowDeltaRows rows) or by a pass before.
 constexpr int kWindowDeltaRows = 1024, kPieceRows = 256;
-template <int D, int KS, bool OWN_DELTA>
-__global__ __launch_bounds__(64 * kGroups * KS, wgs_per_cu(KS)) void window_bwd_f32_kernel(
+template <int D, int KS, int KG, bool OWN_DELTA>
+__global__ __launch_bounds__(64 * KG * KS, wgs_per_cu(KS, KG, D)) void window_bwd_f32_kernel(
     const F32BwdArgs a, const F32WindowBwdArg<true> win, int blocks, int sink_blocks) {
-  __shared__ F32BwdShared<D, KS> sm;
+  __shared__ F32BwdShared<D, KS, KG> sm;
   __shared__ float own_delta[OWN_DELTA ? kWindowDeltaRows : 1];
   const int y = blockIdx.y, far = win.pieces * sink_blocks;
   if (y < far + blocks) {
     const int piece = y < far ? y / sink_blocks + 1 : 0;
     const int blk = y < far ? y - (piece - 1) * sink_blocks : y - far;
-    dkdv_f32_workgroup<D, false, KS, OWN_DELTA, true>(a, blockIdx.x, blk, sm, own_delta, win,
-                                                      piece);
+    dkdv_f32_workgroup<D, false, KS, OWN_DELTA, true, KG>(a, blockIdx.x, blk, sm, own_delta, win,
+                                                          piece);
   } else {
-    dq_f32_workgroup<D, false, KS, OWN_DELTA, true>(a, blockIdx.x, y - far - blocks, sm, {win});
+    dq_f32_workgroup<D, false, KS, OWN_DELTA, true, KG>(a, blockIdx.x, y - far - blocks, sm,
+                                                        {win});
   }
 }
 
@@ -977,7 +998,7 @@ __global__ __launch_bounds__(256) void window_join_f32_kernel(const F32BwdArgs a
   const int i = blockIdx.y * 256 + threadIdx.x, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
   const int which = i / (D / 4) / win.sinks, bh = blockIdx.x;
   if (which > 1) return;
-  const int rows = (win.sinks + 31) / 32 * 32, far = win.far_pieces(row / kRows, a.S);
+  const int rows = (win.sinks + 31) / 32 * 32, far = win.far_pieces(row, a.S);
   if (far == 0) return;  // its workgroup has written the final row
   const float* p = win.partial + ((size_t)bh * (win.pieces + 1) * 2 + which) * rows * D +
                    (size_t)row * D + col;
@@ -1008,12 +1029,29 @@ int bwd_waves_per_group(int BH, int S) {
   return wgs <= (S > 96 ? cus : cus / 4) ? 2 : 1;
 }
 
-// With a window every workgroup's chain is about as long, so two waves per group pay only while
-// the workgroups, one per CU then, all start at once. One -> two, us: forward 24 x 777 (168
-// workgroups) 20.7 -> 17.8, 12 x 2048 (192) 48 -> 35, 48 x 1024 (384) 35 -> 48; backward 12 x 1024
-// (228) 48 -> 39, 24 x 777 (336) 22.6 -> 25.4, 12 x 2048 (384) 80 -> 95.
-int window_f32_waves_per_group(int S, long long wgs) {
-  return S > 96 && wgs <= device_cus() ? 2 : 1;
+// With a window a workgroup's chain is as long as its rows and the window together, so 64 rows by
+// two waves each (KG = 2, KS = 2) have the shortest, and are taken while all such workgroups start at
+// once; then 128 rows by two waves each while those do, one to a CU (at D = 64 only: at 32 a CU holds
+// the other two kinds as well); then one wave each. 41 / 42 / 22 for KG and KS, us: forward 24 x 777
+// x 32 with a window of 100 and 3 sinks (168 workgroups of 128 rows) 20.9 / 20.5 / 16.3, 24 x 2048 x
+// 32 of 256 (384) 31.4 / 30.9 / 26.3, 56 x 1024 x 32 of 128 (448) 24.3 / 26.0 / 28.2, 12 x 1024 x 64 of
+// 256 (96) 33.2 / 29.7 / 25.2, 24 x 777 x 64 of 100 27.7 / 25.6 / 34.2, 48 x 1024 x 64 of 64 29.5 /
+// 40.1 / 41.8; backward 64 x 256 x 32 of 32 (256 of both kinds) 21.1 / 17.7 / 17.0, 28 x 1024 x 32 of
+// 400 (448) 43.3 / 51.9 / 49.1, 8 x 1024 x 64 of 400 (128) 60.8 / 48.5 / 38.8, 16 x 1024 x 64 of 400
+// (256) 61.8 / 50.1 / 65.0, 20 x 1024 x 64 of 400 (320) 67.6 / 65.6 / 81.3.
+// f(KG, KS) for workgroups of `kinds` kinds for each 128 rows and `more` besides, times BH; `twos` is
+// how many workgroups of KG = KS = 2 a CU holds.
+template <int D, typename F>
+void with_window_f32_shape(int BH, int S, int kinds, int more, int twos, F f) {
+  const long long wgs = (long long)BH * (kinds * ((S + kRows - 1) / kRows) + more);
+  const int cus = device_cus();
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 2> two;
+  constexpr std::integral_constant<int, kGroups> all;
+  if (2 * wgs <= (long long)twos * cus) return f(two, two);
+  if constexpr (D == 64)
+    if (S > 96 && wgs <= cus) return f(all, two);
+  f(all, one);
 }
 
 // f(whether to drop, waves per row group) as compile-time constants.
@@ -1039,10 +1077,10 @@ hipError_t fwd_f32_t(float* out, float* lse, const float* q, const float* k, con
   const dim3 grid(BH, (S + kRows - 1) / kRows);
   const DropParams dr = drop_params(drop);
   if (window != nullptr) {
-    with_f32_shape(window_f32_waves_per_group(S, (long long)grid.x * grid.y), false,
-                   [&](auto, auto ks) {
-      fwd_f32_kernel<D, false, ks(), true, true>
-          <<<grid, 64 * kGroups * ks(), 0, stream>>>(out, lse, q, k, v, S, scale, dr, {*window});
+    with_window_f32_shape<D>(BH, S, 1, 0, D == 64 ? 1 : 3, [&](auto kg, auto ks) {
+      const dim3 blocks(BH, (S + 32 * kg() - 1) / (32 * kg()));
+      fwd_f32_kernel<D, false, ks(), true, true, kg()>
+          <<<blocks, 64 * kg() * ks(), 0, stream>>>(out, lse, q, k, v, S, scale, dr, {*window});
     });
     return hipGetLastError();
   }
@@ -1099,8 +1137,11 @@ hipError_t bwd_f32_t(float* dq, float* dk, float* dv, float* delta, const float*
 }
 
 // How a windowed backward is launched: the pieces of its sink keys' later queries, and the bytes
-// of their partials. No pieces where the later queries are few next to the window or in all
-// (short sequences: pieces and their join cost more than the sink blocks' longer chain).
+// of their partials. Small grids last as long as a sink block's chain, and pieces shorten it (24 x
+// 512 x 64 with a window of 100 46 -> 32 us, 24 x 777 x 32 of 400 57 -> 46, 12 x 300 x 32 of 64 17 ->
+// 15); in larger ones pieces and their join cost more than the chain where the later queries are
+// few next to the window or in all (192 x 500 x 64 of 64 113 -> 118, 192 x 1024 x 64 of 400 433 ->
+// 443).
 struct F32WindowPlan {
   int pieces;
   size_t workspace;
@@ -1109,7 +1150,8 @@ F32WindowPlan window_f32_plan(int BH, int S, int D, const Window& w) {
   const long long end = ((long long)kRows + w.window - 2) / 64 * 64 + 64;  // of block 0
   const long long far = S - end;
   F32WindowPlan p{0, 0};
-  if (w.sinks > 0 && far > 0 && (far > end || S > kWindowDeltaRows) && far > 384)
+  const bool small = (long long)BH * S <= 1 << 16 && far > 64;
+  if (w.sinks > 0 && (small || (far > 384 && (far > end || S > kWindowDeltaRows))))
     p.pieces = (int)((far + kPieceRows - 1) / kPieceRows);
   const size_t rows = (size_t)(w.sinks + 31) / 32 * 32;
   if (p.pieces > 0) p.workspace = sizeof(float) * BH * (size_t)(p.pieces + 1) * 2 * rows * D;
@@ -1119,7 +1161,7 @@ F32WindowPlan window_f32_plan(int BH, int S, int D, const Window& w) {
 template <int D>
 hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, float* partial,
                             size_t workspace_bytes, hipStream_t stream) {
-  const int S = args.S, blocks = (S + kRows - 1) / kRows;
+  const int S = args.S;
   const F32WindowPlan plan = window_f32_plan(BH, S, D, w);
   if (plan.workspace > workspace_bytes) return hipErrorInvalidValue;
   F32WindowBwdArg<true> win;
@@ -1127,7 +1169,6 @@ hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, flo
   win.piece_rows = kPieceRows;
   win.pieces = plan.pieces;
   win.partial = partial;
-  const int of = (w.sinks + kRows - 1) / kRows, sink_blocks = of < blocks ? of : blocks;
   // rows that a dK/dV workgroup may walk: all, or a block's window in whole 64s
   const bool own =
       S <= kWindowDeltaRows ||
@@ -1139,15 +1180,16 @@ hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, flo
         args.delta, args.dout, args.out, rows);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  const dim3 grid(BH, plan.pieces * sink_blocks + 2 * blocks);
-  with_f32_shape(window_f32_waves_per_group(S, (long long)grid.x * grid.y), false,
-                 [&](auto, auto ks) {
+  with_window_f32_shape<D>(BH, S, 2, plan.pieces, D == 64 ? 1 : 2, [&](auto kg, auto ks) {
+    constexpr int rows = 32 * kg(), threads = 64 * kg() * ks();
+    const int blocks = (S + rows - 1) / rows, sink_blocks = (w.sinks + rows - 1) / rows;
+    const dim3 grid(BH, plan.pieces * sink_blocks + 2 * blocks);
     if (own)
-      window_bwd_f32_kernel<D, ks(), true>
-          <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, sink_blocks);
+      window_bwd_f32_kernel<D, ks(), kg(), true>
+          <<<grid, threads, 0, stream>>>(args, win, blocks, sink_blocks);
     else
-      window_bwd_f32_kernel<D, ks(), false>
-          <<<grid, 64 * kGroups * ks(), 0, stream>>>(args, win, blocks, sink_blocks);
+      window_bwd_f32_kernel<D, ks(), kg(), false>
+          <<<grid, threads, 0, stream>>>(args, win, blocks, sink_blocks);
     e = hipGetLastError();
   });
   if (e != hipSuccess || plan.pieces == 0) return e;

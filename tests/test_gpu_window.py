@@ -42,6 +42,7 @@ CASES = [
     (300, 300, 32, 90, 4), (1, 1500, 64, 3, 130), (2, 2100, 64, 1000, 4), (1, 2300, 32, 900, 200),
     (1, 1800, 64, 17, 1024), (240, 1100, 64, 80, 4), (240, 1100, 32, 80, 4), (240, 1100, 64, 80, 0),
     (20, 2100, 64, 1000, 4), (20, 2100, 32, 1000, 0), (260, 200, 64, 33, 2), (24, 1024, 32, 200, 40),
+    (12, 1024, 64, 250, 4), (5, 2100, 64, 1000, 4), (6, 1300, 64, 40, 300),
 ]
 
 
