@@ -600,7 +600,7 @@ struct SelectLds {
   int hist[kSelBins];
   uint32_t cand_key[kSelRanked];  // a bin's keys, and their rows
   int cand_row[kSelRanked], cand_rank[kSelRanked];
-  int wave_sum[2][kSelWaves];
+  int wave_sum[kSelWaves];
   int n_cand, digit, left, in_bin;  // the pass's digit, the rank left below it, its bin's size
   uint32_t edge_key;
   int edge_row;
@@ -646,7 +646,49 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
         if (i < L) f(i, held[e]);
       }
     } else {
-      for (int i = tid; i < L; i += kSelThreads) f(i, w[i]);
+      for (int i0 = tid; i0 < L; i0 += kSelHeld * kSelThreads) {
+        float x[kSelHeld];  // in flight together
+#pragma unroll
+        for (int e = 0; e < kSelHeld; ++e) x[e] = w[min(i0 + e * kSelThreads, L - 1)];
+#pragma unroll
+        for (int e = 0; e < kSelHeld; ++e) {
+          const int i = i0 + e * kSelThreads;
+          if (i < L) f(i, x[e]);
+        }
+      }
+    }
+  };
+
+  // put(place, row, weight) for the rows that pick(row, weight) takes, in order: their places are
+  // counted in slabs of kSelHeld rows a thread. Within a slab every wave's loads are in before the
+  // first put, and a place is no later than its row, so put may write over the rows (in place).
+  auto in_order = [&](auto pick, auto put) {
+    int seen = 0;
+    for (int b0 = 0; b0 < L; b0 += kSelHeld * kSelThreads) {
+      float x[kSelHeld];
+#pragma unroll
+      for (int e = 0; e < kSelHeld; ++e)
+        x[e] = HELD ? held[HELD ? e : 0] : w[min(b0 + e * kSelThreads + tid, L - 1)];
+      unsigned long long m[kSelHeld];
+      __syncthreads();  // (hist holds the waves' counts now)
+#pragma unroll
+      for (int e = 0; e < kSelHeld; ++e) {
+        const int i = b0 + e * kSelThreads + tid;
+        m[e] = __ballot(i < L && pick(i, x[e]));
+        if (lane == 0) sm.hist[e * kSelWaves + wave] = __popcll(m[e]);
+      }
+      wait_loads();
+      __syncthreads();
+      static_assert(kSelHeld * kSelWaves == 64, "a lane for each slab and wave");
+      const int n = sm.hist[lane], before = seen + wave_scan(n) - n;
+#pragma unroll
+      for (int e = 0; e < kSelHeld; ++e) {
+        const int at = __shfl(before, e * kSelWaves + wave, 64) +
+                       __popcll(m[e] & ((1ull << lane) - 1));
+        if ((m[e] >> lane) & 1) put(at, b0 + e * kSelThreads + tid, x[e]);
+      }
+      if constexpr (HELD) break;  // (one slab)
+      seen = __shfl(before + n, 63, 64);
     }
   };
 
@@ -674,11 +716,11 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum += c[e] = sm.hist[kSelBins - 1 - (4 * tid + e)];
       const int inc = wave_scan(sum);
-      if (lane == 63) sm.wave_sum[0][wave] = inc;
+      if (lane == 63) sm.wave_sum[wave] = inc;
       __syncthreads();
       int above = inc - sum;
 #pragma unroll
-      for (int v = 0; v < kSelWaves; ++v) above += v < wave ? sm.wave_sum[0][v] : 0;
+      for (int v = 0; v < kSelWaves; ++v) above += v < wave ? sm.wave_sum[v] : 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (above <= rank && rank < above + c[e]) {  // one thread, one bin
@@ -740,22 +782,10 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
       }
       if (shift == 0) {  // more than kSelRanked rows of one weight: the one of that rank, in order
         edge_key = prefix;
-        int seen = 0;
-        for (int t0 = 0; t0 < L; t0 += kSelThreads) {  // (every thread sees the same counts)
-          const int i = t0 + tid;
-          const bool tie = i >= first && i < last && order_key(w[min(i, L - 1)]) == edge_key;
-          const unsigned long long m = __ballot(tie);
-          if (lane == 0) sm.wave_sum[(t0 / kSelThreads) & 1][wave] = __popcll(m);
-          __syncthreads();
-          int at = seen + __popcll(m & ((1ull << lane) - 1));
-#pragma unroll
-          for (int v = 0; v < kSelWaves; ++v) {
-            const int n = sm.wave_sum[(t0 / kSelThreads) & 1][v];
-            at += v < wave ? n : 0;
-            seen += n;
-          }
-          if (tie && at == rank) sm.edge_row = i;
-        }
+        in_order([&](int i, float x) { return i >= first && i < last && order_key(x) == prefix; },
+                 [&](int at, int i, float) {
+                   if (at == rank) sm.edge_row = i;
+                 });
         __syncthreads();
         edge_row = sm.edge_row;
         break;
@@ -767,53 +797,12 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     const uint32_t k = order_key(x);
     return k > edge_key || (k == edge_key && i < edge_row);
   };
-  // in slabs of a row a thread: a row's place is the count of those that stay before it
-  if constexpr (HELD) {
-    unsigned long long m[kSelHeld];
-    __syncthreads();  // (hist holds the slabs' wave counts now)
-#pragma unroll
-    for (int e = 0; e < kSelHeld; ++e) {
-      const int i = e * kSelThreads + tid;
-      m[e] = __ballot(i < L && stays(i, held[e]));
-      if (lane == 0) sm.hist[e * kSelWaves + wave] = __popcll(m[e]);
+  in_order(stays, [&](int at, int i, float x) {
+    if (at < keep) {  // (never past it: `keep` rows stay)
+      kp[at] = i;
+      wo[at] = x;
     }
-    wait_loads();  // in place, other waves write over rows that this one has loaded
-    __syncthreads();
-    static_assert(kSelHeld * kSelWaves == 64, "a lane for each slab and wave");
-    const int n = sm.hist[lane], before = wave_scan(n) - n;
-#pragma unroll
-    for (int e = 0; e < kSelHeld; ++e) {
-      const int at = __shfl(before, e * kSelWaves + wave, 64) +
-                     __popcll(m[e] & ((1ull << lane) - 1));
-      if (((m[e] >> lane) & 1) && at < keep) {  // (never past it: `keep` rows stay)
-        kp[at] = e * kSelThreads + tid;
-        wo[at] = held[e];
-      }
-    }
-  } else {
-    int seen = 0;
-    for (int t0 = 0; t0 < L; t0 += kSelThreads) {
-      const int i = t0 + tid;
-      const float x = w[min(i, L - 1)];
-      const bool s = i < L && stays(i, x);
-      const unsigned long long m = __ballot(s);
-      int* sums = sm.wave_sum[(t0 / kSelThreads) & 1];
-      __syncthreads();
-      if (lane == 0) sums[wave] = __popcll(m);
-      wait_loads();  // as above: at most the slab's own rows are written over, at <= i
-      __syncthreads();
-      int at = seen + __popcll(m & ((1ull << lane) - 1));
-#pragma unroll
-      for (int v = 0; v < kSelWaves; ++v) {
-        at += v < wave ? sums[v] : 0;
-        seen += sums[v];
-      }
-      if (s && at < keep) {
-        kp[at] = i;
-        wo[at] = x;
-      }
-    }
-  }
+  });
 }
 
 // Rows by `kept`, 16 bytes a lane, in a grid over rows: into another cache.
