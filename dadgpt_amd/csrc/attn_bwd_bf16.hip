@@ -1043,9 +1043,15 @@ WindowPlan window_plan(int BH, int S, int D, const Window& w) {
   p.waves_per_group = window_waves_per_group(BH, S, p.one ? 2 : 1);
   const long long far = tiles - end(32 * kWaves / p.waves_per_group);
   if (p.one || w.sinks == 0 || far <= 0) return p;
-  // pieces of even lengths up to 12 tiles (six rounds; of four tiles, B16 H12 T1024 with a window of
-  // 256 takes dQ 56 for 51 us)
-  p.pieces = (int)((far + kMaxPieceTiles - 1) / kMaxPieceTiles);
+  // Pieces of even lengths up to 12 tiles (of four, B16 H12 T1024 with a window of 256 takes dQ 56
+  // for 51 us). Small grids wait for a piece's tiles and for the blocks that add up the partials one
+  // after the other, so there as many tiles as partials, about (12 -> up to sqrt(far), backward, us:
+  // 32 x 799, window 10 24.1 -> 18.5, 12 x 1024, 256 25.0 -> 19.6, 16 x 710, 4 20.0 -> 15.8; but 48 x
+  // 1024, 128 28.5 -> 32.3, 96 x 1024, 128 39.4 -> 42.1).
+  int most = kMaxPieceTiles;
+  if ((long long)BH * S <= 1 << 15)
+    for (most = 4; most < kMaxPieceTiles && most * most < far;) ++most;
+  p.pieces = (int)((far + most - 1) / most);
   p.piece_tiles = (int)((far + p.pieces - 1) / p.pieces);
   p.workspace = sizeof(float) * BH * (size_t)p.pieces * 2 * ((w.sinks + 31) / 32 * 32) * D;
   return p;
