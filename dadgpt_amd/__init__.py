@@ -1,9 +1,9 @@
 """MI355X-native (gfx950) fused causal attention for DadGPT.
 
 The work happens in ``lib/libdadgpt_attn.so`` (hand-written HIP kernels behind the C ABI of
-``include/dadgpt/gpu_attention.h``) and ``lib/libdadgpt_gen.so`` (hipBLASLt GEMMs, the
-materialized attention path and batched GPT-2 generation); ``attention`` and ``gpt2`` are their
-Python mirrors over ctypes.
+``include/dadgpt/gpu_attention.h`` and ``include/dadgpt/kv_cache.h``) and
+``lib/libdadgpt_gen.so`` (hipBLASLt GEMMs, the materialized attention path and batched GPT-2
+generation); ``attention``, ``kv_cache`` and ``gpt2`` are their Python mirrors over ctypes.
 
 Import this package before ``torch``. Both use the HIP runtime, and both use a hipBLASLt:
 PyTorch's ROCm wheel bundles its own (older) hipBLASLt and rocRoller, under the same sonames as
@@ -51,6 +51,6 @@ def _load_native_stack() -> None:
 
 _load_native_stack()
 
-from . import attention  # noqa: E402,F401
+from . import attention, kv_cache  # noqa: E402,F401
 
-__all__ = ["attention", "load_error"]
+__all__ = ["attention", "kv_cache", "load_error"]

@@ -195,7 +195,8 @@ def kv_evict(k_out, v_out, weights_out, kept, lens_out, k, v, weights, lens, n_s
     `budget` rows: its first `sinks`, its last `recent`, and between them those of the largest
     weights, in order, into a cache of max_out rows or (k_out is k, v_out is v) in place. kept
     [n_seq, n_heads, budget] int32 receives the rows' former indices (-1 past the end), lens_out
-    min(lens, budget) (lens_out may be lens)."""
+    min(lens, budget) (lens_out may be lens). weights_out from lens_out on is left as it was: set a
+    row's weight to 0 when a row is appended there."""
     fn = _by_dtype("dadgpt_kv_evict", k.dtype)
     rows = n_seq * n_heads
     po, pp = _ptrs(k.dtype, rows * max_out * d_head, (k_out, v_out), ("k_out", "v_out"))

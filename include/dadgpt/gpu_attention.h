@@ -46,7 +46,7 @@ typedef enum dadgpt_status {
   DADGPT_ERR_INVALID_ARGUMENT = 1, /* null pointer, non-positive size, bad scale */
   DADGPT_ERR_UNSUPPORTED = 2,      /* d_head outside the supported set */
   DADGPT_ERR_HIP = 3,              /* a HIP launch reported an error */
-  DADGPT_ERR_WORKSPACE = 4         /* decode workspace missing or too small */
+  DADGPT_ERR_WORKSPACE = 4         /* workspace missing or too small */
 } dadgpt_status;
 
 /* Message of the last failing call on this thread ("" if none). */

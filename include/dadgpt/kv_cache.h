@@ -79,10 +79,11 @@ int dadgpt_decode_attention_kv8_f32(float* out, const float* q, const uint8_t* k
 
 /* The decode of dadgpt_decode_attention_{bf16,f32}, which also accumulates every key's attention
  * probability: weights_out[s][h][j] = weights[s][h][j] + p_j for j < lens[s], and weights[s][h][j]
- * from there on. weights and weights_out are fp32 [n_seq, n_heads, max_len], 4-byte aligned, and
- * may be one buffer; otherwise they must not overlap. The workspace
- * (dadgpt_decode_weights_workspace_bytes, 0: NULL allowed) needs no initial contents and holds
- * nothing between calls; calls that overlap in time need one each. */
+ * from there on. The caller sets a row's weight (to 0) when it appends the row. weights and
+ * weights_out are fp32 [n_seq, n_heads, max_len], 4-byte aligned, and may be one buffer; otherwise
+ * they must not overlap. The workspace (dadgpt_decode_weights_workspace_bytes, 0: NULL allowed)
+ * needs no initial contents and holds nothing between calls; calls that overlap in time need one
+ * each. */
 size_t dadgpt_decode_weights_workspace_bytes(int n_seq, int n_heads, int max_len, int d_head);
 int dadgpt_decode_attention_weights_bf16(uint16_t* out, float* weights_out, const uint16_t* q,
                                          const uint16_t* k_cache, const uint16_t* v_cache,
@@ -102,7 +103,8 @@ int dadgpt_decode_attention_weights_f32(float* out, float* weights_out, const fl
  * cache is row kept[s][h][r] of the input, r < lens_out[s] = min(lens[s], budget).
  *   k_out, v_out  [n_seq, n_heads, max_out, d_head], max_out >= min(budget, max_len); rows from
  *                 lens_out on are left as they were
- *   weights_out   [n_seq, n_heads, max_out] fp32, 4-byte aligned
+ *   weights_out   [n_seq, n_heads, max_out] fp32, 4-byte aligned; from lens_out on left as they
+ *                 were: a row that is appended there later needs its weight set (to 0)
  *   kept          int32 [n_seq, n_heads, budget], 4-byte aligned; -1 from lens_out on
  *   lens_out      int32 [n_seq], 4-byte aligned; may be lens
  * In place: k_out = k and v_out = v together, with max_out = max_len; weights_out may be weights
