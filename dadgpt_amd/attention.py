@@ -575,6 +575,7 @@ def flash_attention_window_forward_bf16_tokens(out, ld_out: int, lse, q, k, v, l
                                                B: int, H: int, S: int, d_head: int, scale: float,
                                                window: int, sinks: int = 0, stream=None) -> None:
     """Token-major windowed forward (see flash_attention_forward_bf16_tokens)."""
+    _same_device((out, lse, q, k, v))
     _check(lib().dadgpt_flash_attention_window_forward_bf16_tokens(
         _ptr(out), ld_out, _ptr(lse), _ptr(q), _ptr(k), _ptr(v), ld_qkv, B, H, S, d_head, scale,
         window, sinks, _stream_ptr(stream)))
@@ -586,6 +587,7 @@ def flash_attention_window_backward_bf16_tokens(dq, dk, dv, ld_dqkv: int, delta,
                                                 window: int, sinks: int = 0, workspace=None,
                                                 stream=None) -> None:
     """Token-major windowed backward (see flash_attention_backward_bf16_tokens)."""
+    _same_device((dq, dk, dv, delta, dout, out, lse, q, k, v, workspace))
     _check(lib().dadgpt_flash_attention_window_backward_bf16_tokens(
         _ptr(dq), _ptr(dk), _ptr(dv), ld_dqkv, _ptr(delta), _ptr(dout), _ptr(out), ld_out,
         _ptr(lse), _ptr(q), _ptr(k), _ptr(v), ld_qkv, B, H, S, d_head, scale, window, sinks,

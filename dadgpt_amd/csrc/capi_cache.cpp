@@ -173,9 +173,9 @@ int evict(const char* fn, void* k_out, void* v_out, float* wout, int32_t* kept,
     return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: n_seq=%d x n_heads=%d exceeds the launch limits",
                 fn, n_seq, H);
   const int most = budget < max_len ? budget : max_len;
-  if (max_out < most || max_out > 65535L * 256 || most > 65535L * 64)
+  if (max_out < most || max_out > 65535L * 256 || most > 65535L * 64 || budget > 65535L * 256)
     return fail(DADGPT_ERR_INVALID_ARGUMENT,
-                "%s: max_out=%d cannot hold budget=%d of max_len=%d rows, or exceeds the launch "
+                "%s: max_out=%d cannot hold budget=%d of max_len=%d rows, or one exceeds the launch "
                 "limits",
                 fn, max_out, budget, max_len);
   const bool in_place = k_out == k || v_out == v;

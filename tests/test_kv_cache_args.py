@@ -139,6 +139,8 @@ def test_evict_validation(name, size):
     for kw in ({"budget": 0}, {"sinks": -1}, {"recent": -1}, {"sinks": 60}, {"out": 63}, {"n": 0},
                {"L": 0}, {"n": 1 << 21, "h": 2}, {"sinks": 2 ** 31 - 1, "recent": 2 ** 31 - 1}):
         assert call(**kw) == 1, kw
+    # a budget far past any cache: row numbers are counted in 32 bits in steps of a workgroup
+    assert call(budget=2 ** 31 - 1, out=200) == 1 and "launch limits" in A.last_error()
     # in place: both tensors, and caches of one length
     p = _ptrs(9)
     p[0] = p[5]
