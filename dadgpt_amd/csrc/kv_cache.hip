@@ -566,9 +566,8 @@ hipError_t launch_weights_decode_d(T* out, float* wout, const T* q, const T* kc,
 
 // ------------------------------------------------------------------------ eviction
 
-constexpr int kSelThreads = 512, kSelWaves = kSelThreads / 64;
 constexpr int kSelHeld = 8;  // keys a thread holds; longer rows are read again for each pass
-constexpr int kSelRanked = kSelThreads;  // candidates ranked against each other: one a thread at most
+constexpr int kSelRanked = 512;  // candidates ranked against each other: one a thread at most
 // Radix passes from the top: 11, 11 and 10 bits.
 constexpr int kSelBins = 2048;
 
@@ -600,7 +599,7 @@ struct SelectLds {
   int hist[kSelBins];
   uint32_t cand_key[kSelRanked];  // a bin's keys, and their rows
   int cand_row[kSelRanked], cand_rank[kSelRanked];
-  int wave_sum[kSelWaves];
+  int wave_sum[16];
   int n_cand, digit, left, in_bin;  // the pass's digit, the rank left below it, its bin's size
   uint32_t edge_key;
   int edge_row;
@@ -613,11 +612,13 @@ struct SelectLds {
 // kSelRanked rows (mostly after one pass), these are ranked against each other; if the bits run out
 // first, the edge is among rows of one weight, and its row is found by counting them in order.
 // Then the indices that stay, in order, and their weights. HELD: a thread holds its keys (row
-// e * kSelThreads + t); else each pass reads the row again (from the caches).
-template <bool HELD>
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
+// e * NT + t); else each pass reads the row again (from the caches).
+template <int NT, bool HELD>
+__global__ __launch_bounds__(NT) void evict_select_kernel(
     int* __restrict__ kept, float* wout, const float* weights, const int* __restrict__ lens, int H,
     int max_len, int max_out, int budget, int sinks, int recent) {
+  constexpr int NW = NT / 64;
+  static_assert(NT >= kSelRanked && NW <= 16 && kSelBins % NT == 0);
   __shared__ SelectLds sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.x / H;
   const long long hrow = blockIdx.x;
@@ -626,14 +627,14 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   int* kp = kept + hrow * budget;
   float* wo = wout + hrow * max_out;
   const int keep = min(L, budget);
-  for (int i = keep + tid; i < budget; i += kSelThreads) kp[i] = -1;
+  for (int i = keep + tid; i < budget; i += NT) kp[i] = -1;
 
   const int first = min(sinks, L), last = max(first, L - recent);
   float held[HELD ? kSelHeld : 1];
   if constexpr (HELD) {
 #pragma unroll
     for (int e = 0; e < kSelHeld; ++e) {
-      const int i = e * kSelThreads + tid;
+      const int i = e * NT + tid;
       held[e] = i < L ? w[i] : 0.f;
     }
   }
@@ -642,17 +643,17 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     if constexpr (HELD) {
 #pragma unroll
       for (int e = 0; e < kSelHeld; ++e) {
-        const int i = e * kSelThreads + tid;
+        const int i = e * NT + tid;
         if (i < L) f(i, held[e]);
       }
     } else {
-      for (int i0 = tid; i0 < L; i0 += kSelHeld * kSelThreads) {
+      for (int i0 = tid; i0 < L; i0 += kSelHeld * NT) {
         float x[kSelHeld];  // in flight together
 #pragma unroll
-        for (int e = 0; e < kSelHeld; ++e) x[e] = w[min(i0 + e * kSelThreads, L - 1)];
+        for (int e = 0; e < kSelHeld; ++e) x[e] = w[min(i0 + e * NT, L - 1)];
 #pragma unroll
         for (int e = 0; e < kSelHeld; ++e) {
-          const int i = i0 + e * kSelThreads;
+          const int i = i0 + e * NT;
           if (i < L) f(i, x[e]);
         }
       }
@@ -664,28 +665,31 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   // first put, and a place is no later than its row, so put may write over the rows (in place).
   auto in_order = [&](auto pick, auto put) {
     int seen = 0;
-    for (int b0 = 0; b0 < L; b0 += kSelHeld * kSelThreads) {
+    for (int b0 = 0; b0 < L; b0 += kSelHeld * NT) {
       float x[kSelHeld];
 #pragma unroll
       for (int e = 0; e < kSelHeld; ++e)
-        x[e] = HELD ? held[HELD ? e : 0] : w[min(b0 + e * kSelThreads + tid, L - 1)];
+        x[e] = HELD ? held[HELD ? e : 0] : w[min(b0 + e * NT + tid, L - 1)];
       unsigned long long m[kSelHeld];
       __syncthreads();  // (hist holds the waves' counts now)
 #pragma unroll
       for (int e = 0; e < kSelHeld; ++e) {
-        const int i = b0 + e * kSelThreads + tid;
+        const int i = b0 + e * NT + tid;
         m[e] = __ballot(i < L && pick(i, x[e]));
-        if (lane == 0) sm.hist[e * kSelWaves + wave] = __popcll(m[e]);
+        if (lane == 0) sm.hist[e * NW + wave] = __popcll(m[e]);
       }
       wait_loads();
       __syncthreads();
-      static_assert(kSelHeld * kSelWaves == 64, "a lane for each slab and wave");
-      const int n = sm.hist[lane], before = seen + wave_scan(n) - n;
+      constexpr int PER = kSelHeld * NW / 64;  // of the slabs' waves' counts, a lane
+      static_assert(PER == 1 || PER == 2);
+      const int n0 = sm.hist[PER * lane], n = PER == 2 ? n0 + sm.hist[PER * lane + 1] : n0;
+      const int before = seen + wave_scan(n) - n;
 #pragma unroll
       for (int e = 0; e < kSelHeld; ++e) {
-        const int at = __shfl(before, e * kSelWaves + wave, 64) +
-                       __popcll(m[e] & ((1ull << lane) - 1));
-        if ((m[e] >> lane) & 1) put(at, b0 + e * kSelThreads + tid, x[e]);
+        const int c = e * NW + wave;
+        int at = __shfl(before, c / PER, 64) + __popcll(m[e] & ((1ull << lane) - 1));
+        if (PER == 2 && (wave & 1)) at += __shfl(n0, c / PER, 64);
+        if ((m[e] >> lane) & 1) put(at, b0 + e * NT + tid, x[e]);
       }
       if constexpr (HELD) break;  // (one slab)
       seen = __shfl(before + n, 63, 64);
@@ -701,7 +705,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     while (true) {
       const int bits = shift == 10 ? 10 : 11;
       shift -= bits;
-      for (int i = tid; i < kSelBins; i += kSelThreads) sm.hist[i] = 0;
+      for (int i = tid; i < kSelBins; i += NT) sm.hist[i] = 0;
       if (tid == 0) sm.n_cand = 0;
       __syncthreads();
       rows([&](int i, float x) {
@@ -710,21 +714,22 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
           atomicAdd(&sm.hist[(k >> shift) & ((1u << bits) - 1)], 1);
       });
       __syncthreads();
-      // the digit whose rows, counted from the largest down, hold the row of that rank: four bins
+      // the digit whose rows, counted from the largest down, hold the row of that rank: BINS bins
       // a thread, the highest first
-      int c[4], sum = 0;
+      constexpr int BINS = kSelBins / NT;
+      int c[BINS], sum = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum += c[e] = sm.hist[kSelBins - 1 - (4 * tid + e)];
+      for (int e = 0; e < BINS; ++e) sum += c[e] = sm.hist[kSelBins - 1 - (BINS * tid + e)];
       const int inc = wave_scan(sum);
       if (lane == 63) sm.wave_sum[wave] = inc;
       __syncthreads();
       int above = inc - sum;
 #pragma unroll
-      for (int v = 0; v < kSelWaves; ++v) above += v < wave ? sm.wave_sum[v] : 0;
+      for (int v = 0; v < NW; ++v) above += v < wave ? sm.wave_sum[v] : 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < BINS; ++e) {
         if (above <= rank && rank < above + c[e]) {  // one thread, one bin
-          sm.digit = kSelBins - 1 - (4 * tid + e);
+          sm.digit = kSelBins - 1 - (BINS * tid + e);
           sm.left = rank - above;
           sm.in_bin = c[e];
         }
@@ -744,7 +749,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
           }
         });
         __syncthreads();
-        // a wave takes every kSelWaves-th candidate, a lane compares it with one of 64 others (a
+        // a wave takes every NW-th candidate, a lane compares it with one of 64 others (a
         // lane a candidate, walking the others in LDS, took 7k cycles for 30 of them: 18.5 us for
         // the 32 x 12 rows of 2048 that take 10 us now)
         for (int j0 = 0, most = (in_bin + 63) / 64 * 64; j0 < most; j0 += 64) {
@@ -752,18 +757,18 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
           const uint32_t kj = j < in_bin ? sm.cand_key[j] : 0u;
           const int rj = j < in_bin ? sm.cand_row[j] : max_len;
           constexpr int N = 4;  // candidates whose LDS reads are in flight together
-          for (int i = wave; i < in_bin; i += N * kSelWaves) {
+          for (int i = wave; i < in_bin; i += N * NW) {
             uint32_t k[N];
             int row[N];
 #pragma unroll
             for (int u = 0; u < N; ++u) {
-              const int at = min(i + u * kSelWaves, in_bin - 1);
+              const int at = min(i + u * NW, in_bin - 1);
               k[u] = sm.cand_key[at];
               row[u] = sm.cand_row[at];
             }
 #pragma unroll
             for (int u = 0; u < N; ++u) {
-              const int at = i + u * kSelWaves;
+              const int at = i + u * NW;
               const int before = __popcll(__ballot(kj > k[u] || (kj == k[u] && rj < row[u])));
               if (lane == 0 && at < in_bin)
                 sm.cand_rank[at] = j0 == 0 ? before : sm.cand_rank[at] + before;
@@ -967,12 +972,21 @@ hipError_t launch_kv_evict(void* k_out, void* v_out, float* wout, int* kept, int
                            int sinks, int recent, hipStream_t stream) {
   const unsigned rows = (unsigned)(n_seq * H);
   const int row_log2 = __builtin_ctz((unsigned)row_bytes);
-  if (max_len <= kSelHeld * kSelThreads)
-    evict_select_kernel<true><<<rows, kSelThreads, 0, stream>>>(
+  auto select = [&](auto threads, auto held) {
+    evict_select_kernel<threads(), held()><<<rows, threads(), 0, stream>>>(
         kept, wout, weights, lens, H, max_len, max_out, budget, sinks, recent);
+  };
+  // 16 waves for long caches: up to 8192 rows stay in registers, and a pass over more reads half as
+  // often (2 x 3 caches of 8192 rows 39.6 -> 26.2 us, 1 x 12 of 32768 44.9 -> 35.0); from 2048 rows on
+  // while every workgroup has a CU to itself (8 x 12 caches of 4096 29.2 -> 23.8, 32 x 12 46.6 -> 51.7).
+  constexpr std::integral_constant<int, 512> half;
+  constexpr std::integral_constant<int, 1024> full;
+  if (max_len <= kSelHeld * half() && (max_len <= 2048 || rows > (unsigned)device_cus()))
+    select(half, std::true_type{});
+  else if (max_len <= kSelHeld * full())
+    select(full, std::true_type{});
   else
-    evict_select_kernel<false><<<rows, kSelThreads, 0, stream>>>(
-        kept, wout, weights, lens, H, max_len, max_out, budget, sinks, recent);
+    select(full, std::false_type{});
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (k_out == k) {
     evict_in_place_kernel<<<dim3(rows, 1, 2), kInPlaceThreads, 0, stream>>>(
