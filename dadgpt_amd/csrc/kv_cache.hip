@@ -567,7 +567,7 @@ hipError_t launch_weights_decode_d(T* out, float* wout, const T* q, const T* kc,
 // ------------------------------------------------------------------------ eviction
 
 constexpr int kSelHeld = 8;  // keys a thread holds; longer rows are read again for each pass
-constexpr int kSelRanked = 512;  // candidates ranked against each other: one a thread at most
+constexpr int kSelRanked = 512;  // candidates ranked against each other
 // Radix passes from the top: 11, 11 and 10 bits.
 constexpr int kSelBins = 2048;
 
@@ -598,7 +598,7 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)"
 struct SelectLds {
   int hist[kSelBins];
   uint32_t cand_key[kSelRanked];  // a bin's keys, and their rows
-  int cand_row[kSelRanked], cand_rank[kSelRanked];
+  int cand_row[kSelRanked];
   int wave_sum[16];
   int n_cand, digit, left, in_bin;  // the pass's digit, the rank left below it, its bin's size
   uint32_t edge_key;
@@ -618,7 +618,7 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
     int* __restrict__ kept, float* wout, const float* weights, const int* __restrict__ lens, int H,
     int max_len, int max_out, int budget, int sinks, int recent) {
   constexpr int NW = NT / 64;
-  static_assert(NT >= kSelRanked && NW <= 16 && kSelBins % NT == 0);
+  static_assert(NW <= 16 && kSelBins % NT == 0);
   __shared__ SelectLds sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.x / H;
   const long long hrow = blockIdx.x;
@@ -749,36 +749,41 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
           }
         });
         __syncthreads();
-        // a wave takes every NW-th candidate, a lane compares it with one of 64 others (a
-        // lane a candidate, walking the others in LDS, took 7k cycles for 30 of them: 18.5 us for
-        // the 32 x 12 rows of 2048 that take 10 us now)
-        for (int j0 = 0, most = (in_bin + 63) / 64 * 64; j0 < most; j0 += 64) {
-          const int j = j0 + lane;
-          const uint32_t kj = j < in_bin ? sm.cand_key[j] : 0u;
-          const int rj = j < in_bin ? sm.cand_row[j] : max_len;
-          constexpr int N = 4;  // candidates whose LDS reads are in flight together
-          for (int i = wave; i < in_bin; i += N * NW) {
-            uint32_t k[N];
-            int row[N];
+        // a wave takes every NW-th candidate, and its lanes compare the candidate with the others, in
+        // registers, 64 at a time (a lane a candidate, walking the others in LDS, took 7k cycles for
+        // 30 of them: 18.5 us for the 32 x 12 rows of 2048 that take 10 us now)
+        uint32_t kj[kSelRanked / 64];
+        int rj[kSelRanked / 64];
 #pragma unroll
-            for (int u = 0; u < N; ++u) {
-              const int at = min(i + u * NW, in_bin - 1);
-              k[u] = sm.cand_key[at];
-              row[u] = sm.cand_row[at];
-            }
-#pragma unroll
-            for (int u = 0; u < N; ++u) {
-              const int at = i + u * NW;
-              const int before = __popcll(__ballot(kj > k[u] || (kj == k[u] && rj < row[u])));
-              if (lane == 0 && at < in_bin)
-                sm.cand_rank[at] = j0 == 0 ? before : sm.cand_rank[at] + before;
-            }
-          }
+        for (int b = 0; b < kSelRanked / 64; ++b) {
+          kj[b] = 0u, rj[b] = max_len;
+          if (64 * b >= in_bin) break;
+          const int j = 64 * b + lane;
+          if (j < in_bin) kj[b] = sm.cand_key[j], rj[b] = sm.cand_row[j];
         }
-        __syncthreads();
-        if (tid < in_bin && sm.cand_rank[tid] == rank) {
-          sm.edge_key = sm.cand_key[tid];
-          sm.edge_row = sm.cand_row[tid];
+        constexpr int N = 4;  // candidates whose LDS reads are in flight together
+        for (int i = wave; i < in_bin; i += N * NW) {
+          uint32_t k[N];
+          int row[N], before[N] = {};
+#pragma unroll
+          for (int u = 0; u < N; ++u) {
+            const int at = min(i + u * NW, in_bin - 1);
+            k[u] = sm.cand_key[at];
+            row[u] = sm.cand_row[at];
+          }
+#pragma unroll
+          for (int b = 0; b < kSelRanked / 64; ++b) {
+            if (64 * b >= in_bin) break;
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+              before[u] += __popcll(__ballot(kj[b] > k[u] || (kj[b] == k[u] && rj[b] < row[u])));
+          }
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+            if (before[u] == rank && i + u * NW < in_bin && lane == 0) {
+              sm.edge_key = k[u];
+              sm.edge_row = row[u];
+            }
         }
         __syncthreads();
         edge_key = sm.edge_key;
@@ -976,17 +981,21 @@ hipError_t launch_kv_evict(void* k_out, void* v_out, float* wout, int* kept, int
     evict_select_kernel<threads(), held()><<<rows, threads(), 0, stream>>>(
         kept, wout, weights, lens, H, max_len, max_out, budget, sinks, recent);
   };
-  // 16 waves for long caches: up to 8192 rows stay in registers, and a pass over more reads half as
-  // often (2 x 3 caches of 8192 rows 39.6 -> 26.2 us, 1 x 12 of 32768 44.9 -> 35.0); from 2048 rows on
-  // while every workgroup has a CU to itself (8 x 12 caches of 4096 29.2 -> 23.8, 32 x 12 46.6 -> 51.7).
+  // 16 waves for long caches, up to 8192 rows in registers, while every workgroup has a CU to itself (8
+  // -> 16: 8 x 12 caches of 4096 rows 21.0 -> 20.4 us, 2 x 3 of 8192 25.4 -> 20.6, 1 x 12 of 32768 46.1
+  // -> 35.0; but 32 x 12 of 4096 39.7 -> 45.3, 64 x 12 of 8192 82.1 -> 94.3).
   constexpr std::integral_constant<int, 512> half;
   constexpr std::integral_constant<int, 1024> full;
-  if (max_len <= kSelHeld * half() && (max_len <= 2048 || rows > (unsigned)device_cus()))
-    select(half, std::true_type{});
-  else if (max_len <= kSelHeld * full())
-    select(full, std::true_type{});
+  auto select_by = [&](auto threads) {
+    if (max_len <= kSelHeld * threads())
+      select(threads, std::true_type{});
+    else
+      select(threads, std::false_type{});
+  };
+  if (max_len > 2048 && rows <= (unsigned)device_cus())
+    select_by(full);
   else
-    select(full, std::false_type{});
+    select_by(half);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (k_out == k) {
     evict_in_place_kernel<<<dim3(rows, 1, 2), kInPlaceThreads, 0, stream>>>(

@@ -247,7 +247,8 @@ def _weights(n, H, L, seed):
     (3, 2, 1, 64, 1, 0, 0), (8, 2, 50, 32, 7, 2, 3), (8, 3, 300, 64, 100, 4, 32),
     (8, 2, 300, 64, 36, 4, 32), (8, 1, 257, 32, 256, 0, 1), (8, 2, 2500, 64, 600, 1, 0),
     (8, 2, 4100, 32, 2100, 16, 500), (3, 2, 40, 64, 90, 4, 32), (2, 1, 9000, 64, 5000, 0, 0),
-    (2, 150, 2300, 32, 900, 2, 30), (4, 1, 20000, 32, 7000, 4, 100), (8, 2, 8192, 32, 80, 4, 20),
+    (2, 150, 2300, 32, 900, 2, 30), (3, 100, 4500, 32, 900, 2, 30),
+    (4, 1, 20000, 32, 7000, 4, 100), (8, 2, 8192, 32, 80, 4, 20),
 ])
 def test_evict(gpu, dtype, n, H, L, D, budget, sinks, recent):
     k, v = (_randn((n, H, L, D), s, dtype) for s in (1, 2))
