@@ -858,7 +858,9 @@ __device__ __forceinline__ void sink_workgroup(const BwdArgs& a, int bh, int gro
 }
 
 // dQ (which writes delta), the sink keys' pieces in front: they are short, and the dQ workgroups
-// fill in behind them.
+// fill in behind them. B16 H12 T1024 D64, window 256, 4 sinks, token-major: 51 us, 42 of them without
+// sinks; dK/dV 44. Half of either is HBM time (150 MB, 29 us), which a window of 64 comes down to (32
+// and 32 us); P and dS are rounded to bf16 for the products, as without a window.
 constexpr int kMaxPieceTiles = 12;
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, kDqMinBlocks) void window_dq_bf16_kernel(
