@@ -263,6 +263,10 @@ struct WindowBwdArgs : Window {
     if (piece_tiles == 0 && kblk * block_keys < sinks) return last + 1;
     return min(last, ((kblk + 1) * block_keys + window - 2) / kTileRows) + 1;
   }
+  // pieces of the block's sink keys
+  __device__ __forceinline__ int far_pieces(int kblk, int S) const {
+    return ((S - 1) / kTileRows + piece_tiles - block_end(kblk, S)) / piece_tiles;
+  }
   // the partials of sink keys 32 * group .. of one piece: dK, and dV sink_rows() * D further on
   __device__ __forceinline__ int sink_rows() const { return (sinks + 31) / 32 * 32; }
   template <int D>
@@ -878,6 +882,29 @@ __global__ __launch_bounds__(64 * kWaves, kDqMinBlocks) void window_dq_bf16_kern
   constexpr bool kFromDelta = D == 64 || KS == 2;  // as dq_bf16_kernel
   dq_workgroup<D, STRIDED, false, KS, true, kFromDelta, true>(a, blockIdx.x, y - n, tiles, {win});
 }
+// Sums up a long list of partials into its first: kJoinWays threads for four columns, each every
+// kJoinWays-th partial, and their sums in order. dK/dV's workgroups would add one after the other
+// (forward and backward, window 256, us: 1 x 65536 113 -> 69, 1 x 16384 44.9 -> 40.5, 1 x 8192, 11
+// partials 37.9 -> 37.0; but 12 x 8192, window 1024, 10 partials 152.4 -> 155.0).
+constexpr int kJoinWays = 8, kJoinCols = 256 / kJoinWays;
+template <int D>
+__global__ __launch_bounds__(256) void window_join_bf16_kernel(const WindowBwdArgs win, int S) {
+  __shared__ f32x4 sums[kJoinWays][kJoinCols];
+  const int way = threadIdx.x / kJoinCols, at = threadIdx.x % kJoinCols;
+  const int i = blockIdx.y * kJoinCols + at, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
+  const int which = i / (D / 4) / win.sinks;
+  const int far = which > 1 ? 0 : win.far_pieces(row / win.block_keys, S);
+  float* p = win.partials<D>(blockIdx.x, 0, 0) + (size_t)(which * win.sink_rows() + row) * D + col;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int j = way; j < far; j += kJoinWays)
+    sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * win.sink_rows() * D);
+  sums[way][at] = sum;
+  __syncthreads();
+  if (way != 0 || far == 0) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWays; ++w) sum += sums[w][at];
+  *reinterpret_cast<f32x4*>(p) = sum;
+}
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(false)) void window_dkdv_bf16_kernel(
     const BwdArgs a, const WindowBwdArg<true> win) {
@@ -1020,9 +1047,9 @@ hipError_t launch_bwd_bf16_t(bf16* dq, bf16* dk, bf16* dv, float* delta, const b
 
 // How a windowed backward is launched: in one launch or as dQ and then dK/dV, the waves of a row
 // group, the pieces of its sink keys' later queries (in query tiles) and the bytes of their
-// partials.
+// partials, and whether these are joined before dK/dV adds them up.
 struct WindowPlan {
-  bool one;
+  bool one, join;
   int waves_per_group, piece_tiles, pieces;
   size_t workspace;
 };
@@ -1046,15 +1073,14 @@ WindowPlan window_plan(int BH, int S, int D, const Window& w) {
   const long long far = tiles - end(32 * kWaves / p.waves_per_group);
   if (p.one || w.sinks == 0 || far <= 0) return p;
   // Pieces of even lengths up to 12 tiles (of four, B16 H12 T1024 with a window of 256 takes dQ 56
-  // for 51 us). Small grids wait for a piece's tiles and for the blocks that add up the partials one
-  // after the other, so there as many tiles as partials, about (12 -> up to sqrt(far), backward, us:
-  // 32 x 799, window 10 24.1 -> 18.5, 12 x 1024, 256 25.0 -> 19.6, 16 x 710, 4 20.0 -> 15.8; but 48 x
-  // 1024, 128 28.5 -> 32.3, 96 x 1024, 128 39.4 -> 42.1).
-  int most = kMaxPieceTiles;
-  if ((long long)BH * S <= 1 << 15)
-    for (most = 4; most < kMaxPieceTiles && most * most < far;) ++most;
+  // for 51 us); up to four in small grids, which wait for the longest piece (12 -> 4, backward, us: 32 x
+  // 799, window 10 24.1 -> 18.5, 12 x 1024, 256 25.0 -> 19.6, 16 x 710, 4 20.0 -> 15.8; but 48 x 1024, 128
+  // 28.5 -> 32.3, 96 x 1024, 128 39.4 -> 42.1).
+  const bool small = (long long)BH * S <= 1 << 15;
+  const int most = small ? 4 : kMaxPieceTiles;
   p.pieces = (int)((far + most - 1) / most);
   p.piece_tiles = (int)((far + p.pieces - 1) / p.pieces);
+  p.join = p.pieces > (small ? 6 : 12);
   p.workspace = sizeof(float) * BH * (size_t)p.pieces * 2 * ((w.sinks + 31) / 32 * 32) * D;
   return p;
 }
@@ -1085,6 +1111,12 @@ hipError_t launch_window_bwd_bf16_t(const BwdArgs& args, int BH, const Window& w
         <<<dim3(BH, sink_groups * win.pieces + blocks), 64 * kWaves, 0, stream>>>(args, win,
                                                                                   sink_groups);
     if ((e = hipGetLastError()) != hipSuccess) return;
+    if (plan.join) {
+      window_join_bf16_kernel<D>
+          <<<dim3(BH, (w.sinks * (D / 4) * 2 + kJoinCols - 1) / kJoinCols), 256, 0, stream>>>(win, S);
+      if ((e = hipGetLastError()) != hipSuccess) return;
+      win.piece_tiles = S / kTileRows + 1;  // dK/dV has the first partial to add
+    }
     window_dkdv_bf16_kernel<D, strided(), kw()>
         <<<dim3(BH, blocks), 64 * kWaves, 0, stream>>>(args, win);
     e = hipGetLastError();

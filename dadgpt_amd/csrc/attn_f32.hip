@@ -990,21 +990,31 @@ __global__ __launch_bounds__(64 * KG * KS, wgs_per_cu(KS, KG, D)) void window_bw
   }
 }
 
-// The sink rows of dK and dV of blocks with pieces, from the partials, summed in their order: a
-// thread for four columns.
+// The sink rows of dK and dV of blocks with pieces, from the partials: kJoinWays threads for four
+// columns, each summing every kJoinWays-th partial, and their sums in order (BH 1, S 65536, 256
+// pieces: 72 us with one thread for all of them).
+constexpr int kJoinWays = 8, kJoinCols = 256 / kJoinWays;
 template <int D>
 __global__ __launch_bounds__(256) void window_join_f32_kernel(const F32BwdArgs a,
                                                               const F32WindowBwdArgs win) {
-  const int i = blockIdx.y * 256 + threadIdx.x, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
+  __shared__ f32x4 sums[kJoinWays][kJoinCols];
+  const int way = threadIdx.x / kJoinCols, at = threadIdx.x % kJoinCols;
+  const int i = blockIdx.y * kJoinCols + at, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
   const int which = i / (D / 4) / win.sinks, bh = blockIdx.x;
-  if (which > 1) return;
-  const int rows = (win.sinks + 31) / 32 * 32, far = win.far_pieces(row, a.S);
-  if (far == 0) return;  // its workgroup has written the final row
+  const int rows = (win.sinks + 31) / 32 * 32;
+  // without pieces its workgroup has written the final row
+  const int far = which > 1 ? 0 : win.far_pieces(row, a.S);
   const float* p = win.partial + ((size_t)bh * (win.pieces + 1) * 2 + which) * rows * D +
                    (size_t)row * D + col;
-  f32x4 sum = *reinterpret_cast<const f32x4*>(p);
-  for (int j = 1; j <= far; ++j)
-    sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * rows * D);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (far > 0)
+    for (int j = way; j <= far; j += kJoinWays)
+      sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * rows * D);
+  sums[way][at] = sum;
+  __syncthreads();
+  if (way != 0 || far == 0) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWays; ++w) sum += sums[w][at];
   *reinterpret_cast<f32x4*>((which == 0 ? a.dk : a.dv) + ((size_t)bh * a.S + row) * D + col) = sum;
 }
 
@@ -1194,7 +1204,7 @@ hipError_t window_bwd_f32_t(const F32BwdArgs& args, int BH, const Window& w, flo
   });
   if (e != hipSuccess || plan.pieces == 0) return e;
   window_join_f32_kernel<D>
-      <<<dim3(BH, (w.sinks * (D / 4) * 2 + 255) / 256), 256, 0, stream>>>(args, win);
+      <<<dim3(BH, (w.sinks * (D / 4) * 2 + kJoinCols - 1) / kJoinCols), 256, 0, stream>>>(args, win);
   return hipGetLastError();
 }
 

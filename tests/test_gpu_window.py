@@ -43,6 +43,7 @@ CASES = [
     (1, 1800, 64, 17, 1024), (240, 1100, 64, 80, 4), (240, 1100, 32, 80, 4), (240, 1100, 64, 80, 0),
     (20, 2100, 64, 1000, 4), (20, 2100, 32, 1000, 0), (260, 200, 64, 33, 2), (24, 1024, 32, 200, 40),
     (12, 1024, 64, 250, 4), (5, 2100, 64, 1000, 4), (6, 1300, 64, 40, 300),
+    (2, 4500, 64, 30, 40), (1, 6000, 32, 100, 130), (9, 6500, 64, 60, 4),
 ]
 
 
@@ -62,7 +63,7 @@ def test_window_attention(gpu, dtype, BH, S, D, window, sinks):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-@pytest.mark.parametrize("scale", [-0.125, 1.0])
+@pytest.mark.parametrize("scale", [-0.125, 1.0, 0.0, 1e-20])
 def test_window_scales(gpu, dtype, scale):
     """A negative scale, and one that makes the softmax sharp."""
     q, k, v, g = _inputs(2, 333, 64, dtype, seed=5)
