@@ -17,28 +17,43 @@ namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
+// The wave's loads are in. A workgroup barrier alone does not wait for loads in flight, which a
+// store by another wave after it must not overtake.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // ------------------------------------------------------------------------ 8-bit append
 
 constexpr int kAppendWaves = 4;
 constexpr uint32_t kInfBits = 0x7f800000u;
 
-// Eight consecutive source elements as floats.
-__device__ __forceinline__ void load8(float (&x)[8], const bf16* p) {
-  const u32x4 w = ld_g128u(p);
+// Eight consecutive source elements, as they lie in memory until they are looked at.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<bf16> {
+  u32x4 w = {0u, 0u, 0u, 0u};
+  __device__ __forceinline__ void load(const bf16* p) { w = ld_g128u(p); }
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = bf16_lo(w[i]);
-    x[2 * i + 1] = bf16_hi(w[i]);
+    for (int i = 0; i < 4; ++i) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
   }
-}
-__device__ __forceinline__ void load8(float (&x)[8], const float* p) {
-  const u32x4 a = ld_g128u(p), b = ld_g128u(p + 4);
+  // not to be kept as floats from one look to the next
+  __device__ __forceinline__ void keep() { asm("" : "+v"(w)); }
+};
+template <>
+struct Eight<float> {
+  float f[8] = {};
+  __device__ __forceinline__ void load(const float* p) {
+    const u32x4 a = ld_g128u(p), b = ld_g128u(p + 4);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[i] = __uint_as_float(a[i]);
-    x[4 + i] = __uint_as_float(b[i]);
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(a[i]), f[4 + i] = __uint_as_float(b[i]);
   }
-}
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f[i];
+  }
+  __device__ __forceinline__ void keep() {}
+};
 
 // Eight e4m3 codes of x * mul (rounded to nearest even; |x * mul| <= 448, or NaN).
 __device__ __forceinline__ u32x2 to_e4m3(const float (&x)[8], float mul) {
@@ -64,70 +79,84 @@ __device__ __forceinline__ float e4m3_scale(uint32_t a) {
   return __uint_as_float((uint32_t)(max(e, -100) + 127) << 23);
 }
 
-// One wave for each touched block of a (sequence, head) and tensor: D/8 lanes a row, NI rows a
-// lane, all of them loaded before the block's maximum is taken and still in registers when it is
-// known. Grid (heads, K and V: 4 waves a workgroup; touched blocks; sequences), heads fastest, so that
+// WPB waves for each touched block of a (sequence, head) and tensor: D/8 lanes a row, NI rows a lane,
+// all of them loaded before the block's maximum is taken and still in registers when it is known.
+// Grid (heads, K and V: 4 waves a workgroup; touched blocks; sequences), heads fastest, so that
 // neighbours read one stretch of the projection's token-major rows. Bound by that chain (lengths, rows,
-// maximum, codes) more than by HBM: 16 x 12 prompts of 1 to 1024 tokens, 38 MB, 11.2 us; one token
-// for each of 32 x 12 caches 3.5.
-template <typename T, int D, int NI>
+// maximum, codes) more than by HBM: 16 x 12 prompts of 1 to 1024 tokens in blocks of 32, 38 MB, 10.6 us;
+// one token for each of 32 x 12 caches 3.5.
+template <typename T, int D, int NI, int WPB>
 __global__ __launch_bounds__(64 * kAppendWaves) void kv8_append_kernel(
     uint8_t* __restrict__ k8, uint8_t* __restrict__ v8, float* __restrict__ k_scale,
     float* __restrict__ v_scale, const T* __restrict__ k, const T* __restrict__ v,
     const HeadStrides64 ks, const HeadStrides64 vs, const int* __restrict__ lens,
     const int* __restrict__ counts, int H, int rows, int max_len) {
-  constexpr int LPR = D / 8, RPI = 64 / LPR, BLOCK = NI * RPI;
+  constexpr int LPR = D / 8, RPI = 64 / LPR, BLOCK = NI * RPI * WPB;
   const int lane = threadIdx.x & 63, sub = lane % LPR, grp = lane / LPR;
-  const int unit = blockIdx.x * kAppendWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % WPB;
+  const int unit = (blockIdx.x * kAppendWaves + wave) / WPB;
   const bool is_v = unit & 1;
   const int head = unit >> 1, seq = blockIdx.z, at = blockIdx.y;
-  if (head >= H) return;
+  if (head >= H) return;  // (with more than one wave a block, whole workgroups)
   const int begin = clamp_len(lens[seq], max_len);
   const int count = counts == nullptr ? rows : clamp_len(counts[seq], rows);
   const int end = begin + min(count, max_len - begin);
   const int blk = begin / BLOCK + at, lo = blk * BLOCK;
   if (lo >= end || begin >= end) return;
+  const int first = lo + part * NI * RPI + grp;  // the lane's rows: every RPI-th
 
   const HeadStrides64& st = is_v ? vs : ks;
   const T* src = (is_v ? v : k) + seq * st.batch + head * st.head + sub * 8;
   const long long hrow = (long long)seq * H + head;
-  uint8_t* dst = (is_v ? v8 : k8) + (hrow * max_len + lo) * D + sub * 8;
+  uint8_t* dst = (is_v ? v8 : k8) + (hrow * max_len + first) * D + sub * 8;
   float* scale = (is_v ? v_scale : k_scale) + hrow * ((max_len + BLOCK - 1) / BLOCK) + blk;
 
-  float x[NI][8];
-  uint32_t amax = 0;
+  Eight<T> x[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int r = lo + i * RPI + grp;
-    if (r >= begin && r < end) {
-      load8(x[i], src + (long long)(r - begin) * st.row);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-    }
+    const int r = first + i * RPI;
+    if (r >= begin && r < end) x[i].load(src + (long long)(r - begin) * st.row);
   }
   const bool has_old = lo < begin;
   const float s_old = has_old ? *scale : 0.f;
+  uint32_t amax = 0;
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+  for (int i = 0; i < NI; ++i) {
+    float f[8];
+    x[i].floats(f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t a = __float_as_uint(x[i][e]) & 0x7fffffffu;
-      if (a >= kInfBits) x[i][e] = __uint_as_float(0x7fc00000u);  // held as e4m3's NaN
+      const uint32_t a = __float_as_uint(f[e]) & 0x7fffffffu;
       amax = max(amax, a >= kInfBits ? 0u : a);
     }
+    x[i].keep();
+  }
   // (bits of non-negative floats order as the floats do)
-  const uint32_t am = __float_as_uint(lanes::group_max<64>(__uint_as_float(amax)));
+  float most = lanes::group_max<64>(__uint_as_float(amax));
+  if constexpr (WPB > 1) {
+    __shared__ float sm[kAppendWaves];
+    if (lane == 0) sm[wave] = most;
+    wait_loads();  // (s_old: another wave stores the new scale)
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WPB; ++i) most = fmaxf(most, sm[wave - part + i]);
+  }
+  const uint32_t am = __float_as_uint(most);
   const float s_new = fmaxf(s_old, e4m3_scale(am));
   const float inv = 1.0f / s_new;  // exact
   const bool regrow = has_old && s_new > s_old;  // wave-uniform
   const float ratio = s_old * inv;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int r = lo + i * RPI + grp;
-    uint8_t* p = dst + (i * RPI + grp) * D;
+    const int r = first + i * RPI;
+    uint8_t* p = dst + i * RPI * D;
     if (r >= begin && r < end) {
-      *reinterpret_cast<u32x2*>(p) = to_e4m3(x[i], inv);
+      float f[8];
+      x[i].floats(f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // an infinity is held as e4m3's NaN, as NaN is
+        if ((__float_as_uint(f[e]) & 0x7fffffffu) >= kInfBits) f[e] = __uint_as_float(0x7fc00000u);
+      *reinterpret_cast<u32x2*>(p) = to_e4m3(f, inv);
     } else if (regrow && r < begin) {
       const u32x2 w = *reinterpret_cast<const u32x2*>(p);
       float old[8];
@@ -136,7 +165,7 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv8_append_kernel(
       *reinterpret_cast<u32x2*>(p) = to_e4m3(old, ratio);
     }
   }
-  if (lane == 0) *scale = s_new;
+  if (lane == 0 && part == 0) *scale = s_new;
 }
 
 template <typename T, int D>
@@ -145,30 +174,28 @@ hipError_t launch_kv8_append_d(uint8_t* k8, uint8_t* v8, float* k_scale, float* 
                                const HeadStrides64& vs, const int* lens, const int* counts,
                                int n_seq, int H, int rows, int max_len, int block,
                                hipStream_t stream) {
-  const dim3 grid((2 * H + kAppendWaves - 1) / kAppendWaves, kv8_touched_blocks(rows, block), n_seq);
-  auto launch = [&](auto ni) {
-    kv8_append_kernel<T, D, ni()><<<grid, 64 * kAppendWaves, 0, stream>>>(
+  auto launch = [&](auto ni, auto wpb) {
+    const dim3 grid((2 * H * wpb() + kAppendWaves - 1) / kAppendWaves,
+                    kv8_touched_blocks(rows, block), n_seq);
+    kv8_append_kernel<T, D, ni(), wpb()><<<grid, 64 * kAppendWaves, 0, stream>>>(
         k8, v8, k_scale, v_scale, k, v, ks, vs, lens, counts, H, rows, max_len);
+    return hipGetLastError();
   };
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 2> two;
+  constexpr std::integral_constant<int, 4> four;
   switch (block * D / 512) {
     case 1:  // 16 tokens of 32 columns
-      if constexpr (D == 32) {
-        launch(std::integral_constant<int, 1>{});
-        break;
-      }
-      return hipErrorInvalidValue;
-    case 2: launch(std::integral_constant<int, 2>{}); break;
-    case 4: launch(std::integral_constant<int, 4>{}); break;
-    case 8: launch(std::integral_constant<int, 8>{}); break;
+      if constexpr (D == 32) return launch(one, one);
+      break;
+    case 2: return launch(two, one);
+    case 4: return launch(four, one);
+    case 8: return launch(four, two);
     case 16:  // 128 tokens of 64 columns
-      if constexpr (D == 64) {
-        launch(std::integral_constant<int, 16>{});
-        break;
-      }
-      return hipErrorInvalidValue;
-    default: return hipErrorInvalidValue;
+      if constexpr (D == 64) return launch(four, four);
+      break;
   }
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 template <typename T>
@@ -598,10 +625,6 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return x;
 }
-
-// The wave's loads are in. A workgroup barrier alone does not wait for loads in flight, which a
-// store by another wave after it must not overtake.
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 struct SelectLds {
   int hist[kSelBins];
