@@ -95,10 +95,11 @@ def test_append_codes_and_scales(gpu, dtype, n, H, L, D, block, rows):
 
 
 @pytest.mark.gpu
-def test_append_without_counts_and_token_by_token(gpu):
+@pytest.mark.parametrize("D,block", [(64, 32), (64, 64), (64, 128), (32, 128)])
+def test_append_without_counts_and_token_by_token(gpu, D, block):
     """A prompt appended at once and token by token ends with the same scales, and codes that the
     definition gives for that order."""
-    n, H, L, D, block, rows = 3, 2, 80, 64, 32, 75
+    n, H, L, rows = 3, 3, 200, 150
     x = _randn((n, H, rows, D), seed=3) * torch.linspace(0.1, 4, rows, device="cuda")[:, None]
     whole, steps = C.kv8_cache(n, H, L, D, block), C.kv8_cache(n, H, L, D, block)
     C.kv8_append(*whole, x, x, _int([0] * n), None, n, H, rows, L, D, block)
