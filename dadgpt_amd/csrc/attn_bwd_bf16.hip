@@ -253,10 +253,11 @@ struct BwdArgs {
 };
 // The windowed backward's arguments. A dK/dV workgroup walks the query tiles of its key block's
 // window (block_end); a sink key's later queries are `pieces` pieces at most of piece_tiles tiles,
-// whose sums lie in `partial`, fp32 [BH][piece][dK, dV][sink rows, whole 32s][D]. Without pieces
-// (piece_tiles 0) a block with sink keys walks them too.
+// whose sums lie in `partial`, fp32 [BH][piece][dK, dV][sink rows, whole 32s][D]. In one launch the
+// block's own sums lie behind them (slots = pieces + 1). Without pieces (piece_tiles 0) a block with
+// sink keys walks the later queries too.
 struct WindowBwdArgs : Window {
-  int block_keys, piece_tiles, pieces;
+  int block_keys, piece_tiles, pieces, slots;
   float* partial;
   __device__ __forceinline__ int block_end(int kblk, int S) const {
     const int last = (S - 1) / kTileRows;
@@ -271,7 +272,7 @@ struct WindowBwdArgs : Window {
   __device__ __forceinline__ int sink_rows() const { return (sinks + 31) / 32 * 32; }
   template <int D>
   __device__ __forceinline__ float* partials(int bh, int piece, int group) const {
-    return partial + (((size_t)bh * pieces + piece) * 2 * sink_rows() + 32 * group) * D;
+    return partial + (((size_t)bh * slots + piece) * 2 * sink_rows() + 32 * group) * D;
   }
 };
 template <bool WIN>
@@ -358,7 +359,8 @@ __device__ __forceinline__ void add_partials(f32x16 (&acc)[D / 32], const float*
 // One workgroup's dK and dV. OWN_DELTA: delta is computed here, into own_delta (one float for
 // each row from the first tile on); otherwise it is read from a.delta.
 // WIN: the queries of a key block end with its last key's window; what later queries add to sink
-// keys is in the partials that an earlier launch left (sink_workgroup).
+// keys is in the partials that an earlier launch left (sink_workgroup), or, with OWN_DELTA, is added to
+// the block's own sums, which are left there too, by a later one (window_join_rows_kernel).
 template <int D, bool STRIDED, bool DROP, int KS, bool OWN_DELTA, bool WIN = false>
 __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kblk,
                                                BwdTiles<D>& tiles, BwdStats& stats,
@@ -480,8 +482,13 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
       const int far = (S - 1) / kTileRows + 1 - t_end;  // tiles
       if (far > 0 && kw0 < win.sinks) {
         const size_t stride = (size_t)2 * win.sink_rows() * D;
-        add_partials<D>(acc, win.template partials<D>(bh, 0, kw0 / 32) + which * (stride / 2), stride,
-                        (far + win.piece_tiles - 1) / win.piece_tiles, key < win.sinks, lane);
+        if constexpr (OWN_DELTA)
+          store_partial<D>(win.template partials<D>(bh, win.pieces, kw0 / 32) + which * (stride / 2),
+                           acc, key < win.sinks, lane);
+        else
+          add_partials<D>(acc, win.template partials<D>(bh, 0, kw0 / 32) + which * (stride / 2),
+                          stride, (far + win.piece_tiles - 1) / win.piece_tiles, key < win.sinks,
+                          lane);
       }
     }
   };
@@ -882,28 +889,57 @@ __global__ __launch_bounds__(64 * kWaves, kDqMinBlocks) void window_dq_bf16_kern
   constexpr bool kFromDelta = D == 64 || KS == 2;  // as dq_bf16_kernel
   dq_workgroup<D, STRIDED, false, KS, true, kFromDelta, true>(a, blockIdx.x, y - n, tiles, {win});
 }
-// Sums up a long list of partials into its first: kJoinWays threads for four columns, each every
-// kJoinWays-th partial, and their sums in order. dK/dV's workgroups would add one after the other
-// (forward and backward, window 256, us: 1 x 65536 113 -> 69, 1 x 16384 44.9 -> 40.5, 1 x 8192, 11
-// partials 37.9 -> 37.0; but 12 x 8192, window 1024, 10 partials 152.4 -> 155.0).
+// The sum of n partials at p: kJoinWays threads for four columns, each every kJoinWays-th partial, and
+// their sums in order. The first way's thread has it.
 constexpr int kJoinWays = 8, kJoinCols = 256 / kJoinWays;
-template <int D>
-__global__ __launch_bounds__(256) void window_join_bf16_kernel(const WindowBwdArgs win, int S) {
+__device__ __forceinline__ f32x4 join_partials(const float* p, size_t stride, int n) {
   __shared__ f32x4 sums[kJoinWays][kJoinCols];
   const int way = threadIdx.x / kJoinCols, at = threadIdx.x % kJoinCols;
-  const int i = blockIdx.y * kJoinCols + at, col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks;
-  const int which = i / (D / 4) / win.sinks;
-  const int far = which > 1 ? 0 : win.far_pieces(row / win.block_keys, S);
-  float* p = win.partials<D>(blockIdx.x, 0, 0) + (size_t)(which * win.sink_rows() + row) * D + col;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int j = way; j < far; j += kJoinWays)
-    sum += *reinterpret_cast<const f32x4*>(p + (size_t)j * 2 * win.sink_rows() * D);
+  for (int j = way; j < n; j += kJoinWays) sum += *reinterpret_cast<const f32x4*>(p + j * stride);
   sums[way][at] = sum;
   __syncthreads();
-  if (way != 0 || far == 0) return;
 #pragma unroll
   for (int w = 1; w < kJoinWays; ++w) sum += sums[w][at];
-  *reinterpret_cast<f32x4*>(p) = sum;
+  return sum;
+}
+// A workgroup's columns of the sink rows: (dK or dV, row, column), and the row's pieces.
+template <int D>
+struct JoinAt {
+  int col, row, which, far;
+  __device__ __forceinline__ JoinAt(const WindowBwdArgs& win, int S) {
+    const int i = blockIdx.y * kJoinCols + threadIdx.x % kJoinCols;
+    col = i % (D / 4) * 4, row = i / (D / 4) % win.sinks, which = i / (D / 4) / win.sinks;
+    far = which > 1 ? 0 : win.far_pieces(row / win.block_keys, S);
+  }
+};
+// Sums up a long list of partials into its first. dK/dV's workgroups would add one after the other
+// (forward and backward, window 256, us: 1 x 65536 113 -> 69, 1 x 16384 44.9 -> 40.5, 1 x 8192, 11
+// partials 37.9 -> 37.0; but 12 x 8192, window 1024, 10 partials 152.4 -> 155.0).
+template <int D>
+__global__ __launch_bounds__(256) void window_join_bf16_kernel(const WindowBwdArgs win, int S) {
+  const JoinAt<D> at(win, S);
+  const size_t stride = (size_t)2 * win.sink_rows() * D;
+  float* p = win.partials<D>(blockIdx.x, 0, 0) + at.which * (stride / 2) + (size_t)at.row * D + at.col;
+  const f32x4 sum = join_partials(p, stride, at.far);
+  if (threadIdx.x < kJoinCols && at.far > 0) *reinterpret_cast<f32x4*>(p) = sum;
+}
+// The rows of sink keys with pieces, from these and the block's own sums.
+template <int D, bool STRIDED>
+__global__ __launch_bounds__(256) void window_join_rows_kernel(const BwdArgs a,
+                                                               const WindowBwdArgs win) {
+  const JoinAt<D> at(win, a.S);
+  const size_t stride = (size_t)2 * win.sink_rows() * D;
+  const float* p =
+      win.partials<D>(blockIdx.x, 0, 0) + at.which * (stride / 2) + (size_t)at.row * D + at.col;
+  f32x4 sum = join_partials(p, stride, at.far);
+  if (threadIdx.x >= kJoinCols || at.far == 0) return;  // (else its workgroup's row is final)
+  const float mul = at.which == 0 ? a.scale : 1.0f;
+  sum += *reinterpret_cast<const f32x4*>(p + win.pieces * stride);
+  const Slice<D, STRIDED> sl(a.L, blockIdx.x, a.S);
+  bf16* row = at.which == 0 ? sl.row(a.dk, kTDK, at.row) : sl.row(a.dv, kTDV, at.row);
+  *reinterpret_cast<u32x2*>(row + at.col) =
+      u32x2{pack_bf16x2(sum[0] * mul, sum[1] * mul), pack_bf16x2(sum[2] * mul, sum[3] * mul)};
 }
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(false)) void window_dkdv_bf16_kernel(
@@ -913,19 +949,27 @@ __global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(false)) void window_dk
   dkdv_workgroup<D, STRIDED, false, KS, false, true>(a, blockIdx.x, blockIdx.y, tiles, stats,
                                                      nullptr, win);
 }
-// Both in one launch where there are no pieces, delta where it is needed (a block's window of at
-// most kOwnDeltaMaxS rows): the dK/dV workgroups first.
+// All in one launch, delta where it is needed (a block's window of at most kOwnDeltaMaxS rows): the
+// pieces first, if there are any, then dK/dV, then dQ.
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, dkdv_wgs_per_cu(false)) void window_bwd_bf16_kernel(
-    const BwdArgs a, const WindowBwdArg<true> win) {
+    const BwdArgs a, const WindowBwdArg<true> win, int blocks, int sink_groups) {
   __shared__ BwdTiles<D> tiles;
   __shared__ BwdStats stats;
   __shared__ float own_delta[kOwnDeltaMaxS];
-  if (blockIdx.z == 0)
-    dkdv_workgroup<D, STRIDED, false, KS, true, true>(a, blockIdx.x, blockIdx.y, tiles, stats,
-                                                      own_delta, win);
-  else
-    dq_workgroup<D, STRIDED, false, KS, true, true, true>(a, blockIdx.x, blockIdx.y, tiles, {win});
+  static_assert(kMaxPieceTiles * kTileRows <= kOwnDeltaMaxS, "a piece's delta fits");
+  const int y = blockIdx.y, n = sink_groups * win.pieces;
+  if (y < n) {
+    const int piece = y / sink_groups;
+    sink_workgroup<D, STRIDED>(a, blockIdx.x, y - piece * sink_groups, piece, tiles, stats,
+                               own_delta, win);
+  } else if (y < n + blocks) {
+    dkdv_workgroup<D, STRIDED, false, KS, true, true>(a, blockIdx.x, y - n, tiles, stats, own_delta,
+                                                      win);
+  } else {
+    dq_workgroup<D, STRIDED, false, KS, true, true, true>(a, blockIdx.x, y - n - blocks, tiles,
+                                                          {win});
+  }
 }
 
 // How a backward is launched: dQ, then dK/dV (kSeparate); both in one launch with delta
@@ -1050,7 +1094,7 @@ hipError_t launch_bwd_bf16_t(bf16* dq, bf16* dk, bf16* dv, float* delta, const b
 // partials, and whether these are joined before dK/dV adds them up.
 struct WindowPlan {
   bool one, join;
-  int waves_per_group, piece_tiles, pieces;
+  int waves_per_group, piece_tiles, pieces, slots;
   size_t workspace;
 };
 WindowPlan window_plan(int BH, int S, int D, const Window& w) {
@@ -1059,19 +1103,24 @@ WindowPlan window_plan(int BH, int S, int D, const Window& w) {
   auto end = [&](int block_keys) {  // of the first block, in tiles
     return ((long long)block_keys + w.window - 2) / kTileRows + 1;
   };
-  // One launch, as the plain backward, where a workgroup's rows are few enough for its own delta: a
-  // window's without sinks; with sinks, a sequence whose sink blocks need no pieces, as their
-  // later queries are few next to the window or in all (pieces in a launch of their own -> whole,
-  // us: 4 x 300, window 64 20.7 -> 17.5, 192 x 256, 64 33.1 -> 24.6, 96 x 1024, 512 90.6 -> 80.4;
-  // but 12 x 1024, 256 30.5 -> 34.9, 48 x 1024, 128 38.2 -> 53.2).
+  // Sink blocks walk all later queries themselves (`whole`) where these are few, or in large grids few
+  // next to the window: pieces and their join cost more than the longer chain (pieces -> whole,
+  // backward, us: 192 x 256, window 64 21.0 -> 16.7, 180 x 500, 64 38.4 -> 34.9, 96 x 1024, 512 62.9 ->
+  // 59.9; but 12 x 1024, 512 19.2 -> 25.5, 24 x 494, 55 12.0 -> 16.7).
   const long long end128 = end(128), far128 = tiles - end128;
-  const bool whole = w.sinks == 0 || far128 <= 6 || far128 <= end128;
+  const bool few = (long long)BH * S <= 1 << 16;
+  const bool whole =
+      w.sinks == 0 || (few ? far128 <= 2 : far128 <= 6 || far128 <= end128);
+  // One launch, as the plain backward, where a workgroup's rows are few enough for its own delta (two
+  // launches -> one and a join of the sink rows, us: 4 x 1429, window 5 16.6 -> 11.0, 12 x 1024, 256 19.5
+  // -> 15.9, 64 x 700, 64 27.5 -> 19.5; but 96 x 1024, 128 40.1 -> 41.6).
   const bool short_rows = w.window <= kOwnDeltaMaxS - 3 * kTileRows;
-  p.one = bwd_in_one_launch(BH, S, D, false) && whole &&
-          (S <= kOwnDeltaMaxS || (short_rows && w.sinks == 0));
+  p.one = bwd_in_one_launch(BH, S, D, false) &&
+          (whole ? S <= kOwnDeltaMaxS || (short_rows && w.sinks == 0)
+                 : short_rows && (D == 32 || few));
   p.waves_per_group = window_waves_per_group(BH, S, p.one ? 2 : 1);
   const long long far = tiles - end(32 * kWaves / p.waves_per_group);
-  if (p.one || w.sinks == 0 || far <= 0) return p;
+  if ((p.one && whole) || w.sinks == 0 || far <= 0) return p;
   // Pieces of even lengths up to 12 tiles (of four, B16 H12 T1024 with a window of 256 takes dQ 56
   // for 51 us); up to four in small grids, which wait for the longest piece (12 -> 4, backward, us: 32 x
   // 799, window 10 24.1 -> 18.5, 12 x 1024, 256 25.0 -> 19.6, 16 x 710, 4 20.0 -> 15.8; but 48 x 1024, 128
@@ -1080,8 +1129,9 @@ WindowPlan window_plan(int BH, int S, int D, const Window& w) {
   const int most = small ? 4 : kMaxPieceTiles;
   p.pieces = (int)((far + most - 1) / most);
   p.piece_tiles = (int)((far + p.pieces - 1) / p.pieces);
-  p.join = p.pieces > (small ? 6 : 12);
-  p.workspace = sizeof(float) * BH * (size_t)p.pieces * 2 * ((w.sinks + 31) / 32 * 32) * D;
+  p.join = p.one || p.pieces > (small ? 6 : 12);
+  p.slots = p.pieces + (p.one ? 1 : 0);
+  p.workspace = sizeof(float) * BH * (size_t)p.slots * 2 * ((w.sinks + 31) / 32 * 32) * D;
   return p;
 }
 
@@ -1096,14 +1146,19 @@ hipError_t launch_window_bwd_bf16_t(const BwdArgs& args, int BH, const Window& w
   win.block_keys = 32 * kWaves / plan.waves_per_group;
   win.piece_tiles = plan.piece_tiles;
   win.pieces = plan.pieces;
+  win.slots = plan.slots;
   win.partial = partial;
   const int blocks = (S + win.block_keys - 1) / win.block_keys, sink_groups = (w.sinks + 31) / 32;
   hipError_t e = hipSuccess;
   with_shape(plan.waves_per_group, false, !is_contiguous(args.L, S, D),
              [&](auto strided, auto, auto kw) {
+    const dim3 joins(BH, (w.sinks * (D / 4) * 2 + kJoinCols - 1) / kJoinCols);
     if (plan.one) {
       window_bwd_bf16_kernel<D, strided(), kw()>
-          <<<dim3(BH, blocks, 2), 64 * kWaves, 0, stream>>>(args, win);
+          <<<dim3(BH, sink_groups * win.pieces + 2 * blocks), 64 * kWaves, 0, stream>>>(
+              args, win, blocks, sink_groups);
+      if ((e = hipGetLastError()) != hipSuccess || win.pieces == 0) return;
+      window_join_rows_kernel<D, strided()><<<joins, 256, 0, stream>>>(args, win);
       e = hipGetLastError();
       return;
     }
@@ -1112,8 +1167,7 @@ hipError_t launch_window_bwd_bf16_t(const BwdArgs& args, int BH, const Window& w
                                                                                   sink_groups);
     if ((e = hipGetLastError()) != hipSuccess) return;
     if (plan.join) {
-      window_join_bf16_kernel<D>
-          <<<dim3(BH, (w.sinks * (D / 4) * 2 + kJoinCols - 1) / kJoinCols), 256, 0, stream>>>(win, S);
+      window_join_bf16_kernel<D><<<joins, 256, 0, stream>>>(win, S);
       if ((e = hipGetLastError()) != hipSuccess) return;
       win.piece_tiles = S / kTileRows + 1;  // dK/dV has the first partial to add
     }

@@ -171,10 +171,11 @@ def test_window_gradients_against_differences(gpu):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-def test_window_repeats_streams_and_graph_replays(gpu, dtype):
+@pytest.mark.parametrize("BH", [6, 60])
+def test_window_repeats_streams_and_graph_replays(gpu, dtype, BH):
     """The same bits on every call, on another stream, and on every replay of a captured graph with
-    eager work between, for a backward of several pieces."""
-    BH, S, D, window, sinks = 6, 1400, 64, 90, 20
+    eager work between, for backwards of several pieces on a small and a large grid."""
+    S, D, window, sinks = 1400, 64, 90, 20
     q, k, v, g = _inputs(BH, S, D, dtype, seed=13)
     want = {n: x.clone() for n, x in _run(q, k, v, g, 0.125, window, sinks).items()}
     side = torch.cuda.Stream()
