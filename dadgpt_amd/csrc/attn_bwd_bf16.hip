@@ -95,6 +95,17 @@ __global__ __launch_bounds__(256) void delta_bf16_kernel(float* __restrict__ del
   if (valid && part == 0) delta[drow] = acc;
 }
 
+// What two floats lose as a packed pair of bf16 values, as another such pair. The windowed kernels
+// multiply dS as the sum of the two, 16 bits of it. In one bf16 value it adds as much error to dQ and
+// dK as their own rounding does: against 64 bits 1.5 times that of 32-bit arithmetic rounded once (with
+// a window of 4 1.8, as a short row's delta, from the bf16 output, weighs more); in two 1.1 (1.5). B16
+// H12 T1024, window 256, forward and backward 127 us for 119, B1 H12 T8192, window 1024 173 for 150. P
+// stays one value (dV 1.4 times).
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t packed) {
+  asm("" : "+v"(packed));  // (or the compiler would convert again instead of taking the word apart)
+  return pack_bf16x2(a - bf16_lo(packed), b - bf16_hi(packed));
+}
+
 // ---------------------------------------------------------------- dK / dV
 constexpr int kKW = 32;  // keys per wave
 
@@ -118,7 +129,7 @@ constexpr int kKW = 32;  // keys per wave
 // three workgroups per CU, without spilling in the loop. (The strided kernel of one launch with
 // its own delta and one wave per group keeps two registers in scratch and reloads them as it
 // issues a tile.)
-template <int D, bool DROP, bool XA>
+template <int D, bool DROP, bool XA, bool WIN = false>
 __device__ __forceinline__ void dkdv_block(bool mask, f32x16 (&dkacc)[D / 32],
                                            f32x16 (&dvacc)[D / 32], const bf16x8 (&kop)[D / 16],
                                            const bf16x8 (&vop)[D / 16], const bf16* sq,
@@ -169,7 +180,7 @@ __device__ __forceinline__ void dkdv_block(bool mask, f32x16 (&dkacc)[D / 32],
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) dp = mfma32(da[ds], vop[ds], dp);
   }
-  bf16x8 pb[2], dsb[2];
+  bf16x8 pb[2], dsb[2], dsl[2];
   f32x16 nd;  // -delta of the block's queries (dropout only)
   if constexpr (DROP) stats(sdl, nd);
   float pr[16];
@@ -186,7 +197,7 @@ __device__ __forceinline__ void dkdv_block(bool mask, f32x16 (&dkacc)[D / 32],
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    u32x4 wp, wd;
+    u32x4 wp, wd, wl;
 #pragma unroll
     for (int e2 = 0; e2 < 4; ++e2) {
       float p[2], d[2];
@@ -205,9 +216,11 @@ __device__ __forceinline__ void dkdv_block(bool mask, f32x16 (&dkacc)[D / 32],
       }
       wp[e2] = pack_bf16x2(p[0], p[1]);
       wd[e2] = pack_bf16x2(d[0], d[1]);
+      if constexpr (WIN) wl[e2] = pack_rest(d[0], d[1], wd[e2]);
     }
     pb[j] = as_bf16x8(wp);
     dsb[j] = as_bf16x8(wd);
+    if constexpr (WIN) dsl[j] = as_bf16x8(wl);
   }
   uint32_t ta[2][DB] = {};
   if constexpr (XA) tr_addr_xor<D>(ta, lo.tr);
@@ -235,7 +248,10 @@ __device__ __forceinline__ void dkdv_block(bool mask, f32x16 (&dkacc)[D / 32],
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) dkacc[db] = mfma32(t[db][j], dsb[j], dkacc[db]);
+      for (int db = 0; db < DB; ++db) {
+        if constexpr (WIN) dkacc[db] = mfma32(t[db][j], dsl[j], dkacc[db]);
+        dkacc[db] = mfma32(t[db][j], dsb[j], dkacc[db]);
+      }
   }
 }
 
@@ -464,7 +480,7 @@ __device__ __forceinline__ void dkdv_workgroup(const BwdArgs& a, int bh, int kbl
         }
         uint32_t keep = 0;
         if constexpr (DROP) keep = keep_col16(dr, (uint64_t)bh * S + qlo, kw0, lane);
-        dkdv_block<D, DROP, XA>(mask, dkacc, dvacc, kop, vop, cq, cdo, st[cb][0], st[cb][1], qb,
+        dkdv_block<D, DROP, XA, WIN>(mask, dkacc, dvacc, kop, vop, cq, cdo, st[cb][0], st[cb][1], qb,
                                 key - r0, rows_left, lane, a.c, keep, dr.scale, lo);
       }
     }
@@ -590,10 +606,10 @@ __device__ __forceinline__ void dq_chunk(bool diag, f32x16 (&dqacc)[D / 32],
         pr[i] = 32 * kb + 16 * (i / 8) + 8 * hi + i % 8 > qrow_minus_k0 ? 0.f : pr[i];
     }
   }
-  bf16x8 dsb[2];
+  bf16x8 dsb[2], dsl[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    u32x4 w;
+    u32x4 w, wl;
 #pragma unroll
     for (int e2 = 0; e2 < 4; ++e2) {
       float d[2];
@@ -607,14 +623,21 @@ __device__ __forceinline__ void dq_chunk(bool diag, f32x16 (&dqacc)[D / 32],
           d[h] = p * (FROM_DELTA ? dp[8 * j + e] : dp[8 * j + e] + ndl[0]);
       }
       w[e2] = pack_bf16x2(d[0], d[1]);
+      if constexpr (WIN) wl[e2] = pack_rest(d[0], d[1], w[e2]);
     }
     dsb[j] = as_bf16x8(w);
+    if constexpr (WIN) dsl[j] = as_bf16x8(wl);
   }
 #pragma unroll
-  for (int db = 0; db < DB; ++db) {
+  for (int j = 0; j < 2; ++j) {  // A = K^T: lane d = 32db + l32 gets keys 32kb + 16j + 8hi ..
+    bf16x8 kt[DB];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)  // A = K^T: lane d = 32db + l32 gets keys 32kb + 16j + 8hi ..
-      dqacc[db] = mfma32(lds_tr_op<D>(sk, 32 * kb + 16 * j, 32 * db, lane), dsb[j], dqacc[db]);
+    for (int db = 0; db < DB; ++db) kt[db] = lds_tr_op<D>(sk, 32 * kb + 16 * j, 32 * db, lane);
+    if constexpr (WIN)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) dqacc[db] = mfma32(kt[db], dsl[j], dqacc[db]);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dqacc[db] = mfma32(kt[db], dsb[j], dqacc[db]);
   }
 }
 
@@ -836,7 +859,7 @@ __device__ __forceinline__ void sink_workgroup(const BwdArgs& a, int bh, int gro
     if (!mine) continue;
     st[0][lane] *= a.lse_mul;
     st[1][lane] = -own_delta[min(r0 + lane, S - 1) - t0 * kTileRows];
-    dkdv_block<D, false, true>(r0 + kTileRows > S, dkacc, dvacc, kop, vop, tiles.a[at],
+    dkdv_block<D, false, true, true>(r0 + kTileRows > S, dkacc, dvacc, kop, vop, tiles.a[at],
                                tiles.b[at], st[0], st[1], qb, -1, S - r0, lane, a.c, 0, 0.f, lo);
   }
   // waves 2 and 3 to 0 and 1, then dK to wave 0 and dV to wave 1

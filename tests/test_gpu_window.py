@@ -84,6 +84,24 @@ def test_window_large_scores(gpu, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(64, 0), (200, 4)])
+@pytest.mark.parametrize("BH", [4, 120])
+def test_window_gradients_carry_ds_in_two_values(gpu, BH, window, sinks):
+    """dQ and dK in bf16 are off by little more than their own rounding. dS in one bf16 value would
+    add an error of the same size and independent of it (in all 2^0.5 times the rounding's); in two
+    it adds 2^-8 of that, and what is left beside the rounding is delta's error, a sum over d_head
+    of the output's, which is shared by a row's keys and a fraction of either."""
+    q, k, v, g = _inputs(BH, 900, 64, BF, seed=21)
+    got = _run(q, k, v, g, 0.125, window, sinks)
+    pick = slice(0, 4)
+    ref = R.attention(q[pick], k[pick], v[pick], g[pick], 0.125, window, sinks, BF)
+    for name in ("dq", "dk"):
+        exact = ref[name][0]
+        own = (exact.to(BF).double() - exact).norm()
+        assert (got[name][pick].double() - exact).norm() <= 1.25 * own, name
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("S,window", [(1, 1), (100, 100), (321, 4000), (1024, 2 ** 31 - 1)])
 def test_a_window_of_the_sequence_is_the_causal_call(gpu, dtype, S, window):

@@ -53,7 +53,9 @@ def attention(q, k, v, dout, scale, window, sinks, dtype):
     x = dp - delta
     ds = p * x
     e_ds = e_p * x.abs() + p * (e_dp + e_delta + (dp.abs() + delta.abs()) * 2.0 ** -22)
-    e_ds = e_ds + u * ds.abs()
+    # rounded to a bf16 value and the rest to another (a window of the sequence is the causal kernels',
+    # with one)
+    e_ds = e_ds + (u * u if bf16 and window < S else u) * ds.abs()
 
     def grad(a, e_a, b):                            # a b, a computed in the kernel with error e_a
         y = torch.bmm(a, b)
