@@ -892,9 +892,9 @@ __device__ __forceinline__ void sink_workgroup(const BwdArgs& a, int bh, int gro
 }
 
 // dQ (which writes delta), the sink keys' pieces in front: they are short, and the dQ workgroups
-// fill in behind them. B16 H12 T1024 D64, window 256, 4 sinks, token-major: 51 us, 42 of them without
-// sinks; dK/dV 44. Half of either is HBM time (150 MB, 29 us), which a window of 64 comes down to (32
-// and 32 us); P and dS are rounded to bf16 for the products, as without a window.
+// fill in behind them. B16 H12 T1024 D64, window 256, 4 sinks, token-major: 57 us, 46 of them without
+// sinks; dK/dV 51. Half of either is HBM time (150 MB, 29 us), which a window of 64 comes near (34
+// and 34 us).
 constexpr int kMaxPieceTiles = 12;
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, kDqMinBlocks) void window_dq_bf16_kernel(
@@ -1126,6 +1126,7 @@ WindowPlan window_plan(int BH, int S, int D, const Window& w) {
   auto end = [&](int block_keys) {  // of the first block, in tiles
     return ((long long)block_keys + w.window - 2) / kTileRows + 1;
   };
+  // (Times below with dS in one bf16 value; in two all of them are 3 to 15% longer.)
   // Sink blocks walk all later queries themselves (`whole`) where these are few, or in large grids few
   // next to the window: pieces and their join cost more than the longer chain (pieces -> whole,
   // backward, us: 192 x 256, window 64 21.0 -> 16.7, 180 x 500, 64 38.4 -> 34.9, 96 x 1024, 512 62.9 ->
