@@ -127,10 +127,11 @@ __global__ __launch_bounds__(64 * kWaves) void decode_kernel(
       mx = fmaxf(mx, s[i]);
     }
     mx = lanes::wave_max_of_groups<LPR>(mx);  // uniform within each row group already
-    // key0 < L, so key key0 is valid and mx is finite
+    // where every score is -inf, 0 stands in for the maximum: the keys' terms are 0
+    const float base = mx == neg_inf() ? 0.f : mx;
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
-      const float p = fast_exp2(s[i] - mx);  // exactly 0 for masked rows
+      const float p = fast_exp2(s[i] - base);  // exactly 0 for masked rows
       lsum += p;
       float vf[EPL];
       Elem<T>::unpack(vr[i], vf);

@@ -180,8 +180,9 @@ __device__ __forceinline__ void merge_chunks(MergeLds<D, WAVES>& sm, T* out, con
   if (tid < D) {
     // The partials of kMergeBatch chunks are all loaded before any is used (one memory round
     // trip per batch: this merge ends the kernel for the caches that finish last), and the
-    // batches merge online. Every chunk < nch holds a valid key: finite maxima. For
-    // nch <= kMergeBatch this is sum_c l_c 2^(m_c - max) in chunk order, as a two-pass merge.
+    // batches merge online. For nch <= kMergeBatch this is sum_c l_c 2^(m_c - max) in chunk
+    // order, as a two-pass merge. A chunk whose scores are all -inf has that as its maximum and
+    // weighs nothing; while there is no other, 0 stands in for the running maximum.
     constexpr int kMergeBatch = 4;
     float gm = neg_inf(), gl = 0.f, go = 0.f;
     for (int c0 = 0; c0 < nch; c0 += kMergeBatch) {
@@ -197,13 +198,14 @@ __device__ __forceinline__ void merge_chunks(MergeLds<D, WAVES>& sm, T* out, con
 #pragma unroll
       for (int j = 0; j < kMergeBatch; ++j)
         if (c0 + j < nch) bm = fmaxf(bm, mv[j]);
-      const float fo = fast_exp2(gm - bm);  // 0 before the first batch (gl = go = 0 then)
+      const float base = bm == neg_inf() ? 0.f : bm;
+      const float fo = fast_exp2(gm - base);  // 0 before the first batch (gl = go = 0 then)
       gl *= fo;
       go *= fo;
 #pragma unroll
       for (int j = 0; j < kMergeBatch; ++j)
         if (c0 + j < nch) {
-          const float f = fast_exp2(mv[j] - bm);
+          const float f = fast_exp2(mv[j] - base);
           gl += lv[j] * f;
           go += ov[j] * f;
         }

@@ -1,0 +1,80 @@
+"""GPU tests of the one-token calls at scores of -inf and at NaN: the windowed decode, the plain one
+and the 8-bit one, against float64 over the keys that weigh something."""
+import pytest
+import torch
+
+from dadgpt_amd import attention as A
+from dadgpt_amd import kv_cache as C
+from tests import kv_ref as R
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _randn(shape, seed, dtype=F32):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=gen, device="cuda").to(dtype)
+
+
+def _int(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _half(dtype):
+    return 2.0 ** -8 if dtype == BF else 2.0 ** -24
+
+
+def _without(k, v, keep):
+    """The rows of k and v that `keep` marks, in float64."""
+    return k[:, :, keep].double(), v[:, :, keep].double()
+
+
+# (rows, window, sinks, first and last key at -inf): whole waves (64 bf16 keys, 32 fp32 ones) and
+# whole chunks of eight waves, among the sinks, at the window's start, in the middle and at the end;
+# caches of one chunk and of several, the first batch of four chunks whole; windows below, just
+# below and at the cache's length
+MINUS_INF = [
+    (500, 300, 0, 200, 330), (500, 300, 130, 0, 130), (500, 499, 1, 64, 300), (500, 500, 0, 100, 400),
+    (500, 2 ** 31 - 1, 3, 0, 200), (3000, 2000, 600, 0, 600), (3000, 2600, 4, 400, 2999),
+    (3000, 2999, 0, 1, 1500), (3000, 3000, 0, 0, 2200), (3000, 2000, 0, 1500, 2900),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("L,window,sinks,lo,hi", MINUS_INF)
+def test_window_decode_of_scores_of_minus_infinity(gpu, dtype, L, window, sinks, lo, hi):
+    """Keys whose score is -inf weigh 0, also where a wave, a chunk or a batch of chunks holds
+    nothing else: the answer is that of the other visible keys alone."""
+    n, H, D, scale = 2, 2, 64, 0.125
+    q, k, v = (_randn(s, i, dtype) for i, s in enumerate(((n, H, D), (n, H, L, D), (n, H, L, D))))
+    q[..., 0] = 1
+    j = torch.arange(L, device="cuda")
+    seen = (j >= L - window) | (j < sinks)
+    keep = seen & ((j < lo) | (j >= hi))
+    m = int(keep.sum())
+    assert 0 < m < int(seen.sum())
+    ref, bound, _, _ = R.decode(q, *_without(k, v, keep), [m] * n, scale, out_half=_half(dtype))
+    k[:, :, lo:hi, 0] = -float("inf")
+    out = torch.full_like(q, float("nan"))
+    ws = A.decode_workspace(n, H, min(L, window + sinks), D)
+    for _ in range(2):  # the second call finds the workspace as the first left it
+        A.decode_attention_window(out, q, k, v, _int([L] * n), n, H, L, D, scale, window, sinks, ws)
+        assert ((out.double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("L,lo,hi", [(500, 0, 200), (250, 60, 249), (3000, 0, 2200), (3000, 700, 2900)])
+def test_decode_of_scores_of_minus_infinity(gpu, dtype, L, lo, hi):
+    """The same of the decode without a window."""
+    n, H, D, scale = 2, 2, 64, 0.125
+    q, k, v = (_randn(s, 5 + i, dtype) for i, s in enumerate(((n, H, D), (n, H, L, D), (n, H, L, D))))
+    q[..., 0] = 1
+    j = torch.arange(L, device="cuda")
+    keep = (j < lo) | (j >= hi)
+    ref, bound, _, _ = R.decode(q, *_without(k, v, keep), [int(keep.sum())] * n, scale,
+                                out_half=_half(dtype))
+    k[:, :, lo:hi, 0] = -float("inf")
+    out = torch.full_like(q, float("nan"))
+    A.decode_attention(out, q, k, v, _int([L] * n), n, H, L, D, scale, A.decode_workspace(n, H, L, D))
+    assert ((out.double() - ref).abs() <= bound).all()
