@@ -350,9 +350,11 @@ __global__ __launch_bounds__(64 * kKv8Waves) void kv8_decode_kernel(
       mx = fmaxf(mx, s[i]);
     }
     mx = lanes::group_max<64>(mx);
+    // where every score is -inf (past fp32's range), 0 stands in for the maximum
+    const float base = mx == neg_inf() ? 0.f : mx;
 #pragma unroll
     for (int i = 0; i < NLD; ++i) {
-      const float p = fast_exp2(s[i] - mx);  // exactly 0 for masked keys
+      const float p = fast_exp2(s[i] - base);  // exactly 0 for masked keys
       lsum += p;
       const float pv = p * vs[i];
 #pragma unroll

@@ -78,3 +78,39 @@ def test_decode_of_scores_of_minus_infinity(gpu, dtype, L, lo, hi):
     out = torch.full_like(q, float("nan"))
     A.decode_attention(out, q, k, v, _int([L] * n), n, H, L, D, scale, A.decode_workspace(n, H, L, D))
     assert ((out.double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("L,window,sinks,lo,hi", [
+    (500, 0, 0, 0, 256), (500, 400, 4, 160, 448), (6000, 0, 0, 0, 5888), (6000, 0, 0, 1088, 5888),
+    (6000, 5000, 128, 0, 4864)])
+def test_kv8_decode_of_scores_past_fp32(gpu, dtype, L, window, sinks, lo, hi):
+    """Keys whose score lies below fp32's range weigh 0, also where a wave (128 keys), a chunk (1024)
+    or a batch of chunks holds nothing else: the answer is that of the other keys alone."""
+    n, H, D, block, scale = 2, 2, 64, 32, 0.125
+    cache = C.kv8_cache(n, H, L, D, block)
+    for i, (codes, scales) in enumerate(((cache[0], cache[2]), (cache[1], cache[3]))):
+        codes.copy_((_randn((n, H, L, D), 60 + i) * 16).to(C.KV8_DTYPE))
+        scales.fill_(2.0 ** -4)
+    cache[0].view(torch.uint8)[..., 0] = 0
+    q = _randn((n, H, D), 62, dtype)
+    q[..., 0] = 2.0 ** 100
+    j = torch.arange(L, device="cuda")
+    keep = (j < lo) | (j >= hi)
+    if window:
+        keep &= (j >= L - window) | (j < sinks)
+    row = j // block
+    k, v = (R.values(c.view(torch.uint8)) * s.double()[:, :, row, None]
+            for c, s in ((cache[0], cache[2]), (cache[1], cache[3])))
+    ref, bound, _, _ = R.decode(q, *_without(k, v, keep), [int(keep.sum())] * n, scale,
+                                out_half=_half(dtype))
+    # codes of -256 in the column of 2^100, blocks of scale 2^40 there: scores of -2^145
+    cache[0].view(torch.uint8)[:, :, lo:hi, 0] = 0xF8
+    cache[2][:, :, lo // block:hi // block] = 2.0 ** 40
+    out = torch.full_like(q, float("nan"))
+    ws = C.decode_kv8_workspace(n, H, L, D)
+    for _ in range(2):
+        C.decode_attention_kv8(out, q, *cache, _int([L] * n), n, H, L, D, block, scale, window, sinks,
+                               ws)
+        assert ((out.double() - ref).abs() <= bound).all()
