@@ -114,3 +114,34 @@ def test_kv8_decode_of_scores_past_fp32(gpu, dtype, L, window, sinks, lo, hi):
         C.decode_attention_kv8(out, q, *cache, _int([L] * n), n, H, L, D, block, scale, window, sinks,
                                ws)
         assert ((out.double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("L", [200, 2500])
+def test_window_decode_of_a_nan_row_does_not_depend_on_the_window(gpu, dtype, L):
+    """A visible key of NaN makes its (sequence, head) NaN and no other, for windows below, at and
+    past the cache's length."""
+    n, H, D = 2, 2, 64
+    q, k, v = (_randn(s, 70 + i, dtype) for i, s in enumerate(((n, H, D), (n, H, L, D), (n, H, L, D))))
+    k[1, 0, L - 3, 5] = float("nan")
+    ws = A.decode_workspace(n, H, L, D)
+    for window, sinks in ((64, 0), (L - 1, 0), (L - 2, 2), (L, 0), (L, 7), (2 ** 31 - 1, 1)):
+        out = torch.zeros_like(q)
+        A.decode_attention_window(out, q, k, v, _int([L, L]), n, H, L, D, 0.125, window, sinks, ws)
+        bad = torch.isnan(out)
+        assert bad.all(-1).tolist() == bad.any(-1).tolist() == [[False, False], [True, False]], window
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("n,H,L,D", [(5, 3, 1, 64), (6, 3, 250, 32), (6, 2, 1024, 64), (5, 2, 5000, 64)])
+def test_window_decode_of_the_whole_cache_is_the_plain_decode(gpu, dtype, n, H, L, D):
+    q, k, v = (_randn(s, 80 + i, dtype) for i, s in enumerate(((n, H, D), (n, H, L, D), (n, H, L, D))))
+    lens = _int([L, 0, 1, L // 2, L + 5, max(L - 1, 0)][:n])
+    ws = A.decode_workspace(n, H, L, D)
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    A.decode_attention(want, q, k, v, lens, n, H, L, D, 0.125, ws)
+    for window, sinks in ((L, 0), (max(1, L - 3), 4), (2 ** 31 - 1, 1024)):
+        A.decode_attention_window(out, q, k, v, lens, n, H, L, D, 0.125, window, sinks, ws)
+        assert torch.equal(out, want), (window, sinks)
