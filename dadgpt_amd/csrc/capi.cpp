@@ -4,6 +4,7 @@
 // returns a status instead of throwing across the C boundary.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -215,27 +216,86 @@ int check_decode_window(const char* fn, int n_seq, int H, int max_len, int d_hea
                       ws, ws_bytes, ptrs);
 }
 
-// The windowed backward's workspace, and that no gradient shares memory with an input or it: the
-// sink keys' pieces read K and V, and the join writes dK and dV, long after a workgroup has
-// written its own rows. `size` is a tensor's extent in bytes by its index in AttnTensor.
-int check_window_backward(const char* fn, int BH, int S, int d_head, const dadgpt::Window& w,
-                          const void* ws, size_t ws_bytes, const void* const (&tensor)[8],
-                          const size_t (&size)[8]) {
-  const size_t need = dadgpt::window_workspace_bytes(BH, S, d_head, w);
-  if (need > 0 && (ws == nullptr || ws_bytes < need))
+// Whether two [B, H, S, D] tensors of the same strides (elements) have an element in common, the
+// second `off` elements behind the first: whether off is b * batch + h * head + s * row + d for some
+// |b| < B, |h| < H, |s| < S, |d| < D. Searched from the largest stride down, few steps where the
+// tensor's own rows lie apart; rows that do not are not told apart further than kSteps.
+struct StrideDim {
+  long long stride, most;  // most: the largest index
+};
+bool rows_meet(long long off, const StrideDim* dim, const StrideDim* end, long long d, int* steps) {
+  if (dim == end) return off < d && -off < d;
+  long long reach = d - 1;  // of the dimensions after this one
+  for (const StrideDim* x = dim + 1; x != end; ++x) reach += x->stride * x->most;
+  if (dim->stride == 0) return rows_meet(off, dim + 1, end, d, steps);
+  // |off - i * stride| <= reach
+  const long long up = off + reach, low = off - reach;
+  long long i = low >= 0 ? (low + dim->stride - 1) / dim->stride : -(-low / dim->stride);
+  long long last = up >= 0 ? up / dim->stride : -((-up + dim->stride - 1) / dim->stride);
+  if (i < -dim->most) i = -dim->most;
+  if (last > dim->most) last = dim->most;
+  constexpr int kSteps = 4096;
+  for (; i <= last && ++*steps <= kSteps; ++i)
+    if (rows_meet(off - i * dim->stride, dim + 1, end, d, steps)) return true;
+  return false;
+}
+
+// Two gradients of a windowed backward: apart as a whole, or by rows where their strides agree
+// (where they do not, that is the caller's to see to).
+bool gradients_meet(const void* a, const void* b, size_t a_bytes, size_t b_bytes,
+                    const dadgpt::HeadStrides& sa, const dadgpt::HeadStrides& sb, int batch, int H,
+                    int S, int d_head, int elem_bytes) {
+  if (!dadgpt::overlap({a, a_bytes}, {b, b_bytes})) return false;
+  if (a == b) return true;
+  if (sa.batch != sb.batch || sa.head != sb.head || sa.row != sb.row) return false;
+  StrideDim dims[3] = {{sa.batch, batch - 1}, {sa.head, H - 1}, {sa.row, S - 1}};
+  std::sort(dims, dims + 3, [](const StrideDim& x, const StrideDim& y) { return x.stride > y.stride; });
+  const long long off = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / elem_bytes;
+  int steps = 0;
+  return rows_meet(off, dims, dims + 3, d_head, &steps);
+}
+
+// The windowed backward's buffers. No output (dQ, dK, dV, delta, the workspace) shares memory with
+// another or an input: the sink keys' pieces read K and V, and the join writes dK and dV, long after
+// a workgroup has written its own rows. Gradients may lie in one buffer by rows.
+int check_window_backward(const char* fn, int batch, int H, int S, int d_head, int elem_bytes,
+                          const dadgpt::AttnLayout& L, const dadgpt::Window& w, const void* ws,
+                          size_t ws_bytes, const void* const (&tensor)[8], const float* delta,
+                          const float* lse) {
+  static const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv", "lse", "delta"};
+  constexpr int kLse = dadgpt::kAttnTensors, kDelta = kLse + 1, kAll = kDelta + 1;
+  dadgpt::Span span[kAll];
+  for (int t = 0; t < dadgpt::kAttnTensors; ++t)
+    span[t] = {tensor[t], elem_bytes * ((size_t)(batch - 1) * L.t[t].batch +
+                                        (size_t)(H - 1) * L.t[t].head +
+                                        (size_t)(S - 1) * L.t[t].row + d_head)};
+  span[kLse] = {lse, sizeof(float) * batch * H * S};
+  span[kDelta] = {delta, sizeof(float) * batch * H * S};
+  auto meet = [&](int a, int b) {
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: %s overlaps %s", fn, names[a], names[b]);
+  };
+  constexpr int kInputs[] = {dadgpt::kTQ,  dadgpt::kTK,  dadgpt::kTV,
+                             dadgpt::kTO,  dadgpt::kTDO, kLse};
+  for (int g : {(int)dadgpt::kTDQ, (int)dadgpt::kTDK, (int)dadgpt::kTDV, kDelta})
+    for (int t : kInputs)
+      if (dadgpt::overlap(span[g], span[t])) return meet(g, t);
+  for (int g = dadgpt::kTDQ; g <= dadgpt::kTDV; ++g) {
+    if (dadgpt::overlap(span[g], span[kDelta])) return meet(g, kDelta);
+    for (int o = g + 1; o <= dadgpt::kTDV; ++o)
+      if (gradients_meet(tensor[g], tensor[o], span[g].bytes, span[o].bytes, L.t[g], L.t[o], batch, H,
+                         S, d_head, elem_bytes))
+        return meet(g, o);
+  }
+  const size_t need = dadgpt::window_workspace_bytes(batch * H, S, d_head, w);
+  if (need == 0) return DADGPT_OK;
+  if (ws == nullptr || ws_bytes < need)
     return fail(DADGPT_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", fn,
                 ws == nullptr ? 0 : ws_bytes, need);
-  if (need > 0 && reinterpret_cast<uintptr_t>(ws) % 16 != 0)
+  if (reinterpret_cast<uintptr_t>(ws) % 16 != 0)
     return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: workspace is not 16-byte aligned", fn);
-  static const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv"};
-  for (int g = dadgpt::kTDQ; g <= dadgpt::kTDV; ++g) {
-    const dadgpt::Span grad{tensor[g], size[g]};
-    for (int t = dadgpt::kTQ; t <= dadgpt::kTDO; ++t)
-      if (dadgpt::overlap(grad, dadgpt::Span{tensor[t], size[t]}))
-        return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: %s overlaps %s", fn, names[g], names[t]);
-    if (need > 0 && dadgpt::overlap(grad, dadgpt::Span{ws, need}))
-      return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: %s overlaps the workspace", fn, names[g]);
-  }
+  for (int t = 0; t < kAll; ++t)
+    if (dadgpt::overlap(span[t], {ws, need}))
+      return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: %s overlaps the workspace", fn, names[t]);
   return DADGPT_OK;
 }
 
@@ -545,9 +605,9 @@ int dadgpt_flash_attention_window_backward(float* dq, float* dk, float* dv, floa
     return st;
   if (int st = check_window(fn, S, window, sinks)) return st;
   const dadgpt::Window w{window, sinks};
-  const size_t n = sizeof(float) * BH * S * d_head;
-  if (int st = check_window_backward(fn, BH, S, d_head, w, workspace, workspace_bytes,
-                                     {q, k, v, out, dout, dq, dk, dv}, {n, n, n, n, n, n, n, n}))
+  if (int st = check_window_backward(fn, BH, 1, S, d_head, sizeof(float),
+                                     dadgpt::contiguous_layout(S, d_head), w, workspace,
+                                     workspace_bytes, {q, k, v, out, dout, dq, dk, dv}, delta, lse))
     return st;
   return from_hip(dadgpt::launch_window_bwd_f32(dq, dk, dv, delta, dout, out, lse, q, k, v, BH, S,
                                                 d_head, scale, w, workspace, workspace_bytes,
@@ -582,9 +642,9 @@ int dadgpt_flash_attention_window_backward_bf16(uint16_t* dq, uint16_t* dk, uint
     return st;
   if (int st = check_window(fn, S, window, sinks)) return st;
   const dadgpt::Window w{window, sinks};
-  const size_t n = sizeof(uint16_t) * BH * S * d_head;
-  if (int st = check_window_backward(fn, BH, S, d_head, w, workspace, workspace_bytes,
-                                     {q, k, v, out, dout, dq, dk, dv}, {n, n, n, n, n, n, n, n}))
+  if (int st = check_window_backward(fn, BH, 1, S, d_head, sizeof(uint16_t),
+                                     dadgpt::contiguous_layout(S, d_head), w, workspace,
+                                     workspace_bytes, {q, k, v, out, dout, dq, dk, dv}, delta, lse))
     return st;
   return from_hip(dadgpt::launch_window_bwd_bf16(B(dq), B(dk), B(dv), delta, B(dout), B(out), lse,
                                                  B(q), B(k), B(v), BH, S, d_head, scale,
@@ -621,12 +681,8 @@ int dadgpt_flash_attention_window_backward_bf16_strided(
     return st;
   if (int st = check_window(fn, S, window, sinks)) return st;
   const dadgpt::Window w{window, sinks};
-  size_t n[8];
-  for (int t = 0; t < 8; ++t)
-    n[t] = sizeof(uint16_t) * ((size_t)(batch - 1) * L.t[t].batch + (size_t)(H - 1) * L.t[t].head +
-                               (size_t)(S - 1) * L.t[t].row + d_head);
-  if (int st = check_window_backward(fn, batch * H, S, d_head, w, workspace, workspace_bytes,
-                                     {q, k, v, out, dout, dq, dk, dv}, n))
+  if (int st = check_window_backward(fn, batch, H, S, d_head, sizeof(uint16_t), L, w, workspace,
+                                     workspace_bytes, {q, k, v, out, dout, dq, dk, dv}, delta, lse))
     return st;
   return from_hip(dadgpt::launch_window_bwd_bf16(B(dq), B(dk), B(dv), delta, B(dout), B(out), lse,
                                                  B(q), B(k), B(v), batch * H, S, d_head, scale, L,

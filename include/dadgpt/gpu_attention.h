@@ -265,9 +265,11 @@ int dadgpt_decode_attention_f32(float* out, const float* q, const float* k_cache
  * sums over all later queries, which are split and joined through it in a fixed order, so a call
  * repeats bit for bit. The workspace needs no initial contents and holds nothing between calls;
  * calls that overlap in time (two streams, two captured graphs replayed at once) need one each.
- * No output of a windowed backward may overlap another output, an input or the workspace. A
- * gradient whose extent, first to last element, meets an input's or the workspace's is refused, so
- * the gradients' rows may be interleaved with each other's but not with the inputs'. */
+ * No output of a windowed backward (the gradients, delta, the workspace) may overlap another output
+ * or an input, and a call in which one does is refused: by their extents, first to last element, so
+ * gradients may not be interleaved with inputs; gradients of the same strides among each other by
+ * their rows, which may be interleaved. (Gradients of different strides that share a stretch of
+ * memory are the caller's to keep apart.) */
 #define DADGPT_WINDOW_MAX_SINKS 1024
 #define DADGPT_WINDOW_MAX_SEQ (1 << 19)
 size_t dadgpt_flash_attention_window_workspace_bytes(int BH, int S, int d_head, int window,

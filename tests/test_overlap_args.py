@@ -1,0 +1,102 @@
+"""CPU tests of what the windowed backward, the 8-bit and the weighted decode refuse because two of
+a call's buffers share memory or the workspace is not aligned. Every check answers on the host before
+any HIP call: a call whose buffers are apart gets as far as a workspace that is missing (status 4)."""
+import ctypes
+
+import pytest
+
+from dadgpt_amd import attention as A
+from dadgpt_amd import kv_cache as C
+
+FAKE, STEP = 0x1000000, 0x10000000  # non-null addresses, far apart
+
+
+def _ptrs(n):
+    return [FAKE + i * STEP for i in range(n)]
+
+
+# ------------------------------------------------------------- windowed backward
+
+BWD = ("dq", "dk", "dv", "delta", "dout", "out", "lse", "q", "k", "v")
+BH, S, D = 4, 2000, 64
+
+
+def _bwd(name, ptrs, ws=None, wsb=0):
+    return getattr(A.lib(), "dadgpt_flash_attention_window_" + name)(
+        *ptrs, BH, S, D, 0.125, 16, 2, ws, wsb, None)
+
+
+@pytest.mark.parametrize("name,size", [("backward", 4), ("backward_bf16", 2)])
+def test_window_backward_refuses_outputs_over_each_other(name, size):
+    nbytes = {n: BH * S * D * size for n in BWD}
+    nbytes["delta"] = nbytes["lse"] = BH * S * 4
+    need = A.window_workspace_bytes(BH, S, D, 16, 2)
+    assert _bwd(name, _ptrs(10)) == 4  # apart: the missing workspace
+    pairs = [("dq", "dk"), ("dq", "dv"), ("dk", "dv")]
+    pairs += [(g, n) for g in ("dq", "dk", "dv") for n in ("delta", "lse")]
+    pairs += [("delta", n) for n in ("dout", "out", "lse", "q", "k", "v")]
+    for a, b in pairs:
+        # from the same address, with the last bytes shared, with the first bytes shared
+        for at in (0, nbytes[b] - 16, 16 - nbytes[a]):
+            p = _ptrs(10)
+            p[BWD.index(a)] = p[BWD.index(b)] + at
+            assert _bwd(name, p) == 1, (a, b, at)
+            assert f"{a} overlaps {b}" in A.last_error(), (a, b, at, A.last_error())
+        for at in (nbytes[b], -nbytes[a]):  # side by side
+            p = _ptrs(10)
+            p[BWD.index(a)] = p[BWD.index(b)] + at
+            assert _bwd(name, p) == 4, (a, b, at, A.last_error())
+    for n in BWD:
+        p = _ptrs(10)
+        assert _bwd(name, p, p[BWD.index(n)] + nbytes[n] - 16, need) == 1
+        assert f"{n} overlaps the workspace" in A.last_error()
+
+
+def _strides(*rows):
+    return (A.HeadStrides * len(rows))(*[A.HeadStrides(*r) for r in rows])
+
+
+def test_window_backward_in_rows_of_one_buffer():
+    """Gradients side by side in one projection's rows are apart, a column or a head into each other
+    they are not."""
+    B, H = 2, 12
+    d = H * D
+    tok = A.lib().dadgpt_flash_attention_window_backward_bf16_tokens
+    strided = A.lib().dadgpt_flash_attention_window_backward_bf16_strided
+
+    def both(dq, dk, dv, ld):
+        p = _ptrs(10)
+        p[:3] = dq, dk, dv
+        a = tok(p[0], p[1], p[2], ld, p[3], p[4], p[5], d, p[6], p[7], p[8], p[9], 3 * d, B, H, S, D,
+                0.125, 16, 2, None, 0, None)
+        text = A.last_error()
+        g, x, o = (ld * S, D, ld), (3 * d * S, D, 3 * d), (d * S, D, d)
+        b = strided(*p, B, H, S, D, 0.125, 16, 2, _strides(x, x, x, o, o, g, g, g), None, 0, None)
+        assert a == b and text.split(": ")[1:] == A.last_error().split(": ")[1:]
+        return a, text
+
+    base = FAKE
+    assert both(base, base + 2 * d, base + 4 * d, 3 * d)[0] == 4
+    assert both(base + 4 * d, base, base + 2 * d, 3 * d)[0] == 4
+    assert both(base, base + 2 * d, base + 4 * d, 3 * d + 64)[0] == 4
+    for dq, dk, dv, text in (
+            (base, base, base + 2 * d, "dq overlaps dk"),
+            (base, base + 2 * d, base + 2 * d, "dk overlaps dv"),
+            (base, base + 2 * d - 16, base + 4 * d, "dq overlaps dk"),
+            (base, base + 2 * d, base + 4 * d + 16, "dq overlaps dv"),  # into the next row
+            (base + 6 * d * 100, base + 2 * d, base + 6 * d * 1500 + 128, "dq overlaps dv"),
+            (base, base + 2 * d, base + 4 * d - 2 * D, "dk overlaps dv")):
+        status, got = both(dq, dk, dv, 3 * d)
+        assert status == 1 and text in got, (text, got)
+    # one gradient in the gaps of another, a row further down
+    assert both(base, base + 6 * d + 2 * d, base + 4 * d, 3 * d)[0] == 4
+    # head-major buffers: whole slices, side by side and one row into each other
+    h = (H * S * D, S * D, D)
+    n = B * H * S * D * 2
+    p = _ptrs(10)
+    p[1], p[2] = p[0] + n, p[0] - n
+    st = _strides(h, h, h, h, h, h, h, h)
+    assert strided(*p, B, H, S, D, 0.125, 16, 2, st, None, 0, None) == 4
+    p[1] = p[0] + n - 2 * D
+    assert strided(*p, B, H, S, D, 0.125, 16, 2, st, None, 0, None) == 1
+    assert "dq overlaps dk" in A.last_error()
