@@ -97,28 +97,42 @@ int append(const char* fn, uint8_t* k8, uint8_t* v8, float* k_scale, float* v_sc
   const size_t scales = caches * ((max_len + block - 1) / block) * sizeof(float);
   const NamedSpan K{{k8, codes}, "k_cache"}, V{{v8, codes}, "v_cache"};
   const NamedSpan KS{{k_scale, scales}, "k_scale"}, VS{{v_scale, scales}, "v_scale"};
+  auto extent = [&](const dadgpt::HeadStrides64& t) {
+    return sizeof(T) * ((size_t)(n_seq - 1) * t.batch + (size_t)(H - 1) * t.head +
+                        (size_t)(rows - 1) * t.row + d_head);
+  };
   if (int st = check_apart(fn, {K, V, KS, VS},
-                           {{{lens, 4 * (size_t)n_seq}, "lens"},
+                           {{{k, extent(ks)}, "k"},
+                            {{v, extent(vs)}, "v"},
+                            {{lens, 4 * (size_t)n_seq}, "lens"},
                             {{counts, 4 * (size_t)n_seq}, "counts"}}))
     return st;
   return from_hip(launch(ks, vs), fn);
 }
 
-int check_workspace(const char* fn, const void* ws, size_t ws_bytes, size_t need) {
+// The workspace, and that what the call uses of it (`used` bytes) lies apart from its other buffers.
+int check_workspace(const char* fn, const void* ws, size_t ws_bytes, size_t need, size_t used,
+                    std::initializer_list<NamedSpan> others) {
   if (need == 0) return DADGPT_OK;
   if (ws == nullptr || ws_bytes < need)
     return fail(DADGPT_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", fn,
                 ws == nullptr ? 0 : ws_bytes, need);
   if (reinterpret_cast<uintptr_t>(ws) % 16 != 0)
     return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: workspace is not 16-byte aligned", fn);
-  return DADGPT_OK;
+  return check_apart(fn, {{{ws, used}, "the workspace"}}, others);
 }
 
-// Shared checks of the 8-bit decode; *w is the window where there is one.
+// An output row replaces the query that only its own workgroups have read, or lies apart from it.
+NamedSpan query(const void* q, const void* out, size_t bytes) {
+  return {{q == out ? nullptr : q, bytes}, "q"};
+}
+
+// Shared checks of the 8-bit decode (`elem_bytes` of q and out); window 0: none.
 int check_kv8_decode(const char* fn, const void* out, const void* q, const uint8_t* k8,
                      const uint8_t* v8, const float* k_scale, const float* v_scale,
                      const int32_t* lens, int n_seq, int H, int max_len, int d_head, int block,
-                     float scale, int window, int sinks, const void* ws, size_t ws_bytes) {
+                     int elem_bytes, float scale, int window, int sinks, const void* ws,
+                     size_t ws_bytes) {
   if (int st = check_decode_shape(fn, n_seq, H, max_len, d_head, scale, {out, q, k8, v8}))
     return st;
   if (int st = check_words(fn, {{k_scale, "k_scale"}, {v_scale, "v_scale"}, {lens, "lens"}}))
@@ -132,26 +146,39 @@ int check_kv8_decode(const char* fn, const void* out, const void* q, const uint8
     if (int st = check_window(fn, 0, window, sinks)) return st;
     most = dadgpt::visible_keys(max_len, {window, sinks});
   }
+  const size_t caches = (size_t)n_seq * H, row = caches * d_head * elem_bytes;
+  const size_t codes = caches * max_len * d_head;
+  const size_t scales = caches * ((max_len + block - 1) / block) * sizeof(float);
+  const NamedSpan O{{out, row}, "out"}, K{{k8, codes}, "k_cache"}, V{{v8, codes}, "v_cache"};
+  const NamedSpan KS{{k_scale, scales}, "k_scale"}, VS{{v_scale, scales}, "v_scale"};
+  const NamedSpan len{{lens, 4 * (size_t)n_seq}, "lens"};
+  if (int st = check_apart(fn, {O}, {query(q, out, row), K, V, KS, VS, len})) return st;
+  // (counters at its start, partials against its end)
   return check_workspace(fn, ws, ws_bytes,
-                         dadgpt::kv8_decode_workspace_bytes(n_seq, H, most, d_head));
+                         dadgpt::kv8_decode_workspace_bytes(n_seq, H, most, d_head), ws_bytes,
+                         {O, {{q, row}, "q"}, K, V, KS, VS, len});
 }
 
 int check_weights_decode(const char* fn, const void* out, const float* wout, const void* q,
                          const void* kc, const void* vc, const float* weights,
                          const int32_t* lens, int n_seq, int H, int max_len, int d_head,
-                         float scale, const void* ws, size_t ws_bytes) {
+                         int elem_bytes, float scale, const void* ws, size_t ws_bytes) {
   if (int st = check_decode_shape(fn, n_seq, H, max_len, d_head, scale, {out, q, kc, vc}))
     return st;
   if (int st = check_words(
           fn, {{wout, "weights_out"}, {weights, "weights"}, {lens, "lens"}}))
     return st;
-  if (wout != weights) {
-    const size_t n = sizeof(float) * n_seq * H * max_len;
-    if (int st = check_apart(fn, {{{wout, n}, "weights_out"}}, {{{weights, n}, "weights"}}))
-      return st;
-  }
-  return check_workspace(fn, ws, ws_bytes,
-                         dadgpt::weights_decode_workspace_bytes(n_seq, H, max_len, d_head));
+  const size_t caches = (size_t)n_seq * H, row = caches * d_head * elem_bytes;
+  const size_t w = sizeof(float) * caches * max_len, cache = row * max_len;
+  const NamedSpan O{{out, row}, "out"}, W{{wout, w}, "weights_out"};
+  const NamedSpan K{{kc, cache}, "k_cache"}, V{{vc, cache}, "v_cache"};
+  const NamedSpan win{{wout == weights ? nullptr : weights, w}, "weights"};
+  const NamedSpan len{{lens, 4 * (size_t)n_seq}, "lens"};
+  if (int st = check_apart(fn, {O}, {W, query(q, out, row), K, V, {{weights, w}, "weights"}, len}))
+    return st;
+  if (int st = check_apart(fn, {W}, {{{q, row}, "q"}, K, V, win, len})) return st;
+  const size_t need = dadgpt::weights_decode_workspace_bytes(n_seq, H, max_len, d_head);
+  return check_workspace(fn, ws, ws_bytes, need, need, {O, W, {{q, row}, "q"}, K, V, win, len});
 }
 
 int evict(const char* fn, void* k_out, void* v_out, float* wout, int32_t* kept,
@@ -262,8 +289,8 @@ int dadgpt_decode_attention_kv8_bf16(uint16_t* out, const uint16_t* q, const uin
                                      size_t workspace_bytes, void* stream) {
   const char* fn = "dadgpt_decode_attention_kv8_bf16";
   if (int st = check_kv8_decode(fn, out, q, k_cache, v_cache, k_scale, v_scale, lens, n_seq,
-                                n_heads, max_len, d_head, block, scale, window, sinks, workspace,
-                                workspace_bytes))
+                                n_heads, max_len, d_head, block, sizeof(*out), scale, window, sinks,
+                                workspace, workspace_bytes))
     return st;
   const dadgpt::Window w{window, sinks};
   return from_hip(dadgpt::launch_kv8_decode_bf16(
@@ -281,8 +308,8 @@ int dadgpt_decode_attention_kv8_f32(float* out, const float* q, const uint8_t* k
                                     size_t workspace_bytes, void* stream) {
   const char* fn = "dadgpt_decode_attention_kv8_f32";
   if (int st = check_kv8_decode(fn, out, q, k_cache, v_cache, k_scale, v_scale, lens, n_seq,
-                                n_heads, max_len, d_head, block, scale, window, sinks, workspace,
-                                workspace_bytes))
+                                n_heads, max_len, d_head, block, sizeof(*out), scale, window, sinks,
+                                workspace, workspace_bytes))
     return st;
   const dadgpt::Window w{window, sinks};
   return from_hip(dadgpt::launch_kv8_decode_f32(out, q, k_cache, v_cache, k_scale, v_scale, lens,
@@ -304,7 +331,8 @@ int dadgpt_decode_attention_weights_bf16(uint16_t* out, float* weights_out, cons
                                          void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "dadgpt_decode_attention_weights_bf16";
   if (int st = check_weights_decode(fn, out, weights_out, q, k_cache, v_cache, weights, lens, n_seq,
-                                    n_heads, max_len, d_head, scale, workspace, workspace_bytes))
+                                    n_heads, max_len, d_head, sizeof(*out), scale, workspace,
+                                    workspace_bytes))
     return st;
   return from_hip(dadgpt::launch_weights_decode_bf16(
                       B(out), weights_out, B(q), B(k_cache), B(v_cache), weights, lens, n_seq,
@@ -319,7 +347,8 @@ int dadgpt_decode_attention_weights_f32(float* out, float* weights_out, const fl
                                         void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "dadgpt_decode_attention_weights_f32";
   if (int st = check_weights_decode(fn, out, weights_out, q, k_cache, v_cache, weights, lens, n_seq,
-                                    n_heads, max_len, d_head, scale, workspace, workspace_bytes))
+                                    n_heads, max_len, d_head, sizeof(*out), scale, workspace,
+                                    workspace_bytes))
     return st;
   return from_hip(dadgpt::launch_weights_decode_f32(out, weights_out, q, k_cache, v_cache, weights,
                                                     lens, n_seq, n_heads, max_len, d_head, scale,

@@ -6,6 +6,7 @@
  * Conventions, status codes and dadgpt_last_error() as <dadgpt/gpu_attention.h>: device pointers,
  * 16-byte aligned unless an entry says otherwise; every argument checked on the host before any
  * HIP call; work on `stream` (NULL: the null stream) of the current device; nothing allocated.
+ * Outputs and workspaces that overlap each other or an input are refused, except as an entry says.
  * Cache layout [n_seq, n_heads, max_len, d_head] as the decode calls', d_head 32 or 64; lens are
  * DEVICE int32 [n_seq], clamped to [0, max_len].
  */
@@ -54,8 +55,8 @@ int dadgpt_kv8_append_f32(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, fl
                           const int32_t* counts, int n_seq, int n_heads, int rows, int max_len,
                           int d_head, int block, void* stream);
 
-/* Decode attention over an 8-bit cache (q and out bf16 or fp32 [n_seq, n_heads, d_head]; any float
- * scales). window = 0 sees every row below lens[s] (sinks must be 0 then); window >= 1 has the mask
+/* Decode attention over an 8-bit cache (q and out bf16 or fp32 [n_seq, n_heads, d_head], out may be
+ * q; any float scales). window = 0 sees every row below lens[s] (sinks must be 0 then); window >= 1 has the mask
  * of dadgpt_decode_attention_window_*. A length of 0 gives a zero output row. The workspace is as
  * the decode calls': dadgpt_decode_kv8_workspace_bytes (0: NULL allowed), sized for the largest
  * shape it serves, ZERO-FILLED once, and passed whole; every call leaves its counters at zero.
@@ -79,8 +80,8 @@ int dadgpt_decode_attention_kv8_f32(float* out, const float* q, const uint8_t* k
 
 /* The decode of dadgpt_decode_attention_{bf16,f32}, which also accumulates every key's attention
  * probability: weights_out[s][h][j] = weights[s][h][j] + p_j for j < lens[s], and weights[s][h][j]
- * from there on. The caller sets a row's weight (to 0) when it appends the row. weights and
- * weights_out are fp32 [n_seq, n_heads, max_len], 4-byte aligned, and may be one buffer; otherwise
+ * from there on. The caller sets a row's weight (to 0) when it appends the row. out may be q. weights
+ * and weights_out are fp32 [n_seq, n_heads, max_len], 4-byte aligned, and may be one buffer; otherwise
  * they must not overlap. The workspace (dadgpt_decode_weights_workspace_bytes, 0: NULL allowed)
  * needs no initial contents and holds nothing between calls; calls that overlap in time need one
  * each. */

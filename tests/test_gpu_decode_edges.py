@@ -145,3 +145,27 @@ def test_window_decode_of_the_whole_cache_is_the_plain_decode(gpu, dtype, n, H, 
     for window, sinks in ((L, 0), (max(1, L - 3), 4), (2 ** 31 - 1, 1024)):
         A.decode_attention_window(out, q, k, v, lens, n, H, L, D, 0.125, window, sinks, ws)
         assert torch.equal(out, want), (window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("L", [300, 700, 5000])
+def test_decode_into_the_query(gpu, dtype, L):
+    """The 8-bit decode and the decode with weights may write out over q: the bits of a call that
+    does not."""
+    n, H, D, block = 5, 3, 64, 32
+    q, k, v = (_randn(s, 90 + i, dtype) for i, s in enumerate(((n, H, D), (n, H, L, D), (n, H, L, D))))
+    cache = C.kv8_cache(n, H, L, D, block)
+    lens = _int([L, 0, 1, L - 1, L // 2])
+    C.kv8_append(*cache, k, v, _int([0] * n), None, n, H, L, L, D, block)
+    ws8, wsw = C.decode_kv8_workspace(n, H, L, D), C.decode_weights_workspace(n, H, L, D)
+    w = torch.zeros((n, H, L), device="cuda")
+    for window, sinks in ((0, 0), (L // 2, 3)):
+        want, out = torch.empty_like(q), q.clone()
+        C.decode_attention_kv8(want, q, *cache, lens, n, H, L, D, block, 0.125, window, sinks, ws8)
+        C.decode_attention_kv8(out, out, *cache, lens, n, H, L, D, block, 0.125, window, sinks, ws8)
+        assert torch.equal(out, want)
+    want, out, w1, w2 = torch.empty_like(q), q.clone(), w.clone(), w.clone()
+    C.decode_attention_weights(want, w1, q, k, v, w, lens, n, H, L, D, 0.125, wsw)
+    C.decode_attention_weights(out, w2, out, k, v, w, lens, n, H, L, D, 0.125, wsw)
+    assert torch.equal(out, want) and torch.equal(w1, w2)

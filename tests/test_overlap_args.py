@@ -100,3 +100,92 @@ def test_window_backward_in_rows_of_one_buffer():
     p[1] = p[0] + n - 2 * D
     assert strided(*p, B, H, S, D, 0.125, 16, 2, st, None, 0, None) == 1
     assert "dq overlaps dk" in A.last_error()
+
+
+# ------------------------------------------------------------- caches
+
+@pytest.mark.parametrize("name,size", [("bf16", 2), ("f32", 4)])
+def test_weights_decode_refuses_outputs_over_other_buffers(name, size):
+    f = getattr(C.lib(), "dadgpt_decode_attention_weights_" + name)
+    n, h, L, d = 4, 2, 2000, 64
+    names = ("out", "weights_out", "q", "k_cache", "v_cache", "weights", "lens")
+    rows, cache, w = n * h * d * size, n * h * L * d * size, n * h * L * 4
+    nbytes = dict(zip(names, (rows, w, rows, cache, cache, w, 4 * n)))
+    need = C.decode_weights_workspace_bytes(n, h, L, d)
+
+    def call(p, ws=None, wsb=0):
+        return f(*p, n, h, L, d, 0.125, ws, wsb, None)
+
+    assert call(_ptrs(7)) == 4
+    for a, others in (("out", names[1:]), ("weights_out", names[2:])):
+        for b in others:
+            for at in (16, nbytes[b] - 16, 16 - nbytes[a]):
+                if at >= nbytes[b]:
+                    continue
+                p = _ptrs(7)
+                p[names.index(a)] = p[names.index(b)] + at
+                assert call(p) == 1, (a, b, at)
+                assert f"{a} overlaps {b}" in A.last_error(), (a, b, at, A.last_error())
+            for at in ((nbytes[b] + 15) // 16 * 16, -nbytes[a]):
+                p = _ptrs(7)
+                p[names.index(a)] = p[names.index(b)] + at
+                assert call(p) == 4, (a, b, at, A.last_error())
+    for b in ("k_cache", "weights", "lens", "weights_out"):
+        p = _ptrs(7)
+        p[0] = p[names.index(b)]
+        assert call(p) == 1 and f"out overlaps {b}" in A.last_error()
+    p = _ptrs(7)
+    p[1] = p[5]  # in place
+    assert call(p) == 4
+    for b in names:
+        p = _ptrs(7)
+        assert call(p, p[names.index(b)] - need + 16, need) == 1
+        assert f"the workspace overlaps {b}" in A.last_error()
+
+
+@pytest.mark.parametrize("name,size", [("bf16", 2), ("f32", 4)])
+def test_kv8_decode_refuses_its_output_and_workspace_over_inputs(name, size):
+    f = getattr(C.lib(), "dadgpt_decode_attention_kv8_" + name)
+    n, h, L, d, block = 4, 2, 5000, 64, 32
+    names = ("out", "q", "k_cache", "v_cache", "k_scale", "v_scale", "lens")
+    rows, cache, scales = n * h * d * size, n * h * L * d, n * h * 157 * 4
+    nbytes = dict(zip(names, (rows, rows, cache, cache, scales, scales, 4 * n)))
+    need = C.decode_kv8_workspace_bytes(n, h, L, d)
+
+    def call(p, ws=None, wsb=0, window=0):
+        return f(*p, n, h, L, d, block, 0.125, window, 0, ws, wsb, None)
+
+    assert call(_ptrs(7)) == 4
+    for b in names[1:]:
+        for at in (16, nbytes[b] - 16, 16 - rows):
+            if at >= nbytes[b]:
+                continue
+            p = _ptrs(7)
+            p[0] = p[names.index(b)] + at
+            assert call(p) == 1 and f"out overlaps {b}" in A.last_error(), (b, at, A.last_error())
+        p = _ptrs(7)
+        p[0] = p[names.index(b)] + (nbytes[b] + 15) // 16 * 16
+        assert call(p) == 4
+    for b in names:
+        p = _ptrs(7)
+        assert call(p, p[names.index(b)] - need + 16, need) == 1
+        assert f"the workspace overlaps {b}" in A.last_error()
+
+
+@pytest.mark.parametrize("name,size", [("bf16", 2), ("f32", 4)])
+def test_append_refuses_new_rows_that_lie_in_the_cache(name, size):
+    f = getattr(C.lib(), "dadgpt_kv8_append_" + name)
+    n, h, rows, L, d, block = 4, 2, 3, 100, 64, 32
+    st = A.HeadStrides(1 << 12, 64, 768)
+    extent = ((n - 1) * (1 << 12) + (h - 1) * 64 + (rows - 1) * 768 + d) * size
+    cache, scales = n * h * L * d, n * h * 4 * 4
+    names = ("k_cache", "v_cache", "k_scale", "v_scale", "k", "v")
+    nbytes = dict(zip(names, (cache, cache, scales, scales, extent, extent)))
+    for x in ("k", "v"):
+        for c in names[:4]:
+            for at in (0, nbytes[c] - 16, 16 - extent):
+                p = _ptrs(6)
+                p[names.index(x)] = p[names.index(c)] + at
+                got = f(*p, ctypes.byref(st), ctypes.byref(st), FAKE + 6 * STEP, None, n, h, rows, L, d,
+                        block, None)
+                assert got == 1 and f"{c} overlaps {x}" in A.last_error(), (x, c, at)
