@@ -124,6 +124,9 @@ int check_decode(const char* fn, int n_seq, int H, int max_len, int d_head, floa
   if (need > 0 && (ws == nullptr || ws_bytes < need))
     return fail(DADGPT_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", fn,
                 ws == nullptr ? 0 : ws_bytes, need);
+  // its 32-bit counters start there, the fp32 partials a multiple of 16 bytes further on
+  if (need > 0 && reinterpret_cast<uintptr_t>(ws) % 4 != 0)
+    return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: workspace is not 4-byte aligned", fn);
   return DADGPT_OK;
 }
 

@@ -216,8 +216,9 @@ int dadgpt_flash_attention_backward_bf16_tokens(uint16_t* dq, uint16_t* dk, uint
  * d_head 32): then no workspace is needed and NULL may be passed. Longer caches are split
  * into chunks merged inside the same kernel by the last chunk of each cache, through the
  * workspace: per-(sequence, head) arrival counters at its start, fp32 partials packed against
- * its end. Contract: size it for the largest (n_seq, n_heads, max_len, d_head) it will serve,
- * ZERO-FILL it once (hipMemset at allocation), and pass its full size as workspace_bytes on
+ * its end. Contract: 4-byte aligned (checked), sized for the largest (n_seq, n_heads, max_len,
+ * d_head) it will serve (each of the four; a buffer of several shapes' largest byte count is not it),
+ * ZERO-FILLED once (hipMemset at allocation), and its full size passed as workspace_bytes on
  * every call; each call leaves the counters at zero again, so calls of any shape up to the
  * sizing one can share it. Calls that share a workspace must not overlap in time. */
 size_t dadgpt_decode_workspace_bytes(int n_seq, int n_heads, int max_len, int d_head);
