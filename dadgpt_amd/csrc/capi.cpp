@@ -222,7 +222,8 @@ int check_decode_window(const char* fn, int n_seq, int H, int max_len, int d_hea
 // Whether two [B, H, S, D] tensors of the same strides (elements) have an element in common, the
 // second `off` elements behind the first: whether off is b * batch + h * head + s * row + d for some
 // |b| < B, |h| < H, |s| < S, |d| < D. Searched from the largest stride down, few steps where the
-// tensor's own rows lie apart; rows that do not are not told apart further than kSteps.
+// tensor's own rows lie apart; rows that do not are not told apart further than kMeetSteps.
+constexpr int kMeetSteps = 4096;
 struct StrideDim {
   long long stride, most;  // most: the largest index
 };
@@ -237,10 +238,41 @@ bool rows_meet(long long off, const StrideDim* dim, const StrideDim* end, long l
   long long last = up >= 0 ? up / dim->stride : -((-up + dim->stride - 1) / dim->stride);
   if (i < -dim->most) i = -dim->most;
   if (last > dim->most) last = dim->most;
-  constexpr int kSteps = 4096;
-  for (; i <= last && ++*steps <= kSteps; ++i)
+  for (; i <= last && ++*steps <= kMeetSteps; ++i)
     if (rows_meet(off - i * dim->stride, dim + 1, end, d, steps)) return true;
   return false;
+}
+
+// The dimensions of a tensor, the largest stride first.
+struct StrideDims {
+  StrideDim d[3];
+  StrideDims(const dadgpt::HeadStrides& t, int batch, int H, int S)
+      : d{{t.batch, batch - 1}, {t.head, H - 1}, {t.row, S - 1}} {
+    std::sort(d, d + 3, [](const StrideDim& x, const StrideDim& y) { return x.stride > y.stride; });
+  }
+};
+
+// Whether two of a tensor's own rows overlap (a broadcast view's do).
+bool own_rows_meet(const dadgpt::HeadStrides& t, int batch, int H, int S, int d_head) {
+  const StrideDims dims(t, batch, H, S);
+  int steps = 0;
+  for (int x = 0; x < 3; ++x) {  // the first dimension in which the two rows differ
+    long long reach = d_head - 1;
+    for (int y = x + 1; y < 3; ++y) reach += dims.d[y].stride * dims.d[y].most;
+    for (long long i = 1; i <= dims.d[x].most && i * dims.d[x].stride <= reach; ++i) {
+      if (rows_meet(-i * dims.d[x].stride, dims.d + x + 1, dims.d + 3, d_head, &steps)) return true;
+      if (steps > kMeetSteps) return false;
+    }
+  }
+  return false;
+}
+int check_own_rows(const char* fn, const char* name, const dadgpt::HeadStrides& t, int batch, int H,
+                   int S, int d_head) {
+  if (own_rows_meet(t, batch, H, S, d_head))
+    return fail(DADGPT_ERR_INVALID_ARGUMENT,
+                "%s: rows of %s overlap each other (strides {batch %lld, head %lld, row %d})", fn,
+                name, t.batch, t.head, t.row);
+  return DADGPT_OK;
 }
 
 // Two gradients of a windowed backward: apart as a whole, or by rows where their strides agree
@@ -251,11 +283,10 @@ bool gradients_meet(const void* a, const void* b, size_t a_bytes, size_t b_bytes
   if (!dadgpt::overlap({a, a_bytes}, {b, b_bytes})) return false;
   if (a == b) return true;
   if (sa.batch != sb.batch || sa.head != sb.head || sa.row != sb.row) return false;
-  StrideDim dims[3] = {{sa.batch, batch - 1}, {sa.head, H - 1}, {sa.row, S - 1}};
-  std::sort(dims, dims + 3, [](const StrideDim& x, const StrideDim& y) { return x.stride > y.stride; });
+  const StrideDims dims(sa, batch, H, S);
   const long long off = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / elem_bytes;
   int steps = 0;
-  return rows_meet(off, dims, dims + 3, d_head, &steps);
+  return rows_meet(off, dims.d, dims.d + 3, d_head, &steps);
 }
 
 // The windowed backward's buffers. No output (dQ, dK, dV, delta, the workspace) shares memory with
@@ -290,10 +321,12 @@ int check_window_backward(const char* fn, int batch, int H, int S, int d_head, i
         return meet(g, o);
   }
   const size_t need = dadgpt::window_workspace_bytes(batch * H, S, d_head, w);
-  if (need == 0) return DADGPT_OK;
-  if (ws == nullptr || ws_bytes < need)
+  if (need > 0 && (ws == nullptr || ws_bytes < need))
     return fail(DADGPT_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", fn,
                 ws == nullptr ? 0 : ws_bytes, need);
+  for (int g = dadgpt::kTDQ; g <= dadgpt::kTDV; ++g)
+    if (int st = check_own_rows(fn, names[g], L.t[g], batch, H, S, d_head)) return st;
+  if (need == 0) return DADGPT_OK;
   if (reinterpret_cast<uintptr_t>(ws) % 16 != 0)
     return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: workspace is not 16-byte aligned", fn);
   for (int t = 0; t < kAll; ++t)
@@ -665,6 +698,7 @@ int dadgpt_flash_attention_window_forward_bf16_strided(
   if (int st = check_strides(fn, batch, H, S, d_head, strides, 4, &L)) return st;
   if (int st = check_attn(fn, batch * H, S, d_head, scale, {out, lse, q, k, v})) return st;
   if (int st = check_window(fn, S, window, sinks)) return st;
+  if (int st = check_own_rows(fn, "out", L.t[dadgpt::kTO], batch, H, S, d_head)) return st;
   const dadgpt::Window w{window, sinks};
   return from_hip(dadgpt::launch_fwd_bf16(B(out), lse, B(q), B(k), B(v), batch * H, S, d_head,
                                           scale, L, as_stream(stream), nullptr, &w),

@@ -296,7 +296,8 @@ int dadgpt_flash_attention_window_backward_bf16(uint16_t* dq, uint16_t* dk, uint
                                                 void* workspace, size_t workspace_bytes,
                                                 void* stream);
 /* The strided and token-major forms (strides and leading dimensions as above). dq, dk and dv may
- * share one buffer as long as their rows do not overlap. */
+ * share one buffer as long as their rows do not overlap. Inputs may be broadcast (a stride of 0); an
+ * output whose own rows overlap is refused: a shared head's gradient is the sum of its copies'. */
 int dadgpt_flash_attention_window_forward_bf16_strided(
     uint16_t* out, float* lse, const uint16_t* q, const uint16_t* k, const uint16_t* v, int B,
     int H, int S, int d_head, float scale, int window, int sinks,

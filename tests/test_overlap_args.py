@@ -189,3 +189,37 @@ def test_append_refuses_new_rows_that_lie_in_the_cache(name, size):
                 got = f(*p, ctypes.byref(st), ctypes.byref(st), FAKE + 6 * STEP, None, n, h, rows, L, d,
                         block, None)
                 assert got == 1 and f"{c} overlaps {x}" in A.last_error(), (x, c, at)
+
+
+def test_window_strided_refuses_outputs_whose_own_rows_overlap():
+    """An output of a broadcast view (expand: stride 0) or of rows laid into each other would be
+    written by several workgroups; inputs may be broadcast. A call with nothing else wrong gets as far
+    as its workspace's alignment."""
+    B, H = 2, 12
+    need = A.window_workspace_bytes(B * H, S, D, 16, 2)
+    fwd = A.lib().dadgpt_flash_attention_window_forward_bf16_strided
+    bwd = A.lib().dadgpt_flash_attention_window_backward_bf16_strided
+    ok = (H * S * D, S * D, D)
+    names = ("q", "k", "v", "out", "dout", "dq", "dk", "dv")
+
+    def call(**other):
+        st = _strides(*(other.get(n, ok) for n in names))
+        assert bwd(*_ptrs(10), B, H, S, D, 0.125, 16, 2, st, FAKE + 20 * STEP + 8, need, None) == 1
+        return A.last_error()
+
+    assert "not 16-byte aligned" in call()
+    shared = ((H * S * D, 0, D), (0, S * D, D), (S * D, S * D, D), (8, S * D, D),
+              (H * S * D, D - 8, H * D), (S * H * D, D, H * D - 8), (S * D // 2, S * D, D))
+    for name in ("dq", "dk", "dv"):
+        for bad in shared:
+            assert f"rows of {name} overlap" in call(**{name: bad}), (name, bad)
+        # head-major, token-major, tokens before batches, heads outermost, gaps
+        for good in ((S * H * D, D, H * D), (H * D, D, B * H * D), (S * D, B * S * D, D),
+                     (H * S * 128, S * 128, 128), (3 * S * H * D + 64, D, 3 * H * D)):
+            assert "not 16-byte aligned" in call(**{name: good}), (name, good, A.last_error())
+    for name in ("q", "k", "v", "out", "dout"):
+        assert "not 16-byte aligned" in call(**{name: (H * S * D, 0, D)}), name
+    for bad in shared:
+        st = _strides(ok, ok, ok, bad)
+        assert fwd(*_ptrs(5), B, H, S, D, 0.125, 16, 2, st, None) == 1
+        assert "rows of out overlap" in A.last_error()
