@@ -571,14 +571,28 @@ def flash_attention_window_backward_bf16_strided(dq, dk, dv, delta, dout, out, l
         _stream_ptr(stream)))
 
 
+def _token_rows(t, name, rows, ld, width):
+    """Address of a token-major bf16 tensor whose `rows` rows of `width` elements lie ld apart from its
+    first element on, within its storage."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not torch.bfloat16:
+        raise TypeError(f"{name} must be a bfloat16 device tensor")
+    if t.storage_offset() + (rows - 1) * ld + width > t.untyped_storage().nbytes() // 2:
+        raise ValueError(f"{name} is too short for {rows} rows of {width}, {ld} apart")
+    return t.data_ptr()
+
+
 def flash_attention_window_forward_bf16_tokens(out, ld_out: int, lse, q, k, v, ld_qkv: int,
                                                B: int, H: int, S: int, d_head: int, scale: float,
                                                window: int, sinks: int = 0, stream=None) -> None:
     """Token-major windowed forward (see flash_attention_forward_bf16_tokens)."""
+    rows, width = B * S, H * d_head
+    po = _token_rows(out, "out", rows, ld_out, width)
+    pq, pk, pv = (_token_rows(t, n, rows, ld_qkv, width) for t, n in ((q, "q"), (k, "k"), (v, "v")))
+    _require(lse, "lse", torch.float32, B * H * S)
     _same_device((out, lse, q, k, v))
     _check(lib().dadgpt_flash_attention_window_forward_bf16_tokens(
-        _ptr(out), ld_out, _ptr(lse), _ptr(q), _ptr(k), _ptr(v), ld_qkv, B, H, S, d_head, scale,
-        window, sinks, _stream_ptr(stream)))
+        po, ld_out, _ptr(lse), pq, pk, pv, ld_qkv, B, H, S, d_head, scale, window, sinks,
+        _stream_ptr(stream)))
 
 
 def flash_attention_window_backward_bf16_tokens(dq, dk, dv, ld_dqkv: int, delta, dout, out,
@@ -587,11 +601,17 @@ def flash_attention_window_backward_bf16_tokens(dq, dk, dv, ld_dqkv: int, delta,
                                                 window: int, sinks: int = 0, workspace=None,
                                                 stream=None) -> None:
     """Token-major windowed backward (see flash_attention_backward_bf16_tokens)."""
+    rows, width = B * S, H * d_head
+    gq, gk, gv = (_token_rows(t, n, rows, ld_dqkv, width)
+                  for t, n in ((dq, "dq"), (dk, "dk"), (dv, "dv")))
+    pd, po = (_token_rows(t, n, rows, ld_out, width) for t, n in ((dout, "dout"), (out, "out")))
+    pq, pk, pv = (_token_rows(t, n, rows, ld_qkv, width) for t, n in ((q, "q"), (k, "k"), (v, "v")))
+    _require(delta, "delta", torch.float32, B * H * S)
+    _require(lse, "lse", torch.float32, B * H * S)
     _same_device((dq, dk, dv, delta, dout, out, lse, q, k, v, workspace))
     _check(lib().dadgpt_flash_attention_window_backward_bf16_tokens(
-        _ptr(dq), _ptr(dk), _ptr(dv), ld_dqkv, _ptr(delta), _ptr(dout), _ptr(out), ld_out,
-        _ptr(lse), _ptr(q), _ptr(k), _ptr(v), ld_qkv, B, H, S, d_head, scale, window, sinks,
-        *_workspace(workspace), _stream_ptr(stream)))
+        gq, gk, gv, ld_dqkv, _ptr(delta), pd, po, ld_out, _ptr(lse), pq, pk, pv, ld_qkv, B, H, S,
+        d_head, scale, window, sinks, *_workspace(workspace), _stream_ptr(stream)))
 
 
 def decode_attention_window(out, q, k_cache, v_cache, lens, n_seq, n_heads, max_len, d_head, scale,
