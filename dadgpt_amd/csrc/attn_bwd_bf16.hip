@@ -128,7 +128,10 @@ constexpr int kKW = 32;  // keys per wave
 // computed per read: what brings dK/dV (all but the dropout instantiation) to 168 VGPRs,
 // three workgroups per CU, without spilling in the loop. (The strided kernel of one launch with
 // its own delta and one wave per group keeps two registers in scratch and reloads them as it
-// issues a tile.)
+// issues a tile. The windowed kernels at D = 64, with dS in two values and their masks' bounds, keep
+// more there, written before the loop. Bytes a lane, contiguous / strided: window_dkdv with two waves
+// per group 20 / 44, none with one; window_bwd 40 / 64 with two and 8 / 36 with one; window_dq 8 / 20.
+// Reloads in the tile loop, two tiles of it: 4 / 8, 7 / 13, 0 / 5 and 0 / 1.)
 template <int D, bool DROP, bool XA, bool WIN = false>
 __device__ __forceinline__ void dkdv_block(bool mask, f32x16 (&dkacc)[D / 32],
                                            f32x16 (&dvacc)[D / 32], const bf16x8 (&kop)[D / 16],
@@ -893,8 +896,9 @@ __device__ __forceinline__ void sink_workgroup(const BwdArgs& a, int bh, int gro
 
 // dQ (which writes delta), the sink keys' pieces in front: they are short, and the dQ workgroups
 // fill in behind them. B16 H12 T1024 D64, window 256, 4 sinks, token-major: 57 us, 46 of them without
-// sinks; dK/dV 51. Half of either is HBM time (150 MB, 29 us), which a window of 64 comes near (34
-// and 34 us).
+// sinks; dK/dV 51. HBM (223 and 156 MB by the counters: 43 and 30 us at a copy's rate), the matrix
+// pipe (14 and 15 us) and the VALU (11,500 and 10,200 instructions a SIMD, 22 and 19 us at four cycles
+// each) all take a part that the others do not hide. With a window of 64 47 us, 33 without sinks, and 35.
 constexpr int kMaxPieceTiles = 12;
 template <int D, bool STRIDED, int KS>
 __global__ __launch_bounds__(64 * kWaves, kDqMinBlocks) void window_dq_bf16_kernel(
@@ -936,9 +940,11 @@ struct JoinAt {
     far = which > 1 ? 0 : win.far_pieces(row / win.block_keys, S);
   }
 };
-// Sums up a long list of partials into its first. dK/dV's workgroups would add one after the other
-// (forward and backward, window 256, us: 1 x 65536 113 -> 69, 1 x 16384 44.9 -> 40.5, 1 x 8192, 11
-// partials 37.9 -> 37.0; but 12 x 8192, window 1024, 10 partials 152.4 -> 155.0).
+// Sums up a long list of partials into its first. dK/dV's workgroups would add one after the other, the
+// longer the fewer there are to hide it (forward and backward in two launches, window 256, us: 1 x
+// 65536, 85 partials 117 -> 74, 1 x 16384, 63 54.4 -> 37.1, 1 x 8192, 31 37.9 -> 31.0; backward alone 12 x
+// 16384, 21 partials 115.7 -> 112.3, 12 x 12288, window 512, 16 128.6 -> 131.1; forward and backward 12 x
+// 8192, window 1024, 10 174.1 -> 177.2).
 template <int D>
 __global__ __launch_bounds__(256) void window_join_bf16_kernel(const WindowBwdArgs win, int S) {
   const JoinAt<D> at(win, S);
@@ -1126,18 +1132,20 @@ WindowPlan window_plan(int BH, int S, int D, const Window& w) {
   auto end = [&](int block_keys) {  // of the first block, in tiles
     return ((long long)block_keys + w.window - 2) / kTileRows + 1;
   };
-  // (Times below with dS in one bf16 value; in two all of them are 3 to 15% longer.)
   // Sink blocks walk all later queries themselves (`whole`) where these are few, or in large grids few
   // next to the window: pieces and their join cost more than the longer chain (pieces -> whole,
-  // backward, us: 192 x 256, window 64 21.0 -> 16.7, 180 x 500, 64 38.4 -> 34.9, 96 x 1024, 512 62.9 ->
-  // 59.9; but 12 x 1024, 512 19.2 -> 25.5, 24 x 494, 55 12.0 -> 16.7).
+  // backward, 4 sinks, us: 192 x 256, window 64 22.5 -> 18.2, 180 x 500, 64 40.1 -> 36.9, 96 x 1024, 512
+  // 71.2 -> 66.9; but 12 x 1024, 512 22.1 -> 29.5, 24 x 494, 55 12.9 -> 18.7). That is for one launch,
+  // where pieces add a join. As dQ and then dK/dV they add none, and any later query is cut off: 240 x
+  // 500, 64 48.5 -> 48.7, 240 x 500, 256 59.1 -> 61.0, 300 x 600, 256 87.1 -> 89.3, 192 x 1024, 700 133 ->
+  // 134 (192 x 1024, 512 123 -> 119).
   const long long end128 = end(128), far128 = tiles - end128;
   const bool few = (long long)BH * S <= 1 << 16;
   const bool whole =
       w.sinks == 0 || (few ? far128 <= 2 : far128 <= 6 || far128 <= end128);
   // One launch, as the plain backward, where a workgroup's rows are few enough for its own delta (two
-  // launches -> one and a join of the sink rows, us: 4 x 1429, window 5 16.6 -> 11.0, 12 x 1024, 256 19.5
-  // -> 15.9, 64 x 700, 64 27.5 -> 19.5; but 96 x 1024, 128 40.1 -> 41.6).
+  // launches -> one and a join of the sink rows, us: 4 x 1429, window 5 16.6 -> 11.1, 12 x 1024, 256 20.1
+  // -> 16.6, 64 x 700, 64 27.8 -> 20.5; 96 x 1024, 128 43.8 -> 43.9).
   const bool short_rows = w.window <= kOwnDeltaMaxS - 3 * kTileRows;
   p.one = bwd_in_one_launch(BH, S, D, false) &&
           (whole ? S <= kOwnDeltaMaxS || (short_rows && w.sinks == 0)
@@ -1145,10 +1153,10 @@ WindowPlan window_plan(int BH, int S, int D, const Window& w) {
   p.waves_per_group = window_waves_per_group(BH, S, p.one ? 2 : 1);
   const long long far = tiles - end(32 * kWaves / p.waves_per_group);
   if ((p.one && whole) || w.sinks == 0 || far <= 0) return p;
-  // Pieces of even lengths up to 12 tiles (of four, B16 H12 T1024 with a window of 256 takes dQ 56
-  // for 51 us); up to four in small grids, which wait for the longest piece (12 -> 4, backward, us: 32 x
-  // 799, window 10 24.1 -> 18.5, 12 x 1024, 256 25.0 -> 19.6, 16 x 710, 4 20.0 -> 15.8; but 48 x 1024, 128
-  // 28.5 -> 32.3, 96 x 1024, 128 39.4 -> 42.1).
+  // Pieces of even lengths up to 12 tiles; up to four in small grids, which wait for the longest piece
+  // (12 -> 4, backward in two launches, us: 32 x 799, window 10 24.7 -> 18.6, 12 x 1024, 256 24.9 -> 19.9,
+  // 16 x 710, 4 20.4 -> 15.9; but 48 x 1024, 128 29.2 -> 32.5, 96 x 1024, 128 42.9 -> 46.4, 192 x 1024, 256
+  // 94.1 -> 97.4).
   const bool small = (long long)BH * S <= 1 << 15;
   const int most = small ? 4 : kMaxPieceTiles;
   p.pieces = (int)((far + most - 1) / most);

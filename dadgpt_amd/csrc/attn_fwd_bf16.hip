@@ -237,7 +237,8 @@ __device__ __forceinline__ void fwd_softmax_pv(f32x16 (&s)[NQB], f32x16 (&oacc)[
 // and the workgroup's first visible key, waves leave out chunks none of their queries sees, and
 // chunks that some of them see in part are masked by comparison. A query may see nothing of its
 // wave's first chunks; its maximum stays -inf until it does (finite_max). B16 H12 T1024 D64, window
-// 256, 4 sinks: 28 us (causal 37; reading and writing its 100 MB alone 20).
+// 256, 4 sinks: 28 us (causal 37), 146 MB by the counters, a copy's rate, for the 100 MB of its inputs
+// and outputs: neighbouring blocks read a window's keys again.
 template <int D, bool STRIDED, bool DROP, int KS, bool FRESH = false, bool WIN = false>
 __global__ __launch_bounds__(64 * kWaves, kMinBlocks)
 __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_kernel(

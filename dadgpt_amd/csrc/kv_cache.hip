@@ -83,8 +83,8 @@ __device__ __forceinline__ float e4m3_scale(uint32_t a) {
 // all of them loaded before the block's maximum is taken and still in registers when it is known.
 // Grid (heads, K and V: 4 waves a workgroup; touched blocks; sequences), heads fastest, so that
 // neighbours read one stretch of the projection's token-major rows. Bound by that chain (lengths, rows,
-// maximum, codes) more than by HBM: 16 x 12 prompts of 1 to 1024 tokens in blocks of 32, 38 MB, 10.6 us;
-// one token for each of 32 x 12 caches 3.5.
+// maximum, codes, once a workgroup) more than by HBM: 16 x 12 prompts of 1 to 1024 tokens in blocks of
+// 32, 38 MB, 11.5 us in bf16, 63 MB, 14.6 in fp32; one token for each of 32 x 12 caches 3.4.
 template <typename T, int D, int NI, int WPB>
 __global__ __launch_bounds__(64 * kAppendWaves) void kv8_append_kernel(
     uint8_t* __restrict__ k8, uint8_t* __restrict__ v8, float* __restrict__ k_scale,
@@ -220,7 +220,8 @@ hipError_t launch_kv8_append_t(uint8_t* k8, uint8_t* v8, float* k_scale, float* 
 // a chunk of keys per 8-wave workgroup, 16-byte loads that cover whole key rows (16 codes a lane: 4
 // lanes a row at D = 64), all of a wave's loads issued before any arithmetic, chunks of one cache
 // merged by the last to arrive. 8 x 12 caches of 1 to 32768 rows, 200 MB, 35 us, 5.7 TB/s; 32 x 12
-// of 1 to 1024, 25 MB, 7.8 us, of which a launch with next to nothing to read is 4.
+// of 1 to 1024, 25 MB, 8.1 us, of which a launch with next to nothing to read is 4. Windowed: 32 x 12
+// of 1 to 1024 under 256 5.6, 8 x 12 of 1 to 32768 under 4096, 47 MB, 11.0.
 constexpr int kKv8Waves = 8;
 constexpr int kKv8Loads = 8;  // 16-byte loads per lane and tensor
 template <int D>
@@ -409,8 +410,8 @@ hipError_t launch_kv8_decode_d(T* out, const T* q, const uint8_t* k8, const uint
 // maximum and sum. A cache of one chunk has them in the workgroup; longer ones leave scores and
 // partials in the workspace for weights_kernel.
 // ONE: a workgroup runs through its cache's chunks, two at most, and needs neither. 16 x 12 caches
-// of 1 to 8192 rows of 64 bf16, 206 MB, 36 us and 6 for weights_kernel; 32 x 12 of 1 to 1024, 52 MB,
-// 12 us.
+// of 1 to 8192 rows of 64 bf16, 206 MB, 35 us and 5.4 for weights_kernel; 32 x 12 of 1 to 1024, 52 MB,
+// 13 us. In place as into another buffer.
 constexpr int kWWaves = 8, kWLoads = 8, kWChunks = 2;
 template <typename T, int D>
 __host__ __device__ constexpr int weights_chunk_keys() {
@@ -850,9 +851,8 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
   });
 }
 
-// Rows by `kept`, 16 bytes a lane, in a grid over rows: into another cache.
-// The rows that stay, into another cache: a copy (32 x 12 caches, 512 of up to 2048 rows of 128 bytes,
-// K and V, 91 MB, 17.4 us, 5.2 TB/s).
+// The rows that stay, into another cache, by `kept`, 16 bytes a lane, in a grid over rows: a copy (32 x
+// 12 caches, 512 of up to 2048 rows of 128 bytes, K and V, 91 MB, 17.3 us, 5.3 TB/s).
 constexpr int kMoveThreads = 256, kMovePer = 4;
 __global__ __launch_bounds__(kMoveThreads) void evict_gather_kernel(
     char* __restrict__ k_out, char* __restrict__ v_out, int* lens_out, const char* __restrict__ k,
@@ -885,7 +885,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_gather_kernel(
 
 // The same within a cache: one workgroup per (sequence, head) and tensor, in passes of kInPlaceRows
 // rows. A row moves down or stays (kept[r] >= r), so a pass writes only rows that earlier passes
-// or itself have read.
+// or itself have read. Rows that stay where they are are read too and not written: the 32 x 12 caches
+// above take 15.4 us, and 8.5 where every cache is within its budget.
 constexpr int kInPlaceThreads = 1024, kInPlacePer = 4;
 __global__ __launch_bounds__(kInPlaceThreads) void evict_in_place_kernel(
     char* k, char* v, int* lens_out, const int* lens, const int* __restrict__ kept, int H,
