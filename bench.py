@@ -100,8 +100,8 @@ def event_time_ms(fn, reps, stream):
 # The sources of the profiled kernels: the traffic summary records their digest at profiling
 # time, so a bench line can say whether its traffic figures describe the kernels it timed.
 KERNEL_SOURCES = [os.path.join(ROOT, "dadgpt_amd", "csrc", n) for n in (
-    "attn_fwd_bf16.hip", "attn_bwd_bf16.hip", "decode.hip", "tiles.hpp", "common.hpp",
-    "lanes.hpp", "dropout.hpp", "kernels.hpp")]
+    "attn_fwd_bf16.hip", "attn_bwd_bf16.hip", "decode.hip", "decode.hpp", "window.hpp",
+    "tiles.hpp", "common.hpp", "lanes.hpp", "dropout.hpp", "kernels.hpp")]
 
 
 def kernel_sources_digest():
