@@ -100,7 +100,8 @@ __global__ __launch_bounds__(256) void delta_bf16_kernel(float* __restrict__ del
 // dK as their own rounding does: against 64 bits 1.5 times that of 32-bit arithmetic rounded once (with
 // a window of 4 1.8, as a short row's delta, from the bf16 output, weighs more); in two 1.1 (1.5). B16
 // H12 T1024, window 256, forward and backward 127 us for 119, B1 H12 T8192, window 1024 173 for 150. P
-// stays one value (dV 1.4 times).
+// stays one value (dV 1.4 times), and delta is formed from the bf16 output (a term of dS that a row's
+// keys share).
 __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t packed) {
   asm("" : "+v"(packed));  // (or the compiler would convert again instead of taking the word apart)
   return pack_bf16x2(a - bf16_lo(packed), b - bf16_hi(packed));

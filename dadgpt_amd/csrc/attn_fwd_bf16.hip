@@ -238,7 +238,9 @@ __device__ __forceinline__ void fwd_softmax_pv(f32x16 (&s)[NQB], f32x16 (&oacc)[
 // chunks that some of them see in part are masked by comparison. A query may see nothing of its
 // wave's first chunks; its maximum stays -inf until it does (finite_max). B16 H12 T1024 D64, window
 // 256, 4 sinks: 28 us (causal 37), 146 MB by the counters, a copy's rate, for the 100 MB of its inputs
-// and outputs: neighbouring blocks read a window's keys again.
+// and outputs: neighbouring blocks read a window's keys again. P enters P V as one bf16 value, as in the
+// causal kernel: the output is off by 1.25 times what 32-bit arithmetic rounded once is, and a second
+// value would be two more products for each four.
 template <int D, bool STRIDED, bool DROP, int KS, bool FRESH = false, bool WIN = false>
 __global__ __launch_bounds__(64 * kWaves, kMinBlocks)
 __attribute__((amdgpu_num_vgpr(512 / (kMinBlocks * kWaves / 4)))) void fwd_bf16_kernel(
