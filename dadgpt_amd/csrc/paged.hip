@@ -1,0 +1,119 @@
+// Appending to paged caches for gfx950: the new rows of ragged sequences out of a fused projection's
+// output into the pages that the block table names, q and k rotated on the way (one launch for what
+// would be three: rotation, and a scatter each of k and v). Bound by HBM, and for a token a sequence by
+// the launch and the chain row_start, lens -> page -> store.
+#include "common.hpp"
+#include "paged.hpp"
+#include "rope.hpp"
+#include "serving.hpp"
+
+namespace dadgpt {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T>
+struct AppendArgs {
+  T *k_pages, *v_pages, *q_out;
+  const T *q, *k, *v;
+  long long ld_out, ld_q, ld_kv;
+  PagedStep p;
+  Rope r;
+  int heads_q, groups;  // query heads to move (0 without q); of all heads: a thread takes g, g + groups, ..
+};
+
+// Grid (rows of a sequence, sequences). Consecutive threads run along a head's chunks, then the heads
+// of a row, which lie side by side in the projection's output.
+template <typename T, int VEC, bool INTER, int HPT>
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs<T> a) {
+  const paged::NewRows seq(a.p, blockIdx.y);
+  const int D = a.p.D, chunks = D / (2 * VEC);
+  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t c = id % chunks, j = id / chunks;
+  const int t = j / a.groups, g = j % a.groups;
+  const int token = seq.token + t;
+  if (t >= seq.count || token < 0) return;
+  const rotary::Chunk pair = rotary::chunk_of<VEC, INTER>(c, a.r.rot_dim);
+  const rotary::Chunk flat{{2 * (int)c * VEC, 2 * (int)c * VEC + VEC}, false};
+  const int page = a.p.table[(size_t)blockIdx.y * a.p.max_pages + token / a.p.page];
+  const bool held = paged::is_page(a.p, page);
+  const long long row = seq.first + t;
+
+  T* dst[HPT];
+  rotary::Piece<T, VEC> x[HPT][2];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int head = i * a.groups + g, kh = head - a.heads_q, vh = kh - a.p.Hkv;
+    const rotary::Chunk& ch = vh >= 0 ? flat : pair;
+    const T* src;
+    if (kh < 0) {
+      src = a.q + row * a.ld_q + head * D;
+      dst[i] = a.q_out + row * a.ld_out + head * D;
+    } else {
+      const int h = vh >= 0 ? vh : kh;
+      src = (vh >= 0 ? a.v : a.k) + row * a.ld_kv + h * D;
+      dst[i] = held && vh < a.p.Hkv ? (vh >= 0 ? a.v_pages : a.k_pages) +
+                                          paged::page_row(a.p, page, h, token % a.p.page)
+                                    : nullptr;
+    }
+    if (dst[i] == nullptr) continue;
+    x[i][0].load(src + ch.at[0]);
+    x[i][1].load(src + ch.at[1]);
+  }
+  if (pair.rotated) {
+    const auto turn = rotary::turn_of<VEC>(a.r.freqs + c * VEC, token, a.r.magnitude, false);
+#pragma unroll
+    for (int i = 0; i < HPT; ++i)
+      if (i * a.groups + g < a.heads_q + a.p.Hkv)
+        rotary::turn_pieces<T, VEC, INTER>(x[i][0], x[i][1], turn);
+  }
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    if (dst[i] == nullptr) continue;
+    const rotary::Chunk& ch = i * a.groups + g >= a.heads_q + a.p.Hkv ? flat : pair;
+    x[i][0].store(dst[i] + ch.at[0]);
+    x[i][1].store(dst[i] + ch.at[1]);
+  }
+}
+
+template <typename T>
+hipError_t launch_append_t(T* k_pages, T* v_pages, T* q_out, long long ld_out, const T* q,
+                           long long ld_q, const T* k, const T* v, long long ld_kv, const PagedStep& p, const Rope& r,
+                           hipStream_t stream) {
+  AppendArgs<T> a{k_pages, v_pages, q_out, q, k, v, ld_out, ld_q, ld_kv, p, r, q ? p.H : 0, 0};
+  const int heads = a.heads_q + 2 * p.Hkv;
+  auto run = [&](auto vec, auto inter) {
+    const long long chunks = p.D / (2 * vec());
+    const int hpt = rotary::heads_per_thread((long long)p.rows * chunks, heads);
+    a.groups = (heads + hpt - 1) / hpt;
+    const dim3 grid((unsigned)((p.max_rows * chunks * a.groups + kThreads - 1) / kThreads), p.n_seq);
+    switch (hpt) {
+      case 1: paged_append_kernel<T, vec(), inter(), 1><<<grid, kThreads, 0, stream>>>(a); break;
+      case 2: paged_append_kernel<T, vec(), inter(), 2><<<grid, kThreads, 0, stream>>>(a); break;
+      case 4: paged_append_kernel<T, vec(), inter(), 4><<<grid, kThreads, 0, stream>>>(a); break;
+      default: paged_append_kernel<T, vec(), inter(), 8><<<grid, kThreads, 0, stream>>>(a); break;
+    }
+    return hipGetLastError();
+  };
+  auto with = [&](auto vec) {
+    return r.interleaved ? run(vec, std::true_type{}) : run(vec, std::false_type{});
+  };
+  if constexpr (sizeof(T) == 2)
+    if (rotary::wide<T>(r.rot_dim, p.D)) return with(std::integral_constant<int, 8>{});
+  return with(std::integral_constant<int, 4>{});
+}
+
+}  // namespace
+
+hipError_t launch_paged_append_bf16(bf16* k_pages, bf16* v_pages, bf16* q_out, long long ld_out,
+                                    const bf16* q, long long ld_q, const bf16* k, const bf16* v,
+                                    long long ld_kv, const PagedStep& step, const Rope& rope, hipStream_t stream) {
+  return launch_append_t<bf16>(k_pages, v_pages, q_out, ld_out, q, ld_q, k, v, ld_kv, step, rope, stream);
+}
+hipError_t launch_paged_append_f32(float* k_pages, float* v_pages, float* q_out, long long ld_out,
+                                   const float* q, long long ld_q, const float* k, const float* v,
+                                   long long ld_kv, const PagedStep& step, const Rope& rope, hipStream_t stream) {
+  return launch_append_t<float>(k_pages, v_pages, q_out, ld_out, q, ld_q, k, v, ld_kv, step, rope, stream);
+}
+
+}  // namespace dadgpt

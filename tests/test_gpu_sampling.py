@@ -1,0 +1,169 @@
+"""GPU tests of the sampling: tokens equal to the definition's (serving_ref, sums in extended precision) for
+rows whose decisions lie further from a border than the sums are off, and probabilities to fp32."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from dadgpt_amd import sampling
+from tests import serving_ref as S
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+# Weights are multiples of 2^-44 of the largest: a sum of n is off by less than n 2^-45 of it, and the
+# exponentials by 1e-14 of each weight.
+MARGIN = 1e-8
+
+
+def _sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    rows = logits.shape[0]
+
+    def dev(x, dtype=F32):
+        return None if x is None else torch.tensor(x, dtype=dtype).cuda()
+    tokens = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    probs = torch.full((rows,), -7.0, device="cuda")
+    sampling.sample(tokens, probs, logits.cuda() if not logits.is_cuda else logits, dev(u),
+                    dev(temperature), dev(top_k, torch.int32), dev(top_p), dev(min_p))
+    torch.cuda.synchronize()
+    return tokens.cpu().tolist(), probs.cpu().tolist()
+
+
+def _check(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    tokens, probs = _sample(logits, u, temperature, top_k, top_p, min_p)
+    x, checked = logits.float().cpu().numpy(), 0
+    for r in range(len(u)):
+        want, p, margin = S.sample(x[r], np.float32(u[r]), 1.0 if temperature is None else temperature[r],
+                                   0 if top_k is None else top_k[r], 1.0 if top_p is None else top_p[r],
+                                   0.0 if min_p is None else min_p[r])
+        if margin < MARGIN:
+            continue
+        checked += 1
+        assert tokens[r] == want, (r, tokens[r], want, margin)
+        assert abs(probs[r] - p) <= 2.0 ** -23 * p + 1e-30
+    assert checked >= 0.9 * len(u)
+
+
+def _logits(rows, vocab, seed, dtype, spread=3.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn((rows, vocab), generator=gen) * spread).to(dtype)
+
+
+def _uniforms(rows, seed):
+    return torch.rand(rows, generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("vocab", [1, 2, 5, 63, 1000, 4096, 4097, 8193, 50257, 70001])
+def test_settings(gpu, vocab, dtype):
+    rows = 24
+    x, u = _logits(rows, vocab, vocab, dtype), _uniforms(rows, vocab + 1)
+    pick = [(t, k, p, m) for t in (0.7, 1.0, 1.7) for k, p, m in
+            ((0, 1.0, 0.0), (1, 1.0, 0.0), (40, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.05),
+             (200, 0.8, 0.01), (5000, 0.5, 0.0), (3, 0.999, 0.3))]
+    assert len(pick) == rows
+    _check(x, u, *(list(z) for z in zip(*pick)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_defaults_and_draws(gpu, dtype):
+    """No settings; the draw follows the probabilities (4096 draws of one row: each of the likeliest
+    tokens within five standard deviations)."""
+    x = _logits(1, 300, 3, dtype, 1.5)
+    rows = 4096
+    u = ((torch.arange(rows) + 0.5) / rows).tolist()
+    tokens, _ = _sample(x.expand(rows, 300), u)
+    p = torch.softmax(x[0].double(), 0)
+    n = torch.bincount(torch.tensor(tokens), minlength=300).double()
+    assert ((n - rows * p).abs() <= 1.0 + 1e-6).all()  # evenly spaced numbers: within one
+    _check(x.expand(64, 300).contiguous(), _uniforms(64, 4))
+
+
+def test_edges_of_the_settings(gpu):
+    x = _logits(1, 777, 5, F32)
+    inf, nan = math.inf, math.nan
+    rows = [  # u, temperature, top_k, top_p, min_p
+        (0.5, 0.0, 0, 1.0, 0.0), (0.5, -1.0, 7, 0.5, 0.1), (0.5, nan, 0, 1.0, 0.0),
+        (0.5, inf, 0, 1.0, 0.0), (0.5, 1e-30, 0, 1.0, 0.0), (0.9, 1e-3, 50, 0.9, 0.0),
+        (0.5, 1.0, -3, 1.0, 0.0), (0.5, 1.0, 776, 1.0, 0.0), (0.5, 1.0, 777, 1.0, 0.0),
+        (0.5, 1.0, 10000, 1.0, 0.0), (0.5, 1.0, 0, 0.0, 0.0), (0.5, 1.0, 0, -1.0, 0.0),
+        (0.5, 1.0, 0, nan, 0.0), (0.5, 1.0, 0, 1.5, 0.0), (0.5, 1.0, 0, 1.0, 1.0),
+        (0.5, 1.0, 0, 1.0, 2.0), (0.5, 1.0, 0, 1.0, nan), (0.5, 1.0, 0, 1.0, -0.5),
+        (0.0, 1.0, 0, 1.0, 0.0), (nan, 1.0, 0, 1.0, 0.0), (-0.5, 1.0, 0, 1.0, 0.0),
+        (1.0, 1.0, 0, 1.0, 0.0), (2.0, 1.0, 5, 1.0, 0.0), (0.99999994, 1.0, 0, 0.95, 0.0),
+        (0.3, 100.0, 0, 0.9, 0.0), (0.3, 1e4, 20, 0.9, 0.5)]
+    _check(x.expand(len(rows), 777).contiguous(), *(list(z) for z in zip(*rows)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_ties(gpu, dtype):
+    """Equal logits: the lowest indices stay. 3000 ties are more than are compared each with each."""
+    for vocab, at in ((50, [3, 9, 20, 21, 40]), (50257, list(range(100, 50257, 16)))):
+        x = torch.full((1, vocab), -2.0)
+        x[0, at] = 1.5
+        x[0, at[1]] = 4.0
+        x[0, 0], x[0, 1] = 0.0, -0.0  # equal
+        x = x.to(dtype)
+        rows = [(u, 1.0, k, p, m) for u in (0.0, 0.41, 0.77, 0.9999) for k, p, m in
+                ((2, 1.0, 0.0), (4, 1.0, 0.0), (0, 0.31, 0.0), (len(at) + 1, 1.0, 0.0),
+                 (len(at) + 1, 0.97, 0.0), (3, 0.6, 0.01), (0, 0.5, 0.0), (0, 1.0, 0.05))]
+        _check(x.expand(len(rows), vocab).contiguous(), *(list(z) for z in zip(*rows)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_all_equal(gpu, dtype):
+    rows = [(u, 1.0, k, p, 0.0) for u in (0.0, 0.3, 0.70001) for k, p in
+            ((0, 1.0), (17, 1.0), (0, 0.25003), (5000, 0.50007))]
+    _check(torch.full((len(rows), 50257), 2.5, dtype=dtype), *(list(z) for z in zip(*rows)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_special_logits(gpu, dtype):
+    """NaN and -inf are never picked, +inf alone is where there is one, nothing left: -1."""
+    inf, nan = math.inf, math.nan
+    V, rows = 90, []
+    for x in ([nan] * V, [-inf] * V, [nan, -inf] * (V // 2), [-inf] * 50 + [1.0] + [nan] * 39,
+              [1.0] * 40 + [inf] + [2.0] * 48 + [inf], [inf] * V, [nan, inf, 3.0] * 30,
+              [3.0e38] + [-3.0e38] * 88 + [1.0], [0.0] + [nan] * 80 + [-1e30] * 9):
+        rows += [x] * 4
+    u = [0.0, 0.4, 0.6, 0.999] * 9
+    x = torch.tensor(rows).to(dtype)
+    _check(x, u)
+    _check(x, u, [0.8] * 36, [3] * 36, [0.9] * 36, [0.1] * 36)
+    _check(x, u, [0.0] * 36)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_strides(gpu, dtype):
+    """Rows at any pitch and alignment: slices of a wider buffer, one row expanded."""
+    rows, vocab = 6, 1003
+    wide = _logits(rows, vocab + 13, 9, dtype).cuda()
+    u, k = _uniforms(rows, 10), [0, 1, 20, 0, 300, 2]
+    for lo in range(5):
+        x = wide[:, lo:lo + vocab]
+        _check(x, u, None, k, [0.9] * rows)
+
+
+def test_largest_vocabulary(gpu):
+    x = _logits(3, sampling.MAX_VOCAB, 11, F32)
+    _check(x, [0.2, 0.5, 0.9], [1.0, 0.9, 1.1], [0, 1000, 0], [1.0, 1.0, 0.9], [0.0, 0.0, 0.0])
+
+
+def test_no_probabilities_and_graph(gpu):
+    x = _logits(8, 5000, 12, F32).cuda()
+    u = torch.tensor(_uniforms(8, 13)).cuda()
+    p = torch.full((8,), 0.9, device="cuda")
+    tokens, probs = torch.zeros(8, dtype=torch.int32, device="cuda"), torch.zeros(8, device="cuda")
+    sampling.sample(tokens, None, x, u, top_p=p)
+    got = torch.zeros_like(tokens)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        sampling.sample(got, probs, x, u, top_p=p)
+    for i in range(3):
+        sampling.sample(tokens, None, x, u, top_p=p)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, tokens)
+        x.add_(torch.randn(x.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(i)))
+        u.copy_(torch.tensor(_uniforms(8, 20 + i)))
