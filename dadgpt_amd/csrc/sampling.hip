@@ -1,16 +1,18 @@
 // Picking tokens by given random numbers for gfx950: temperature, top-k, top-p, min-p and the draw, one
 // workgroup a row and one launch.
 //
-// The filters all keep a head of the row's descending order, so most of a row need only be compared with
-// a bound that no element which stays lies below. In turn: the largest logit; with top-p, the sum Z of all
-// weights; the bound (top-k: the k-th largest of the threads' maxima, which k elements reach, or for a
-// large k a guess from a sample, checked by counting; top-p: the logit of weight (1 - p) Z / vocab, as all
-// elements below it together weigh less than (1 - p) Z; min-p: its own); the elements that reach it, at
-// most 8192, into LDS; and there the cuts and the draw, each the search for the element at which a
-// running sum (of ones or of weights, by logit or by index) crosses a target: a histogram over 1024
-// buckets, the bucket of the crossing, and its few elements compared each with each. Rows with more
-// candidates (a huge top-k, flat weights) search over the row itself, and the draw, as that of a row
-// without filters, goes by the sums of the row's pieces in order.
+// The filters all keep a head of the row's descending order. In turn: the largest logit; a histogram
+// below it of counts (top-k) or counts and weights (top-p), which gives the bucket where the running
+// sum crosses the target; the elements down to that bucket into LDS; and there the cuts and the draw,
+// each the search for the element at which a running sum (of ones or of weights, by logit or by index)
+// crosses its target. Up to 64 elements one wave adds up for each lane what lies above its own; more are
+// searched by a finer histogram and the few elements of its bucket. Rows that keep more than 8192
+// elements search over the row itself, and the draw there, as that of a row without filters, goes by
+// the sums of the waves' stretches of the row.
+//
+// The histogram has 16 columns, one for each lane of a row of 16: however the logits are spread, four
+// lanes of an atomic meet in a bank at most (with one column, 785 wave-wide pairs of atomics on 50257
+// logits of a usual spread took 45 us).
 //
 // A pick must not depend on the order in which weights are added: they are computed in double (relative
 // error below 1e-13) and held as multiples of 2^-44 of the largest one, in 64-bit integers, whose sums
@@ -26,16 +28,13 @@
 namespace dadgpt {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kPiece = 4 * kThreads;        // elements that the workgroup takes at a time, 4 a lane
-constexpr int kMostPieces = (1 << 19) / kPiece + 1;
-constexpr int kBuckets = kThreads;          // of a histogram: one for each thread to scan
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kLevels = 64, kColumns = 16;  // buckets of the row's histogram, copies of each
+constexpr int kBuckets = kThreads;          // of a search's: one for each thread to scan
 constexpr int kFew = kThreads;              // elements of a bucket that are compared each with each
-constexpr int kPerThread = 8, kList = kPerThread * kThreads;  // candidates
-constexpr int kMostK = kThreads / 2;        // top-k by the threads' maxima
+constexpr int kPerThread = 16, kList = kPerThread * kThreads;  // candidates
 constexpr int kOne = 44;                    // weights are multiples of 2^-44
 constexpr float kFaintest = 31.0f;          // e^-31 < 2^-44.7: weighs nothing
-constexpr float kMostFinite = 3.4028234663852886e38f;
 
 typedef unsigned long long u64;
 
@@ -61,12 +60,16 @@ __device__ __forceinline__ u64 dpp64(u64 x) {
   const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
   return (u64)hi << 32 | lo;
 }
-// Sum over the lanes up to and with this one.
-__device__ __forceinline__ u64 wave_scan(u64 x) {
+// Sum over the lanes of its row of 16, and over all, up to and with this one.
+__device__ __forceinline__ u64 row_scan(u64 x) {
   x += dpp64<0x111>(x);  // row_shr:1, 2, 4, 8
   x += dpp64<0x112>(x);
   x += dpp64<0x114>(x);
   x += dpp64<0x118>(x);
+  return x;
+}
+__device__ __forceinline__ u64 wave_scan(u64 x) {
+  x = row_scan(x);
   x += dpp64<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
   x += dpp64<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
   return x;
@@ -85,9 +88,18 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 struct Shared {
   u64 list[kList];                  // the candidates, as order_of
   u64 few[kFew], few_weight[kFew];  // a bucket's elements
-  u64 weight[kBuckets];             // a histogram
-  uint32_t count[kBuckets];
-  u64 piece[kMostPieces * kWaves];  // sums of the waves' pieces, in the row's order
+  union {
+    struct {
+      u64 weight[kLevels][kColumns];      // the row's histogram
+      uint32_t count[kLevels][kColumns];
+    } row;
+    struct {
+      u64 weight[kBuckets];         // a search's
+      uint32_t count[kBuckets];
+    } search;
+  };
+  u64 level_weight[kLevels];
+  uint32_t level_count[kLevels];
   double root[64];                  // 2^(i / 64)
   u64 wave_sum[2][kWaves];          // (in turn, so that one barrier a use is enough)
   uint32_t wave_max[2][kWaves];
@@ -139,7 +151,7 @@ template <>
 struct Four<float> {
   f32x4 w;
   __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const f32x4*>(p); }
-  __device__ __forceinline__ void set(int e, float x) { w[e] = x; }
+  __device__ __forceinline__ void set(int e, float x) { w[e] = x; }  // (in the order of e)
   __device__ __forceinline__ float get(int e) const { return w[e]; }
 };
 template <>
@@ -155,39 +167,59 @@ struct Four<bf16> {
   }
 };
 
-// Element `index` of the row lies in lane (index + shift) / 4 of piece (index + shift) / kPiece, so that
-// four neighbours are one aligned load wherever the row starts.
-template <typename T>
+// The row in stretches, one for each wave, in order; a wave goes through its own in pieces of 256
+// elements, four neighbours a lane. Element `index` is number index + shift of them, so that four
+// neighbours are one aligned load wherever the row starts. NP > 0: a row of at most NP pieces a wave,
+// which stays in registers for the passes over all of it; 0: they read it again (from L2).
+template <typename T, int NP>
 struct Row {
   const T* row;
-  int vocab, shift, pieces, tid, lane, wave;
+  Four<T> kept[NP > 0 ? NP : 1];
+  int vocab, shift, pieces, first, tid, lane, wave;
   bool infinite;  // the largest logit is +inf: those count as 0, all others as -inf
   int turn_max = 0, turn_sum = 0;
   Shared& sm;
 
   __device__ __forceinline__ Row(const T* base, int n, Shared& shared)
       : row(base), vocab(n), shift((int)(reinterpret_cast<uintptr_t>(base) / sizeof(T) % 4)),
-        pieces((n + shift + kPiece - 1) / kPiece), tid(threadIdx.x), lane(threadIdx.x & 63),
-        wave(threadIdx.x >> 6), infinite(false), sm(shared) {}
+        pieces((n + shift + 256 * kWaves - 1) / (256 * kWaves)), tid(threadIdx.x),
+        lane(threadIdx.x & 63), wave(threadIdx.x >> 6), infinite(false), sm(shared) {
+    first = wave * pieces * 256 + 4 * lane - shift;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) load(kept[i], i);
+  }
 
   __device__ __forceinline__ void load(Four<T>& x, int piece) const {
-    const int at = piece * kPiece + 4 * tid - shift;
-    if (at >= 0 && at + 4 <= vocab) {
+    const int at = index(piece, 0);
+    if (piece < pieces && at >= 0 && at + 4 <= vocab) {
       x.load(row + at);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        x.set(e, at + e >= 0 && at + e < vocab ? row[at + e] : static_cast<T>(neg_inf()));
+        x.set(e, piece < pieces && at + e >= 0 && at + e < vocab ? row[at + e]
+                                                                : static_cast<T>(neg_inf()));
     }
   }
+  __device__ __forceinline__ int index(int piece, int e) const { return first + piece * 256 + e; }
   __device__ __forceinline__ float value(const Four<T>& x, int e) const {
     const float v = x.get(e);
-    return !infinite ? v : v == __builtin_inff() ? 0.f : neg_inf();
+    return !infinite ? v : only_inf(v);
   }
-  // f(piece, the lane's four elements), N pieces at a time and the next N in flight meanwhile (a piece
-  // past the end: -inf)
+  static __device__ __forceinline__ float only_inf(float v) {
+    return v == __builtin_inff() ? 0.f : neg_inf();
+  }
+  __device__ __forceinline__ void set_infinite() {
+    infinite = true;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const Four<T> x = kept[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) kept[i].set(e, static_cast<T>(only_inf(x.get(e))));
+    }
+  }
+  // f(piece, the lane's four elements), N pieces at a time and the next N in flight meanwhile
   template <int N, typename F>
-  __device__ __forceinline__ void each_piece(F f) const {
+  __device__ __forceinline__ void each_again(F f) const {
     Four<T> next[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) load(next[i], i);
@@ -206,8 +238,19 @@ struct Row {
       }
     }
   }
-  __device__ __forceinline__ int index(int piece, int e) const {
-    return piece * kPiece + 4 * tid + e - shift;
+  // (pieces past the end, there for the sake of whole Ns, are all -inf.) AGAIN: from memory, where the
+  // registers are needed for other things
+  template <bool AGAIN, typename F>
+  __device__ __forceinline__ void each_piece(F f) const {
+    if constexpr (NP > 0 && !AGAIN) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const float v[4] = {kept[i].get(0), kept[i].get(1), kept[i].get(2), kept[i].get(3)};
+        f(i, v);
+      }
+    } else {
+      each_again<4>(f);
+    }
   }
 
   // The largest of a value from each thread.
@@ -239,76 +282,164 @@ struct Row {
 
   // The index at which the sum of measure(x, index) in the row's order reaches `target(sum of all)`,
   // which is above 0 and at most that sum.
-  template <typename M, typename G>
+  template <bool AGAIN, typename M, typename G>
   __device__ __forceinline__ int in_order(M measure, G target_of, u64& all) {
-    each_piece<2>([&](int i, const float (&x)[4]) {
-      u64 s = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s += measure(x[e], index(i, e));
-      s = wave_scan(s);
-      if (lane == 63 && i < pieces) sm.piece[i * kWaves + wave] = s;
-    });
-    __syncthreads();
-    const int n = pieces * kWaves, per = (n + kThreads - 1) / kThreads, first = tid * per;
     u64 mine = 0;
-    for (int i = first; i < min(n, first + per); ++i) mine += sm.piece[i];
-    u64 at = before(mine, all);
-    const u64 target = target_of(all);
-    if (at < target && at + mine >= target) {
-      int i = first;
-      while (at + sm.piece[i] < target) at += sm.piece[i++];
-      sm.bucket = i;
-      sm.found_above = at;
-    }
+    each_piece<AGAIN>([&](int i, const float (&x)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine += measure(x[e], index(i, e));
+    });
+    u64* to = sm.wave_sum[turn_sum ^= 1];
+    const u64 stretch = wave_scan(mine);
+    if (lane == 63) to[wave] = stretch;
     __syncthreads();
-    const int hit = sm.bucket;
-    if (wave == hit % kWaves) {  // this wave's piece: its lanes, then the lane's elements
-      const int i = hit / kWaves;
-      Four<T> x;
-      load(x, i);
-      u64 w[4], s = 0;
+    u64 at = 0, sum = 0, my_sum = 0;
+    all = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += w[e] = measure(value(x, e), index(i, e));
-      u64 to = sm.found_above + wave_scan(s);
-      if (to >= target && to - s < target) {
-        to -= s;
-        int e = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w == wave) at = all, my_sum = to[w];
+      all += to[w];
+    }
+    sum = at + my_sum;
+    const u64 target = target_of(all);
+    if (at < target && sum >= target) {  // this wave's stretch: its pieces, lanes, the lane's elements
+      for (int i = 0; i < pieces; ++i) {
+        Four<T> x;
+        load(x, i);
+        u64 w[4], s = 0;
 #pragma unroll
-        for (int y = 0; y < 3; ++y)
-          if (e == y && to + w[y] < target) to += w[y], ++e;
-        sm.token = index(i, e);
+        for (int e = 0; e < 4; ++e) s += w[e] = measure(value(x, e), index(i, e));
+        const u64 upto = at + wave_scan(s);
+        if (__builtin_amdgcn_ballot_w64(upto >= target) == 0) {
+          at = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(upto >> 32), 63) << 32 |
+               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)upto, 63);
+          continue;
+        }
+        if (upto >= target && upto - s < target) {
+          u64 x = upto - s;
+          int e = 0;
+#pragma unroll
+          for (int y = 0; y < 3; ++y)
+            if (e == y && x + w[y] < target) x += w[y], ++e;
+          sm.token = index(i, e);
+        }
+        break;
       }
     }
     __syncthreads();
     return sm.token;
   }
 
+  // A histogram over buckets bucket_of(x) (kLevels: none), descending, of counts and measure(x, index)
+  // (0: not counted). The bucket at which the sum of measures (and `over`) reaches target_of(sum of
+  // all): its number (kLevels: nowhere), the elements in it and down to its end, and the sums of all
+  // and of what lies above it.
+  struct Level {
+    int bucket;
+    uint32_t own, count;
+    u64 all, over;
+  };
+  __device__ __forceinline__ static u64 lane_of(u64 x, int i) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, i);
+  }
+  template <bool WEIGHTS, bool AGAIN, typename B, typename M, typename G>
+  __device__ __forceinline__ Level histogram(B bucket_of, M measure, G target_of, u64 over = 0) {
+    for (int i = tid; i < kLevels * kColumns; i += kThreads) {
+      sm.row.count[0][i] = 0;
+      if constexpr (WEIGHTS) sm.row.weight[0][i] = 0;
+    }
+    __syncthreads();
+    const int column = lane % kColumns;
+    each_piece<AGAIN>([&](int i, const float (&x)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int b = bucket_of(x[e]);
+        if (b >= kLevels) continue;
+        const u64 w = measure(x[e], index(i, e));
+        if (w == 0) continue;
+        atomicAdd(&sm.row.count[b][column], 1u);
+        if constexpr (WEIGHTS) atomicAdd(&sm.row.weight[b][column], w);
+      }
+    });
+    __syncthreads();
+    for (int i = tid; i < kLevels * kColumns; i += kThreads) {
+      const u64 n = row_scan((u64)sm.row.count[0][i]);
+      const u64 w = WEIGHTS ? row_scan(sm.row.weight[0][i]) : n;
+      if (lane % kColumns == kColumns - 1)
+        sm.level_count[i / kColumns] = (uint32_t)n, sm.level_weight[i / kColumns] = w;
+    }
+    __syncthreads();
+    // (every wave for itself)
+    static_assert(kLevels == 64 && kColumns == 16, "a lane a bucket, a row of lanes its copies");
+    const u64 w = sm.level_weight[lane], upto = wave_scan(w) + over;
+    const u64 own = sm.level_count[lane], n = wave_scan(own);
+    Level r;
+    r.all = lane_of(upto, 63);
+    const u64 target = target_of(r.all);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(upto - w < target && upto >= target);
+    const int at = hit != 0 ? __builtin_ctzll(hit) : 63;
+    r.bucket = hit != 0 ? at : kLevels;
+    r.own = (uint32_t)lane_of(own, at);
+    r.count = (uint32_t)lane_of(n, at);
+    r.over = lane_of(upto - w, at);
+    return r;
+  }
+
+  // Appends the elements with good(x) to sm.list; their number (those past kList are not held).
+  template <bool AGAIN, typename P>
+  __device__ __forceinline__ int collect(P good) {
+    if (tid == 0) sm.listed = 0;
+    __syncthreads();
+    each_piece<AGAIN>([&](int i, const float (&x)[4]) {
+      uint64_t in[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in[e] = __builtin_amdgcn_ballot_w64(good(x[e]));
+      if ((in[0] | in[1] | in[2] | in[3]) == 0) return;  // wave-uniform
+      uint32_t at = 0;
+      if (lane == 0)
+        at = atomicAdd(&sm.listed, (uint32_t)(__builtin_popcountll(in[0]) + __builtin_popcountll(in[1]) +
+                                              __builtin_popcountll(in[2]) + __builtin_popcountll(in[3])));
+      at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32),
+                                                           __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], 0));
+        if ((in[e] >> lane & 1) != 0 && to < (uint32_t)kList) sm.list[to] = order_of(x[e], index(i, e));
+        at += __builtin_popcountll(in[e]);
+      }
+    });
+    __syncthreads();
+    return (int)sm.listed;
+  }
+
   // The element at which the sum of weights, taken in descending order of the elements' numbers, reaches
   // target_of(sum of all); 0 where it does not. each(lo, hi, f) calls f(number, weight) for the
   // elements of those numbers that have a weight; no two have the same number.
+  // (`over`: the sum of weights above hi)
   template <typename Each, typename G>
-  __device__ __forceinline__ u64 search(Each each, u64 lo, u64 hi, G target_of) {
-    u64 over = 0, target = 0;  // over: what lies above the current range
+  __device__ __forceinline__ u64 search(const Each& each, u64 lo, u64 hi, G target_of, u64 over = 0) {
+    u64 target = 0;
     while (true) {
       const float per = (float)kBuckets / ((float)(hi - lo) + 1.0f);
       auto bucket = [&](u64 k) { return min((int)((float)(hi - k) * per), kBuckets - 1); };
-      sm.weight[tid] = 0;
-      sm.count[tid] = 0;
+      sm.search.weight[tid] = 0;
+      sm.search.count[tid] = 0;
       if (tid == 0) sm.bucket = kBuckets, sm.listed = 0;
       __syncthreads();
       each(lo, hi, [&](u64 k, u64 w) {
         const int b = bucket(k);
-        atomicAdd(&sm.weight[b], w);
-        atomicAdd(&sm.count[b], 1u);
+        atomicAdd(&sm.search.weight[b], w);
+        atomicAdd(&sm.search.count[b], 1u);
       });
       __syncthreads();
       u64 all;
-      const u64 w = sm.weight[tid], upto = over + before(w, all);
+      const u64 w = sm.search.weight[tid], upto = over + before(w, all);
       if (target == 0) target = target_of(all);
       if (upto < target && upto + w >= target) {
         sm.bucket = tid;
         sm.found_above = upto;
-        sm.bucket_count = sm.count[tid];
+        sm.bucket_count = sm.search.count[tid];
       }
       __syncthreads();
       const int b = sm.bucket;
@@ -387,86 +518,194 @@ struct Pick {
   u64 all;  // the weights' sum that it was drawn from; 0: taken, not drawn
 };
 
-// Over the whole row; hi: the largest key.
-template <typename T>
-__device__ Pick pick_from_row(Row<T>& row, const Settings& s, const Weigher& weigh, uint32_t hi) {
+// Buckets of equal width below `top`, the last one with all that lies lower; and those of one bucket, in
+// 64 equal parts of it.
+struct Levels {
+  float top, per;
+  __device__ __forceinline__ int operator()(float x) const {
+    return x > neg_inf() ? (int)fminf((top - x) * per, (float)(kLevels - 1)) : kLevels;
+  }
+};
+struct Parts {
+  Levels levels;
+  int bucket;
+  __device__ __forceinline__ int operator()(float x) const {
+    const float t = (levels.top - x) * levels.per - (float)bucket;
+    return x > neg_inf() && t >= 0.f && t < 1.0f ? (int)(t * (float)kLevels) : kLevels;
+  }
+};
+
+// Elements of sm.list, kPerThread of them with every thread, each of weight 1.
+__device__ __forceinline__ Elements<kPerThread> listed(const Shared& sm, int tid, int n) {
+  Elements<kPerThread> x;
+#pragma unroll
+  for (int j = 0; j < kPerThread; ++j) {
+    const int i = tid + j * kThreads;
+    x.number[j] = i < n ? sm.list[i] : 0;
+    x.weight[j] = i < n ? 1 : 0;
+  }
+  return x;
+}
+
+// Over the whole row, where more stays than the list holds; hi: the largest key, `first`: the row's
+// histogram for the first filter.
+template <typename T, int NP>
+__device__ __forceinline__ Pick pick_from_row(Row<T, NP>& row, const Settings& s, const Weigher& weigh,
+                                              uint32_t hi, float per_k, float per_p,
+                                              const typename Row<T, NP>::Level& first) {
   u64 cut = 1ull << 32;  // what stays: numbers from here on
   const u64 most = (u64)hi << 32 | 0xffffffffu;
-  auto each = [&](auto weight) {
-    return [&row, weight](u64 lo, u64 hi, auto f) {
-      row.template each_piece<2>([&](int i, const float (&x)[4]) {
+  const float top = (float)weigh.top;
+  // The number at which the sum of weigh_of(x, number) reaches its target: by the row's histogram and the
+  // elements of its bucket, or, if they are too many (ties), in the row.
+  auto cut_at = [&](auto by_weight, float per, auto target_of, bool known) {
+    auto weight = [&](float x, u64 k) -> u64 {
+      if constexpr (by_weight())
+        return weigh(x) & (k >= cut ? ~u64(0) : 0);
+      else
+        return 1;
+    };
+    auto measure = [&](float x, int i) { return weight(x, order_of(x, i)); };
+    const Levels levels{top, per};
+    auto at = known ? first : row.template histogram<by_weight(), true>(levels, measure, target_of);
+    const u64 target = target_of(at.all);
+    auto among = [&](auto bucket_of) -> u64 {  // (the elements that weigh nothing are not in `own`)
+      const int n =
+          row.template collect<true>([&](float x) { return bucket_of(x) == at.bucket; });
+      if (n > kList) return 0;
+      Elements<kPerThread> x = listed(row.sm, row.tid, n);
+      uint32_t low = 0;
+#pragma unroll
+      for (int j = 0; j < kPerThread; ++j)
+        if (x.weight[j] != 0) {
+          low = max(low, (uint32_t)(~x.number[j] >> 32));
+          x.weight[j] = weight(logit_of((uint32_t)(x.number[j] >> 32)), x.number[j]);
+        }
+      const uint32_t least = ~row.largest(low);
+      return row.search(x, (u64)least << 32, most, [&](u64) { return target; }, at.over);
+    };
+    u64 found = 0;
+    if (at.own <= (uint32_t)kList) {
+      found = among(levels);
+    } else if (at.bucket < kLevels - 1) {
+      const Parts parts{levels, at.bucket};
+      at = row.template histogram<by_weight(), true>(parts, measure, [&](u64) { return target; }, at.over);
+      if (at.own <= (uint32_t)kList) found = among(parts);
+    }
+    if (found != 0) return found;
+    auto each = [&](u64 lo, u64 hi, auto f) {
+      row.template each_again<2>([&](int i, const float (&x)[4]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const u64 k = order_of(x[e], row.index(i, e));
           if (k >= lo && k <= hi) {
-            const u64 w = weight(x[e]);
+            const u64 w = weight(x[e], k);
             if (w != 0) f(k, w);
           }
         }
       });
     };
+    return row.search(each, cut, most, [&](u64) { return target; });
   };
-  if (s.k < row.vocab) {
-    const u64 at = row.search(each([](float) { return u64(1); }), cut, most,
-                              [&](u64) { return (u64)s.k; });
-    cut = max(cut, at);
-  }
-  if (s.p < 1.0f) {
-    const u64 faint = (u64)key_of((float)weigh.top - kFaintest * s.temperature) << 32;
-    const u64 at = row.search(each([&](float x) { return weigh(x); }), max(cut, faint), most,
-                              [&](u64 all) { return reaching(s.p, all); });
-    cut = max(cut, at);
-  }
+  if (s.k < row.vocab)
+    cut = max(cut, cut_at(std::false_type{}, per_k, [&](u64) { return (u64)s.k; }, true));
+  if (s.p < 1.0f)
+    cut = max(cut, cut_at(std::true_type{}, per_p, [&](u64 all) { return reaching(s.p, all); },
+                          s.k == row.vocab));
   Pick pick;
-  pick.token = row.in_order(
+  pick.token = row.template in_order<true>(
       [&](float x, int i) -> u64 {
-        if (order_of(x, i) < cut) return 0;
-        if (s.min_p > 0.f && weigh.exact(x) < (double)s.min_p) return 0;
-        return weigh(x);
+        // (no branch: one would leave each weight's latency bare)
+        const u64 w = weigh(x) & (order_of(x, i) >= cut ? ~u64(0) : 0);
+        return s.min_p > 0.f && weigh.exact(x) < (double)s.min_p ? 0 : w;
       },
       [&](u64 all) { return exceeding(s.u, all); }, pick.all);
   return pick;
 }
 
+// Of a number and a weight a lane (0: none; no two numbers are the same): the sum of the weights of the
+// lanes with larger numbers.
+__device__ __forceinline__ u64 above_in_wave(u64 number, u64 weight, int n) {
+  u64 sum = 0;
+  for (int i = 0; i < n; ++i) {
+    const u64 k = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(number >> 32), i) << 32 |
+                  (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)number, i);
+    const u64 w = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(weight >> 32), i) << 32 |
+                  (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)weight, i);
+    sum += k > number ? w : 0;
+  }
+  return sum;
+}
+__device__ __forceinline__ u64 wave_total(u64 x) {
+  x = wave_scan(x);
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, 63);
+}
+
+// pick_from_list for up to 64 candidates, in one wave; the answer is in every lane.
+__device__ __forceinline__ Pick pick_in_wave(const Settings& s, const Weigher& weigh, u64 number, int n,
+                                             u64 z, int lane) {
+  u64 w = 0;
+  if (lane < n) {
+    w = weigh(logit_of((uint32_t)(number >> 32)));
+    if (s.min_p > 0.f && !(s.p < 1.0f) && weigh.exact(logit_of((uint32_t)(number >> 32))) < (double)s.min_p)
+      w = 0;
+  }
+  if (s.k < n && above_in_wave(number, lane < n ? 1 : 0, n) >= (u64)s.k) w = 0;
+  if (s.p < 1.0f) {
+    const u64 all = z != 0 ? z : wave_total(w);
+    if (above_in_wave(number, w, n) >= reaching(s.p, all)) w = 0;
+    if (s.min_p > 0.f && w != 0 &&
+        weigh.exact(logit_of((uint32_t)(number >> 32))) < (double)s.min_p)
+      w = 0;
+  }
+  Pick pick;
+  pick.all = wave_total(w);
+  const u64 at = (uint32_t)number, before = above_in_wave(at, w, n);  // ~index: the lowest first
+  const u64 target = exceeding(s.u, pick.all);
+  const uint64_t hit = __builtin_amdgcn_ballot_w64(w != 0 && before < target && before + w >= target);
+  pick.token = (int)~(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)number, __builtin_ctzll(hit));
+  return pick;
+}
+
 // Among the n candidates in sm.list, which hold every element that can stay; z: the weights' sum that
 // top-p goes by, 0 for that of the first k.
-template <typename T>
-__device__ Pick pick_from_list(Row<T>& row, const Settings& s, const Weigher& weigh, uint32_t hi, int n,
+template <typename T, int NP>
+__device__ __forceinline__ Pick pick_from_list(Row<T, NP>& row, const Settings& s, const Weigher& weigh, uint32_t hi, int n,
                                u64 z) {
   Shared& sm = row.sm;
-  Elements<kPerThread> x;
+  Elements<kPerThread> x = listed(sm, row.tid, n);
   uint32_t low = 0;
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) {
-    const int i = row.tid + j * kThreads;
-    x.number[j] = i < n ? sm.list[i] : 0;
-    x.weight[j] = i < n ? 1 : 0;
-    if (i < n) low = max(low, (uint32_t)(~x.number[j] >> 32));
-  }
+  for (int j = 0; j < kPerThread; ++j)
+    if (x.weight[j] != 0) low = max(low, (uint32_t)(~x.number[j] >> 32));
   const u64 most = (u64)hi << 32 | 0xffffffffu;
   u64 cut = (u64)~row.largest(low) << 32;
   if (s.k < n) cut = row.search(x, cut, most, [&](u64) { return (u64)s.k; });
   u64 sum = 0;
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) {
-    if (j * kThreads >= n) break;
-    x.weight[j] = x.number[j] >= cut && j * kThreads + row.tid < n ? weigh(logit_of(x.number[j] >> 32)) : 0;
-    sum += x.weight[j];
-  }
+  for (int j = 0; j < kPerThread; ++j)
+    if (j * kThreads < n) {
+      x.weight[j] = j * kThreads + row.tid < n && x.number[j] >= cut
+                        ? weigh(logit_of((uint32_t)(x.number[j] >> 32)))
+                        : 0;
+      sum += x.weight[j];
+    }
   if (s.p < 1.0f) {
     if (z == 0) row.before(sum, z);
-    cut = row.search(x, cut, most, [&](u64) { return reaching(s.p, z); });  // (0: not reached)
+    cut = row.search(x, cut, most, [&](u64) { return reaching(s.p, z); });
   }
   sum = 0;
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) {
-    if (j * kThreads >= n) break;
-    if (x.number[j] < cut ||
-        (s.min_p > 0.f && weigh.exact(logit_of(x.number[j] >> 32)) < (double)s.min_p))
-      x.weight[j] = 0;
-    x.number[j] = (uint32_t)x.number[j];  // ~index: the lowest first
-    sum += x.weight[j];
-  }
+  for (int j = 0; j < kPerThread; ++j)
+    if (j * kThreads < n) {
+      if (x.number[j] < cut ||
+          (s.min_p > 0.f &&
+           weigh.exact(logit_of((uint32_t)(x.number[j] >> 32))) < (double)s.min_p))
+        x.weight[j] = 0;
+      x.number[j] = (uint32_t)x.number[j];  // ~index: the lowest first
+      sum += x.weight[j];
+    }
   Pick pick;
   row.before(sum, pick.all);
   const u64 at = row.search(x, (uint32_t)~(row.vocab - 1), 0xffffffffu,
@@ -475,14 +714,14 @@ __device__ Pick pick_from_list(Row<T>& row, const Settings& s, const Weigher& we
   return pick;
 }
 
-template <typename T>
+template <typename T, int NP>
 __global__ __launch_bounds__(kThreads) void sample_kernel(
     int* __restrict__ tokens, float* __restrict__ probs, const T* __restrict__ logits, long long ld,
     int vocab, const SampleSettings set) {
   __shared__ Shared sm;
   const int r = blockIdx.x;
   const T* base = logits + r * ld;
-  Row<T> row(base, vocab, sm);
+  Row<T, NP> row(base, vocab, sm);
   const int tid = row.tid;
 
   Settings s;
@@ -499,7 +738,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(
   if (tid < 64) sm.root[tid] = exp2(tid / 64.0);
 
   float mine = neg_inf();
-  row.template each_piece<4>([&](int, const float (&x)[4]) {
+  row.template each_piece<false>([&](int, const float (&x)[4]) {
     mine = fmaxf(fmaxf(fmaxf(fmaxf(mine, x[0]), x[1]), x[2]), x[3]);
   });
   uint32_t hi = row.largest(key_of(mine));
@@ -511,7 +750,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(
   };
   if (hi == 0) return answer(-1, 0.f);  // nothing to pick
   if (logit_of(hi) == __builtin_inff()) {
-    row.infinite = true;
+    row.set_infinite();
     mine = mine == __builtin_inff() ? 0.f : neg_inf();
     hi = key_of(0.f);
   }
@@ -519,7 +758,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(
   if (s.k == 1) {
     uint32_t first = 0;  // ~index
     if (mine == top)     // (only some threads: their elements once more)
-      row.template each_piece<2>([&](int i, const float (&x)[4]) {
+      row.template each_again<4>([&](int i, const float (&x)[4]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (x[e] == top) first = max(first, (uint32_t)~row.index(i, e));
@@ -534,87 +773,73 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(
     const double x = (double)top + log(0.5 * w) * (double)s.temperature;
     return (float)(x - fabs(x) * 0x1p-22);
   };
-  // The bound, as a logit: every element that can stay reaches it.
-  const u64 most = (u64)hi << 32 | 0xffffffffu;
-  float bound = neg_inf();
+  auto finish = [&](const Pick& pick) {
+    Four<T> x;
+    x.set(0, base[pick.token]);
+    answer(pick.token, (float)(weigh.exact(row.value(x, 0)) * 0x1p44 / (double)pick.all));
+  };
+  int n = kList + 1;  // candidates
+  typename Row<T, NP>::Level at{};
   u64 z = 0;
-  bool bounded = vocab <= kList;
-  if (!bounded && s.k < vocab) {
-    if (s.k <= kMostK) {
-      // (fewer threads with an element than k: 0, no bound)
-      const Elements<1> x{{order_of(mine, tid)}, {mine > neg_inf() ? u64(1) : 0}};
-      const uint32_t low = ~row.largest(x.weight[0] != 0 ? ~key_of(mine) : 0u);
-      const u64 at = row.search(x, (u64)low << 32, most, [&](u64) { return (u64)s.k; });
-      if (at != 0) bound = logit_of((uint32_t)(at >> 32));
-      bounded = true;
-    } else if (s.k <= kList * 2 / 3) {
-      // one piece from the middle: a tenth more of it than k's share, and three standard deviations
-      Four<T> four;
-      row.load(four, row.pieces / 2);
-      Elements<4> x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = row.value(four, e);
-        x.number[e] = order_of(v, 4 * tid + e);
-        x.weight[e] = v > neg_inf() ? 1 : 0;
-      }
-      const float share = 1.1f * (float)s.k * (float)kPiece / (float)vocab;
-      const u64 at = row.search(x, 0, most, [&](u64) { return (u64)(share + 3.0f * sqrtf(share)); });
-      if (at != 0) bound = logit_of((uint32_t)(at >> 32));
-      bounded = at != 0;
+  // buckets a unit of logit: for top-k down to the smallest maximum of a thread, which that many elements
+  // reach if every thread has one, and further for a larger k; for top-p down to what weighs nothing
+  float per_k = 0.f, per_p = (float)(kLevels - 1) / (kFaintest * s.temperature);
+  if (!(per_p < 0x1p100f)) per_p = 0x1p100f;
+  if (s.k < vocab) {
+    const uint32_t low = ~row.largest(~key_of(mine));
+    const float range = low != 0 ? 1.02f * (top - logit_of(low)) : kFaintest;
+    per_k = (float)(kLevels - 1) / (s.k <= kThreads ? range : 2.0f * range);
+    if (!(per_k < 0x1p100f)) per_k = 0x1p100f;
+  }
+  if (vocab <= kList && (s.k < vocab || s.p < 1.0f)) {
+    n = row.template collect<false>([](float x) { return x > neg_inf(); });
+  } else if (s.k < vocab || s.p < 1.0f) {
+    const bool by_k = s.k < vocab;
+    const Levels levels{top, by_k ? per_k : per_p};
+    if (by_k)
+      at = row.template histogram<false, false>(levels, [](float, int) { return u64(1); },
+                                         [&](u64) { return (u64)s.k; });
+    else
+      at = row.template histogram<true, false>(levels, [&](float x, int) { return weigh(x); },
+                                        [&](u64 all) { return reaching(s.p, all); });
+    if (!by_k) z = at.all;
+    if (at.count <= (uint32_t)kList) {
+      // (a bound: the last bucket's is all that is above -inf)
+      const float end = at.bucket < kLevels - 1 ? (float)(at.bucket + 1) : __builtin_inff();
+      n = row.template collect<false>([&](float x) { return (top - x) * levels.per < end; });
     }
-  } else if (!bounded && s.p < 1.0f) {
-    u64 sum = 0;
-    row.template each_piece<2>([&](int, const float (&x)[4]) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += weigh(x[e]);
-    });
-    row.before(sum, z);
-    bound = logit_at((1.0 - (double)fmaxf(s.p, 0.f)) * (double)z / 0x1p44 / vocab);
-    bounded = true;
+  } else if (s.min_p > 0.f) {
+    const float bound = fmaxf(logit_at(s.min_p), -3.4028234663852886e38f);
+    n = row.template collect<false>([&](float x) { return x >= bound; });
   }
-  // (top-p after top-k goes by the weights of the first k, also of those below min-p; after no top-k by Z,
-  // which is known unless everything is a candidate)
-  if (s.min_p > 0.f && !(s.p < 1.0f && z == 0)) {
-    bound = fmaxf(bound, logit_at(s.min_p));
-    bounded = true;
+  if (s.k == vocab && s.p == 1.0f && s.min_p == 0.f) {
+    Pick pick;
+    pick.token = row.template in_order<false>(
+        [&](float x, int) { return weigh(x); }, [&](u64 all) { return exceeding(s.u, all); }, pick.all);
+    return finish(pick);
   }
-  Pick pick;
-  bool picked = false;
-  if (bounded) {
-    bound = fmaxf(bound, -kMostFinite);
-    if (tid == 0) sm.listed = 0;
-    __syncthreads();
-    row.template each_piece<4>([&](int i, const float (&x)[4]) {
-      if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= bound) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (x[e] >= bound) {
-            const uint32_t at = atomicAdd(&sm.listed, 1u);
-            if (at < (uint32_t)kList) sm.list[at] = order_of(x[e], row.index(i, e));
-          }
-      }
-    });
-    __syncthreads();
-    const int n = (int)sm.listed;
-    // (by the sample, k elements at least; otherwise the list holds what stays by its bound)
-    if (n <= kList && (n >= s.k || s.k <= kMostK || s.k == vocab || vocab <= kList)) {
-      pick = pick_from_list(row, s, weigh, hi, n, z);
-      picked = true;
+  if (n <= 64) {
+    if (row.wave == 0) {
+      const u64 number = row.lane < n ? sm.list[row.lane] : 0;
+      finish(pick_in_wave(s, weigh, number, n, z, row.lane));
     }
-    __syncthreads();
+    return;
   }
-  if (!picked) pick = pick_from_row(row, s, weigh, hi);
-  Four<T> x;
-  x.set(0, base[pick.token]);
-  answer(pick.token, (float)(weigh.exact(row.value(x, 0)) * 0x1p44 / (double)pick.all));
+  finish(n <= kList ? pick_from_list(row, s, weigh, hi, n, z) : pick_from_row(row, s, weigh, hi, per_k, per_p, at));
 }
 
 template <typename T>
 hipError_t launch_sample_t(int* tokens, float* probs, const T* logits, long long ld, int rows,
                            int vocab, const SampleSettings& set, hipStream_t stream) {
-  sample_kernel<T><<<rows, kThreads, 0, stream>>>(tokens, probs, logits, ld, vocab, set);
-  return hipGetLastError();
+  auto run = [&](auto np) {
+    sample_kernel<T, np()><<<rows, kThreads, 0, stream>>>(tokens, probs, logits, ld, vocab, set);
+    return hipGetLastError();
+  };
+  // pieces of 256 elements for each of the 8 waves; up to 25 of them stay in registers (100 for fp32)
+  const int pieces = (vocab + 3 + 256 * kWaves - 1) / (256 * kWaves);
+  if (pieces <= 8) return run(std::integral_constant<int, 8>{});
+  if (pieces <= 25) return run(std::integral_constant<int, 25>{});
+  return run(std::integral_constant<int, 0>{});
 }
 
 }  // namespace
