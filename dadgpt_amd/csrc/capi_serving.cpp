@@ -331,7 +331,7 @@ int attend(const char* fn, T* out, int64_t ld_out, const T* q, int64_t ld_q, con
   if (flat_meets(K, O)) return overlaps(fn, "out", "k_pages");
   if (flat_meets(V, O)) return overlaps(fn, "out", "v_pages");
   if (int st = check_step_apart(fn, s, O)) return st;
-  const size_t need = dadgpt::paged_workspace_needed(s);
+  const size_t need = dadgpt::paged_workspace_needed(s, elem);
   if (need > 0) {
     if (ws == nullptr || ws_bytes < need)
       return fail(DADGPT_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", fn,

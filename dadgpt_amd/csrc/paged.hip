@@ -26,7 +26,7 @@ struct AppendArgs {
 // of a row, which lie side by side in the projection's output.
 template <typename T, int VEC, bool INTER, int HPT>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs<T> a) {
-  const paged::NewRows seq(a.p, blockIdx.y);
+  const auto seq = paged::NewRows::of<true>(a.p, blockIdx.y);
   const int D = a.p.D, chunks = D / (2 * VEC);
   const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t c = id % chunks, j = id / chunks;

@@ -69,7 +69,7 @@ __device__ __forceinline__ Work find_work(const TileArgs<T>& a, int lane) {
     for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
       int n = 0;
       if (s0 + lane < a.p.n_seq) {
-        const paged::NewRows r(a.p, s0 + lane);
+        const auto r = paged::NewRows::of<false>(a.p, s0 + lane);
         n = (int)(((long long)r.count * a.group + kTile - 1) / kTile);
       }
       int upto = n;
@@ -90,8 +90,10 @@ __device__ __forceinline__ Work find_work(const TileArgs<T>& a, int lane) {
   }
   Work w{};
   if (seq >= a.p.n_seq) return w;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  tile = __builtin_amdgcn_readfirstlane(tile);
   w.seq = seq;
-  const paged::NewRows r(a.p, seq);
+  const auto r = paged::NewRows::of<true>(a.p, seq);
   w.row0 = tile * kTile;
   w.rows = (int)min((long long)kTile, (long long)r.count * a.group - w.row0);
   if (w.none()) return w;
@@ -122,23 +124,31 @@ __device__ __forceinline__ void st_agent2(float* p, float a, float b) {
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// e^x or, in the bf16 kernel, whose maxima are in log2 units, 2^x; 0 at -inf.
-template <typename T>
+// 2^x where the maxima are in log2 units, e^x where they are in natural-log ones (the fp32 tiles); 0 at
+// -inf.
+template <bool LOG2>
 __device__ __forceinline__ float weight_of(float x) {
-  if constexpr (sizeof(T) == 2)
+  if constexpr (LOG2)
     return fast_exp2(x);
   else
     return x == neg_inf() ? 0.f : exp_acc(x);
 }
 
+__device__ __forceinline__ void ld_agent2(const float* p, float& a, float& b) {
+  const uint64_t w = __hip_atomic_load(const_cast<uint64_t*>(reinterpret_cast<const uint64_t*>(p)),
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  a = __uint_as_float((uint32_t)w);
+  b = __uint_as_float((uint32_t)(w >> 32));
+}
+
 // Parts of one row's sums: maximum, weights, weighted values. A part whose scores are all -inf weighs
 // nothing.
-template <typename T>
+template <bool LOG2>
 struct Merged {
   float m = neg_inf(), l = 0.f, o = 0.f;
   __device__ __forceinline__ void add(float m1, float l1, float o1) {
     const float mn = fmaxf(m, m1), base = mn == neg_inf() ? 0.f : mn;
-    const float f0 = weight_of<T>(m - base), f1 = weight_of<T>(m1 - base);
+    const float f0 = weight_of<LOG2>(m - base), f1 = weight_of<LOG2>(m1 - base);
     m = mn;
     l = l * f0 + l1 * f1;
     o = o * f0 + o1 * f1;
@@ -147,11 +157,11 @@ struct Merged {
 };
 // The partials of chunks c0 .. c1 - 1 of one element (`at`: its row's first partial, `col`), eight
 // loaded before any is used.
-template <typename T>
-__device__ __forceinline__ Merged<T> merge_chunks_of(const float* at, size_t pitch, int col, int c0,
+template <bool LOG2>
+__device__ __forceinline__ Merged<LOG2> merge_chunks_of(const float* at, size_t pitch, int col, int c0,
                                                      int c1) {
   constexpr int N = 8;
-  Merged<T> r;
+  Merged<LOG2> r;
   for (int c = c0; c < c1; c += N) {
     float m[N], l[N], o[N];
 #pragma unroll
@@ -168,34 +178,85 @@ __device__ __forceinline__ Merged<T> merge_chunks_of(const float* at, size_t pit
   return r;
 }
 
-// The last workgroup of a tile to arrive: every chunk's partial is written. `lds`: kFew * D * kWaves * 3
-// floats. Few rows: a wave takes every element for a quarter of the chunks.
-constexpr int kFew = 8;
-template <typename T, int D>
+// The last workgroup of a tile to arrive: every chunk's partial is written. Up to FEW rows, a wave takes
+// every element for its share of the chunks; `lds` has room for FEW * D * WAVES Merged.
+constexpr int kFew = 8, kMergeChunks = 16;
+template <bool LOG2, int WAVES, int FEW, typename T, int D>
 __device__ __forceinline__ void merge_tile(const TileArgs<T>& a, const Work& w, const float* part,
-                                           float* lds) {
+                                           void* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t pitch = (size_t)a.part_rows * (D + 2);
   auto store = [&](int e, float x) {
     const RowPlace at = row_place<D>(w, a.group, e / D);
     a.out[(w.first + at.t) * a.ld_out + at.col + e % D] = Elem<T>::from(x);
   };
+  auto merge = [&](int e, int c0, int c1) {
+    return merge_chunks_of<LOG2>(part + (e / D) * (D + 2), pitch, e % D, c0, c1);
+  };
   const int n = w.rows * D;
-  if (w.rows > kFew) {
-    for (int e = tid; e < n; e += kThreads)
-      store(e, merge_chunks_of<T>(part + (e / D) * (D + 2), pitch, e % D, 0, w.chunks).value());
+  if (w.rows > FEW) {
+    if (w.chunks <= kMergeChunks && w.rows <= kTile && WAVES == kWaves) {
+      // every row's maximum and sum once, as a factor for each chunk; then a thread adds up pairs of
+      // columns, 16 of them and so as many loads of a chunk in flight
+      float(*factor)[kTile] = reinterpret_cast<float(*)[kTile]>(lds);
+      for (int r = tid; r < w.rows; r += 64 * WAVES) {
+        float m[kMergeChunks], l[kMergeChunks], most = neg_inf(), sum = 0.f;
+        const float* at = part + (size_t)r * (D + 2);
+#pragma unroll
+        for (int c = 0; c < kMergeChunks; ++c) {
+          const int x = min(c, w.chunks - 1);
+          ld_agent2(at + x * pitch, m[c], l[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < kMergeChunks; ++c)
+          if (c < w.chunks) most = fmaxf(most, m[c]);
+        const float base = most == neg_inf() ? 0.f : most;
+#pragma unroll
+        for (int c = 0; c < kMergeChunks; ++c)
+          if (c < w.chunks) m[c] = weight_of<LOG2>(m[c] - base), sum += l[c] * m[c];
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+        for (int c = 0; c < kMergeChunks; ++c)
+          if (c < w.chunks) factor[c][r] = m[c] * inv;
+      }
+      __syncthreads();
+      constexpr int P = kTile * D / 2 / (64 * WAVES);  // pairs a thread
+      float x[P], y[P];
+#pragma unroll
+      for (int j = 0; j < P; ++j) x[j] = y[j] = 0.f;
+      for (int c = 0; c < w.chunks; ++c) {
+        float u[P], v[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const int e = 2 * min(tid + j * 64 * WAVES, n / 2 - 1);
+          ld_agent2(part + c * pitch + (size_t)(e / D) * (D + 2) + 2 + e % D, u[j], v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const float f = factor[c][2 * min(tid + j * 64 * WAVES, n / 2 - 1) / D];
+          x[j] = fmaf(u[j], f, x[j]);
+          y[j] = fmaf(v[j], f, y[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const int e = 2 * (tid + j * 64 * WAVES);
+        if (e < n) store(e, x[j]), store(e + 1, y[j]);
+      }
+      return;
+    }
+    for (int e = tid; e < n; e += 64 * WAVES) store(e, merge(e, 0, w.chunks).value());
     return;
   }
-  Merged<T>* all = reinterpret_cast<Merged<T>*>(lds);
-  const int c0 = w.chunks * wave / kWaves, c1 = w.chunks * (wave + 1) / kWaves;
-  for (int e = lane; e < n; e += 64)
-    all[wave * kFew * D + e] = merge_chunks_of<T>(part + (e / D) * (D + 2), pitch, e % D, c0, c1);
+  Merged<LOG2>* all = reinterpret_cast<Merged<LOG2>*>(lds);
+  const int c0 = w.chunks * wave / WAVES, c1 = w.chunks * (wave + 1) / WAVES;
+  for (int e = lane; e < n; e += 64) all[wave * FEW * D + e] = merge(e, c0, c1);
   __syncthreads();
-  for (int e = tid; e < n; e += kThreads) {
-    Merged<T> r = all[e];
+  for (int e = tid; e < n; e += 64 * WAVES) {
+    Merged<LOG2> r = all[e];
 #pragma unroll
-    for (int x = 1; x < kWaves; ++x) {
-      const Merged<T>& y = all[x * kFew * D + e];
+    for (int x = 1; x < WAVES; ++x) {
+      const Merged<LOG2>& y = all[x * FEW * D + e];
       r.add(y.m, y.l, y.o);
     }
     store(e, r.value());
@@ -263,7 +324,7 @@ __device__ __forceinline__ void join_waves(const WaveRows<D>& r, f32x16 (&o)[D /
       const int from = x * r.groups + r.grp;
       const float m1 = ml[from][0][lane], mn = fmaxf(m, m1);
       const float base = mn == neg_inf() ? 0.f : mn;
-      const float f0 = weight_of<T>(m - base), f1 = weight_of<T>(m1 - base);
+      const float f0 = weight_of<sizeof(T) == 2>(m - base), f1 = weight_of<sizeof(T) == 2>(m1 - base);
       m = mn;
       l = l * f0 + ml[from][1][lane] * f1;
 #pragma unroll
@@ -280,7 +341,7 @@ __device__ __forceinline__ void leave_partial(const TileArgs<T>& a, const Work& 
                                               float l, float* lds, int* flag, int lane) {
   const int l32 = lane & 31, hi = lane >> 5;
   const size_t unit = (size_t)blockIdx.y * a.p.Hkv + blockIdx.x;
-  float* part = a.part + unit * a.n_chunk * a.part_rows * (D + 2);
+  float* part = tile_partials<D>(a);
   if (r.owner() && r.q0 + l32 < w.rows) {
     float* row = part + ((size_t)blockIdx.z * a.part_rows + r.q0 + l32) * (D + 2);
     if (hi == 0) st_agent2(row, m, l);
@@ -293,7 +354,8 @@ __device__ __forceinline__ void leave_partial(const TileArgs<T>& a, const Work& 
         st_agent2(to + 2, o[db][4 * g + 2], o[db][4 * g + 3]);
       }
   }
-  if (last_to_arrive(a.counter + unit, w.chunks, flag)) merge_tile<T, D>(a, w, part, lds);
+  if (last_to_arrive(a.counter + unit, w.chunks, flag))
+    merge_tile<sizeof(T) == 2, kWaves, kFew, T, D>(a, w, part, lds);
 }
 
 // The pages of a tile's four groups of 16 tokens, the first of them token `key`.
@@ -306,8 +368,173 @@ __device__ __forceinline__ Pages pages_at(const TileArgs<T>& a, const Work& w, i
   Pages g;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    g.id[i] = table[min((key + 16 * i) >> a.page_log2, a.p.max_pages - 1)];
+    g.id[i] = paged::ld_uniform(table + min((key + 16 * i) >> a.page_log2, a.p.max_pages - 1));
   return g;
+}
+
+// The partials of the workgroup's tile.
+template <int D, typename T>
+__device__ __forceinline__ float* tile_partials(const TileArgs<T>& a) {
+  const size_t unit = (size_t)blockIdx.y * a.p.Hkv + blockIdx.x;
+  return a.part + unit * a.n_chunk * a.part_rows * (D + 2);
+}
+
+// Merges the waves' results in LDS into the output, or into the chunk's partial; true in the last
+// workgroup of a tile of several chunks.
+template <bool LOG2, int W, int ROWS, typename T, int D>
+__device__ __forceinline__ bool merge_waves(const TileArgs<T>& a, const Work& w,
+                                            const float (&o)[W][ROWS][D], const float (&m)[W][ROWS],
+                                            const float (&l)[W][ROWS], int* flag) {
+  float* part = tile_partials<D>(a);
+  for (int e = threadIdx.x; e < w.rows * D; e += 64 * W) {
+    const int r = e / D, col = e % D;
+    Merged<LOG2> x;
+#pragma unroll
+    for (int i = 0; i < W; ++i) x.add(m[i][r], l[i][r], o[i][r][col]);
+    if (w.chunks == 1) {
+      const RowPlace p = row_place<D>(w, a.group, r);
+      a.out[(w.first + p.t) * a.ld_out + p.col + col] = Elem<T>::from(x.value());
+    } else {
+      float* to = part + ((size_t)blockIdx.z * a.part_rows + r) * (D + 2);
+      st_agent(to + 2 + col, x.o);
+      if (col == 0) st_agent2(to, x.m, x.l);
+    }
+  }
+  return w.chunks > 1 &&
+         last_to_arrive(a.counter + (size_t)blockIdx.y * a.p.Hkv + blockIdx.x, w.chunks, flag);
+}
+
+// ------------------------------------------------------------------------ a few rows
+
+// NR rows (1 to 4: a token of as many query heads, or a few tokens): products on the VALU, as decode.hip's.
+// Every 16-byte load of a wave covers whole rows of a page, all of a wave's loads are in flight before any
+// arithmetic, and nothing passes through LDS before the waves are merged. A chunk is one round of loads of
+// eight waves: `chunk` is few_keys().
+constexpr int kRowWaves = 8, kRowLoads = 8;
+template <typename T, int D>
+__host__ __device__ constexpr int few_keys() {
+  return kRowWaves * kRowLoads * 64 / (D / Elem<T>::kPer16B);
+}
+
+template <typename T, int D, int NR>
+__global__ __launch_bounds__(64 * kRowWaves) void paged_rows_kernel(const TileArgs<T> a) {
+  constexpr int EPL = Elem<T>::kPer16B, LPR = D / EPL, KPL = 64 / LPR, NLD = kRowLoads;
+  constexpr int KW = NLD * KPL, W = kRowWaves;
+  static_assert(KPL <= 16, "the rows of a load lie in one page");
+  struct Waves {
+    float o[W][NR][D], m[W][NR], l[W][NR];
+  };
+  // the waves' results; in the end merged chunks
+  __shared__ __attribute__((aligned(16))) char lds[W * NR * D * sizeof(Merged<true>)];
+  static_assert(sizeof(lds) >= sizeof(Waves), "the waves' results fit");
+  Waves& sm = *reinterpret_cast<Waves*>(lds);
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, sub = lane % LPR, grp = lane / LPR;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Work w = find_work(a, lane);
+  if (w.none()) return;
+  const int head = blockIdx.x, key0 = w.key0 + wave * KW;
+
+  float m[NR], l[NR], o[NR][EPL];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    m[r] = neg_inf();
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[r][e] = 0.f;
+  }
+  if (key0 < w.key1) {  // wave-uniform
+    // Rows past the end take the place of the last one, loads past it of the wave's first: in a page, and
+    // masked below.
+    const int* table = a.p.table + (size_t)w.seq * a.p.max_pages;
+    bool bad[NLD], any_bad = false;
+    size_t at[NLD];
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+      const int ki = key0 + i * KPL, k = ki < w.key1 ? ki : key0;
+      const int id = paged::ld_uniform(table + (k >> a.page_log2));
+      bad[i] = !paged::is_page(a.p, id);
+      any_bad = any_bad || bad[i];
+      at[i] = paged::page_row(a.p, bad[i] ? 0 : id, head, k & (a.p.page - 1));  // (there is a page 0)
+    }
+    u32x4 q[NR];
+    int after[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const RowPlace p = row_place<D>(w, a.group, min(r, w.rows - 1));
+      after[r] = w.token + p.t;
+      q[r] = ld_g128u(a.q + (w.first + p.t) * a.ld_q + p.col + sub * EPL);
+    }
+    u32x4 kr[NLD], vr[NLD];
+    auto row = [&](int i) {
+      const int left = w.key1 - 1 - (key0 + i * KPL);  // below 0: the wave's first row
+      return (size_t)max(min(grp, left), 0) * D + sub * EPL;
+    };
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) kr[i] = ld_stream(a.k_pages + at[i] + row(i));
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) vr[i] = ld_stream(a.v_pages + at[i] + row(i));
+    __builtin_amdgcn_sched_barrier(0);  // all of them stay in flight
+    if (any_bad) {
+#pragma unroll
+      for (int i = 0; i < NLD; ++i)
+        if (bad[i]) kr[i] = u32x4{0u, 0u, 0u, 0u}, vr[i] = u32x4{0u, 0u, 0u, 0u};
+    }
+    float s[NR][NLD];
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+      const int key = key0 + i * KPL + grp;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float x = lanes::group_sum<LPR>(Elem<T>::dot(q[r], kr[i])) * a.scale;
+        const bool seen = key < w.key1 && !bad[i] && (NR == 1 || key <= after[r]);
+        s[r][i] = seen ? x : neg_inf();
+        m[r] = fmaxf(m[r], s[r][i]);
+      }
+    }
+    float base[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      m[r] = lanes::wave_max_of_groups<LPR>(m[r]);
+      base[r] = m[r] == neg_inf() ? 0.f : m[r];
+    }
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+      float v[EPL];
+      Elem<T>::unpack(vr[i], v);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float p = fast_exp2(s[r][i] - base[r]);
+        l[r] += p;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(p, v[e], o[r][e]);
+      }
+    }
+    // over the row groups: lanes with the same columns
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      if constexpr (LPR < 8) {
+        l[r] += __shfl_xor(l[r], LPR, 64);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[r][e] += __shfl_xor(o[r][e], LPR, 64);
+      }
+      constexpr int K0 = LPR < 8 ? 8 : LPR;
+      l[r] = lanes::sum_across<K0>(l[r]);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[r][e] = lanes::sum_across<K0>(o[r][e]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    if (grp == 0) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) sm.o[wave][r][sub * EPL + e] = o[r][e];
+    }
+    if (lane == 0) sm.m[wave][r] = m[r], sm.l[wave][r] = l[r];
+  }
+  __syncthreads();
+  if (merge_waves<true, W, NR, T, D>(a, w, sm.o, sm.m, sm.l, &flag))
+    merge_tile<true, W, NR, T, D>(a, w, tile_partials<D>(a), lds);
 }
 
 // ------------------------------------------------------------------------ bf16
@@ -364,9 +591,283 @@ struct Stage {
   }
 };
 
+// A row's running state in a wave: maximum and sum of its weights, O^T.
+template <int D>
+struct Running {
+  f32x16 o[D / 32];
+  float m = neg_inf(), l = 0.f;
+  __device__ __forceinline__ Running() {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
+  }
+};
+
+// 32 keys, the first of them token c0: rows 32 i .. of the tiles ck and cv. bad0, bad1: their first and
+// second 16 have no page.
+template <int D>
+__device__ __forceinline__ void keys32(Running<D>& x, const bf16* ck, const bf16* cv, int i, int c0,
+                                       bool bad0, bool bad1, const WaveRows<D>& r,
+                                       const bf16x8 (&q)[D / 16], float scale, int lane) {
+  constexpr int DB = D / 32;
+  const int l32 = lane & 31, hi = lane >> 5;
+  f32x16 s{};
+#pragma unroll
+  for (int ds = 0; ds < D / 16; ++ds)
+    s = mfma32(lds_op(ck, rm_off<D>(32 * i + sigma32(l32), 2 * ds + hi)), q[ds], s);
+  if (c0 + 31 > r.all_see || bad0 || bad1) {
+    const int last = r.after - c0 - 8 * hi;
+#pragma unroll
+    for (int y = 0; y < 16; ++y)
+      if (reg_row(y, 0) > last || (y < 8 ? bad0 : bad1)) s[y] = neg_inf();
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  bf16x8 va[DB][2], p[2];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) va[db][j] = lds_tr_op<D>(cv, 32 * i + 16 * j, 32 * db, lane);
+  float sum = weights_bf16(p, s, scale, x.m);
+  // 2^64 or more, inf, or NaN (a row's first keys: m is -inf), compared on the bits; both halves of a
+  // row take the row's decision, and no other row's bits depend on it
+  const bool need = __float_as_uint(sum) >= __float_as_uint(kMaxP);
+  if (__builtin_amdgcn_ballot_w64(need) != 0) {
+    float mx = s[0];
+#pragma unroll
+    for (int y = 1; y < 16; ++y) mx = fmaxf(mx, s[y]);
+    mx = max_halves(mx) * scale;
+    const float mn = or_halves(need) ? fmaxf(x.m, mx) : x.m;
+    const float base = mn == neg_inf() ? 0.f : mn;  // no key seen yet weighs anything
+    const float f = fast_exp2(x.m - base);
+    x.m = mn;
+    x.l *= f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) x.o[db] *= f;
+    sum = weights_bf16(p, s, scale, base);
+  }
+  x.l += sum;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) x.o[db] = mfma32(va[db][j], p[j], x.o[db]);
+}
+
+// The owners' rows into the output, through the wave's own stretch of LDS, so that a store instruction
+// covers whole heads.
+template <int D>
+__device__ __forceinline__ void store_rows(const TileArgs<bf16>& a, const Work& w,
+                                           const WaveRows<D>& r, const Running<D>& x, bf16* lds,
+                                           int lane) {
+  constexpr int C = D / 8;
+  if (!r.owner()) return;
+  const int l32 = lane & 31, hi = lane >> 5;
+  bf16* rows = lds + r.grp * 32 * D;
+  const float inv = x.l == 0.f ? 0.f : 1.0f / x.l;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 4 * db + g;
+      u32x2 y;
+      y[0] = pack_bf16x2(x.o[db][4 * g] * inv, x.o[db][4 * g + 1] * inv);
+      y[1] = pack_bf16x2(x.o[db][4 * g + 2] * inv, x.o[db][4 * g + 3] * inv);
+      *reinterpret_cast<u32x2*>(rows + l32 * D + ((c ^ (l32 % C)) << 3) + 4 * hi) = y;
+    }
+#pragma unroll
+  for (int n = 0; n < 32 * C / 64; ++n) {
+    const int i = (n * 64 + lane) / C, c = (n * 64 + lane) % C;
+    const u32x4 y = *reinterpret_cast<const u32x4*>(rows + i * D + ((c ^ (i % C)) << 3));
+    if (r.q0 + i < w.rows) {
+      const RowPlace at = row_place<D>(w, a.group, r.q0 + i);
+      *reinterpret_cast<u32x4*>(a.out + (w.first + at.t) * a.ld_out + at.col + 8 * c) = y;
+    }
+  }
+}
+
+// The lane's query, columns 16 ds + 8 hi + 0 .. 7.
+template <int D>
+__device__ __forceinline__ void load_query(bf16x8 (&q)[D / 16], const TileArgs<bf16>& a,
+                                           const Work& w, const WaveRows<D>& r, int hi) {
+  const bf16* row = a.q + (w.first + r.mine.t) * a.ld_q + r.mine.col + 8 * hi;
+#pragma unroll
+  for (int ds = 0; ds < D / 16; ++ds) q[ds] = ld_g128(row + 16 * ds);
+}
+// (once the direct loads' wait is over: the compiler, which does not see those, has none to add then)
+template <int D>
+__device__ __forceinline__ void take_query(bf16x8 (&q)[D / 16], bool negate) {
+#pragma unroll
+  for (int ds = 0; ds < D / 16; ++ds) {
+    asm volatile("" : "+v"(q[ds]));
+    if (negate) q[ds] = neg_bf16x8(q[ds]);
+  }
+}
+
+// Up to 16 NB rows, a chunk of 512 keys (1024 at D = 32) for eight waves: a wave takes 64 (128) keys in one
+// round, K straight into registers and V through its own stretch of LDS, everything in flight at once and
+// no barrier until the waves are merged. (The kernel below, with a tile of 64 keys in flight for the
+// workgroup, is a chain of as many memory latencies as a chunk has tiles.) On v_mfma_f32_16x16x32_bf16:
+//   S^T[16 keys][16 rows] = K Q^T   A = K as it lies in memory: lane l holds key l % 16, columns 8 (l / 16)
+//                                   .. + 7 of each 32
+//   O^T[16 columns][16 rows] += V^T P^T over 32 keys, V^T by ds_read_b64_tr_b16
+// Of 32 keys, the two tiles of scores take 8 g + r and 8 g + 4 + r as their rows 4 g + r (r < 4): the
+// lanes l / 16 = g then hold the weights of keys 8 g .. + 7, the other product's operand.
+typedef __attribute__((ext_vector_type(4))) float acc16;
+__device__ __forceinline__ acc16 mfma16(const bf16x8& a, const bf16x8& b, const acc16& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+constexpr int kMidWaves = 8;
+template <int D>
+__host__ __device__ constexpr int mid_wave_keys() {
+  return 64 * 64 / D;
+}
+
+template <int D, int NB>
+__global__ __launch_bounds__(64 * kMidWaves, 4) void paged_mid_bf16_kernel(const TileArgs<bf16> a) {
+  constexpr int KW = mid_wave_keys<D>(), NJ = KW / 32, NG = KW / 16, DS = D / 32, DB = D / 16;
+  constexpr int W = kMidWaves, ROWS = 16 * NB;
+  struct Waves {
+    float o[W][ROWS][D], m[W][ROWS], l[W][ROWS];
+  };
+  constexpr size_t kV = sizeof(bf16) * W * KW * D, kFewBytes = sizeof(Merged<true>) * W * kFew * D;
+  constexpr size_t kBytes = kV > sizeof(Waves) ? kV : sizeof(Waves);
+  // V; then the waves' results; in the end merged chunks
+  __shared__ __attribute__((aligned(16))) char lds[kBytes > kFewBytes ? kBytes : kFewBytes];
+  __shared__ int flag;
+  Waves& sm = *reinterpret_cast<Waves*>(lds);
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Work w = find_work(a, lane);
+  if (w.none()) return;
+  const int head = blockIdx.x, key0 = w.key0 + wave * KW;
+
+  float m[NB], l[NB];
+  acc16 o[NB][DB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    m[b] = neg_inf();
+    l[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[b][d] = acc16{0.f, 0.f, 0.f, 0.f};
+  }
+  if (key0 < w.key1) {  // wave-uniform
+    // The pages of the wave's groups of 16 tokens. What has none is read from the wave's first page, or
+    // from page 0, and masked; V has zeros in its place.
+    const int* table = a.p.table + (size_t)w.seq * a.p.max_pages;
+    bool there[NG], bad[NG];
+    size_t at[NG];
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int k = key0 + 16 * i < w.key1 ? key0 + 16 * i : key0;
+      const int id = paged::ld_uniform(table + (k >> a.page_log2));
+      bad[i] = !paged::is_page(a.p, id);
+      there[i] = key0 + 16 * i < w.key1 && !bad[i];
+      at[i] = paged::page_row(a.p, bad[i] ? 0 : id, head, k & (a.p.page - 1));
+    }
+    bf16x8 q[NB][DS], kr[NJ][2][DS];
+    int after[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const RowPlace p = row_place<D>(w, a.group, min(16 * b + l16, w.rows - 1));
+      after[b] = w.token + p.t;
+      const bf16* row = a.q + (w.first + p.t) * a.ld_q + p.col + 8 * g4;
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) q[b][ds] = ld_g128(row + 32 * ds);
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        // row l16 of the tile: token 8 (l16 / 4) + 4 t + l16 % 4 of the 32, in group 2 j or 2 j + 1
+        const int k = 8 * (l16 >> 2) + 4 * t + (l16 & 3), i = 2 * j + (l16 >> 3);
+        const int left = w.key1 - 1 - (key0 + 16 * i);  // below 0: the wave's first row
+        const size_t more = at[2 * j + 1] - at[2 * j], base = at[2 * j] + (l16 >> 3 ? more : 0);
+        const bf16* row = a.k_pages + base + (size_t)max(min(k & 15, left), 0) * D + 8 * g4;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+          kr[j][t][ds] = as_bf16x8(ld_stream(row + 32 * ds));
+      }
+    const Stage<D> stage(lane);
+    bf16* v = reinterpret_cast<bf16*>(lds) + wave * KW * D;
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+      stage(v, a.v_pages + at[i], w.key1 - key0 - 16 * i, there[i], i, lane);
+    wait_vm_lds<0>();
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) {
+        asm volatile("" : "+v"(q[b][ds]));
+        if (a.negate) q[b][ds] = neg_bf16x8(q[b][ds]);
+      }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      acc16 s[NJ][2];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          s[j][t] = acc16{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ds = 0; ds < DS; ++ds) s[j][t] = mfma16(kr[j][t][ds], q[b][ds], s[j][t]);
+          // register r: key 8 g4 + 4 t + r of these 32, of group 2 j or 2 j + 1
+          const int last = min(after[b], w.key1 - 1) - (key0 + 32 * j + 8 * g4 + 4 * t);
+          const bool none = (bad[2 * j] && g4 < 2) || (bad[2 * j + 1] && g4 >= 2);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (r > last || none) s[j][t][r] = neg_inf();
+            m[b] = fmaxf(m[b], s[j][t][r]);
+          }
+        }
+      m[b] = lanes::max_xor32(lanes::max_xor16(m[b])) * a.scale;
+      const float base = m[b] == neg_inf() ? 0.f : m[b];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        u32x4 p;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; r += 2) {
+            const float p0 = fast_exp2(fmaf(s[j][t][r], a.scale, -base));
+            const float p1 = fast_exp2(fmaf(s[j][t][r + 1], a.scale, -base));
+            l[b] += p0 + p1;
+            p[2 * t + r / 2] = pack_bf16x2(p0, p1);
+          }
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          s16x4 x[2];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int row = 32 * j + 8 * g4 + 4 * half + (l16 >> 2), col = 16 * d + 4 * (l16 & 3);
+            const lds_bf16* at = (const lds_bf16*)v + row * D + (((col >> 3) ^ swz<D>(row)) << 3) +
+                                 (col & 7);
+            x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+          }
+          const bf16x8 vt = __builtin_bit_cast(
+              bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          o[b][d] = mfma16(vt, as_bf16x8(p), o[b][d]);
+        }
+      }
+      l[b] = lanes::sum_xor32(lanes::sum_xor16(l[b]));
+    }
+  }
+  __syncthreads();  // every wave is done with V
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int row = 16 * b + l16;
+    if (row >= w.rows) continue;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      *reinterpret_cast<f32x4*>(&sm.o[wave][row][16 * d + 4 * g4]) =
+          f32x4{o[b][d][0], o[b][d][1], o[b][d][2], o[b][d][3]};
+    if (g4 == 0) sm.m[wave][row] = m[b], sm.l[wave][row] = l[b];
+  }
+  __syncthreads();
+  if (merge_waves<true, W, ROWS, bf16, D>(a, w, sm.o, sm.m, sm.l, &flag))
+    merge_tile<true, W, kFew, bf16, D>(a, w, tile_partials<D>(a), lds);
+}
+
 template <int D>
 __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<bf16> a) {
-  constexpr int DS = D / 16, DB = D / 32;
+  constexpr int DB = D / 32;
   // two tiles of K, two of V; in the end the waves' partials, output rows or merged chunks
   __shared__ __attribute__((aligned(16))) bf16 lds[4 * kTileRows * D];
   bf16 *const sk[2] = {lds, lds + kTileRows * D};
@@ -375,7 +876,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
   __shared__ int flag;
   static_assert(sizeof(lds) >= (kWaves - 1) * DB * sizeof(AccLds), "waves' partials fit");
   static_assert(sizeof(lds) >= kWaves * 32 * D * sizeof(bf16), "output rows fit");
-  static_assert(sizeof(lds) >= kFew * D * kWaves * sizeof(Merged<bf16>), "merged chunks fit");
+  static_assert(sizeof(lds) >= kFew * D * kWaves * sizeof(Merged<true>), "merged chunks fit");
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -383,11 +884,9 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
   if (w.none()) return;
   const WaveRows<D> r(w, a.group, wave, l32);
 
-  // the lane's query, columns 16 ds + 8 hi + 0 .. 7 (rows past the last repeat it)
-  const bf16* qrow = a.q + (w.first + r.mine.t) * a.ld_q + r.mine.col + 8 * hi;
-  bf16x8 qop[DS];
-#pragma unroll
-  for (int ds = 0; ds < DS; ++ds) qop[ds] = ld_g128(qrow + 16 * ds);
+  bf16x8 q[D / 16];
+  load_query<D>(q, a, w, r, hi);
+
   const int head = blockIdx.x, n_tiles = w.key1 > w.key0 ? (w.key1 - w.key0 + 63) / 64 : 0;
   const Stage<D> stage(lane);
   auto load = [&](int t, const Pages& g, bf16* tk, bf16* tv) {
@@ -399,11 +898,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
     stage(tv, a.v_pages + at, left, there, wave, lane);
   };
 
-  f32x16 o[DB];
-#pragma unroll
-  for (int db = 0; db < DB; ++db) o[db] = f32x16{};
-  float m = neg_inf(), l = 0.f;
-
+  Running<D> x;
   Pages now{}, next{};
   if (n_tiles > 0) {
     now = pages_at(a, w, w.key0);
@@ -412,11 +907,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
   }
   wait_vm_lds<0>();
   __builtin_amdgcn_s_barrier();
-#pragma unroll
-  for (int ds = 0; ds < DS; ++ds) {
-    asm volatile("" : "+v"(qop[ds]));
-    if (a.negate) qop[ds] = neg_bf16x8(qop[ds]);
-  }
+  take_query<D>(q, a.negate);
 
   auto tile = [&](int t, const bf16* ck, const bf16* cv, bf16* nk, bf16* nv) {
     const int k0 = w.key0 + 64 * t;
@@ -430,47 +921,8 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
       const int c0 = k0 + 32 * i;
       if (!r.active || ((2 * t + i) & (r.ks - 1)) != r.sub || c0 > r.some_see || c0 >= w.key1)
         continue;
-      const bool bad0 = !paged::is_page(a.p, now.id[2 * i]);
-      const bool bad1 = !paged::is_page(a.p, now.id[2 * i + 1]);
-      f32x16 s{};
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds)
-        s = mfma32(lds_op(ck, rm_off<D>(32 * i + sigma32(l32), 2 * ds + hi)), qop[ds], s);
-      if (c0 + 31 > r.all_see || bad0 || bad1) {
-        const int last = r.after - c0 - 8 * hi;
-#pragma unroll
-        for (int x = 0; x < 16; ++x)
-          if (reg_row(x, 0) > last || (x < 8 ? bad0 : bad1)) s[x] = neg_inf();
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      bf16x8 va[DB][2], p[2];
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) va[db][j] = lds_tr_op<D>(cv, 32 * i + 16 * j, 32 * db, lane);
-      float sum = weights_bf16(p, s, a.scale, m);
-      // 2^64 or more, inf, or NaN (a row's first keys: m is -inf), compared on the bits; both halves of
-      // a row take the row's decision, and no other row's bits depend on it
-      const bool need = __float_as_uint(sum) >= __float_as_uint(kMaxP);
-      if (__builtin_amdgcn_ballot_w64(need) != 0) {
-        float mx = s[0];
-#pragma unroll
-        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, s[x]);
-        mx = max_halves(mx) * a.scale;
-        const float mn = or_halves(need) ? fmaxf(m, mx) : m;
-        const float base = mn == neg_inf() ? 0.f : mn;  // no key seen yet weighs anything
-        const float f = fast_exp2(m - base);
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] *= f;
-        sum = weights_bf16(p, s, a.scale, base);
-      }
-      l += sum;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) o[db] = mfma32(va[db][j], p[j], o[db]);
+      keys32<D>(x, ck, cv, i, c0, !paged::is_page(a.p, now.id[2 * i]),
+                !paged::is_page(a.p, now.id[2 * i + 1]), r, q, a.scale, lane);
     }
     now = next;
     next = after_next;
@@ -481,37 +933,10 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
     tile(t, sk[0], sv[0], sk[1], sv[1]);
     if (t + 1 < n_tiles) tile(t + 1, sk[1], sv[1], sk[0], sv[0]);
   }
-  l = sum_halves(l);
-
-  join_waves<bf16, D>(r, o, m, l, lds, sm_ml, lane);
-  if (w.chunks == 1) {
-    if (!r.owner()) return;
-    // rows through the wave's own stretch of LDS, so that a store instruction covers whole heads
-    constexpr int C = D / 8;
-    bf16* rows = lds + r.grp * 32 * D;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int c = 4 * db + g;
-        u32x2 x;
-        x[0] = pack_bf16x2(o[db][4 * g] * inv, o[db][4 * g + 1] * inv);
-        x[1] = pack_bf16x2(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
-        *reinterpret_cast<u32x2*>(rows + l32 * D + ((c ^ (l32 % C)) << 3) + 4 * hi) = x;
-      }
-#pragma unroll
-    for (int n = 0; n < 32 * C / 64; ++n) {
-      const int i = (n * 64 + lane) / C, c = (n * 64 + lane) % C;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(rows + i * D + ((c ^ (i % C)) << 3));
-      if (r.q0 + i < w.rows) {
-        const RowPlace at = row_place<D>(w, a.group, r.q0 + i);
-        *reinterpret_cast<u32x4*>(a.out + (w.first + at.t) * a.ld_out + at.col + 8 * c) = x;
-      }
-    }
-    return;
-  }
-  leave_partial<bf16, D>(a, w, r, o, m, l, reinterpret_cast<float*>(lds), &flag, lane);
+  x.l = sum_halves(x.l);
+  join_waves<bf16, D>(r, x.o, x.m, x.l, lds, sm_ml, lane);
+  if (w.chunks == 1) return store_rows<D>(a, w, r, x, lds, lane);
+  leave_partial<bf16, D>(a, w, r, x.o, x.m, x.l, reinterpret_cast<float*>(lds), &flag, lane);
 }
 
 // ------------------------------------------------------------------------ fp32
@@ -549,7 +974,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<f
   __shared__ int flag;
   static_assert(sizeof(planes) >= (kWaves - 1) * DB * sizeof(AccLds), "waves' partials fit");
   static_assert(sizeof(planes) >= kWaves * 32 * kPitch * sizeof(float), "output rows fit");
-  static_assert(sizeof(planes) >= kFew * D * kWaves * sizeof(Merged<float>), "merged chunks fit");
+  static_assert(sizeof(planes) >= kFew * D * kWaves * sizeof(Merged<false>), "merged chunks fit");
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -663,7 +1088,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<f
 
 // ------------------------------------------------------------------------ host
 
+// The kernel of a step, by the rows of a (sequence, KV head): the VALU's up to 2 (fp32: 4); bf16 up to 32: a
+// wave for itself; tiles of 128. At 8 sequences of 1 to 32768 tokens, 4 KV heads of 64, in bf16, the first two
+// take 31 and 40 us with one row, 41 and 41 with 2, 47 and 42 with 3; the tiles 49 with 3, where the second
+// still takes 49 with 8 and 57 with 16.
+enum Path { kRows, kMid, kTiles };
+constexpr int kMostMid = 32;
+constexpr int most_rows(int elem) { return elem == 2 ? 2 : 4; }
+Path path_of(const PagedStep& s, int elem) {
+  const long long rows = (long long)s.max_rows * (s.H / s.Hkv);
+  return rows <= most_rows(elem) ? kRows : elem == 2 && rows <= kMostMid ? kMid : kTiles;
+}
+
 struct Plan {
+  Path path;
   int tiles, chunk, n_chunk, part_rows;
   size_t counters, partials;  // bytes
 };
@@ -676,18 +1114,30 @@ long long tiles_of(int n_seq, long long group, int rows, int max_rows) {
   const long long per_seq = (max_rows * group + kTile - 1) / kTile;
   return std::min(n_seq * per_seq, n_seq + rows * group / kTile);
 }
+int mid_keys_of(int D) { return kMidWaves * (D == 64 ? mid_wave_keys<64>() : mid_wave_keys<32>()); }
+int few_keys_of(int elem, int D) {
+  return elem == 2 ? (D == 64 ? few_keys<bf16, 64>() : few_keys<bf16, 32>())
+                   : (D == 64 ? few_keys<float, 64>() : few_keys<float, 32>());
+}
 
 // Tiles of the step's list, keys of a workgroup, and what the workspace holds. The lengths are on the
 // device: the grid has room for every sequence at its longest.
-Plan plan_of(const PagedStep& s) {
+Plan plan_of(const PagedStep& s, int elem) {
   const long long group = s.H / s.Hkv, max_len = (long long)s.max_pages * s.page;
   Plan p{};
+  p.path = path_of(s, elem);
   p.tiles = (int)tiles_of(s.n_seq, group, s.rows, s.max_rows);
   p.part_rows = (int)std::min(s.max_rows * group, (long long)kTile);
   const long long units = (long long)p.tiles * s.Hkv;
-  const long long want = (wanted() + units - 1) / units;
-  const long long chunk = std::max<long long>(kLeastKeys, (max_len + want - 1) / want);
-  p.chunk = (int)((chunk + 63) / 64 * 64);
+  if (p.path == kRows) {
+    p.chunk = few_keys_of(elem, s.D);
+  } else if (p.path == kMid) {
+    p.chunk = mid_keys_of(s.D);
+  } else {
+    const long long want = (wanted() + units - 1) / units;
+    const long long chunk = std::max<long long>(kLeastKeys, (max_len + want - 1) / want);
+    p.chunk = (int)((chunk + 255) / 256 * 256);
+  }
   p.n_chunk = (int)((max_len + p.chunk - 1) / p.chunk);
   if (p.n_chunk > 1) {
     p.counters = counter_bytes(p.tiles, s.Hkv);
@@ -700,7 +1150,7 @@ template <typename T, typename F>
 hipError_t launch_paged_t(T* out, long long ld_out, const T* q, long long ld_q, const T* k_pages,
                           const T* v_pages, const PagedStep& s, float scale, void* workspace,
                           size_t workspace_bytes, F launch) {
-  const Plan plan = plan_of(s);
+  const Plan plan = plan_of(s, sizeof(T));
   TileArgs<T> a{};
   a.out = out, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages;
   a.ld_out = ld_out, a.ld_q = ld_q, a.p = s;
@@ -712,34 +1162,58 @@ hipError_t launch_paged_t(T* out, long long ld_out, const T* q, long long ld_q, 
   // weighs the same, as at a scale of 0 (as attn_fwd_bf16.hip).
   a.scale = sizeof(T) == 2 ? fmaxf(fabsf(scale) * kLog2e, 1e-30f) : scale;
   a.negate = scale < 0.f;
+  if (plan.path == kRows) a.scale = scale * kLog2e;  // (masked after it)
   if (plan.n_chunk > 1) {
     // the caller checked workspace_bytes >= paged_workspace_needed(); partials against its end
     const size_t at = (workspace_bytes - plan.partials) & ~(size_t)15;
     a.counter = static_cast<unsigned*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + at);
   }
-  launch(a, dim3(s.Hkv, plan.tiles, plan.n_chunk));
+  launch(a, dim3(s.Hkv, plan.tiles, plan.n_chunk), plan.path);
   return hipGetLastError();
+}
+
+template <typename T>
+void launch_rows(const TileArgs<T>& a, dim3 grid, hipStream_t stream) {
+  auto run = [&](auto d) {
+    switch (a.part_rows) {
+      case 1: paged_rows_kernel<T, d(), 1><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
+      case 2: paged_rows_kernel<T, d(), 2><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
+      case 3: paged_rows_kernel<T, d(), 3><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
+      default: paged_rows_kernel<T, d(), 4><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
+    }
+  };
+  if (a.p.D == 64)
+    run(std::integral_constant<int, 64>{});
+  else
+    run(std::integral_constant<int, 32>{});
 }
 
 }  // namespace
 
-size_t paged_workspace_needed(const PagedStep& step) {
-  const Plan p = plan_of(step);
+size_t paged_workspace_needed(const PagedStep& step, int elem) {
+  const Plan p = plan_of(step, elem);
   return p.n_chunk > 1 ? p.counters + p.partials + 16 : 0;
 }
 
-// Of n tiles x KV heads, n < wanted(), a plan makes at most ceil(max_len / kLeastKeys) chunks each and
-// wanted() + n workgroups in all; more than that are not cut. The bound grows with every argument.
+// Of n tiles x KV heads, n < wanted(), a plan of tiles makes at most ceil(max_len / kLeastKeys) chunks each
+// and wanted() + n workgroups in all, more than that are not cut; that of a few rows makes n_seq x KV heads
+// times ceil(max_len / their chunk). Both bounds grow with every argument.
 size_t paged_workspace_bytes(const PagedStep& s) {
   const long long group = s.H / s.Hkv, max_len = (long long)s.max_pages * s.page;
   const long long chunks = (max_len + kLeastKeys - 1) / kLeastKeys;
   if (chunks <= 1) return 0;
-  const long long units =
-      std::min(tiles_of(s.n_seq, group, s.rows, s.max_rows) * s.Hkv, wanted());
-  const long long parts = std::min(units * chunks, wanted() + units);
-  const long long part_rows = std::min(s.max_rows * group, (long long)kTile);
-  return counter_bytes((int)units, 1) + sizeof(float) * parts * part_rows * (s.D + 2) + 16;
+  const long long row = sizeof(float) * (s.D + 2);
+  const long long units = std::min(tiles_of(s.n_seq, group, s.rows, s.max_rows) * s.Hkv, wanted());
+  const long long tiled = std::min(units * chunks, wanted() + units) *
+                          std::min(s.max_rows * group, (long long)kTile) * row;
+  long long few = 0;
+  if (group <= kMostMid) {
+    const int keys = std::min({few_keys_of(2, s.D), few_keys_of(4, s.D), mid_keys_of(s.D)});
+    few = (long long)s.n_seq * s.Hkv * ((max_len + keys - 1) / keys) *
+          std::min<long long>(s.max_rows * group, kMostMid) * row;
+  }
+  return counter_bytes((int)std::max(units, (long long)s.n_seq * s.Hkv), 1) + std::max(tiled, few) + 16;
 }
 
 hipError_t launch_paged_attention_bf16(bf16* out, long long ld_out, const bf16* q, long long ld_q,
@@ -748,8 +1222,22 @@ hipError_t launch_paged_attention_bf16(bf16* out, long long ld_out, const bf16* 
                                        size_t workspace_bytes, hipStream_t stream) {
   return launch_paged_t<bf16>(
       out, ld_out, q, ld_q, k_pages, v_pages, step, scale, workspace, workspace_bytes,
-      [&](const TileArgs<bf16>& a, dim3 grid) {
-        if (step.D == 64)
+      [&](const TileArgs<bf16>& a, dim3 grid, Path path) {
+        if (path == kRows) {
+          launch_rows(a, grid, stream);
+        } else if (path == kMid) {
+          auto run = [&](auto d, auto nb) {
+            paged_mid_bf16_kernel<d(), nb()><<<grid, 64 * kMidWaves, 0, stream>>>(a);
+          };
+          constexpr std::integral_constant<int, 64> d64;
+          constexpr std::integral_constant<int, 32> d32;
+          constexpr std::integral_constant<int, 1> one;
+          constexpr std::integral_constant<int, 2> two;
+          if (step.D == 64)
+            a.part_rows <= 16 ? run(d64, one) : run(d64, two);
+          else
+            a.part_rows <= 16 ? run(d32, one) : run(d32, two);
+        } else if (step.D == 64)
           paged_bf16_kernel<64><<<grid, kThreads, 0, stream>>>(a);
         else
           paged_bf16_kernel<32><<<grid, kThreads, 0, stream>>>(a);
@@ -762,8 +1250,10 @@ hipError_t launch_paged_attention_f32(float* out, long long ld_out, const float*
                                       size_t workspace_bytes, hipStream_t stream) {
   return launch_paged_t<float>(
       out, ld_out, q, ld_q, k_pages, v_pages, step, scale, workspace, workspace_bytes,
-      [&](const TileArgs<float>& a, dim3 grid) {
-        if (step.D == 64)
+      [&](const TileArgs<float>& a, dim3 grid, Path path) {
+        if (path == kRows)
+          launch_rows(a, grid, stream);
+        else if (step.D == 64)
           paged_f32_kernel<64><<<grid, kThreads, 0, stream>>>(a);
         else
           paged_f32_kernel<32><<<grid, kThreads, 0, stream>>>(a);

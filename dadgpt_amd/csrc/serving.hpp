@@ -48,7 +48,7 @@ hipError_t launch_paged_append_f32(float* k_pages, float* v_pages, float* q_out,
 
 // Bytes that this step's launch uses, and those that serve it and every step with no larger n_seq, rows,
 // max_rows and max_pages.
-size_t paged_workspace_needed(const PagedStep& step);
+size_t paged_workspace_needed(const PagedStep& step, int elem_bytes);
 size_t paged_workspace_bytes(const PagedStep& step);
 hipError_t launch_paged_attention_bf16(bf16* out, long long ld_out, const bf16* q, long long ld_q,
                                        const bf16* k_pages, const bf16* v_pages,

@@ -28,7 +28,7 @@ PAGED_SYMBOLS = (
 
 # Tokens that a page can have (of one KV head), and those that a sequence can (the header's
 # DADGPT_PAGED_MAX_LEN).
-PAGES, MAX_LEN = (16, 32, 64, 128), 1 << 24
+PAGES, MAX_LEN = (16, 32, 64, 128), 65535 * 256
 
 _lib = None
 

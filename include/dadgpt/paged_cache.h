@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define DADGPT_PAGED_MAX_LEN (1 << 24)
+#define DADGPT_PAGED_MAX_LEN (65535 * 256)
 
 /* Writes the new rows into the pages, rotating q and k on the way as dadgpt_rope_* (<dadgpt/rope.h>)
  * with each row's token number as its position; freqs NULL: no rotation (rot_dim 0 then).

@@ -134,7 +134,7 @@ STEP_REFUSALS = [(dict(n_seq=0), 1, "positive"), (dict(H=0), 1, "positive"), (di
                  (dict(n_pages=0), 1, "positive"), (dict(max_pages=-1), 1, "positive"),
                  (dict(H=5), 1, "no multiple"), (dict(page=8), 1, "page=8"), (dict(page=48), 1, "page=48"),
                  (dict(page=256), 1, "page=256"), (dict(D=128), 2, "d_head"), (dict(D=16), 2, "d_head"),
-                 (dict(max_pages=(1 << 20) + 1), 1, "tokens"),
+                 (dict(max_pages=65535 * 16 + 1), 1, "tokens"),
                  (dict(n_seq=65536), 1, "launch limits"), (dict(rows=(1 << 24) + 1), 1, "launch limits")]
 
 
