@@ -17,9 +17,9 @@ __device__ __forceinline__ int ld_uniform(const int* p) {
   return *reinterpret_cast<constant_int*>(reinterpret_cast<uintptr_t>(p));
 }
 
-// The new rows of sequence s (UNIFORM: the same in every lane): rows first .. first + count - 1 of the step (clamped, so that no value
-// of the device arrays leads out of a buffer), the token number of the first, and the tokens after the
-// last. Token numbers are below 0 where the count exceeds the length.
+// The new rows of sequence s (UNIFORM: the same in every lane): rows first .. first + count - 1 of the step
+// (clamped, so that no value of the device arrays leads out of a buffer), the token number of the first,
+// and the tokens after the last. Token numbers are below 0 where the count exceeds the length.
 struct NewRows {
   int first, count, token, len;
   template <bool UNIFORM>

@@ -41,69 +41,127 @@ struct TileArgs {
   long long ld_out, ld_q;
   PagedStep p;
   int group, page_log2;
-  int chunk, n_chunk;   // keys of a workgroup, chunks of the longest cache
-  int part_rows;        // rows that a partial has room for
-  bool one_tile;        // every sequence has one tile at most
+  int chunk, n_chunk;   // a few rows: keys of a workgroup, chunks of the longest cache
+  int slots;            // tiles: partials of a KV head that there is room for
+  int rows, part_pitch; // the most of a tile; floats of its partial of a chunk
   float scale;          // fp32: as it is; bf16: |scale| log2 e
   bool negate;          // scale < 0 (bf16)
-  float* part;          // [tile][KV head][chunk][part_rows][D + 2]: maximum, sum, unnormalised output
-  unsigned* counter;    // [tile][KV head]
+  float* part;          // partials: maximum, sum, unnormalised output of every row
+  unsigned* counter;    // one for each partial; a tile uses its first chunk's
 };
 
-// What a workgroup does: tile `tile` of the step's list (every sequence's tiles one after the other),
-// KV head `head`, keys key0 .. key1 - 1.
+// What a workgroup does: the rows of a tile, KV head `head`, keys key0 .. key1 - 1 of chunk `chunk`.
 struct Work {
+  int head, chunk, chunks;        // (of the tile)
   int seq, row0, rows;            // first row of the tile in the sequence's rows x heads, rows in it
   int first, token, key0, key1;   // row of the step of the sequence's first token, that token's number
-  int chunks;                     // of the tile
+  int part0, part_step;           // the partial of its chunk 0, and how far apart those of its chunks are
   __device__ __forceinline__ bool none() const { return rows <= 0; }
+  // rows from row0 on, chunk `chunk` of `keys` keys each; a cache of `whole` tokens or fewer stays in one
+  template <typename T>
+  __device__ __forceinline__ void take(const TileArgs<T>& a, const paged::NewRows& r, int keys,
+                                       int whole) {
+    rows = (int)min((long long)kTile, (long long)r.count * a.group - row0);
+    if (none()) return;
+    first = r.first;
+    token = r.token;
+    const int seen = token + (row0 + rows - 1) / a.group + 1;  // by the tile's last row
+    chunks = seen > keys && r.len > whole ? (seen + keys - 1) / keys : 1;
+    if (chunk >= chunks) rows = 0;
+    key0 = chunk * keys;
+    key1 = chunks == 1 ? seen : min(seen, key0 + keys);
+  }
 };
 
+// A few rows: a sequence is one tile, in chunks of a.chunk keys; the grid is (KV head, sequence, chunk).
 template <typename T>
-__device__ __forceinline__ Work find_work(const TileArgs<T>& a, int lane) {
-  int seq = blockIdx.y, tile = 0;
-  if (!a.one_tile) {
-    // the sequence whose tiles hold this one: 64 sequences at a time, their tiles summed up over lanes
-    int left = blockIdx.y;
-    seq = a.p.n_seq;
-    for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
-      int n = 0;
-      if (s0 + lane < a.p.n_seq) {
-        const auto r = paged::NewRows::of<false>(a.p, s0 + lane);
-        n = (int)(((long long)r.count * a.group + kTile - 1) / kTile);
-      }
-      int upto = n;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(upto, d, 64);
-        if (lane >= d) upto += y;
-      }
-      const uint64_t reach = __builtin_amdgcn_ballot_w64(upto > left);
-      if (reach != 0) {
-        const int at = __builtin_ctzll(reach);
-        seq = s0 + at;
-        tile = left - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
-        break;
-      }
-      left -= __builtin_amdgcn_readlane(upto, 63);
-    }
-  }
+__device__ __forceinline__ Work find_few(const TileArgs<T>& a) {
   Work w{};
-  if (seq >= a.p.n_seq) return w;
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  tile = __builtin_amdgcn_readfirstlane(tile);
-  w.seq = seq;
-  const auto r = paged::NewRows::of<true>(a.p, seq);
-  w.row0 = tile * kTile;
-  w.rows = (int)min((long long)kTile, (long long)r.count * a.group - w.row0);
-  if (w.none()) return w;
-  w.first = r.first;
-  w.token = r.token;
-  const int seen = r.token + (w.row0 + w.rows - 1) / a.group + 1;  // by the tile's last row
-  w.chunks = seen > a.chunk ? (seen + a.chunk - 1) / a.chunk : 1;
-  if ((int)blockIdx.z >= w.chunks) w.rows = 0;
-  w.key0 = blockIdx.z * a.chunk;
-  w.key1 = min(seen, w.key0 + a.chunk);
+  w.head = blockIdx.x, w.seq = blockIdx.y, w.chunk = blockIdx.z;
+  w.part0 = (w.seq * a.p.Hkv + w.head) * a.n_chunk;
+  w.part_step = 1;
+  w.take(a, paged::NewRows::of<true>(a.p, w.seq), a.chunk, a.chunk);
+  return w;
+}
+
+// Tiles of 128 rows: the grid is (KV head, place in a list). The list is every sequence's tiles, once for
+// each chunk of its keys. How long a chunk is follows from the lengths, which only the device has: all the
+// tiles' keys, shared out evenly over kShares workgroups, three a CU; longer where there are more tiles
+// than that, which even each other out. So a cache that is far from its room still fills the machine, and
+// one long sequence among short ones is cut. Merging chunks costs about 6 us of waiting, as much as a few
+// tiles: a chunk has kLeastKeys at least, and in bf16 a sequence that is not twice as long stays whole.
+// In bf16, 12 heads of 64, against equal parts of the longest cache: chunks of up to 512 rows of 8 prompts
+// of up to 8192 tokens 67 us (75), 64 sequences of up to 1024 tokens with up to 256 rows 28 (29), one of
+// 32768 with 512 rows 48 (55).
+constexpr int kShares = 768;
+template <typename T>
+constexpr int kLeastKeys = sizeof(T) == 2 ? 512 : 256;
+template <typename T>
+constexpr int kWhole = sizeof(T) == 2 ? 2 : 1;  // chunks
+template <typename T>
+__device__ __forceinline__ Work find_tile(const TileArgs<T>& a, int lane) {
+  // tiles and tokens of sequence s0 + lane
+  auto count = [&](int s, int& tiles, int& len, uint64_t& keys) {
+    tiles = 0, len = 0, keys = 0;
+    if (s >= a.p.n_seq) return;
+    const auto r = paged::NewRows::of<false>(a.p, s);
+    tiles = (int)(((long long)r.count * a.group + kTile - 1) / kTile);
+    len = max(r.token + r.count, 0);
+    keys = (uint64_t)tiles * max(len - r.count / 2, (len + 1) / 2);  // about those that the rows see
+  };
+  int tiles, len;
+  unsigned all_tiles = 0;
+  uint64_t keys, all_keys = 0;
+  for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
+    count(s0 + lane, tiles, len, keys);
+    all_tiles += tiles, all_keys += keys;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    all_tiles += __shfl_xor(all_tiles, d, 64);
+    all_keys += __shfl_xor((unsigned long long)all_keys, d, 64);
+  }
+  const float share = (float)all_keys * a.p.Hkv * (1.0f / kShares) *
+                      fmaxf(1.0f, (float)all_tiles * a.p.Hkv * (1.0f / kShares));
+  const int chunk = max(kLeastKeys<T>, ((int)fminf(share, (float)(1 << 24)) + 64) / 64 * 64);
+
+  Work w{};
+  w.head = blockIdx.x;
+  w.seq = -1;
+  // the sequence whose places in the list hold this one: 64 sequences at a time, summed up over lanes
+  int left = blockIdx.y, parts_before = 0, n_tiles = 0;
+  for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
+    if (a.p.n_seq > 64) count(s0 + lane, tiles, len, keys);
+    const int cuts = len > kWhole<T> * chunk ? (len + chunk - 1) / chunk : 1;
+    const int places = tiles * cuts, parts = cuts > 1 ? places : 0;
+    int upto = places, parts_upto = parts;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(upto, d, 64), y = __shfl_up(parts_upto, d, 64);
+      if (lane >= d) upto += x, parts_upto += y;
+    }
+    const uint64_t reach = __builtin_amdgcn_ballot_w64(upto > left);
+    if (reach != 0) {
+      const int at = __builtin_ctzll(reach);
+      w.seq = s0 + at;
+      n_tiles = __builtin_amdgcn_readlane(tiles, at);
+      left -= __builtin_amdgcn_readlane(upto - places, at);
+      parts_before += __builtin_amdgcn_readlane(parts_upto - parts, at);
+      // (a list that the arrays make longer than the step has room for: its tiles there are left out)
+      if (parts_before + __builtin_amdgcn_readlane(parts, at) > a.slots) return w;
+      break;
+    }
+    left -= __builtin_amdgcn_readlane(upto, 63);
+    parts_before += __builtin_amdgcn_readlane(parts_upto, 63);
+  }
+  if (w.seq < 0) return w;
+  w.chunk = __builtin_amdgcn_readfirstlane(left / n_tiles);
+  const int tile = n_tiles - 1 - (left - w.chunk * n_tiles);  // the last rows, which see most, first
+  w.row0 = __builtin_amdgcn_readfirstlane(tile * kTile);
+  w.part0 = (parts_before + tile) * a.p.Hkv + w.head;
+  w.part_step = n_tiles * a.p.Hkv;
+  const int keys_each = __builtin_amdgcn_readfirstlane(chunk);
+  w.take(a, paged::NewRows::of<true>(a.p, w.seq), keys_each, kWhole<T> * keys_each);
   return w;
 }
 
@@ -114,10 +172,16 @@ struct RowPlace {
 template <int D>
 __device__ __forceinline__ RowPlace row_place(const Work& w, int group, int r) {
   const uint32_t x = w.row0 + r, t = x / (uint32_t)group;
-  return RowPlace{(int)t, (int)((blockIdx.x * group + (x - t * group)) * D)};
+  return RowPlace{(int)t, (int)((w.head * group + (x - t * group)) * D)};
 }
 
 // ------------------------------------------------------------------------ merging
+
+// The partial of chunk `c` of the workgroup's tile.
+template <typename T>
+__device__ __forceinline__ float* partial(const TileArgs<T>& a, const Work& w, int c) {
+  return a.part + (w.part0 + c * (size_t)w.part_step) * a.part_pitch;
+}
 
 __device__ __forceinline__ void st_agent2(float* p, float a, float b) {
   const uint64_t w = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
@@ -180,12 +244,12 @@ __device__ __forceinline__ Merged<LOG2> merge_chunks_of(const float* at, size_t 
 
 // The last workgroup of a tile to arrive: every chunk's partial is written. Up to FEW rows, a wave takes
 // every element for its share of the chunks; `lds` has room for FEW * D * WAVES Merged.
-constexpr int kFew = 8, kMergeChunks = 16;
+constexpr int kFew = 8;
 template <bool LOG2, int WAVES, int FEW, typename T, int D>
 __device__ __forceinline__ void merge_tile(const TileArgs<T>& a, const Work& w, const float* part,
                                            void* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const size_t pitch = (size_t)a.part_rows * (D + 2);
+  const size_t pitch = a.part_pitch;
   auto store = [&](int e, float x) {
     const RowPlace at = row_place<D>(w, a.group, e / D);
     a.out[(w.first + at.t) * a.ld_out + at.col + e % D] = Elem<T>::from(x);
@@ -195,56 +259,6 @@ __device__ __forceinline__ void merge_tile(const TileArgs<T>& a, const Work& w, 
   };
   const int n = w.rows * D;
   if (w.rows > FEW) {
-    if (w.chunks <= kMergeChunks && w.rows <= kTile && WAVES == kWaves) {
-      // every row's maximum and sum once, as a factor for each chunk; then a thread adds up pairs of
-      // columns, 16 of them and so as many loads of a chunk in flight
-      float(*factor)[kTile] = reinterpret_cast<float(*)[kTile]>(lds);
-      for (int r = tid; r < w.rows; r += 64 * WAVES) {
-        float m[kMergeChunks], l[kMergeChunks], most = neg_inf(), sum = 0.f;
-        const float* at = part + (size_t)r * (D + 2);
-#pragma unroll
-        for (int c = 0; c < kMergeChunks; ++c) {
-          const int x = min(c, w.chunks - 1);
-          ld_agent2(at + x * pitch, m[c], l[c]);
-        }
-#pragma unroll
-        for (int c = 0; c < kMergeChunks; ++c)
-          if (c < w.chunks) most = fmaxf(most, m[c]);
-        const float base = most == neg_inf() ? 0.f : most;
-#pragma unroll
-        for (int c = 0; c < kMergeChunks; ++c)
-          if (c < w.chunks) m[c] = weight_of<LOG2>(m[c] - base), sum += l[c] * m[c];
-        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-#pragma unroll
-        for (int c = 0; c < kMergeChunks; ++c)
-          if (c < w.chunks) factor[c][r] = m[c] * inv;
-      }
-      __syncthreads();
-      constexpr int P = kTile * D / 2 / (64 * WAVES);  // pairs a thread
-      float x[P], y[P];
-#pragma unroll
-      for (int j = 0; j < P; ++j) x[j] = y[j] = 0.f;
-      for (int c = 0; c < w.chunks; ++c) {
-        float u[P], v[P];
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-          const int e = 2 * min(tid + j * 64 * WAVES, n / 2 - 1);
-          ld_agent2(part + c * pitch + (size_t)(e / D) * (D + 2) + 2 + e % D, u[j], v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-          const float f = factor[c][2 * min(tid + j * 64 * WAVES, n / 2 - 1) / D];
-          x[j] = fmaf(u[j], f, x[j]);
-          y[j] = fmaf(v[j], f, y[j]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < P; ++j) {
-        const int e = 2 * (tid + j * 64 * WAVES);
-        if (e < n) store(e, x[j]), store(e + 1, y[j]);
-      }
-      return;
-    }
     for (int e = tid; e < n; e += 64 * WAVES) store(e, merge(e, 0, w.chunks).value());
     return;
   }
@@ -334,28 +348,62 @@ __device__ __forceinline__ void join_waves(const WaveRows<D>& r, f32x16 (&o)[D /
   __syncthreads();
 }
 
-// A tile of several chunks: leaves this one's partial, and in the last workgroup to arrive merges all.
-template <typename T, int D>
-__device__ __forceinline__ void leave_partial(const TileArgs<T>& a, const Work& w,
-                                              const WaveRows<D>& r, const f32x16 (&o)[D / 32], float m,
-                                              float l, float* lds, int* flag, int lane) {
-  const int l32 = lane & 31, hi = lane >> 5;
-  const size_t unit = (size_t)blockIdx.y * a.p.Hkv + blockIdx.x;
-  float* part = tile_partials<D>(a);
-  if (r.owner() && r.q0 + l32 < w.rows) {
-    float* row = part + ((size_t)blockIdx.z * a.part_rows + r.q0 + l32) * (D + 2);
-    if (hi == 0) st_agent2(row, m, l);
+// A row's running state in a wave: maximum and sum of its weights, O^T.
+template <int D>
+struct Running {
+  f32x16 o[D / 32];
+  float m = neg_inf(), l = 0.f;
+  __device__ __forceinline__ Running() {
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float* to = row + 2 + 32 * db + 8 * g + 4 * hi;
-        st_agent2(to, o[db][4 * g], o[db][4 * g + 1]);
-        st_agent2(to + 2, o[db][4 * g + 2], o[db][4 * g + 3]);
-      }
+    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
   }
-  if (last_to_arrive(a.counter + unit, w.chunks, flag))
-    merge_tile<sizeof(T) == 2, kWaves, kFew, T, D>(a, w, part, lds);
+};
+
+// A tile of several chunks: the owners leave their sums as the lanes hold them, so that every store of a
+// wave is 512 bytes in a row; in the last workgroup to arrive the waves that share rows take every chunk in
+// turn and are joined again, and true is returned.
+__host__ __device__ constexpr int group_floats(int D) { return 64 * (2 + D / 2); }  // of 32 rows
+template <typename T, int D>
+__device__ __forceinline__ bool merge_chunks(const TileArgs<T>& a, const Work& w,
+                                             const WaveRows<D>& r, Running<D>& x, void* lds,
+                                             float (*ml)[2][64], int* flag, int lane) {
+  constexpr int N = D / 2;  // of O^T in a lane
+  const int place = r.grp * group_floats(D) + 2 * lane;
+  if (r.owner()) {
+    float* to = partial(a, w, w.chunk) + place;
+    st_agent2(to, x.m, x.l);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) st_agent2(to + 64 * (2 + i), x.o[i / 16][i % 16], x.o[i / 16][i % 16 + 1]);
+  }
+  if (!last_to_arrive(a.counter + w.part0, w.chunks, flag)) return false;
+  x = Running<D>();
+  if (r.active) {
+    float m[2], l[2], o[2][N];
+    auto load = [&](int b, int c) {
+      const float* at = partial(a, w, min(c, w.chunks - 1)) + place;
+      ld_agent2(at, m[b], l[b]);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) ld_agent2(at + 64 * (2 + i), o[b][i], o[b][i + 1]);
+    };
+    auto add = [&](int b, int c) {
+      if (c >= w.chunks) return;
+      const float mn = fmaxf(x.m, m[b]), base = mn == neg_inf() ? 0.f : mn;
+      const float f0 = weight_of<sizeof(T) == 2>(x.m - base), f1 = weight_of<sizeof(T) == 2>(m[b] - base);
+      x.m = mn;
+      x.l = x.l * f0 + l[b] * f1;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x.o[i / 16][i % 16] = x.o[i / 16][i % 16] * f0 + o[b][i] * f1;
+    };
+    load(0, r.sub);
+    for (int c = r.sub; c < w.chunks; c += 2 * r.ks) {
+      load(1, c + r.ks);
+      add(0, c);
+      if (c + 2 * r.ks < w.chunks) load(0, c + 2 * r.ks);
+      add(1, c + r.ks);
+    }
+  }
+  join_waves<T, D>(r, x.o, x.m, x.l, lds, ml, lane);
+  return true;
 }
 
 // The pages of a tile's four groups of 16 tokens, the first of them token `key`.
@@ -372,20 +420,12 @@ __device__ __forceinline__ Pages pages_at(const TileArgs<T>& a, const Work& w, i
   return g;
 }
 
-// The partials of the workgroup's tile.
-template <int D, typename T>
-__device__ __forceinline__ float* tile_partials(const TileArgs<T>& a) {
-  const size_t unit = (size_t)blockIdx.y * a.p.Hkv + blockIdx.x;
-  return a.part + unit * a.n_chunk * a.part_rows * (D + 2);
-}
-
 // Merges the waves' results in LDS into the output, or into the chunk's partial; true in the last
 // workgroup of a tile of several chunks.
 template <bool LOG2, int W, int ROWS, typename T, int D>
 __device__ __forceinline__ bool merge_waves(const TileArgs<T>& a, const Work& w,
                                             const float (&o)[W][ROWS][D], const float (&m)[W][ROWS],
                                             const float (&l)[W][ROWS], int* flag) {
-  float* part = tile_partials<D>(a);
   for (int e = threadIdx.x; e < w.rows * D; e += 64 * W) {
     const int r = e / D, col = e % D;
     Merged<LOG2> x;
@@ -395,13 +435,13 @@ __device__ __forceinline__ bool merge_waves(const TileArgs<T>& a, const Work& w,
       const RowPlace p = row_place<D>(w, a.group, r);
       a.out[(w.first + p.t) * a.ld_out + p.col + col] = Elem<T>::from(x.value());
     } else {
-      float* to = part + ((size_t)blockIdx.z * a.part_rows + r) * (D + 2);
+      float* to = partial(a, w, w.chunk) + (size_t)r * (D + 2);
       st_agent(to + 2 + col, x.o);
       if (col == 0) st_agent2(to, x.m, x.l);
     }
   }
   return w.chunks > 1 &&
-         last_to_arrive(a.counter + (size_t)blockIdx.y * a.p.Hkv + blockIdx.x, w.chunks, flag);
+         last_to_arrive(a.counter + w.part0, w.chunks, flag);
 }
 
 // ------------------------------------------------------------------------ a few rows
@@ -431,9 +471,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void paged_rows_kernel(const TileAr
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, sub = lane % LPR, grp = lane / LPR;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Work w = find_work(a, lane);
+  const Work w = find_few(a);
   if (w.none()) return;
-  const int head = blockIdx.x, key0 = w.key0 + wave * KW;
+  const int head = w.head, key0 = w.key0 + wave * KW;
 
   float m[NR], l[NR], o[NR][EPL];
 #pragma unroll
@@ -534,7 +574,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void paged_rows_kernel(const TileAr
   }
   __syncthreads();
   if (merge_waves<true, W, NR, T, D>(a, w, sm.o, sm.m, sm.l, &flag))
-    merge_tile<true, W, NR, T, D>(a, w, tile_partials<D>(a), lds);
+    merge_tile<true, W, NR, T, D>(a, w, partial(a, w, 0), lds);
 }
 
 // ------------------------------------------------------------------------ bf16
@@ -557,8 +597,7 @@ __device__ __forceinline__ float weights_bf16(bf16x8 (&p)[2], const f32x16& s, f
   return sum;
 }
 
-// A wave's 16 tokens of a tile of K or V: `rows` of them exist (the others take the last one's place;
-// they are masked, and must be finite where the last one is), `id` names their page; nothing to read: zeros.
+// A wave's 16 tokens of a tile of K or V; nothing to read: zeros.
 template <int D>
 struct Stage {
   static constexpr int C = D / 8, PER = 16 * C / 64;  // pieces a row, instructions a wave
@@ -570,8 +609,17 @@ struct Stage {
       off[n] = (uint32_t)(row * D + (c ^ swz<D>(row)) * 8) * 2u;
     }
   }
-  __device__ __forceinline__ void operator()(bf16* tile, const bf16* src, int rows, bool there,
-                                             int wave, int lane) const {
+  // `rows` of the 16 exist: the others take the last one's place (they are masked, and must be finite where
+  // the last one is)
+  __device__ __forceinline__ void clip(int rows, int lane) {
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int r = (n * 64 + lane) / C;
+      if (r >= rows) off[n] -= (uint32_t)((r - rows + 1) * D * 2);
+    }
+  }
+  __device__ __forceinline__ void operator()(bf16* tile, const bf16* src, bool there, int wave,
+                                             int lane) const {
     bf16* to = tile + wave * 16 * D;
     if (!there) {
 #pragma unroll
@@ -580,33 +628,49 @@ struct Stage {
       return;
     }
 #pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      uint32_t o = off[n];
-      if (rows < 16) {
-        const int r = (n * 64 + lane) / C;
-        if (r >= rows) o -= (uint32_t)((r - rows + 1) * D * 2);
-      }
-      dma_lds16_sbase(src, o, to + n * 64 * 8);
-    }
+    for (int n = 0; n < PER; ++n) dma_lds16_sbase(src, off[n], to + n * 64 * 8);
   }
 };
 
-// A row's running state in a wave: maximum and sum of its weights, O^T.
-template <int D>
-struct Running {
-  f32x16 o[D / 32];
-  float m = neg_inf(), l = 0.f;
-  __device__ __forceinline__ Running() {
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
+// Where a workgroup's groups of 16 tokens lie: lane i knows it of group i of 64, 16 tiles, so that a tile
+// costs a wave two v_readlane. (As scalar lookups and products for each tile, these were half of the scalar
+// instructions, which were as many as the vector ones.)
+struct Groups {
+  uint32_t lo, hi;       // the first element
+  uint64_t there, bad;   // has tokens of the workgroup and a page; has no page
+  int next;              // page of group 64 + lane
+  template <typename T>
+  __device__ __forceinline__ Groups(const TileArgs<T>& a, const Work& w, int lane) {
+    next = look(a, w, lane);
+    advance(a, w, 0, lane);
+  }
+  template <typename T>
+  __device__ __forceinline__ static int look(const TileArgs<T>& a, const Work& w, int group) {
+    const int page = (w.key0 + 16 * group) >> a.page_log2;
+    return a.p.table[(size_t)w.seq * a.p.max_pages + min(page, a.p.max_pages - 1)];
+  }
+  // to groups 64 b .. 64 b + 63
+  template <typename T>
+  __device__ __forceinline__ void advance(const TileArgs<T>& a, const Work& w, int b, int lane) {
+    const int key = w.key0 + 16 * (64 * b + lane);
+    const bool page = paged::is_page(a.p, next);
+    const size_t at = paged::page_row(a.p, page ? next : 0, w.head, key & (a.p.page - 1));
+    lo = (uint32_t)at, hi = (uint32_t)(at >> 32);
+    there = __builtin_amdgcn_ballot_w64(page && key < w.key1);
+    bad = __builtin_amdgcn_ballot_w64(!page);
+    next = look(a, w, 64 * (b + 1) + lane);
+  }
+  __device__ __forceinline__ size_t at(int i) const {
+    return (size_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, i) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)lo, i);
   }
 };
 
-// 32 keys, the first of them token c0: rows 32 i .. of the tiles ck and cv. bad0, bad1: their first and
-// second 16 have no page.
+// 32 keys, the first of them token c0: rows 32 i .. of the tiles ck and cv. `bad`: bits 0 and 1, their first
+// and second 16 have no page; mask: that, or some of the rows do not see them all.
 template <int D>
 __device__ __forceinline__ void keys32(Running<D>& x, const bf16* ck, const bf16* cv, int i, int c0,
-                                       bool bad0, bool bad1, const WaveRows<D>& r,
+                                       bool mask, uint32_t bad, const WaveRows<D>& r,
                                        const bf16x8 (&q)[D / 16], float scale, int lane) {
   constexpr int DB = D / 32;
   const int l32 = lane & 31, hi = lane >> 5;
@@ -614,7 +678,8 @@ __device__ __forceinline__ void keys32(Running<D>& x, const bf16* ck, const bf16
 #pragma unroll
   for (int ds = 0; ds < D / 16; ++ds)
     s = mfma32(lds_op(ck, rm_off<D>(32 * i + sigma32(l32), 2 * ds + hi)), q[ds], s);
-  if (c0 + 31 > r.all_see || bad0 || bad1) {
+  if (mask) {
+    const bool bad0 = (bad & 1) != 0, bad1 = (bad & 2) != 0;
     const int last = r.after - c0 - 8 * hi;
 #pragma unroll
     for (int y = 0; y < 16; ++y)
@@ -735,9 +800,9 @@ __global__ __launch_bounds__(64 * kMidWaves, 4) void paged_mid_bf16_kernel(const
   Waves& sm = *reinterpret_cast<Waves*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Work w = find_work(a, lane);
+  const Work w = find_few(a);
   if (w.none()) return;
-  const int head = blockIdx.x, key0 = w.key0 + wave * KW;
+  const int head = w.head, key0 = w.key0 + wave * KW;
 
   float m[NB], l[NB];
   acc16 o[NB][DB];
@@ -785,11 +850,14 @@ __global__ __launch_bounds__(64 * kMidWaves, 4) void paged_mid_bf16_kernel(const
         for (int ds = 0; ds < DS; ++ds)
           kr[j][t][ds] = as_bf16x8(ld_stream(row + 32 * ds));
       }
-    const Stage<D> stage(lane);
+    Stage<D> stage(lane);
     bf16* v = reinterpret_cast<bf16*>(lds) + wave * KW * D;
 #pragma unroll
-    for (int i = 0; i < NG; ++i)
-      stage(v, a.v_pages + at[i], w.key1 - key0 - 16 * i, there[i], i, lane);
+    for (int i = 0; i < NG; ++i) {
+      const int left = w.key1 - key0 - 16 * i;
+      if (there[i] && left < 16) stage.clip(left, lane);  // (the last group that is there)
+      stage(v, a.v_pages + at[i], there[i], i, lane);
+    }
     wait_vm_lds<0>();
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -862,7 +930,7 @@ __global__ __launch_bounds__(64 * kMidWaves, 4) void paged_mid_bf16_kernel(const
   }
   __syncthreads();
   if (merge_waves<true, W, ROWS, bf16, D>(a, w, sm.o, sm.m, sm.l, &flag))
-    merge_tile<true, W, kFew, bf16, D>(a, w, tile_partials<D>(a), lds);
+    merge_tile<true, W, kFew, bf16, D>(a, w, partial(a, w, 0), lds);
 }
 
 template <int D>
@@ -876,56 +944,49 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
   __shared__ int flag;
   static_assert(sizeof(lds) >= (kWaves - 1) * DB * sizeof(AccLds), "waves' partials fit");
   static_assert(sizeof(lds) >= kWaves * 32 * D * sizeof(bf16), "output rows fit");
-  static_assert(sizeof(lds) >= kFew * D * kWaves * sizeof(Merged<true>), "merged chunks fit");
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Work w = find_work(a, lane);
+  const Work w = find_tile(a, lane);
   if (w.none()) return;
   const WaveRows<D> r(w, a.group, wave, l32);
 
   bf16x8 q[D / 16];
   load_query<D>(q, a, w, r, hi);
 
-  const int head = blockIdx.x, n_tiles = w.key1 > w.key0 ? (w.key1 - w.key0 + 63) / 64 : 0;
-  const Stage<D> stage(lane);
-  auto load = [&](int t, const Pages& g, bf16* tk, bf16* tv) {
-    const int key = w.key0 + 64 * t + 16 * wave, left = w.key1 - key;
-    const int id = wave == 0 ? g.id[0] : wave == 1 ? g.id[1] : wave == 2 ? g.id[2] : g.id[3];
-    const bool there = left > 0 && paged::is_page(a.p, id);
-    const size_t at = there ? paged::page_row(a.p, id, head, key & (a.p.page - 1)) : 0;
-    stage(tk, a.k_pages + at, left, there, wave, lane);
-    stage(tv, a.v_pages + at, left, there, wave, lane);
+  const int head = w.head, n_tiles = w.key1 > w.key0 ? (w.key1 - w.key0 + 63) / 64 : 0;
+  Stage<D> stage(lane);
+  Groups g(a, w, lane);
+  auto load = [&](int t, bf16* tk, bf16* tv) {
+    if (t % 16 == 0 && t > 0) g.advance(a, w, t / 16, lane);
+    const int i = 4 * (t % 16) + wave;
+    const bool there = (g.there >> i & 1) != 0;
+    const size_t at = g.at(i);
+    const int left = w.key1 - (w.key0 + 64 * t + 16 * wave);
+    if (there && left < 16) stage.clip(left, lane);
+    stage(tk, a.k_pages + at, there, wave, lane);
+    stage(tv, a.v_pages + at, there, wave, lane);
   };
 
   Running<D> x;
-  Pages now{}, next{};
-  if (n_tiles > 0) {
-    now = pages_at(a, w, w.key0);
-    load(0, now, sk[0], sv[0]);
-    if (n_tiles > 1) next = pages_at(a, w, w.key0 + 64);
-  }
+  if (n_tiles > 0) load(0, sk[0], sv[0]);
   wait_vm_lds<0>();
   __builtin_amdgcn_s_barrier();
   take_query<D>(q, a.negate);
 
+  // blocks of 32 keys that some of the wave's rows see, and that all of them do
+  const int some = !r.active ? 0 : (min(r.some_see + 1, w.key1) - w.key0 + 31) / 32;
+  const int all = (r.all_see + 1 - w.key0) / 32;
   auto tile = [&](int t, const bf16* ck, const bf16* cv, bf16* nk, bf16* nv) {
-    const int k0 = w.key0 + 64 * t;
-    Pages after_next = next;
-    if (t + 1 < n_tiles) {
-      load(t + 1, next, nk, nv);
-      if (t + 2 < n_tiles) after_next = pages_at(a, w, k0 + 128);
-    }
+    const uint32_t bad = (uint32_t)(g.bad >> 4 * (t % 16)) & 15;
+    if (t + 1 < n_tiles) load(t + 1, nk, nv);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int c0 = k0 + 32 * i;
-      if (!r.active || ((2 * t + i) & (r.ks - 1)) != r.sub || c0 > r.some_see || c0 >= w.key1)
-        continue;
-      keys32<D>(x, ck, cv, i, c0, !paged::is_page(a.p, now.id[2 * i]),
-                !paged::is_page(a.p, now.id[2 * i + 1]), r, q, a.scale, lane);
+      const int block = 2 * t + i;
+      if (((block & (r.ks - 1)) == r.sub) & (block < some))
+        keys32<D>(x, ck, cv, i, w.key0 + 32 * block, (block >= all) | (bad != 0), bad >> 2 * i, r, q,
+                  a.scale, lane);
     }
-    now = next;
-    next = after_next;
     wait_vm_lds<0>();
     __builtin_amdgcn_s_barrier();
   };
@@ -935,8 +996,8 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
   }
   x.l = sum_halves(x.l);
   join_waves<bf16, D>(r, x.o, x.m, x.l, lds, sm_ml, lane);
-  if (w.chunks == 1) return store_rows<D>(a, w, r, x, lds, lane);
-  leave_partial<bf16, D>(a, w, r, x.o, x.m, x.l, reinterpret_cast<float*>(lds), &flag, lane);
+  if (w.chunks > 1 && !merge_chunks<bf16, D>(a, w, r, x, lds, sm_ml, &flag, lane)) return;
+  store_rows<D>(a, w, r, x, lds, lane);
 }
 
 // ------------------------------------------------------------------------ fp32
@@ -974,22 +1035,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<f
   __shared__ int flag;
   static_assert(sizeof(planes) >= (kWaves - 1) * DB * sizeof(AccLds), "waves' partials fit");
   static_assert(sizeof(planes) >= kWaves * 32 * kPitch * sizeof(float), "output rows fit");
-  static_assert(sizeof(planes) >= kFew * D * kWaves * sizeof(Merged<false>), "merged chunks fit");
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Work w = find_work(a, lane);
+  const Work w = find_tile(a, lane);
   if (w.none()) return;
   const WaveRows<D> r(w, a.group, wave, l32);
 
   X3 q[D / 16];  // the lane's query, split
   load_split_row<D>(q, a.q + (w.first + r.mine.t) * a.ld_q + r.mine.col, hi);
-  f32x16 o[DB];
-#pragma unroll
-  for (int db = 0; db < DB; ++db) o[db] = zero16();
-  float m = neg_inf(), l = 0.f;
+  Running<D> x;
+  f32x16(&o)[DB] = x.o;
+  float &m = x.m, &l = x.l;
 
-  const int head = blockIdx.x, n_tiles = w.key1 > w.key0 ? (w.key1 - w.key0 + 63) / 64 : 0;
+  const int head = w.head, n_tiles = w.key1 > w.key0 ? (w.key1 - w.key0 + 63) / 64 : 0;
   Pages now{}, next{};
   PageTile<D> tk, tv;
   if (n_tiles > 0) {
@@ -1061,29 +1120,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<f
   l = sum_halves(l);
   __syncthreads();  // the tiles are read: partials and output rows go there
   join_waves<float, D>(r, o, m, l, planes, sm_ml, lane);
-  if (w.chunks == 1) {
-    if (!r.owner()) return;
-    float* rows = reinterpret_cast<float*>(planes) + r.grp * 32 * kPitch;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(rows + l32 * kPitch + 32 * db + 8 * g + 4 * hi) =
-            f32x4{o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv,
-                  o[db][4 * g + 3] * inv};
-#pragma unroll
-    for (int n = 0; n < 32 * D / 4 / 64; ++n) {
-      const int i = (n * 64 + lane) / (D / 4), c = (n * 64 + lane) % (D / 4);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(rows + i * kPitch + 4 * c);
-      if (r.q0 + i < w.rows) {
-        const RowPlace at = row_place<D>(w, a.group, r.q0 + i);
-        *reinterpret_cast<f32x4*>(a.out + (w.first + at.t) * a.ld_out + at.col + 4 * c) = x;
-      }
-    }
+  if (w.chunks > 1 &&
+      !merge_chunks<float, D>(a, w, r, x, planes, sm_ml, &flag, lane))
     return;
+  if (!r.owner()) return;
+  float* rows = reinterpret_cast<float*>(planes) + r.grp * 32 * kPitch;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(rows + l32 * kPitch + 32 * db + 8 * g + 4 * hi) =
+          f32x4{o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv,
+                o[db][4 * g + 3] * inv};
+#pragma unroll
+  for (int n = 0; n < 32 * D / 4 / 64; ++n) {
+    const int i = (n * 64 + lane) / (D / 4), c = (n * 64 + lane) % (D / 4);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(rows + i * kPitch + 4 * c);
+    if (r.q0 + i < w.rows) {
+      const RowPlace at = row_place<D>(w, a.group, r.q0 + i);
+      *reinterpret_cast<f32x4*>(a.out + (w.first + at.t) * a.ld_out + at.col + 4 * c) = x;
+    }
   }
-  leave_partial<float, D>(a, w, r, o, m, l, reinterpret_cast<float*>(planes), &flag, lane);
 }
 
 // ------------------------------------------------------------------------ host
@@ -1102,17 +1160,22 @@ Path path_of(const PagedStep& s, int elem) {
 
 struct Plan {
   Path path;
-  int tiles, chunk, n_chunk, part_rows;
+  int tiles, chunk, n_chunk, slots, rows, part_pitch;
   size_t counters, partials;  // bytes
 };
 
-// Workgroups that a step is cut into where it has fewer tiles: about eight a CU.
-long long wanted() { return 8LL * (device_cus() > 0 ? device_cus() : 256); }
-constexpr int kLeastKeys = 256;  // of a chunk
-
-long long tiles_of(int n_seq, long long group, int rows, int max_rows) {
-  const long long per_seq = (max_rows * group + kTile - 1) / kTile;
-  return std::min(n_seq * per_seq, n_seq + rows * group / kTile);
+long long tiles_of(const PagedStep& s) {
+  const long long group = s.H / s.Hkv, per_seq = (s.max_rows * group + kTile - 1) / kTile;
+  return std::min(s.n_seq * per_seq, s.n_seq + s.rows * group / kTile);
+}
+// Of find_tile()'s list: with T the sum that it shares out, the tiles' lengths add up to 2 T at most, and a
+// chunk has T Hkv / kShares keys at least, so a KV head has no more than 2 kShares / Hkv chunks besides the
+// first ones; and no more than twice that of tiles that are cut.
+long long places_of(const PagedStep& s) { return tiles_of(s) + 2 * kShares / s.Hkv + 1; }
+long long slots_of(const PagedStep& s) {
+  const long long most = ((long long)s.max_pages * s.page + 255) / 256;  // (a chunk has 256 keys at least)
+  return most <= 1 ? 0
+                   : std::min({places_of(s), 4LL * kShares / s.Hkv + 1, tiles_of(s) * most});
 }
 int mid_keys_of(int D) { return kMidWaves * (D == 64 ? mid_wave_keys<64>() : mid_wave_keys<32>()); }
 int few_keys_of(int elem, int D) {
@@ -1120,29 +1183,25 @@ int few_keys_of(int elem, int D) {
                    : (D == 64 ? few_keys<float, 64>() : few_keys<float, 32>());
 }
 
-// Tiles of the step's list, keys of a workgroup, and what the workspace holds. The lengths are on the
-// device: the grid has room for every sequence at its longest.
+// The lengths are on the device: there is room for every sequence at its longest.
 Plan plan_of(const PagedStep& s, int elem) {
   const long long group = s.H / s.Hkv, max_len = (long long)s.max_pages * s.page;
   Plan p{};
   p.path = path_of(s, elem);
-  p.tiles = (int)tiles_of(s.n_seq, group, s.rows, s.max_rows);
-  p.part_rows = (int)std::min(s.max_rows * group, (long long)kTile);
-  const long long units = (long long)p.tiles * s.Hkv;
-  if (p.path == kRows) {
-    p.chunk = few_keys_of(elem, s.D);
-  } else if (p.path == kMid) {
-    p.chunk = mid_keys_of(s.D);
+  p.rows = (int)std::min(s.max_rows * group, (long long)kTile);
+  long long parts = 0;
+  if (p.path == kTiles) {
+    p.part_pitch = (p.rows + 31) / 32 * group_floats(s.D);
+    p.slots = (int)slots_of(s);
+    parts = (long long)p.slots * s.Hkv;
   } else {
-    const long long want = (wanted() + units - 1) / units;
-    const long long chunk = std::max<long long>(kLeastKeys, (max_len + want - 1) / want);
-    p.chunk = (int)((chunk + 255) / 256 * 256);
+    p.part_pitch = p.rows * (s.D + 2);
+    p.chunk = p.path == kRows ? few_keys_of(elem, s.D) : mid_keys_of(s.D);
+    p.n_chunk = (int)((max_len + p.chunk - 1) / p.chunk);
+    if (p.n_chunk > 1) parts = (long long)s.n_seq * s.Hkv * p.n_chunk;
   }
-  p.n_chunk = (int)((max_len + p.chunk - 1) / p.chunk);
-  if (p.n_chunk > 1) {
-    p.counters = counter_bytes(p.tiles, s.Hkv);
-    p.partials = sizeof(float) * units * p.n_chunk * p.part_rows * (s.D + 2);
-  }
+  p.counters = parts * sizeof(unsigned);
+  p.partials = parts * p.part_pitch * sizeof(float);
   return p;
 }
 
@@ -1156,27 +1215,29 @@ hipError_t launch_paged_t(T* out, long long ld_out, const T* q, long long ld_q, 
   a.ld_out = ld_out, a.ld_q = ld_q, a.p = s;
   a.group = s.H / s.Hkv;
   a.page_log2 = __builtin_ctz((unsigned)s.page);
-  a.chunk = plan.chunk, a.n_chunk = plan.n_chunk, a.part_rows = plan.part_rows;
-  a.one_tile = (long long)s.max_rows * a.group <= kTile;
+  a.chunk = plan.chunk, a.n_chunk = plan.n_chunk, a.slots = plan.slots;
+  a.rows = plan.rows, a.part_pitch = plan.part_pitch;
   // bf16: masked scores are -inf before they are scaled, so the factor is kept above 0: at 1e-30 every score
   // weighs the same, as at a scale of 0 (as attn_fwd_bf16.hip).
   a.scale = sizeof(T) == 2 ? fmaxf(fabsf(scale) * kLog2e, 1e-30f) : scale;
   a.negate = scale < 0.f;
   if (plan.path == kRows) a.scale = scale * kLog2e;  // (masked after it)
-  if (plan.n_chunk > 1) {
+  if (plan.partials > 0) {
     // the caller checked workspace_bytes >= paged_workspace_needed(); partials against its end
     const size_t at = (workspace_bytes - plan.partials) & ~(size_t)15;
     a.counter = static_cast<unsigned*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + at);
   }
-  launch(a, dim3(s.Hkv, plan.tiles, plan.n_chunk), plan.path);
+  const dim3 grid = plan.path == kTiles ? dim3(s.Hkv, (unsigned)places_of(s))
+                                        : dim3(s.Hkv, s.n_seq, plan.n_chunk);
+  launch(a, grid, plan.path);
   return hipGetLastError();
 }
 
 template <typename T>
 void launch_rows(const TileArgs<T>& a, dim3 grid, hipStream_t stream) {
   auto run = [&](auto d) {
-    switch (a.part_rows) {
+    switch (a.rows) {
       case 1: paged_rows_kernel<T, d(), 1><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
       case 2: paged_rows_kernel<T, d(), 2><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
       case 3: paged_rows_kernel<T, d(), 3><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
@@ -1193,27 +1254,25 @@ void launch_rows(const TileArgs<T>& a, dim3 grid, hipStream_t stream) {
 
 size_t paged_workspace_needed(const PagedStep& step, int elem) {
   const Plan p = plan_of(step, elem);
-  return p.n_chunk > 1 ? p.counters + p.partials + 16 : 0;
+  return p.partials > 0 ? p.counters + p.partials + 16 : 0;
 }
 
-// Of n tiles x KV heads, n < wanted(), a plan of tiles makes at most ceil(max_len / kLeastKeys) chunks each
-// and wanted() + n workgroups in all, more than that are not cut; that of a few rows makes n_seq x KV heads
-// times ceil(max_len / their chunk). Both bounds grow with every argument.
+// The larger of what tiles and a few rows take, each of which grows with every argument.
 size_t paged_workspace_bytes(const PagedStep& s) {
   const long long group = s.H / s.Hkv, max_len = (long long)s.max_pages * s.page;
-  const long long chunks = (max_len + kLeastKeys - 1) / kLeastKeys;
-  if (chunks <= 1) return 0;
-  const long long row = sizeof(float) * (s.D + 2);
-  const long long units = std::min(tiles_of(s.n_seq, group, s.rows, s.max_rows) * s.Hkv, wanted());
-  const long long tiled = std::min(units * chunks, wanted() + units) *
-                          std::min(s.max_rows * group, (long long)kTile) * row;
+  const long long tile_rows = std::min((s.max_rows * group + 31) / 32 * 32, (long long)kTile);
+  const long long tiled = slots_of(s) * s.Hkv * (sizeof(unsigned) + sizeof(float) * tile_rows * (s.D + 4));
   long long few = 0;
   if (group <= kMostMid) {
     const int keys = std::min({few_keys_of(2, s.D), few_keys_of(4, s.D), mid_keys_of(s.D)});
-    few = (long long)s.n_seq * s.Hkv * ((max_len + keys - 1) / keys) *
-          std::min<long long>(s.max_rows * group, kMostMid) * row;
+    const long long n_chunk = (max_len + keys - 1) / keys;
+    if (n_chunk > 1)
+      few = s.n_seq * s.Hkv * n_chunk *
+            (sizeof(unsigned) +
+             sizeof(float) * std::min<long long>(s.max_rows * group, kMostMid) * (s.D + 2));
   }
-  return counter_bytes((int)std::max(units, (long long)s.n_seq * s.Hkv), 1) + std::max(tiled, few) + 16;
+  const long long most = std::max(tiled, few);
+  return most > 0 ? most + 16 : 0;
 }
 
 hipError_t launch_paged_attention_bf16(bf16* out, long long ld_out, const bf16* q, long long ld_q,
@@ -1234,9 +1293,9 @@ hipError_t launch_paged_attention_bf16(bf16* out, long long ld_out, const bf16* 
           constexpr std::integral_constant<int, 1> one;
           constexpr std::integral_constant<int, 2> two;
           if (step.D == 64)
-            a.part_rows <= 16 ? run(d64, one) : run(d64, two);
+            a.rows <= 16 ? run(d64, one) : run(d64, two);
           else
-            a.part_rows <= 16 ? run(d32, one) : run(d32, two);
+            a.rows <= 16 ? run(d32, one) : run(d32, two);
         } else if (step.D == 64)
           paged_bf16_kernel<64><<<grid, kThreads, 0, stream>>>(a);
         else
