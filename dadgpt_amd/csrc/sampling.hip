@@ -530,8 +530,10 @@ struct Parts {
   Levels levels;
   int bucket;
   __device__ __forceinline__ int operator()(float x) const {
+    // (whether x is in the bucket is for Levels to say: this difference may be rounded once, and then lies
+    // below 0 for an x at the bucket's edge)
     const float t = (levels.top - x) * levels.per - (float)bucket;
-    return x > neg_inf() && t >= 0.f && t < 1.0f ? (int)(t * (float)kLevels) : kLevels;
+    return levels(x) == bucket ? min(max((int)(t * (float)kLevels), 0), kLevels - 1) : kLevels;
   }
 };
 

@@ -134,6 +134,20 @@ def test_special_logits(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_ties_at_a_buckets_edge(gpu, dtype):
+    """More candidates than the list holds, most of them at a logit whose distance from the largest, in
+    buckets, rounds up to the edge of one: 11.75 * 63 / (31 t) in fp32 is 19 and exactly a little less."""
+    t = 1.2567912340164185
+    per = np.float32(63) / (np.float32(31) * np.float32(t))
+    assert np.float32(11.75) * per == 19 and 11.75 * float(per) < 19
+    row = torch.tensor([0.0] + [-11.75] * 20000 + [-12.0] * 12000 + [-20.0] * 100)
+    row = row[torch.randperm(len(row), generator=torch.Generator().manual_seed(5))]
+    ps = [0.5, 0.6, 0.75, 0.8, 0.9, 0.97]
+    x = row.to(dtype).repeat(2 * len(ps), 1)
+    _check(x, _uniforms(len(x), 6), [t] * len(x), [0] * len(ps) + [30000] * len(ps), ps + ps)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_strides(gpu, dtype):
     """Rows at any pitch and alignment: slices of a wider buffer, one row expanded."""
     rows, vocab = 6, 1003
