@@ -530,8 +530,9 @@ struct Parts {
   Levels levels;
   int bucket;
   __device__ __forceinline__ int operator()(float x) const {
-    // (whether x is in the bucket is for Levels to say: this difference may be rounded once, and then lies
-    // below 0 for an x at the bucket's edge)
+    // Every use of this has to give an element the same part: Levels says whether it is in the bucket at
+    // all, and the difference is rounded after the product, not once with it in some uses.
+#pragma clang fp contract(off)
     const float t = (levels.top - x) * levels.per - (float)bucket;
     return levels(x) == bucket ? min(max((int)(t * (float)kLevels), 0), kLevels - 1) : kLevels;
   }
