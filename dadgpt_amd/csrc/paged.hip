@@ -19,80 +19,57 @@ struct AppendArgs {
   long long ld_out, ld_q, ld_kv;
   PagedStep p;
   Rope r;
-  int heads_q, groups;  // query heads to move (0 without q); of all heads: a thread takes g, g + groups, ..
+  int heads_q;  // query heads to move (0 without q)
 };
 
 // Grid (rows of a sequence, sequences). Consecutive threads run along a head's chunks, then the heads
 // of a row, which lie side by side in the projection's output.
-template <typename T, int VEC, bool INTER, int HPT>
+template <typename T, int VEC, bool INTER>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs<T> a) {
   const auto seq = paged::NewRows::of<true>(a.p, blockIdx.y);
-  const int D = a.p.D, chunks = D / (2 * VEC);
+  const int D = a.p.D, chunks = D / (2 * VEC), heads = a.heads_q + 2 * a.p.Hkv;
   const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t c = id % chunks, j = id / chunks;
-  const int t = j / a.groups, g = j % a.groups;
+  const int t = j / heads, head = j % heads;
   const int token = seq.token + t;
   if (t >= seq.count || token < 0) return;
-  const rotary::Chunk pair = rotary::chunk_of<VEC, INTER>(c, a.r.rot_dim);
-  const rotary::Chunk flat{{2 * (int)c * VEC, 2 * (int)c * VEC + VEC}, false};
-  const int page = a.p.table[(size_t)blockIdx.y * a.p.max_pages + token / a.p.page];
-  const bool held = paged::is_page(a.p, page);
+  const int kh = head - a.heads_q, vh = kh - a.p.Hkv;
   const long long row = seq.first + t;
-
-  T* dst[HPT];
-  rotary::Piece<T, VEC> x[HPT][2];
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    const int head = i * a.groups + g, kh = head - a.heads_q, vh = kh - a.p.Hkv;
-    const rotary::Chunk& ch = vh >= 0 ? flat : pair;
-    const T* src;
-    if (kh < 0) {
-      src = a.q + row * a.ld_q + head * D;
-      dst[i] = a.q_out + row * a.ld_out + head * D;
-    } else {
-      const int h = vh >= 0 ? vh : kh;
-      src = (vh >= 0 ? a.v : a.k) + row * a.ld_kv + h * D;
-      dst[i] = held && vh < a.p.Hkv ? (vh >= 0 ? a.v_pages : a.k_pages) +
-                                          paged::page_row(a.p, page, h, token % a.p.page)
-                                    : nullptr;
-    }
-    if (dst[i] == nullptr) continue;
-    x[i][0].load(src + ch.at[0]);
-    x[i][1].load(src + ch.at[1]);
+  const T* src;
+  T* dst;
+  if (kh < 0) {
+    src = a.q + row * a.ld_q + head * D;
+    dst = a.q_out + row * a.ld_out + head * D;
+  } else {
+    const int page = a.p.table[(size_t)blockIdx.y * a.p.max_pages + token / a.p.page];
+    if (!paged::is_page(a.p, page)) return;
+    const int h = vh >= 0 ? vh : kh;
+    src = (vh >= 0 ? a.v : a.k) + row * a.ld_kv + h * D;
+    dst = (vh >= 0 ? a.v_pages : a.k_pages) + paged::page_row(a.p, page, h, token % a.p.page);
   }
-  if (pair.rotated) {
-    const auto turn = rotary::turn_of<VEC>(a.r.freqs + c * VEC, token, a.r.magnitude, false);
-#pragma unroll
-    for (int i = 0; i < HPT; ++i)
-      if (i * a.groups + g < a.heads_q + a.p.Hkv)
-        rotary::turn_pieces<T, VEC, INTER>(x[i][0], x[i][1], turn);
-  }
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    if (dst[i] == nullptr) continue;
-    const rotary::Chunk& ch = i * a.groups + g >= a.heads_q + a.p.Hkv ? flat : pair;
-    x[i][0].store(dst[i] + ch.at[0]);
-    x[i][1].store(dst[i] + ch.at[1]);
-  }
+  const rotary::Chunk ch =
+      vh >= 0 ? rotary::Chunk{{2 * (int)c * VEC, 2 * (int)c * VEC + VEC}, false}
+              : rotary::chunk_of<VEC, INTER>(c, a.r.rot_dim);
+  rotary::Piece<T, VEC> x, y;
+  x.load(src + ch.at[0]);
+  y.load(src + ch.at[1]);
+  if (ch.rotated)
+    rotary::turn_pieces<T, VEC, INTER>(
+        x, y, rotary::turn_of<VEC, sizeof(T) == 2>(a.r.freqs + c * VEC, token, a.r.magnitude, false));
+  x.store(dst + ch.at[0]);
+  y.store(dst + ch.at[1]);
 }
 
 template <typename T>
 hipError_t launch_append_t(T* k_pages, T* v_pages, T* q_out, long long ld_out, const T* q,
                            long long ld_q, const T* k, const T* v, long long ld_kv, const PagedStep& p, const Rope& r,
                            hipStream_t stream) {
-  AppendArgs<T> a{k_pages, v_pages, q_out, q, k, v, ld_out, ld_q, ld_kv, p, r, q ? p.H : 0, 0};
+  AppendArgs<T> a{k_pages, v_pages, q_out, q, k, v, ld_out, ld_q, ld_kv, p, r, q ? p.H : 0};
   const int heads = a.heads_q + 2 * p.Hkv;
   auto run = [&](auto vec, auto inter) {
     const long long chunks = p.D / (2 * vec());
-    const int hpt = rotary::heads_per_thread((long long)p.rows * chunks, heads);
-    a.groups = (heads + hpt - 1) / hpt;
-    const dim3 grid((unsigned)((p.max_rows * chunks * a.groups + kThreads - 1) / kThreads), p.n_seq);
-    switch (hpt) {
-      case 1: paged_append_kernel<T, vec(), inter(), 1><<<grid, kThreads, 0, stream>>>(a); break;
-      case 2: paged_append_kernel<T, vec(), inter(), 2><<<grid, kThreads, 0, stream>>>(a); break;
-      case 4: paged_append_kernel<T, vec(), inter(), 4><<<grid, kThreads, 0, stream>>>(a); break;
-      default: paged_append_kernel<T, vec(), inter(), 8><<<grid, kThreads, 0, stream>>>(a); break;
-    }
+    const dim3 grid((unsigned)((p.max_rows * chunks * heads + kThreads - 1) / kThreads), p.n_seq);
+    paged_append_kernel<T, vec(), inter()><<<grid, kThreads, 0, stream>>>(a);
     return hipGetLastError();
   };
   auto with = [&](auto vec) {

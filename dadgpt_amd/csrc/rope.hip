@@ -2,9 +2,11 @@
 // gradients back. y = magnitude R(position * f) x pair by pair, so the transposed map, the backward, is
 // the rotation by the negative angle with the same magnitude, and one kernel does both.
 //
-// Bound by HBM: every element is read and written once (4 operations an element). The angles cost
-// more than the rotation (a double product and a sincospi for each pair of a token), so a thread
-// computes those of its pairs once and takes up to eight heads of the token.
+// Bound by HBM: every element is read and written once (4 operations an element). A thread turns one
+// chunk of one head, so that the waves are many and short and loads, angles and stores of different ones
+// overlap: B16 T1024, q and k of 12 heads of 64 in bf16, one way, takes 24 us (4.2 TB/s; a copy 19.5 us),
+// B1 T32768, 10 heads of 64 in fp32, 34 us (5.0 TB/s). (Several heads a thread share its angles, but
+// with 2, 4 and 8 of them these took 25, 27 and 27 us, and 36, 40 and 45.)
 #include "common.hpp"
 #include "rope.hpp"
 #include "serving.hpp"
@@ -21,73 +23,50 @@ struct RopeArgs {
   const int* positions;
   RopeShape s;
   Rope r;
-  int groups;          // of heads: a thread takes heads g, g + groups, ..
   bool tokens_first;   // consecutive threads along the tokens of a head, not along the heads
   uint32_t n;
 };
 
 // Consecutive threads run along a head's chunks and then along what lies next in memory: the heads of a
 // token, or the tokens of a head.
-template <typename T, int VEC, bool INTER, int HPT>
+template <typename T, int VEC, bool INTER>
 __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeArgs<T> a) {
   const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
   if (id >= a.n) return;
-  const int D = a.s.D, S = a.s.S, chunks = D / (2 * VEC);
-  const uint32_t c = id % chunks, j = id / chunks, tokens = (uint32_t)a.s.B * S;
-  const uint32_t token = a.tokens_first ? j % tokens : j / a.groups;
-  const uint32_t g = a.tokens_first ? j / tokens : j % a.groups;
-  const uint32_t b = token / S, row = token - b * S;
+  const uint32_t chunks = a.s.D / (2 * VEC), heads = a.s.H + a.s.Hkv, tokens = (uint32_t)a.s.B * a.s.S;
+  const uint32_t c = id % chunks, j = id / chunks;
+  const uint32_t token = a.tokens_first ? j % tokens : j / heads;
+  const uint32_t head = a.tokens_first ? j / tokens : j % heads;
+  const uint32_t b = token / a.s.S, row = token - b * a.s.S;
   const rotary::Chunk ch = rotary::chunk_of<VEC, INTER>(c, a.r.rot_dim);
 
-  const T* src[HPT];
-  T* dst[HPT];
-  rotary::Piece<T, VEC> x[HPT][2];
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    const int head = i * a.groups + g;
-    const bool is_k = head >= a.s.H;
-    const int h = is_k ? head - a.s.H : head;
-    const Strides64 from = a.s.t[is_k ? 1 : 0], to = a.s.t[is_k ? 3 : 2];
-    src[i] = (is_k ? a.k : a.q) + (b * from.batch + h * from.head + row * from.row);
-    dst[i] = (is_k ? a.k_out : a.q_out) + (b * to.batch + h * to.head + row * to.row);
-    if (head >= a.s.H + a.s.Hkv) dst[i] = nullptr;
-    if (dst[i] == nullptr) continue;
-    x[i][0].load(src[i] + ch.at[0]);
-    x[i][1].load(src[i] + ch.at[1]);
-  }
+  const bool is_k = head >= (uint32_t)a.s.H;
+  const uint32_t h = is_k ? head - a.s.H : head;
+  const Strides64 from = a.s.t[is_k ? 1 : 0], to = a.s.t[is_k ? 3 : 2];
+  const T* src = (is_k ? a.k : a.q) + (b * from.batch + h * from.head + row * from.row);
+  T* dst = (is_k ? a.k_out : a.q_out) + (b * to.batch + h * to.head + row * to.row);
+  rotary::Piece<T, VEC> x, y;
+  x.load(src + ch.at[0]);
+  y.load(src + ch.at[1]);
   if (ch.rotated) {
     const int pos = a.positions == nullptr ? (int)row : a.positions[token];
-    const auto turn = rotary::turn_of<VEC>(a.r.freqs + c * VEC, pos, a.r.magnitude, a.r.inverse);
-#pragma unroll
-    for (int i = 0; i < HPT; ++i) rotary::turn_pieces<T, VEC, INTER>(x[i][0], x[i][1], turn);
+    rotary::turn_pieces<T, VEC, INTER>(
+        x, y, rotary::turn_of<VEC, sizeof(T) == 2>(a.r.freqs + c * VEC, pos, a.r.magnitude, a.r.inverse));
   }
-#pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    if (dst[i] == nullptr) continue;
-    x[i][0].store(dst[i] + ch.at[0]);
-    x[i][1].store(dst[i] + ch.at[1]);
-  }
+  x.store(dst + ch.at[0]);
+  y.store(dst + ch.at[1]);
 }
 
 template <typename T>
 hipError_t launch_rope_t(T* q_out, T* k_out, const T* q, const T* k, const RopeShape& s,
                          const Rope& r, const int* positions, hipStream_t stream) {
-  RopeArgs<T> a{q_out, k_out, q, k, positions, s, r, 0, false, 0};
+  RopeArgs<T> a{q_out, k_out, q, k, positions, s, r, false, 0};
   const int heads = s.H + s.Hkv;
   const Strides64& t = s.H > 0 ? s.t[0] : s.t[1];
   a.tokens_first = t.row < t.head;
   auto run = [&](auto vec, auto inter) {
-    const long long per_head = (long long)s.B * s.S * (s.D / (2 * vec()));
-    const int hpt = rotary::heads_per_thread(per_head, heads);
-    a.groups = (heads + hpt - 1) / hpt;
-    a.n = (uint32_t)(per_head * a.groups);
-    const unsigned grid = (a.n + kThreads - 1) / kThreads;
-    switch (hpt) {
-      case 1: rope_kernel<T, vec(), inter(), 1><<<grid, kThreads, 0, stream>>>(a); break;
-      case 2: rope_kernel<T, vec(), inter(), 2><<<grid, kThreads, 0, stream>>>(a); break;
-      case 4: rope_kernel<T, vec(), inter(), 4><<<grid, kThreads, 0, stream>>>(a); break;
-      default: rope_kernel<T, vec(), inter(), 8><<<grid, kThreads, 0, stream>>>(a); break;
-    }
+    a.n = (uint32_t)((long long)s.B * s.S * heads * (s.D / (2 * vec())));
+    rope_kernel<T, vec(), inter()><<<(a.n + kThreads - 1) / kThreads, kThreads, 0, stream>>>(a);
     return hipGetLastError();
   };
   auto with = [&](auto vec) {

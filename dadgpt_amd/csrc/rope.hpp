@@ -1,6 +1,6 @@
 // Rotary positions, for the kernels that move heads from one place to another (rope.hip, paged.hip):
-// a thread owns the same 2 VEC elements of several heads of one token, VEC pairs or, past rot_dim,
-// elements that are only copied, and computes the token's VEC angles once for all of them.
+// a thread owns 2 VEC elements of a head of a token, VEC pairs or, past rot_dim, elements that are only
+// copied.
 #pragma once
 
 #include "common.hpp"
@@ -16,8 +16,10 @@ struct Turn {
 };
 
 // The angle pos * f in turns, reduced in double (its error is pos * f * 2^-52 and below 2^-24 of what
-// is left), then the library's sin(pi x) and cos(pi x), which need no reduction of their own.
-template <int VEC>
+// is left), then the library's sin(pi x) and cos(pi x), which need no reduction of their own; for bf16
+// (FAST) the instructions for sin and cos of a number of turns, whose error, below 2^-20, is far below
+// half a step of the result, 2^-9.
+template <int VEC, bool FAST>
 __device__ __forceinline__ Turn<VEC> turn_of(const double* __restrict__ freqs, int pos,
                                              float magnitude, bool inverse) {
   constexpr double kTurns = 0.15915494309189533577;  // 1 / 2 pi
@@ -27,7 +29,10 @@ __device__ __forceinline__ Turn<VEC> turn_of(const double* __restrict__ freqs, i
     const double a = (double)pos * (freqs[e] * kTurns);
     const float x = (float)(a - __builtin_rint(a));
     float s, c;
-    sincospif(2.0f * x, &s, &c);
+    if constexpr (FAST)
+      s = __builtin_amdgcn_sinf(x), c = __builtin_amdgcn_cosf(x);
+    else
+      sincospif(2.0f * x, &s, &c);
     t.c[e] = c * magnitude;
     t.s[e] = (inverse ? -s : s) * magnitude;
   }
@@ -106,15 +111,6 @@ __device__ __forceinline__ void turn_pieces(Piece<T, VEC>& a, Piece<T, VEC>& b,
 template <typename T>
 inline bool wide(int rot_dim, int D) {
   return sizeof(T) == 2 && rot_dim % 16 == 0 && D % 16 == 0;
-}
-
-// Heads a thread takes of `heads`: as many as leave the GPU this many threads (8 waves of 64 a SIMD's
-// worth for 256 CUs would be 524,288; past 262,144 nothing is gained: B16 T1024 with 24 heads, see
-// rope.hip), at most 8, which is what the loads in flight of one thread hold.
-inline int heads_per_thread(long long threads_per_head, int heads) {
-  int n = 1;
-  while (n < 8 && threads_per_head * heads >= 2LL * n * 262144) n *= 2;
-  return n;
 }
 
 }  // namespace rotary
