@@ -1,7 +1,9 @@
 // Appending to paged caches for gfx950: the new rows of ragged sequences out of a fused projection's
 // output into the pages that the block table names, q and k rotated on the way (one launch for what
-// would be three: rotation, and a scatter each of k and v). Bound by HBM, and for a token a sequence by
-// the launch and the chain row_start, lens -> page -> store.
+// would be three: rotation, and a scatter each of k and v), one chunk of one head a thread (as
+// rope.hip). Bound by HBM, and for a token a sequence by the launch and the chain row_start, lens -> page
+// -> store: 8192 tokens of 16 prompts, 12 heads of 64 in bf16, 15.7 us (4.8 TB/s; a copy 14.6 us); one
+// token of 32 sequences 3.4 us of 13, the rest is the call's.
 #include "common.hpp"
 #include "paged.hpp"
 #include "rope.hpp"

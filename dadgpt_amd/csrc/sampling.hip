@@ -10,17 +10,22 @@
 // elements search over the row itself, and the draw there, as that of a row without filters, goes by
 // the sums of the waves' stretches of the row.
 //
-// The histogram has 16 columns, one for each lane of a row of 16: however the logits are spread, four
-// lanes of an atomic meet in a bank at most (with one column, 785 wave-wide pairs of atomics on 50257
-// logits of a usual spread took 45 us).
+// The histogram has 256 buckets, so that a bucket of a row of usual spread fits the list (with 64 of
+// them, flat rows of 50257 had 9000 to 16000 elements in the one that top-p ends in, and needed a second
+// histogram of it), and 8 columns, one for every eighth lane: however the logits are spread, eight lanes
+// of an atomic meet in a bank at most. (With one column, 785 wave-wide pairs of atomics on 50257 logits of
+// a usual spread took 45 us.)
 //
 // A pick must not depend on the order in which weights are added: they are computed in double (relative
 // error below 1e-13) and held as multiples of 2^-44 of the largest one, in 64-bit integers, whose sums
 // are exact in any order, histogram atomics among them. What that rounds off, 2^-45 a weight at
 // random, moves a border by about 1e-11 of the sum for 50257 of them.
 //
-// Bound by one CU's operations on a row: two or three an element and pass, about 20 for a weight. The
-// row (200 KB of fp32 for 50257 logits) comes from L2 after the first pass.
+// Bound by one CU's operations on a row: two or three an element and pass, about 20 for a weight, and
+// between passes by barriers and chains in LDS. The row (200 KB of fp32 for 50257 logits) comes from L2
+// after the first pass. 50257 logits, us: one row, top-k of 40, 19; 32 rows of all kinds 75; 512 rows of bf16
+// with top-p 204. 32 rows of one kind: no filter 25, top-k of 40 20, of 5000 40, top-p of 0.9 44 (spread of
+// 4) to 95 (of 0.5: 40000 tokens stay), and 320 with all logits equal.
 #include "common.hpp"
 #include "lanes.hpp"
 #include "serving.hpp"
@@ -29,7 +34,7 @@ namespace dadgpt {
 namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
-constexpr int kLevels = 64, kColumns = 16;  // buckets of the row's histogram, copies of each
+constexpr int kLevels = 256, kColumns = 8;  // buckets of the row's histogram, copies of each
 constexpr int kBuckets = kThreads;          // of a search's: one for each thread to scan
 constexpr int kFew = kThreads;              // elements of a bucket that are compared each with each
 constexpr int kPerThread = 16, kList = kPerThread * kThreads;  // candidates
@@ -66,6 +71,13 @@ __device__ __forceinline__ u64 row_scan(u64 x) {
   x += dpp64<0x112>(x);
   x += dpp64<0x114>(x);
   x += dpp64<0x118>(x);
+  return x;
+}
+// The sum over lanes l - 7 to l of a row.
+__device__ __forceinline__ u64 sum_of_8(u64 x) {
+  x += dpp64<0x111>(x);
+  x += dpp64<0x112>(x);
+  x += dpp64<0x114>(x);
   return x;
 }
 __device__ __forceinline__ u64 wave_scan(u64 x) {
@@ -364,25 +376,36 @@ struct Row {
     });
     __syncthreads();
     for (int i = tid; i < kLevels * kColumns; i += kThreads) {
-      const u64 n = row_scan((u64)sm.row.count[0][i]);
-      const u64 w = WEIGHTS ? row_scan(sm.row.weight[0][i]) : n;
+      const u64 n = sum_of_8((u64)sm.row.count[0][i]);
+      const u64 w = WEIGHTS ? sum_of_8(sm.row.weight[0][i]) : n;
       if (lane % kColumns == kColumns - 1)
         sm.level_count[i / kColumns] = (uint32_t)n, sm.level_weight[i / kColumns] = w;
     }
     __syncthreads();
     // (every wave for itself)
-    static_assert(kLevels == 64 && kColumns == 16, "a lane a bucket, a row of lanes its copies");
-    const u64 w = sm.level_weight[lane], upto = wave_scan(w) + over;
-    const u64 own = sm.level_count[lane], n = wave_scan(own);
+    static_assert(kLevels == 4 * 64 && kColumns == 8, "four buckets a lane, eight lanes a bucket's copies");
+    u64 w[4], n[4], sum = 0, number = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sum += w[e] = sm.level_weight[4 * lane + e];
+      number += n[e] = sm.level_count[4 * lane + e];
+    }
+    const u64 upto = wave_scan(sum) + over;
     Level r;
     r.all = lane_of(upto, 63);
     const u64 target = target_of(r.all);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(upto - w < target && upto >= target);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(upto - sum < target && upto >= target);
     const int at = hit != 0 ? __builtin_ctzll(hit) : 63;
-    r.bucket = hit != 0 ? at : kLevels;
+    // (each lane as if it were the one)
+    u64 above = upto - sum, count = wave_scan(number) - number + n[0], own = n[0];
+    int e = 0;
+#pragma unroll
+    for (int y = 0; y < 3; ++y)
+      if (e == y && above + w[y] < target) above += w[y], own = n[y + 1], count += own, ++e;
+    r.bucket = hit != 0 ? 4 * at + __builtin_amdgcn_readlane(e, at) : kLevels;
     r.own = (uint32_t)lane_of(own, at);
-    r.count = (uint32_t)lane_of(n, at);
-    r.over = lane_of(upto - w, at);
+    r.count = (uint32_t)lane_of(count, at);
+    r.over = lane_of(above, at);
     return r;
   }
 
@@ -519,7 +542,7 @@ struct Pick {
 };
 
 // Buckets of equal width below `top`, the last one with all that lies lower; and those of one bucket, in
-// 64 equal parts of it.
+// kLevels equal parts of it.
 struct Levels {
   float top, per;
   __device__ __forceinline__ int operator()(float x) const {

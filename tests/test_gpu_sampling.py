@@ -134,7 +134,7 @@ def test_special_logits(gpu, dtype):
 
 
 def _edge(t, distance, place):
-    per = np.float32(63) / (np.float32(31) * np.float32(t))
+    per = np.float32(255) / (np.float32(31) * np.float32(t))
     assert np.float32(distance) * per == place and distance * float(per) < place
 
 
@@ -148,23 +148,23 @@ def _check_flat(t, row, ps, dtype):
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_ties_at_a_buckets_edge(gpu, dtype, many):
     """More candidates than the list holds, `many` of them at a logit whose distance from the largest, in
-    buckets, rounds up to the edge of one: 11.75 * 63 / (31 t) in fp32 is 19 and exactly a little less."""
-    t = 1.2567912340164185
-    _edge(t, 11.75, 19)
-    row = [0.0] + [-11.75] * many + [-11.875] * 6000 + [-12.0] * 6000 + [-20.0] * 100
-    w = np.exp(np.array([0.0, -11.75, -11.875, -12.0]) / t) * [1, many, 6000, 6000]
+    buckets, rounds up to the edge of one: 11.75 * 255 / (31 t) in fp32 is 73 and exactly a little less."""
+    t = 1.324016809463501
+    _edge(t, 11.75, 73)
+    row = [0.0] + [-11.75] * many + [-11.8125] * 12000 + [-20.0] * 100
+    w = np.exp(np.array([0.0, -11.75, -11.8125]) / t) * [1, many, 12000]
     ends = np.cumsum(w) / w.sum()
-    ps = [float(ends[i] + f * (ends[i + 1] - ends[i])) for i in range(3) for f in (0.3, 0.8)]
+    ps = [float(ends[i] + f * (ends[i + 1] - ends[i])) for i in range(2) for f in (0.3, 0.6, 0.9)]
     _check_flat(t, row, ps, dtype)
 
 
 @pytest.mark.parametrize("many", [300, 4000])
 def test_ties_at_the_edge_of_a_buckets_part(gpu, many):
-    """The same at the edge of one of the 64 parts of a bucket of more than the list holds."""
-    t = 1.188039779663086
-    _edge(t, 11.5, 19 + 43 / 64)
-    row = [0.0] + [-11.25] * 9000 + [-11.5] * many + [-11.505] * 3000 + [-20.0] * 100
-    w = np.exp(np.array([0.0, -11.25, -11.5, -11.505]) / t) * [1, 9000, many, 3000]
+    """The same at the edge of one of the 256 parts of a bucket of more than the list holds."""
+    t = 1.1700055599212646
+    _edge(t, 11.5, 80 + 218 / 256)
+    row = [0.0] + [-11.4375] * 9000 + [-11.5] * many + [-11.5004] * 3000 + [-20.0] * 100
+    w = np.exp(np.array([0.0, -11.4375, -11.5, -11.5004]) / t) * [1, 9000, many, 3000]
     ends = np.cumsum(w) / w.sum()
     ps = [float(ends[i] + f * (ends[i + 1] - ends[i])) for i in (1, 2) for f in (0.3, 0.6, 0.9)]
     _check_flat(t, row, ps, F32)
