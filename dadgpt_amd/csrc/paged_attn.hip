@@ -2,23 +2,32 @@
 // and both in one call.
 //
 // Work. The queries that share a KV head are rows of one product: row r of a (sequence, KV head) is
-// query head r % G of its group for new token r / G, so that K and V are read once for the group. A
-// workgroup owns 128 of these rows, and `chunk` keys of those that they see; the chunks of one tile
-// leave fp32 partials, which the last workgroup to arrive merges (as decode.hip, whose header says why
-// relaxed agent-scope accesses order that).
+// query head r % G of its group for new token r / G, so that K and V are read once for the group. A few
+// rows are one tile, 128 a tile otherwise; a workgroup owns a tile's rows for a chunk of the keys that
+// they see. The chunks of one tile leave fp32 partials, which the last workgroup to arrive merges (as
+// decode.hip, whose header says why relaxed agent-scope accesses order that).
 //
-// The keys are walked in tiles of 64. A tile is four groups of 16 tokens, each within a page (a page
-// holds 16 at least): a wave stages one group of K and V by direct global -> LDS loads from wherever
-// the block table puts it, tile t + 1 in flight while tile t is multiplied. Scores, softmax and P V are
-// those of the bf16 forward (attn_fwd_bf16.hip): S^T = K Q^T with Q in registers, a lane a row,
-// P straight from the score registers into O^T += V^T P^T, and a running maximum that moves only when
-// weights would reach 2^64.
+// Three kernels, by the rows (path_of): paged_rows_kernel on the VALU, paged_mid_bf16_kernel in 16-row
+// matrix tiles, and the tiles below. The first two are bound by HBM and by the chain row_start, lens ->
+// page -> keys -> merge, and have all of a workgroup's loads in flight at once: 32 sequences of 1 to 1024
+// tokens, 12 heads of 64 in bf16, 14 us (50 MB, 3.6 TB/s), 8 of 1 to 32768 with three rows for each of 4 KV
+// heads 34 to 40 us (134 MB, 3.4 to 3.9 TB/s).
 //
-// Where a tile has fewer rows than 128, two or four waves share 32 rows and take every second or fourth
-// 32 keys; their results are merged at the end.
+// Tiles (bf16). The keys are walked in tiles of 64. A tile is four groups of 16 tokens, each within a page
+// (a page holds 16 at least): a wave stages one group of K and V by direct global -> LDS loads from
+// wherever the block table puts it, tile t + 1 in flight while tile t is multiplied. Scores, softmax and
+// P V are those of the bf16 forward (attn_fwd_bf16.hip): S^T = K Q^T with Q in registers, a lane a row,
+// P straight from the score registers into O^T += V^T P^T, rounded to bf16 there as in the forward, and a
+// running maximum that moves only when weights would reach 2^64. Where a tile has fewer rows than 128, two
+// or four waves share 32 rows and take every second or fourth 32 keys; their results are merged at the end.
+// Bound by VALU and matrix pipe, in waves that depend on themselves: 8 prompts' chunks of up to 512 rows
+// over up to 8192 tokens, 12 heads, 54 to 67 us (25 GFLOP, up to 460 TFLOP/s); 512 rows over 32768 tokens
+// 48 us (540 TFLOP/s). A third buffer, four workgroups a CU (spills) and neighbouring tiles on one XCD
+// were no faster.
 //
 // fp32: the same walk with the products of x3.hpp (six bf16 products for an fp32 one), tiles loaded
-// into registers and split into three bf16 planes as they are stored, maxima in natural-log units.
+// into registers and split into three bf16 planes as they are stored, maxima in natural-log units. 8 prompts'
+// chunks as above over up to 4096 tokens: 136 us (12 GFLOP, 89 TFLOP/s of the 154 of a library product).
 #include "common.hpp"
 #include "decode.hpp"
 #include "lanes.hpp"
@@ -1257,22 +1266,21 @@ size_t paged_workspace_needed(const PagedStep& step, int elem) {
   return p.partials > 0 ? p.counters + p.partials + 16 : 0;
 }
 
-// The larger of what tiles and a few rows take, each of which grows with every argument.
+// The most counters and the most partials, of tiles or of a few rows, each of which grows with every argument:
+// counters lie at the front and partials at the end, so that a step's partials never reach another's counters,
+// which stay at zero between calls.
 size_t paged_workspace_bytes(const PagedStep& s) {
   const long long group = s.H / s.Hkv, max_len = (long long)s.max_pages * s.page;
   const long long tile_rows = std::min((s.max_rows * group + 31) / 32 * 32, (long long)kTile);
-  const long long tiled = slots_of(s) * s.Hkv * (sizeof(unsigned) + sizeof(float) * tile_rows * (s.D + 4));
-  long long few = 0;
+  long long counters = slots_of(s) * s.Hkv, floats = counters * tile_rows * (s.D + 4);
   if (group <= kMostMid) {
     const int keys = std::min({few_keys_of(2, s.D), few_keys_of(4, s.D), mid_keys_of(s.D)});
     const long long n_chunk = (max_len + keys - 1) / keys;
-    if (n_chunk > 1)
-      few = s.n_seq * s.Hkv * n_chunk *
-            (sizeof(unsigned) +
-             sizeof(float) * std::min<long long>(s.max_rows * group, kMostMid) * (s.D + 2));
+    const long long parts = n_chunk > 1 ? s.n_seq * s.Hkv * n_chunk : 0;
+    counters = std::max(counters, parts);
+    floats = std::max(floats, parts * std::min<long long>(s.max_rows * group, kMostMid) * (s.D + 2));
   }
-  const long long most = std::max(tiled, few);
-  return most > 0 ? most + 16 : 0;
+  return counters > 0 ? counters * sizeof(unsigned) + floats * sizeof(float) + 16 : 0;
 }
 
 hipError_t launch_paged_attention_bf16(bf16* out, long long ld_out, const bf16* q, long long ld_q,

@@ -76,6 +76,33 @@ def test_long_caches_split(gpu, dtype, Hkv, G, D, len_):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_workspace_of_prompts_and_tokens(gpu, dtype):
+    """One workspace for a step of prompts' chunks and a step of single tokens in turn, whose partials are
+    fewer and larger than those of the tokens: each gets the bits it gets with one of its own. The caches are
+    long; their pages are shared, as prefixes are."""
+    n, Hkv, D, page, max_pages = 64, 4, 64, 128, 128
+    gen = torch.Generator().manual_seed(9)
+    kp, vp = (torch.randn((24, Hkv, page, D), generator=gen).to(dtype).cuda() for _ in range(2))
+    table = torch.randint(0, 24, (n, max_pages), generator=gen).int().cuda()
+    lens = torch.randint(9000, page * max_pages, (n,), generator=gen).int().cuda()
+    q = torch.randn((n * 48, Hkv, D), generator=gen).to(dtype).cuda()
+    ws = P.paged_workspace(q, kp, table, 48)
+
+    def step(rows, ws):
+        start = (torch.arange(n + 1) * rows).int().cuda()
+        out = torch.empty_like(q[:n * rows])
+        P.paged_attention(out, q[:n * rows], kp, vp, table, start, lens, rows, 0.125,
+                          torch.zeros_like(ws) if ws is own else ws)
+        torch.cuda.synchronize()
+        return out
+    own = ws.clone()
+    assert P.paged_workspace(q[:n], kp, table, 1).numel() < ws.numel()
+    want = {rows: step(rows, own) for rows in (48, 1, 20)}
+    for rows in (48, 1, 20, 1, 48):
+        assert torch.equal(step(rows, ws), want[rows]), rows
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_chunk_equals_one_token_at_a_time(gpu, dtype):
     """A chunk's rows are the rows of its tokens alone, up to both forms' bounds."""
     st = S.Step([150, 70], [50, 70], 4, 2, 64, 32, dtype, seed=4)
