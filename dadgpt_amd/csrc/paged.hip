@@ -64,8 +64,8 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs
 
 template <typename T>
 hipError_t launch_append_t(T* k_pages, T* v_pages, T* q_out, long long ld_out, const T* q,
-                           long long ld_q, const T* k, const T* v, long long ld_kv, const PagedStep& p, const Rope& r,
-                           hipStream_t stream) {
+                           long long ld_q, const T* k, const T* v, long long ld_kv,
+                           const PagedStep& p, const Rope& r, hipStream_t stream) {
   AppendArgs<T> a{k_pages, v_pages, q_out, q, k, v, ld_out, ld_q, ld_kv, p, r, q ? p.H : 0};
   const int heads = a.heads_q + 2 * p.Hkv;
   auto run = [&](auto vec, auto inter) {
@@ -86,12 +86,14 @@ hipError_t launch_append_t(T* k_pages, T* v_pages, T* q_out, long long ld_out, c
 
 hipError_t launch_paged_append_bf16(bf16* k_pages, bf16* v_pages, bf16* q_out, long long ld_out,
                                     const bf16* q, long long ld_q, const bf16* k, const bf16* v,
-                                    long long ld_kv, const PagedStep& step, const Rope& rope, hipStream_t stream) {
+                                    long long ld_kv, const PagedStep& step, const Rope& rope,
+                                    hipStream_t stream) {
   return launch_append_t<bf16>(k_pages, v_pages, q_out, ld_out, q, ld_q, k, v, ld_kv, step, rope, stream);
 }
 hipError_t launch_paged_append_f32(float* k_pages, float* v_pages, float* q_out, long long ld_out,
                                    const float* q, long long ld_q, const float* k, const float* v,
-                                   long long ld_kv, const PagedStep& step, const Rope& rope, hipStream_t stream) {
+                                   long long ld_kv, const PagedStep& step, const Rope& rope,
+                                    hipStream_t stream) {
   return launch_append_t<float>(k_pages, v_pages, q_out, ld_out, q, ld_q, k, v, ld_kv, step, rope, stream);
 }
 

@@ -697,8 +697,8 @@ __device__ __forceinline__ Pick pick_in_wave(const Settings& s, const Weigher& w
 // Among the n candidates in sm.list, which hold every element that can stay; z: the weights' sum that
 // top-p goes by, 0 for that of the first k.
 template <typename T, int NP>
-__device__ __forceinline__ Pick pick_from_list(Row<T, NP>& row, const Settings& s, const Weigher& weigh, uint32_t hi, int n,
-                               u64 z) {
+__device__ __forceinline__ Pick pick_from_list(Row<T, NP>& row, const Settings& s,
+                                               const Weigher& weigh, uint32_t hi, int n, u64 z) {
   Shared& sm = row.sm;
   Elements<kPerThread> x = listed(sm, row.tid, n);
   uint32_t low = 0;
@@ -851,7 +851,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(
     }
     return;
   }
-  finish(n <= kList ? pick_from_list(row, s, weigh, hi, n, z) : pick_from_row(row, s, weigh, hi, per_k, per_p, at));
+  finish(n <= kList ? pick_from_list(row, s, weigh, hi, n, z)
+                    : pick_from_row(row, s, weigh, hi, per_k, per_p, at));
 }
 
 template <typename T>
