@@ -213,6 +213,85 @@ def test_many_sequences(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_many_sequences_in_chunks(gpu, dtype):
+    """More sequences than the lanes of a wave, some of whose caches are cut and some not."""
+    n = 100
+    counts = [0] * n
+    for s, c in ((0, 150), (1, 33), (62, 140), (63, 2), (64, 1), (65, 300), (98, 129), (99, 64)):
+        counts[s] = c
+    lens = [c + (0, 3000, 100, 5000)[s % 4] if c else 5 for s, c in enumerate(counts)]
+    st = S.Step(lens, counts, 2, 2, 32, 64, dtype, seed=13)
+    _check(st, _attend(st))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129])
+def test_rows_of_every_kernel(gpu, dtype, rows):
+    """The numbers of rows at which another kernel or another share of the waves takes over, over caches of
+    one and of several chunks; D alternates."""
+    D = 64 if rows % 2 else 32
+    for group in (1, rows) if rows < 64 else (1,):
+        count = rows // group
+        st = S.Step([count + 1400, count, count + 40], [count] * 3, group, 1, D, 16, dtype, seed=14)
+        _check(st, _attend(st))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_far_pages(gpu, dtype):
+    """Pages behind the element 2^32 of a cache: the bits of the same pages at its start, read and written."""
+    n_pages, Hkv, page, D = (1 << 32) // (8 * 128 * 64) + 24, 8, 128, 64
+    far = n_pages - 20
+    kp, vp = (torch.empty((n_pages, Hkv, page, D), dtype=dtype, device="cuda") for _ in range(2))
+    gen = torch.Generator().manual_seed(15)
+    for x in (kp, vp):
+        x[:20] = torch.randn((20, Hkv, page, D), generator=gen).to(dtype)
+    lens, freqs = [1200, 1100], R.rope_frequencies(64)
+    table = torch.arange(20).view(2, 10).int()
+    for rows in (1, 3, 40):  # of a KV head: the three kernels
+        counts = torch.tensor([0, rows, 2 * rows]).int().cuda()
+        new = torch.randn((2 * rows, 3 * Hkv, D), generator=gen).to(dtype).cuda()
+        outs = []
+        for start in (0, far):
+            if start:
+                kp[far:], vp[far:] = kp[:20], vp[:20]
+            at = (table + start).cuda()
+            q, k, v = new.clone().split(Hkv, 1)
+            length = torch.tensor(lens).int().cuda()
+            P.paged_append(kp, vp, q, q, k, v, at, counts, length, rows, freqs, False)
+            out = torch.empty((2 * rows, Hkv, D), dtype=dtype, device="cuda")
+            P.paged_attention(out, q, kp, vp, at, counts, length, rows, 0.125,
+                              P.paged_workspace(q, kp, at, rows))
+            outs.append(out)
+        torch.cuda.synchronize()
+        assert torch.equal(*outs), rows
+        assert torch.equal(kp[far:], kp[:20]) and torch.equal(vp[far:], vp[:20])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_graph_of_a_prompts_step_replays(gpu, dtype):
+    """The same graph for chunks that are cut and that are not, and for sequences that have none."""
+    st = S.Step([4000, 200, 90], [100, 60, 90], 2, 1, 64, 32, dtype, seed=16, max_pages=125)
+    q, kp, vp, table, starts, lens = (st.cuda(x) for x in ("q", "k_pages", "v_pages", "table", "starts",
+                                                           "lens"))
+    ws, out = P.paged_workspace(q, kp, table, 100), torch.zeros_like(q)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        P.paged_attention(out, q, kp, vp, table, starts, lens, 100, 0.125, ws)
+    for i, (now, rows) in enumerate((([4000, 200, 90], [100, 60, 90]), ([300, 200, 4000], [50, 100, 100]),
+                                     ([4000, 0, 1], [99, 0, 1]), ([4000, 200, 90], [100, 60, 90]))):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        starts.copy_(torch.tensor([0, rows[0], rows[0] + rows[1], sum(rows)], dtype=torch.int32))
+        table[:, 63:].copy_(table[:, :62])  # (a place for every token)
+        graph.replay()
+        got = out.clone()
+        want = torch.zeros_like(q)
+        P.paged_attention(want, q, kp, vp, table, starts, lens, 100, 0.125, ws)
+        torch.cuda.synchronize()
+        assert torch.equal(got[:sum(rows)], want[:sum(rows)]), i
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_graph_replays(gpu, dtype):
     """A captured step follows lengths, rows and pages in device memory."""
     st = S.Step([900, 40, 300], [1, 1, 1], 4, 2, 64, 16, dtype, seed=12, max_pages=64)
