@@ -3,9 +3,9 @@
 //
 // The filters all keep a head of the row's descending order. In turn: the largest logit; a histogram
 // below it of counts (top-k) or counts and weights (top-p), which gives the bucket where the running
-// sum crosses the target; the elements down to that bucket into LDS; and there the cuts and the draw,
-// each the search for the element at which a running sum (of ones or of weights, by logit or by index)
-// crosses its target. Up to 64 elements one wave adds up for each lane what lies above its own; more are
+// sum crosses the target; the indexes of the elements down to that bucket into LDS; and among those the
+// cuts and the draw, each the search for the element at which a running sum (of ones or of weights, by
+// logit or by index) crosses its target. Up to 64 elements one wave adds up for each lane what lies above its own; more are
 // searched by a finer histogram and the few elements of its bucket. Rows that keep more than 8192
 // elements search over the row itself, and the draw there, as that of a row without filters, goes by
 // the sums of the waves' stretches of the row.
@@ -23,10 +23,11 @@
 //
 // Bound by one CU's operations on a row: two or three an element and pass, about 20 for a weight, and
 // between passes by barriers and chains in LDS. The row (200 KB of fp32 for 50257 logits) comes from L2
-// after the first pass. 50257 logits, us: one row, top-k of 40, 19; 32 rows of all kinds 75; 512 rows of bf16
-// with top-p 204. 32 rows of one kind: no filter 25, top-k of 40 20, of 5000 40, top-p of 0.9 44 (spread of
+// after the first pass. 50257 logits, us: one row, top-k of 40, 18; 32 rows of all kinds 73; 512 rows of bf16
+// with top-p 153. 32 rows of one kind: no filter 25, top-k of 40 20, of 5000 40, top-p of 0.9 44 (spread of
 // 4) to 95 (of 0.5: 40000 tokens stay), and 320 with all logits equal.
 #include "common.hpp"
+#include "kernels.hpp"
 #include "lanes.hpp"
 #include "serving.hpp"
 
@@ -98,7 +99,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 }
 
 struct Shared {
-  u64 list[kList];                  // the candidates, as order_of
+  int list[kList];                  // the candidates' indexes
   u64 few[kFew], few_weight[kFew];  // a bucket's elements
   union {
     struct {
@@ -265,6 +266,13 @@ struct Row {
     }
   }
 
+  // The number (order_of) of a listed element.
+  __device__ __forceinline__ u64 number_of(int i) const {
+    Four<T> x;
+    x.set(0, row[i]);
+    return order_of(value(x, 0), i);
+  }
+
   // The largest of a value from each thread.
   __device__ __forceinline__ uint32_t largest(uint32_t x) {
     uint32_t* to = sm.wave_max[turn_max ^= 1];
@@ -428,7 +436,7 @@ struct Row {
       for (int e = 0; e < 4; ++e) {
         const uint32_t to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32),
                                                            __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], 0));
-        if ((in[e] >> lane & 1) != 0 && to < (uint32_t)kList) sm.list[to] = order_of(x[e], index(i, e));
+        if ((in[e] >> lane & 1) != 0 && to < (uint32_t)kList) sm.list[to] = index(i, e);
         at += __builtin_popcountll(in[e]);
       }
     });
@@ -561,13 +569,14 @@ struct Parts {
   }
 };
 
-// Elements of sm.list, kPerThread of them with every thread, each of weight 1.
-__device__ __forceinline__ Elements<kPerThread> listed(const Shared& sm, int tid, int n) {
+// The listed elements, kPerThread of them with every thread, each of weight 1.
+template <typename T, int NP>
+__device__ __forceinline__ Elements<kPerThread> listed(const Row<T, NP>& row, int n) {
   Elements<kPerThread> x;
 #pragma unroll
   for (int j = 0; j < kPerThread; ++j) {
-    const int i = tid + j * kThreads;
-    x.number[j] = i < n ? sm.list[i] : 0;
+    const int i = row.tid + j * kThreads;
+    x.number[j] = i < n ? row.number_of(row.sm.list[i]) : 0;
     x.weight[j] = i < n ? 1 : 0;
   }
   return x;
@@ -599,7 +608,7 @@ __device__ __forceinline__ Pick pick_from_row(Row<T, NP>& row, const Settings& s
       const int n =
           row.template collect<true>([&](float x) { return bucket_of(x) == at.bucket; });
       if (n > kList) return 0;
-      Elements<kPerThread> x = listed(row.sm, row.tid, n);
+      Elements<kPerThread> x = listed(row, n);
       uint32_t low = 0;
 #pragma unroll
       for (int j = 0; j < kPerThread; ++j)
@@ -700,7 +709,7 @@ template <typename T, int NP>
 __device__ __forceinline__ Pick pick_from_list(Row<T, NP>& row, const Settings& s,
                                                const Weigher& weigh, uint32_t hi, int n, u64 z) {
   Shared& sm = row.sm;
-  Elements<kPerThread> x = listed(sm, row.tid, n);
+  Elements<kPerThread> x = listed(row, n);
   uint32_t low = 0;
 #pragma unroll
   for (int j = 0; j < kPerThread; ++j)
@@ -741,7 +750,7 @@ __device__ __forceinline__ Pick pick_from_list(Row<T, NP>& row, const Settings& 
 }
 
 template <typename T, int NP>
-__global__ __launch_bounds__(kThreads) void sample_kernel(
+__global__ __launch_bounds__(kThreads, NP == 0 ? 4 : 2) void sample_kernel(
     int* __restrict__ tokens, float* __restrict__ probs, const T* __restrict__ logits, long long ld,
     int vocab, const SampleSettings set) {
   __shared__ Shared sm;
@@ -846,7 +855,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(
   }
   if (n <= 64) {
     if (row.wave == 0) {
-      const u64 number = row.lane < n ? sm.list[row.lane] : 0;
+      const u64 number = row.lane < n ? row.number_of(sm.list[row.lane]) : 0;
       finish(pick_in_wave(s, weigh, number, n, z, row.lane));
     }
     return;
@@ -862,8 +871,11 @@ hipError_t launch_sample_t(int* tokens, float* probs, const T* logits, long long
     sample_kernel<T, np()><<<rows, kThreads, 0, stream>>>(tokens, probs, logits, ld, vocab, set);
     return hipGetLastError();
   };
-  // pieces of 256 elements for each of the 8 waves; up to 25 of them stay in registers (100 for fp32)
+  // Pieces of 256 elements for each of the 8 waves; up to 25 of them stay in registers (100 for fp32).
+  // With more rows than CUs, two workgroups on a CU, in 128 registers each and with the row from L2, hide
+  // more than that saves (512 rows of 50257 in bf16: 153 us, 203 with the rows in registers).
   const int pieces = (vocab + 3 + 256 * kWaves - 1) / (256 * kWaves);
+  if (rows > (device_cus() > 0 ? device_cus() : 256)) return run(std::integral_constant<int, 0>{});
   if (pieces <= 8) return run(std::integral_constant<int, 8>{});
   if (pieces <= 25) return run(std::integral_constant<int, 25>{});
   return run(std::integral_constant<int, 0>{});

@@ -66,6 +66,17 @@ def test_settings(gpu, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("vocab", [7, 1000, 9001])
+def test_more_rows_than_cus(gpu, vocab, dtype):
+    rows = 320
+    x, u = _logits(rows, vocab, 100 + vocab, dtype), _uniforms(rows, vocab + 2)
+    pick = [((0.6, 1.0, 1.9)[r % 3], *((0, 1.0, 0.0), (1, 1.0, 0.0), (40, 1.0, 0.0), (0, 0.9, 0.0),
+                                       (0, 1.0, 0.05), (200, 0.8, 0.01), (0, 0.999, 0.0))[r % 7])
+            for r in range(rows)]
+    _check(x, u, *(list(z) for z in zip(*pick)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_defaults_and_draws(gpu, dtype):
     """No settings; the draw follows the probabilities (4096 draws of one row: each of the likeliest
     tokens within five standard deviations)."""
