@@ -11,7 +11,7 @@
 // matrix tiles, and the tiles below. The first two are bound by HBM and by the chain row_start, lens ->
 // page -> keys -> merge, and have all of a workgroup's loads in flight at once: 32 sequences of 1 to 1024
 // tokens, 12 heads of 64 in bf16, 14 us (50 MB, 3.6 TB/s), 8 of 1 to 32768 with three rows for each of 4 KV
-// heads 34 to 40 us (134 MB, 3.4 to 3.9 TB/s).
+// heads 34 to 43 us (134 MB, 3.1 to 3.9 TB/s).
 //
 // Tiles (bf16). The keys are walked in tiles of 64. A tile is four groups of 16 tokens, each within a page
 // (a page holds 16 at least): a wave stages one group of K and V by direct global -> LDS loads from
