@@ -441,7 +441,9 @@ struct Row {
       }
     });
     __syncthreads();
-    return (int)sm.listed;
+    const int n = (int)sm.listed;
+    __syncthreads();  // (the next collect or search begins by setting it to 0)
+    return n;
   }
 
   // The element at which the sum of weights, taken in descending order of the elements' numbers, reaches

@@ -215,3 +215,23 @@ def test_no_probabilities_and_graph(gpu):
         assert torch.equal(got, tokens)
         x.add_(torch.randn(x.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(i)))
         u.copy_(torch.tensor(_uniforms(8, 20 + i)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [16, 320])
+def test_a_bucket_that_top_k_leaves_a_part_of(gpu, rows, dtype):
+    """top-p ends in a bucket of which top-k left fewer elements than the candidate list holds and which has
+    many more: the list is given up for the row itself. Every call and every row of equal settings answers the
+    same."""
+    x = torch.full((rows, 50257), 2.5)
+    x[1::2, :300] = 3.0
+    x, p = x.to(dtype), [0.50007] * rows
+    u, k = [0.03, 0.37, 0.71, 0.96] * (rows // 4), [5000, 8000, 8000, 5000] * (rows // 4)
+    if rows == 16:
+        _check(x, u, None, k, p)
+    x = x[:4].repeat(rows // 4, 1).cuda()
+    first = _sample(x, u, None, k, p)
+    for got in first:
+        assert got == got[:4] * (rows // 4)
+    for _ in range(3):
+        assert _sample(x, u, None, k, p) == first
