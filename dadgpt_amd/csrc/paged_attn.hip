@@ -1035,6 +1035,26 @@ struct PageTile {
   __device__ __forceinline__ f32x4 piece(int i) const { return r[i]; }
 };
 
+// The three planes of a product of x3.hpp leave NaN of an infinity (inf - inf in the split, or cross terms of
+// unlike signs): what the first planes' product makes infinite is infinite, and counts as that. (An element
+// that rounds to an infinity in bf16, above 3.39e38, is taken for one.)
+template <int D>
+__device__ __forceinline__ void infinite_scores(f32x16& s, const bf16* planes, int row0,
+                                                const X3 (&q)[D / 16], int lane) {
+  bool odd = false;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) odd = odd || !(fabsf(s[x]) < __builtin_inff());
+  if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
+  const int krow = row0 + sigma32(lane & 31), hi = lane >> 5;
+  f32x16 first = zero16();
+#pragma unroll
+  for (int ds = 0; ds < D / 16; ++ds)
+    first = mfma32(lds_op(planes, rm_off<D>(krow, 2 * ds + hi)), q[ds].v[0], first);
+#pragma unroll
+  for (int x = 0; x < 16; ++x)
+    if (fabsf(first[x]) == __builtin_inff()) s[x] = first[x];
+}
+
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<float> a) {
   constexpr int DB = D / 32, kPlane = 3 * kTileRows * D, kPitch = D + 4;
@@ -1091,9 +1111,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<f
       f32x16 s = score_tile_p<D, kTileRows>(planes, 32 * i, q, lane);
       float sum;
       f32x16 p;
-      auto weights = [&]() {
+      auto weights = [&](float base, auto infinite) {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) p[x] = exp_acc(fmaf(s[x], a.scale, -m));
+        for (int x = 0; x < 16; ++x) {
+          const float y = fmaf(s[x], a.scale, -base);
+          p[x] = exp_acc(y);
+          if constexpr (infinite()) p[x] = y == neg_inf() ? 0.f : p[x];
+        }
         if (partly) {
 #pragma unroll
           for (int x = 0; x < 16; ++x)
@@ -1103,22 +1127,25 @@ __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<f
 #pragma unroll
         for (int x = 1; x < 16; ++x) sum += p[x];
       };
-      weights();
-      // as in the bf16 kernel; a row that needs it sees a key of these
+      weights(m, std::false_type{});
+      // as in the bf16 kernel; a row that needs it sees a key of these. (A score of -inf makes the sum NaN
+      // here: exp_acc wants finite numbers.)
       const bool need = __float_as_uint(sum) >= __float_as_uint(kMaxW);
       if (__builtin_amdgcn_ballot_w64(need) != 0) {
+        infinite_scores<D>(s, planes, 32 * i, q, lane);
         float mx = neg_inf();
 #pragma unroll
         for (int x = 0; x < 16; ++x)
           if (!(partly && hidden(x))) mx = fmaxf(mx, s[x] * a.scale);
         mx = max_halves(mx);
         const float mn = or_halves(need) ? fmaxf(m, mx) : m;
-        const float f = m == neg_inf() ? 0.f : exp_acc(m - mn);
+        const float base = mn == neg_inf() ? 0.f : mn;  // no key seen yet weighs anything
+        const float f = weight_of<false>(m - base);
         m = mn;
         l *= f;
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[db] *= f;
-        weights();
+        weights(base, std::true_type{});
       }
       l += sum;
       accumulate_t_p<D, kTileRows>(o, planes + kPlane, 32 * i, p, lane);

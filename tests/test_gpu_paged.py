@@ -399,3 +399,39 @@ def test_append_in_place_query(gpu):
                    st.cuda("starts"), st.cuda("lens"), 20, freqs)
     assert torch.equal(x[:, :4], qo) and torch.equal(kp2, kp) and torch.equal(vp2, vp)
     assert torch.equal(x[:, 4:], torch.cat((st.k, st.v), 1).cuda())
+
+
+def _without(st, skip):
+    """The same step, without the tokens 0 .. skip[s] - 1 (whole pages) of sequence s."""
+    less = S.Step(st.lens, st.counts, st.H, st.Hkv, st.D, st.page, st.dtype, seed=0)
+    less.q, less.k_pages, less.v_pages, less.n_pages = st.q, st.k_pages, st.v_pages, st.n_pages
+    less.table = st.table.clone()
+    for s, n in enumerate(skip):
+        less.table[s, :n // st.page] = -1
+    return less
+
+
+# rows of a KV head: the kernels of a few rows, of up to 32, and the tiles, whose waves share 32 rows by four
+# and by two
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [1, 4, 5, 20, 40])
+@pytest.mark.parametrize("how", ["infinite", "overflow", "far overflow"])
+def test_scores_of_minus_infinity(gpu, dtype, rows, how):
+    """Keys that score -inf (an infinite element, or finite ones whose product overflows) weigh nothing,
+    wherever the first of them are; a row that has no other key gets zeros. The scores of a far overflow differ
+    by enough that parts of a product overflow to either side."""
+    st = S.Step([900, 192 + rows, 130], [rows, rows, 1], 2, 2, 64, 64, dtype, seed=30)
+    skip = [704, 128, 192]  # of 900 (into the second chunk), of some, of all of the third's 130
+    big = {"infinite": (1.0, -math.inf), "overflow": (2.0 ** 70, -1.234 * 2.0 ** 70),
+           "far overflow": (1.377 * 2.0 ** 100, -1.234 * 2.0 ** 100)}[how]
+    st.q[:, :, 5] = big[0]
+    st.k_pages[..., 5] = 0.0  # (of what is seen: the large element of q must not matter)
+    for s, n in enumerate(skip):
+        for j in range(min(n, st.lens[s])):
+            page, slot = st.place(s, j)
+            st.k_pages[page, :, slot, 5] = big[1]
+    out = _attend(st)
+    assert (out[-1] == 0).all()
+    want, bound = _without(st, skip).attention(1.0 / 8)
+    got = out.cpu().double()[:-1]
+    assert ((got - want[:-1]).abs() <= bound[:-1]).all()
