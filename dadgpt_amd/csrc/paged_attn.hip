@@ -1055,6 +1055,41 @@ __device__ __forceinline__ void infinite_scores(f32x16& s, const bf16* planes, i
     if (fabsf(first[x]) == __builtin_inff()) s[x] = first[x];
 }
 
+// accumulate_t_p, with such values in the product of the first planes alone.
+template <int D>
+__device__ __forceinline__ void accumulate_infinite(f32x16 (&acc)[D / 32], const bf16* planes, int row0,
+                                                    const f32x16& p, int lane) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p[8 * j + e];
+    const X3 pb = split3(x);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      u32x4 a[3];
+#pragma unroll
+      for (int pl = 0; pl < 3; ++pl)
+        a[pl] = as_u32x4(lds_tr_op<D>(planes + pl * kTileRows * D, row0 + 16 * j, 32 * db, lane));
+      const bf16x8 all = as_bf16x8(a[0]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = (a[0][e] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
+        const uint32_t hi = (a[0][e] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
+#pragma unroll
+        for (int pl = 0; pl < 3; ++pl) a[pl][e] &= ~(lo | hi);
+      }
+      const X3 v{{as_bf16x8(a[0]), as_bf16x8(a[1]), as_bf16x8(a[2])}};
+      acc[db] = mfma32(v.v[1], pb.v[1], acc[db]);  // (in mfma_x6's order)
+      acc[db] = mfma32(v.v[2], pb.v[0], acc[db]);
+      acc[db] = mfma32(v.v[0], pb.v[2], acc[db]);
+      acc[db] = mfma32(v.v[1], pb.v[0], acc[db]);
+      acc[db] = mfma32(v.v[0], pb.v[1], acc[db]);
+      acc[db] = mfma32(all, pb.v[0], acc[db]);
+    }
+  }
+}
+
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<float> a) {
   constexpr int DB = D / 32, kPlane = 3 * kTileRows * D, kPitch = D + 4;
@@ -1078,83 +1113,102 @@ __global__ __launch_bounds__(kThreads, 2) void paged_f32_kernel(const TileArgs<f
   float &m = x.m, &l = x.l;
 
   const int head = w.head, n_tiles = w.key1 > w.key0 ? (w.key1 - w.key0 + 63) / 64 : 0;
-  Pages now{}, next{};
-  PageTile<D> tk, tv;
-  if (n_tiles > 0) {
-    now = pages_at(a, w, w.key0);
-    tk.load(a, a.k_pages, now, head, w.key0, w.key1);
-    tv.load(a, a.v_pages, now, head, w.key0, w.key1);
-    if (n_tiles > 1) next = pages_at(a, w, w.key0 + 64);
-  }
-  for (int t = 0; t < n_tiles; ++t) {
-    const int k0 = w.key0 + 64 * t;
-    __syncthreads();  // the last tile's reads are done
-    store_x3<D, kTileRows>(tk, planes);
-    store_x3<D, kTileRows>(tv, planes + kPlane);
-    Pages after_next = next;
-    if (t + 1 < n_tiles) {
-      tk.load(a, a.k_pages, next, head, k0 + 64, w.key1);
-      tv.load(a, a.v_pages, next, head, k0 + 64, w.key1);
-      if (t + 2 < n_tiles) after_next = pages_at(a, w, k0 + 128);
+  // The walk over the tiles. INFINITE: for scores and values that are infinite, which become NaN otherwise.
+  auto walk = [&](auto infinite) {
+    Pages now{}, next{};
+    PageTile<D> tk, tv;
+    if (n_tiles > 0) {
+      now = pages_at(a, w, w.key0);
+      tk.load(a, a.k_pages, now, head, w.key0, w.key1);
+      tv.load(a, a.v_pages, now, head, w.key0, w.key1);
+      if (n_tiles > 1) next = pages_at(a, w, w.key0 + 64);
     }
-    __syncthreads();
+    for (int t = 0; t < n_tiles; ++t) {
+      const int k0 = w.key0 + 64 * t;
+      __syncthreads();  // the last tile's reads are done
+      store_x3<D, kTileRows>(tk, planes);
+      store_x3<D, kTileRows>(tv, planes + kPlane);
+      Pages after_next = next;
+      if (t + 1 < n_tiles) {
+        tk.load(a, a.k_pages, next, head, k0 + 64, w.key1);
+        tv.load(a, a.v_pages, next, head, k0 + 64, w.key1);
+        if (t + 2 < n_tiles) after_next = pages_at(a, w, k0 + 128);
+      }
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c0 = k0 + 32 * i;
-      if (!r.active || ((2 * t + i) & (r.ks - 1)) != r.sub || c0 > r.some_see || c0 >= w.key1)
-        continue;
-      const bool bad0 = !paged::is_page(a.p, now.id[2 * i]);
-      const bool bad1 = !paged::is_page(a.p, now.id[2 * i + 1]);
-      const bool partly = c0 + 31 > r.all_see || bad0 || bad1;
-      const int last = r.after - c0 - 8 * hi;
-      auto hidden = [&](int x) { return reg_row(x, 0) > last || (x < 8 ? bad0 : bad1); };
-      f32x16 s = score_tile_p<D, kTileRows>(planes, 32 * i, q, lane);
-      float sum;
-      f32x16 p;
-      auto weights = [&](float base, auto infinite) {
+      for (int i = 0; i < 2; ++i) {
+        const int c0 = k0 + 32 * i;
+        if (!r.active || ((2 * t + i) & (r.ks - 1)) != r.sub || c0 > r.some_see || c0 >= w.key1)
+          continue;
+        const bool bad0 = !paged::is_page(a.p, now.id[2 * i]);
+        const bool bad1 = !paged::is_page(a.p, now.id[2 * i + 1]);
+        const bool partly = c0 + 31 > r.all_see || bad0 || bad1;
+        const int last = r.after - c0 - 8 * hi;
+        auto hidden = [&](int x) { return reg_row(x, 0) > last || (x < 8 ? bad0 : bad1); };
+        f32x16 s = score_tile_p<D, kTileRows>(planes, 32 * i, q, lane);
+        if constexpr (infinite()) infinite_scores<D>(s, planes, 32 * i, q, lane);
+        float sum;
+        f32x16 p;
+        auto weights = [&](float base) {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const float y = fmaf(s[x], a.scale, -base);
-          p[x] = exp_acc(y);
-          if constexpr (infinite()) p[x] = y == neg_inf() ? 0.f : p[x];
-        }
-        if (partly) {
+          for (int x = 0; x < 16; ++x) {
+            const float y = fmaf(s[x], a.scale, -base);
+            p[x] = exp_acc(y);
+            if constexpr (infinite()) p[x] = y == neg_inf() ? 0.f : p[x];  // (exp_acc's is NaN)
+          }
+          if (partly) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+              if (hidden(x)) p[x] = 0.f;
+          }
+          sum = p[0];
+#pragma unroll
+          for (int x = 1; x < 16; ++x) sum += p[x];
+        };
+        weights(m);
+        // as in the bf16 kernel; a row that needs it sees a key of these
+        const bool need = __float_as_uint(sum) >= __float_as_uint(kMaxW);
+        if (__builtin_amdgcn_ballot_w64(need) != 0) {
+          float mx = neg_inf();
 #pragma unroll
           for (int x = 0; x < 16; ++x)
-            if (hidden(x)) p[x] = 0.f;
+            if (!(partly && hidden(x))) mx = fmaxf(mx, s[x] * a.scale);
+          mx = max_halves(mx);
+          const float mn = or_halves(need) ? fmaxf(m, mx) : m;
+          const float base = mn == neg_inf() ? 0.f : mn;  // no key seen yet weighs anything
+          const float f = weight_of<false>(m - base);
+          m = mn;
+          l *= f;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db] *= f;
+          weights(base);
         }
-        sum = p[0];
-#pragma unroll
-        for (int x = 1; x < 16; ++x) sum += p[x];
-      };
-      weights(m, std::false_type{});
-      // as in the bf16 kernel; a row that needs it sees a key of these. (A score of -inf makes the sum NaN
-      // here: exp_acc wants finite numbers.)
-      const bool need = __float_as_uint(sum) >= __float_as_uint(kMaxW);
-      if (__builtin_amdgcn_ballot_w64(need) != 0) {
-        infinite_scores<D>(s, planes, 32 * i, q, lane);
-        float mx = neg_inf();
-#pragma unroll
-        for (int x = 0; x < 16; ++x)
-          if (!(partly && hidden(x))) mx = fmaxf(mx, s[x] * a.scale);
-        mx = max_halves(mx);
-        const float mn = or_halves(need) ? fmaxf(m, mx) : m;
-        const float base = mn == neg_inf() ? 0.f : mn;  // no key seen yet weighs anything
-        const float f = weight_of<false>(m - base);
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] *= f;
-        weights(base, std::true_type{});
+        l += sum;
+        if constexpr (infinite())
+          accumulate_infinite<D>(o, planes + kPlane, 32 * i, p, lane);
+        else
+          accumulate_t_p<D, kTileRows>(o, planes + kPlane, 32 * i, p, lane);
       }
-      l += sum;
-      accumulate_t_p<D, kTileRows>(o, planes + kPlane, 32 * i, p, lane);
+      now = next;
+      next = after_next;
     }
-    now = next;
-    next = after_next;
+    __syncthreads();  // the tiles are read
+  };
+  if (tid == 0) flag = 0;
+  walk(std::false_type{});
+  // (a NaN in a sum stays, so that one look at the end is enough, and costs no tile anything)
+  bool nan = !(l == l);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) nan = nan || !(o[db][i] == o[db][i]);
+  if (nan) flag = 1;
+  __syncthreads();
+  if (__builtin_amdgcn_readfirstlane(flag) != 0) {
+    x = Running<D>();
+    walk(std::true_type{});
   }
   l = sum_halves(l);
-  __syncthreads();  // the tiles are read: partials and output rows go there
   join_waves<float, D>(r, o, m, l, planes, sm_ml, lane);
   if (w.chunks > 1 &&
       !merge_chunks<float, D>(a, w, r, x, planes, sm_ml, &flag, lane))

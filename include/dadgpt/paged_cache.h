@@ -61,9 +61,9 @@ int dadgpt_paged_append_f32(float* k_pages, float* v_pages, float* q_out, int64_
 /* out = softmax(scale q k^T) v for every new row, over its sequence's tokens up to and with its own.
  * Row r of q (out) holds n_heads * d_head elements from r * ld_q (ld_out) on; out may be q (ld_out =
  * ld_q). A row none of whose keys weighs anything (it lies before token 0, all its pages are missing,
- * all its scores are -inf) gets zeros. A NaN key or value makes the rows that see it NaN; values
- * that a row does not see, but that another row of the step sees, may reach it as 0 * v: a NaN or infinity
- * there can make it NaN too.
+ * all its scores are -inf) gets zeros. A NaN key or value makes the rows that see it NaN, an infinite value
+ * its column infinite; values that a row does not see, but that another row of the step sees, may reach it as
+ * 0 * v: a NaN or infinity there can make it NaN too. (fp32 elements above 3.39e38 may count as infinite.)
  * The workspace is as the decode calls': dadgpt_paged_workspace_bytes (0: NULL allowed) of this shape, or
  * of one with larger n_seq, rows, max_rows or max_pages, ZERO-FILLED once, 16-byte aligned, and passed
  * whole; every call leaves its counters at zero. Calls that share one must not overlap in time. */

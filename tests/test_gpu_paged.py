@@ -435,3 +435,24 @@ def test_scores_of_minus_infinity(gpu, dtype, rows, how):
     want, bound = _without(st, skip).attention(1.0 / 8)
     got = out.cpu().double()[:-1]
     assert ((got - want[:-1]).abs() <= bound[:-1]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [1, 4, 5, 20, 40])
+def test_infinite_values(gpu, dtype, rows):
+    """An infinite value makes its column of the rows that see it infinite, two of unlike signs or a NaN make it
+    NaN; other columns are what they were."""
+    st = S.Step([700 + rows, 60 + rows], [rows, rows], 2, 1, 64, 16, dtype, seed=31)
+    before = _attend(st).cpu()
+    for s, j, col, x in ((0, 3, 7, math.inf), (0, 600, 40, -math.inf), (0, 5, 41, math.inf),
+                         (0, 650, 41, -math.inf), (0, 9, 42, math.nan), (1, 50, 0, -math.inf)):
+        page, slot = st.place(s, j)
+        st.v_pages[page, :, slot, col] = x
+    got = _attend(st).cpu()
+    a, b = got[:rows], got[rows:]
+    assert (a[..., 7] == math.inf).all() and (a[..., 40] == -math.inf).all()
+    assert torch.isnan(a[..., 41:43]).all() and (b[..., 0] == -math.inf).all()
+    left = [c for c in range(64) if c not in (7, 40, 41, 42)]
+    want, bound = st.attention(1.0 / 8)
+    assert torch.equal(b[..., 1:], before[rows:, :, 1:])
+    assert ((a.double() - want[:rows]).abs() <= bound[:rows])[..., left].all()
