@@ -295,8 +295,9 @@ int append(const char* fn, T* k_pages, T* v_pages, T* q_out, int64_t ld_out, con
     if (int st = check_step_apart(fn, s, c)) return st;
   }
   if (q_out != nullptr) {
+    const bool in_place = q_out == q && ld_out == ld_q;
     for (const View& x : in)
-      if (!(x.p == q && q_out == q && ld_out == ld_q) && meet(QO, x)) return overlaps(fn, "q_out", x.name);
+      if (!(in_place && &x == &in[0]) && meet(QO, x)) return overlaps(fn, "q_out", x.name);
     if (flat_meets(f, QO)) return overlaps(fn, "q_out", "freqs");
     if (int st = check_step_apart(fn, s, QO)) return st;
   }

@@ -178,6 +178,17 @@ def test_append_refusals(name):
 
 
 @pytest.mark.parametrize("name", ["bf16", "f32"])
+def test_append_in_place_is_of_q_alone(name):
+    """q_out may be q; where k or v begin at the same address, the call would overwrite what it reads."""
+    fn = getattr(P.lib(), "dadgpt_paged_append_" + name)
+    for k, v, what in ((_at(3), _at(2), "k"), (_at(2), _at(3), "v"), (_at(3), _at(3), "k")):
+        for H, heads in ((4, 4), (2, 2)):
+            status = fn(_at(0), _at(1), _at(3), heads * 64, _at(3), heads * 64, k, v, 256, _at(4), _at(5),
+                        _at(6), *_step(dict(H=H)), _at(7), 64, 0, 1.0, None)
+            assert status == 1 and "q_out overlaps " + what in A.last_error()
+
+
+@pytest.mark.parametrize("name", ["bf16", "f32"])
 def test_attention_refusals(name):
     fn, size = getattr(P.lib(), "dadgpt_paged_attention_" + name), 2 if name == "bf16" else 4
 
