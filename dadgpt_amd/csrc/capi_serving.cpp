@@ -318,13 +318,11 @@ int attend(const char* fn, T* out, int64_t ld_out, const T* q, int64_t ld_q, con
   if (int st = check_pitch(fn, "ld_q", ld_q, wq)) return st;
   if (!std::isfinite(scale))
     return fail(DADGPT_ERR_INVALID_ARGUMENT, "%s: scale must be finite", fn);
-  // tiles of 128 rows along grid.y, each sequence with one of its own that is not full, and up to 2049 places
-  // for what is cut
-  if (s.n_seq + (long long)s.rows * (s.H / s.Hkv) / 128 > 65535 - 2049)
+  const int elem = sizeof(T);
+  if (!dadgpt::paged_fits(s, elem))
     return fail(DADGPT_ERR_INVALID_ARGUMENT,
                 "%s: n_seq=%d and rows=%d x %d query heads to a KV head exceed the launch limits", fn,
                 s.n_seq, s.rows, s.H / s.Hkv);
-  const int elem = sizeof(T);
   const View O = token_rows(out, "out", s.rows, ld_out, wq, elem);
   const View Q = token_rows(q, "q", s.rows, ld_q, wq, elem);
   const View K = flat(k_pages, cache_bytes(s, elem), "k_pages");

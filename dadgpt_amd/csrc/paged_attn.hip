@@ -1342,6 +1342,10 @@ void launch_rows(const TileArgs<T>& a, dim3 grid, hipStream_t stream) {
 
 }  // namespace
 
+bool paged_fits(const PagedStep& step, int elem) {
+  return path_of(step, elem) != kTiles || places_of(step) <= 65535;  // (of n_seq: the caller's check)
+}
+
 size_t paged_workspace_needed(const PagedStep& step, int elem) {
   const Plan p = plan_of(step, elem);
   return p.partials > 0 ? p.counters + p.partials + 16 : 0;

@@ -46,6 +46,8 @@ hipError_t launch_paged_append_f32(float* k_pages, float* v_pages, float* q_out,
                                    const float* q, long long ld_q, const float* k, const float* v,
                                    long long ld_kv, const PagedStep& step, const Rope& rope, hipStream_t stream);
 
+// Whether the step's grid is within the launch limits.
+bool paged_fits(const PagedStep& step, int elem_bytes);
 // Bytes that this step's launch uses, and those that serve it and every step with no larger n_seq, rows,
 // max_rows and max_pages.
 size_t paged_workspace_needed(const PagedStep& step, int elem_bytes);

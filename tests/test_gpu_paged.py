@@ -456,3 +456,35 @@ def test_infinite_values(gpu, dtype, rows):
     want, bound = st.attention(1.0 / 8)
     assert torch.equal(b[..., 1:], before[rows:, :, 1:])
     assert ((a.double() - want[:rows]).abs() <= bound[:rows])[..., left].all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [65535, (65535 - 769 - 60000) * 128])
+def test_largest_grids(gpu, dtype, rows):
+    """A token of each of 65535 sequences, and as many tiles as a grid has room for, over shared pages: some of
+    the first, last and other sequences against the same sequence in a step of its own."""
+    gen = torch.Generator().manual_seed(32)
+    n, page, D, max_pages = (65535 if rows == 65535 else 60000), 16, 32, 64
+    kp, vp = (torch.randn((90, 2, page, D), generator=gen).to(dtype).cuda() for _ in range(2))
+    table = torch.randint(0, 90, (n, max_pages), generator=gen).int().cuda()
+    counts = torch.ones(n, dtype=torch.long)
+    more = rows - n
+    at = torch.randperm(n - 1, generator=gen)[:more // 999]
+    counts[at] += 999
+    counts[-1] += more - 999 * len(at)  # (the last one too)
+    assert int(counts.sum()) == rows and int(counts.max()) <= 1000
+    lens = torch.minimum(counts + torch.randint(0, 1000, (n,), generator=gen), torch.tensor(1024))
+    starts = torch.cat((torch.zeros(1, dtype=torch.long), counts.cumsum(0)))
+    q = torch.randn((rows, 2, D), generator=gen).to(dtype).cuda()
+    out, most = torch.full_like(q, 7.0), int(counts.max())
+    P.paged_attention(out, q, kp, vp, table, starts.int().cuda(), lens.int().cuda(), most, 0.25,
+                      P.paged_workspace(q, kp, table, most))
+    torch.cuda.synchronize()
+    for s in [0, 1, n // 2, n - 2, n - 1, *(at[:3].tolist())]:
+        a, b = int(starts[s]), int(starts[s + 1])
+        st = S.Step([int(lens[s])], [b - a], 2, 2, D, page, dtype, seed=0)
+        st.q, st.k_pages, st.v_pages, st.n_pages = q[a:b].cpu(), kp.cpu(), vp.cpu(), 90
+        st.table, st.max_pages = table[s:s + 1].cpu(), max_pages
+        some = torch.arange(0, b - a, max(1, (b - a) // 20))
+        want, bound = st.attention(0.25)
+        assert ((out[a:b].cpu().double() - want).abs() <= bound)[some].all(), s

@@ -223,6 +223,26 @@ def test_attention_refusals(name):
         _refused(call, (1, "the workspace overlaps " + what), ws=_at(x), **split)
 
 
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+def test_the_largest_steps(name):
+    """Steps are refused for their grid from its limit on, 65535 workgroups of a KV head, not before: a token
+    of each of 65535 sequences, and tiles of 128 rows (with up to 2 * 768 / n_kv_heads + 1 places for chunks)."""
+    fn = getattr(P.lib(), "dadgpt_paged_attention_" + name)
+
+    def call(n_seq, rows, max_rows):
+        step = dict(n_seq=n_seq, H=2, Hkv=2, rows=rows, max_rows=max_rows, n_pages=9, page=16, max_pages=512,
+                    D=64)
+        status = fn(_at(0), 128, _at(100), 128, _at(200), _at(300), _at(400), _at(500), _at(600),
+                    *step.values(), 0.125, None, 0, None)
+        return status, A.last_error()
+    for n_seq, rows, max_rows in ((65535, 65535, 1), (60000, (65535 - 769 - 60000) * 128, 1000),
+                                  (1, 65535 * 128 - 769 * 128, 65535 * 128 - 769 * 128)):
+        status, text = call(n_seq, rows, max_rows)
+        assert status == 4 and "workspace" in text, text
+    status, text = call(60000, (65535 - 769 - 60000 + 1) * 128, 1000)
+    assert status == 1 and "launch limits" in text
+
+
 def _workspace(kw):
     s = {**STEPS, **kw}
     return [s[k] for k in ("n_seq", "H", "Hkv", "rows", "max_rows", "page", "max_pages", "D")]
