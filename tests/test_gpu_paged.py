@@ -488,3 +488,24 @@ def test_largest_grids(gpu, dtype, rows):
         some = torch.arange(0, b - a, max(1, (b - a) // 20))
         want, bound = st.attention(0.25)
         assert ((out[a:b].cpu().double() - want).abs() <= bound)[some].all(), s
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("shape", [([9000, 3000, 8500], [1, 1, 1], 4, 4), ([9000, 700, 4000], [2, 1, 0], 2, 1),
+                                   ([9000, 8000], [8, 3], 2, 2), ([9000, 200], [300, 200], 2, 2)],
+                         ids=["one row", "four rows", "eight rows", "tiles"])
+def test_all_counters_return_to_zero(gpu, dtype, shape):
+    """Counters lie in front and partials against the end: in a workspace of twice the size everything in the
+    front half is zero after a call."""
+    lens, counts, H, Hkv = shape
+    st = S.Step(lens, counts, H, Hkv, 64, 128, dtype, seed=33)
+    q, kp, table = st.cuda("q"), st.cuda("k_pages"), st.cuda("table")
+    size = P.paged_workspace(q, kp, table, max(counts)).numel()
+    ws = torch.zeros(2 * size, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, 7.0)
+    for _ in range(2):
+        P.paged_attention(out, q, kp, st.cuda("v_pages"), table, st.cuda("starts"), st.cuda("lens"),
+                          max(counts), 0.125, ws)
+        torch.cuda.synchronize()
+        assert int(ws[:size].max()) == 0 and int(ws[size:].max()) > 0
+    _check(st, out)
