@@ -828,8 +828,10 @@ __global__ __launch_bounds__(kThreads, NP == 0 ? 4 : 2) void sample_kernel(
     per_k = (float)(kLevels - 1) / (s.k <= kThreads ? range : 2.0f * range);
     if (!(per_k < 0x1p100f)) per_k = 0x1p100f;
   }
+  bool by_bound = false;  // the candidates are the logits from `bound` on
+  float bound = -3.4028234663852886e38f;
   if (vocab <= kList && (s.k < vocab || s.p < 1.0f)) {
-    n = row.template collect<false>([](float x) { return x > neg_inf(); });
+    by_bound = true;
   } else if (s.k < vocab || s.p < 1.0f) {
     const bool by_k = s.k < vocab;
     const Levels levels{top, by_k ? per_k : per_p};
@@ -841,14 +843,16 @@ __global__ __launch_bounds__(kThreads, NP == 0 ? 4 : 2) void sample_kernel(
                                         [&](u64 all) { return reaching(s.p, all); });
     if (!by_k) z = at.all;
     if (at.count <= (uint32_t)kList) {
-      // (a bound: the last bucket's is all that is above -inf)
-      const float end = at.bucket < kLevels - 1 ? (float)(at.bucket + 1) : __builtin_inff();
-      n = row.template collect<false>([&](float x) { return (top - x) * levels.per < end; });
+      // (the last bucket's lower end is the lowest logit, also where the distance overflows)
+      by_bound = at.bucket >= kLevels - 1;
+      const float end = (float)(at.bucket + 1);
+      if (!by_bound) n = row.template collect<false>([&](float x) { return (top - x) * levels.per < end; });
     }
   } else if (s.min_p > 0.f) {
-    const float bound = fmaxf(logit_at(s.min_p), -3.4028234663852886e38f);
-    n = row.template collect<false>([&](float x) { return x >= bound; });
+    by_bound = true;
+    bound = fmaxf(logit_at(s.min_p), bound);
   }
+  if (by_bound) n = row.template collect<false>([&](float x) { return x >= bound; });
   if (s.k == vocab && s.p == 1.0f && s.min_p == 0.f) {
     Pick pick;
     pick.token = row.template in_order<false>(

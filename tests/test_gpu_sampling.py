@@ -235,3 +235,24 @@ def test_a_bucket_that_top_k_leaves_a_part_of(gpu, rows, dtype):
         assert got == got[:4] * (rows // 4)
     for _ in range(3):
         assert _sample(x, u, None, k, p) == first
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_distances_that_overflow(gpu, dtype):
+    """Logits further apart than fp32 reaches, at temperatures where the lower ones still weigh something: fewer
+    candidates than the list holds, in a row that is longer. At an infinite temperature, and of the first 3000 of
+    4000 equal ones, all weights are 2^44 units: sums and their parts by fp32 numbers are exact, also at a
+    border. Otherwise sums of 4000 largest weights and more are off by 6000 * 2^-45 / 4000 and 1e-14 of
+    themselves, less than 1e-12, and no decision lies as near a border."""
+    x = torch.full((9000,), -math.inf)
+    at = torch.randperm(9000, generator=torch.Generator().manual_seed(7))
+    x[at[:4000]], x[at[4000:6000]] = 2.0e38, -2.0e38
+    inf = math.inf
+    rows = [(u, t, k, p, 0.0) for u in (0.2, 0.6, 0.99) for t in (1.0e38, inf)
+            for k, p in ((5000, 1.0), (5000, 0.93), (0, 0.95), (6000, 1.0), (3000, 1.0), (0, 1.0))]
+    x = x.to(dtype).repeat(len(rows), 1)
+    tokens, probs = _sample(x, *(list(z) for z in zip(*rows)))
+    for r, (u, t, k, p, _) in enumerate(rows):
+        want, prob, margin = S.sample(x[r].float().numpy(), np.float32(u), t, k, p)
+        assert margin >= 1e-12 or t == inf or k == 3000
+        assert tokens[r] == want and abs(probs[r] - prob) <= 2.0 ** -23 * prob, r
