@@ -767,7 +767,7 @@ __global__ __launch_bounds__(kThreads, NP == 0 ? 4 : 2) void sample_kernel(
   s.p = set.top_p == nullptr ? 1.0f : set.top_p[r];
   s.min_p = set.min_p == nullptr ? 0.0f : set.min_p[r];
   s.u = set.uniforms[r];
-  s.u = s.u > 0.f ? s.u : 0.f;
+  s.u = s.u > 0.f ? fminf(s.u, 1.0f) : 0.f;
   if (!(s.temperature > 0.f) || s.min_p > 1.0f) s.temperature = 1.0f, s.k = 1;  // the first largest
   if (s.k <= 0 || s.k > vocab) s.k = vocab;
   if (!(s.p < 1.0f)) s.p = 1.0f;

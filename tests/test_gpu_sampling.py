@@ -256,3 +256,14 @@ def test_distances_that_overflow(gpu, dtype):
         want, prob, margin = S.sample(x[r].float().numpy(), np.float32(u), t, k, p)
         assert margin >= 1e-12 or t == inf or k == 3000
         assert tokens[r] == want and abs(probs[r] - prob) <= 2.0 ** -23 * prob, r
+
+
+@pytest.mark.parametrize("vocab", [40, 5000, 9001])
+def test_uniforms_far_outside(gpu, vocab):
+    """What is outside [0, 1) counts as the nearest end, however far: above, the last token that stayed."""
+    x, u = _logits(1, vocab, 21, F32), [1.0, 2.0, 1e10, 3.0e38, math.inf, -1e-30, -3.0e38, -math.inf]
+    for k, p in ((0, 1.0), (30, 1.0), (0, 0.99), (3000, 0.9999)):
+        tokens, probs = _sample(x.expand(8, vocab).contiguous(), u, None, [k] * 8, [p] * 8)
+        for i in range(8):
+            want, prob, _ = S.sample(x[0].numpy(), np.float32(min(max(u[i], 0.0), 1.0)), 1.0, k, p)
+            assert tokens[i] == want and abs(probs[i] - prob) <= 2.0 ** -23 * prob, (k, p, u[i])
