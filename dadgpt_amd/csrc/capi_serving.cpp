@@ -165,6 +165,7 @@ int rope(const char* fn, T* q_out, T* k_out, const T* q, const T* k,
                     fn, names[i], (long long)t.batch, (long long)t.head, (long long)t.row);
     shape.t[i] = Strides64{t.batch, t.head, t.row};
   }
+  // threads: 8 for a head of a row at most, numbered in 32 bits
   if ((long long)batch * S > (1LL << 31) / 8 ||
       (long long)batch * S * (H + (long long)Hkv) > (1LL << 31) / 8)
     return fail(DADGPT_ERR_INVALID_ARGUMENT,

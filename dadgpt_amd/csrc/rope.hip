@@ -79,10 +79,6 @@ hipError_t launch_rope_t(T* q_out, T* k_out, const T* q, const T* k, const RopeS
 
 }  // namespace
 
-long long rope_threads(const RopeShape& s) {
-  return (long long)s.B * s.S * (s.D / 8) * (s.H + s.Hkv);
-}
-
 hipError_t launch_rope_bf16(bf16* q_out, bf16* k_out, const bf16* q, const bf16* k,
                             const RopeShape& shape, const Rope& rope, const int* positions,
                             hipStream_t stream) {

@@ -24,8 +24,6 @@ struct RopeShape {
   int B, H, Hkv, S, D;
   Strides64 t[4];
 };
-// Threads that a call makes: the host keeps them below 2^31.
-long long rope_threads(const RopeShape& s);
 hipError_t launch_rope_bf16(bf16* q_out, bf16* k_out, const bf16* q, const bf16* k,
                             const RopeShape& shape, const Rope& rope, const int* positions,
                             hipStream_t stream);
