@@ -62,7 +62,7 @@ hipError_t launch_rope_t(T* q_out, T* k_out, const T* q, const T* k, const RopeS
                          const Rope& r, const int* positions, hipStream_t stream) {
   RopeArgs<T> a{q_out, k_out, q, k, positions, s, r, false, 0};
   const int heads = s.H + s.Hkv;
-  const Strides64& t = s.H > 0 ? s.t[0] : s.t[1];
+  const Strides64& t = s.t[0];
   a.tokens_first = t.row < t.head;
   auto run = [&](auto vec, auto inter) {
     a.n = (uint32_t)((long long)s.B * s.S * heads * (s.D / (2 * vec())));

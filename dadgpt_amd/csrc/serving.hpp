@@ -12,7 +12,7 @@ struct Strides64 {
   long long batch, head, row;
 };
 
-// Rotary positions of q [B, H, S, D] and k [B, Hkv, S, D] (H or Hkv may be 0). Strides in the order
+// Rotary positions of q [B, H, S, D] and k [B, Hkv, S, D] (Hkv may be 0). Strides in the order
 // q, k, q_out, k_out; `magnitude` multiplies the rotated elements, `inverse` turns them back.
 struct Rope {
   const double* freqs;
