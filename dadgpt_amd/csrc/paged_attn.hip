@@ -455,10 +455,10 @@ __device__ __forceinline__ bool merge_waves(const TileArgs<T>& a, const Work& w,
 
 // ------------------------------------------------------------------------ a few rows
 
-// NR rows (1 to 4: a token of as many query heads, or a few tokens): products on the VALU, as decode.hip's.
-// Every 16-byte load of a wave covers whole rows of a page, all of a wave's loads are in flight before any
-// arithmetic, and nothing passes through LDS before the waves are merged. A chunk is one round of loads of
-// eight waves: `chunk` is few_keys().
+// NR rows (1 to most_rows(): a token of as many query heads, or a few tokens): products on the VALU, as
+// decode.hip's. Every 16-byte load of a wave covers whole rows of a page, all of a wave's loads are in flight
+// before any arithmetic, and nothing passes through LDS before the waves are merged. A chunk is one round of
+// loads of eight waves: `chunk` is few_keys().
 constexpr int kRowWaves = 8, kRowLoads = 8;
 template <typename T, int D>
 __host__ __device__ constexpr int few_keys() {
@@ -1327,12 +1327,13 @@ hipError_t launch_paged_t(T* out, long long ld_out, const T* q, long long ld_q, 
 template <typename T>
 void launch_rows(const TileArgs<T>& a, dim3 grid, hipStream_t stream) {
   auto run = [&](auto d) {
-    switch (a.rows) {
-      case 1: paged_rows_kernel<T, d(), 1><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
-      case 2: paged_rows_kernel<T, d(), 2><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
-      case 3: paged_rows_kernel<T, d(), 3><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
-      default: paged_rows_kernel<T, d(), 4><<<grid, 64 * kRowWaves, 0, stream>>>(a); break;
+    auto rows = [&](auto nr) { paged_rows_kernel<T, d(), nr()><<<grid, 64 * kRowWaves, 0, stream>>>(a); };
+    if (a.rows == 1) return rows(std::integral_constant<int, 1>{});
+    if constexpr (most_rows(sizeof(T)) > 2) {
+      if (a.rows == 4) return rows(std::integral_constant<int, 4>{});
+      if (a.rows == 3) return rows(std::integral_constant<int, 3>{});
     }
+    rows(std::integral_constant<int, 2>{});
   };
   if (a.p.D == 64)
     run(std::integral_constant<int, 64>{});
