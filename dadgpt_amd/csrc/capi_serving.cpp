@@ -21,9 +21,6 @@ using dadgpt::Rope;
 using dadgpt::Span;
 using dadgpt::Strides64;
 
-const bf16* B(const uint16_t* p) { return reinterpret_cast<const bf16*>(p); }
-bf16* B(uint16_t* p) { return reinterpret_cast<bf16*>(p); }
-
 constexpr int64_t kMostPitch = 1 << 24;
 
 int check_aligned(const char* fn, const char* name, const void* p, uintptr_t bytes) {

@@ -963,7 +963,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_bf16_kernel(const TileArgs<
   bf16x8 q[D / 16];
   load_query<D>(q, a, w, r, hi);
 
-  const int head = w.head, n_tiles = w.key1 > w.key0 ? (w.key1 - w.key0 + 63) / 64 : 0;
+  const int n_tiles = w.key1 > w.key0 ? (w.key1 - w.key0 + 63) / 64 : 0;
   Stage<D> stage(lane);
   Groups g(a, w, lane);
   auto load = [&](int t, bf16* tk, bf16* tv) {

@@ -710,7 +710,6 @@ __device__ __forceinline__ Pick pick_in_wave(const Settings& s, const Weigher& w
 template <typename T, int NP>
 __device__ __forceinline__ Pick pick_from_list(Row<T, NP>& row, const Settings& s,
                                                const Weigher& weigh, uint32_t hi, int n, u64 z) {
-  Shared& sm = row.sm;
   Elements<kPerThread> x = listed(row, n);
   uint32_t low = 0;
 #pragma unroll
