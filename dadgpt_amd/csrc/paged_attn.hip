@@ -588,7 +588,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void paged_rows_kernel(const TileAr
 
 // ------------------------------------------------------------------------ bf16
 
-// Weights exp2(s c - m) as bf16 operands of the next product; their fp32 sum.
+// Weights exp2(s c - m) as bf16 operands of the next product, rounded once as the bf16 forward's; their fp32
+// sum. (Weights in two parts, as the kernel for up to 32 rows has them, would take the error from 1.25 to 1.4
+// times that of the result's rounding to 1.0, and 8 chunks of 256 rows over up to 8192 tokens, 12 heads of 64,
+// from 47 to 54 us, 512 rows over 32768 from 75 to 94; in two parts for tiles of up to 32 rows alone, 52 and 85.)
 __device__ __forceinline__ float weights_bf16(bf16x8 (&p)[2], const f32x16& s, float c, float m) {
   float sum = 0.f;
 #pragma unroll
@@ -783,10 +786,21 @@ __device__ __forceinline__ void take_query(bf16x8 (&q)[D / 16], bool negate) {
 //                                   .. + 7 of each 32
 //   O^T[16 columns][16 rows] += V^T P^T over 32 keys, V^T by ds_read_b64_tr_b16
 // Of 32 keys, the two tiles of scores take 8 g + r and 8 g + 4 + r as their rows 4 g + r (r < 4): the
-// lanes l / 16 = g then hold the weights of keys 8 g .. + 7, the other product's operand.
+// lanes l / 16 = g then hold the weights of keys 8 g .. + 7, the other product's operand. Weights are the sum
+// of two bf16 numbers, good to 2^-15, so that a decode step's results are as exact whichever of the kernels for
+// a few rows it takes; one number, as in the tiles, costs 0.6 us less of 43 (8 sequences of 4096 to 32768
+// tokens, three rows for each of 4 KV heads). The first is cut off, and the second a 2^-20 of the weight
+// larger than the rest: neither is 0 or of another sign than the weight, so an infinite value's products are
+// the infinity.
 typedef __attribute__((ext_vector_type(4))) float acc16;
 __device__ __forceinline__ acc16 mfma16(const bf16x8& a, const bf16x8& b, const acc16& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t cut_pair(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ float rest_of(float p) {
+  return fmaf(p, 1.0f + 0x1p-20f, -__uint_as_float(__float_as_uint(p) & 0xffff0000u));
 }
 constexpr int kMidWaves = 8;
 template <int D>
@@ -898,7 +912,7 @@ __global__ __launch_bounds__(64 * kMidWaves, 4) void paged_mid_bf16_kernel(const
       const float base = m[b] == neg_inf() ? 0.f : m[b];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        u32x4 p;
+        u32x4 p, rest;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -906,7 +920,8 @@ __global__ __launch_bounds__(64 * kMidWaves, 4) void paged_mid_bf16_kernel(const
             const float p0 = fast_exp2(fmaf(s[j][t][r], a.scale, -base));
             const float p1 = fast_exp2(fmaf(s[j][t][r + 1], a.scale, -base));
             l[b] += p0 + p1;
-            p[2 * t + r / 2] = pack_bf16x2(p0, p1);
+            p[2 * t + r / 2] = cut_pair(p0, p1);
+            rest[2 * t + r / 2] = pack_bf16x2(rest_of(p0), rest_of(p1));
           }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
@@ -920,6 +935,7 @@ __global__ __launch_bounds__(64 * kMidWaves, 4) void paged_mid_bf16_kernel(const
           }
           const bf16x8 vt = __builtin_bit_cast(
               bf16x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          o[b][d] = mfma16(vt, as_bf16x8(rest), o[b][d]);
           o[b][d] = mfma16(vt, as_bf16x8(p), o[b][d]);
         }
       }

@@ -509,3 +509,19 @@ def test_all_counters_return_to_zero(gpu, dtype, shape):
         torch.cuda.synchronize()
         assert int(ws[:size].max()) == 0 and int(ws[size:].max()) > 0
     _check(st, out)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 16, 17, 32])
+@pytest.mark.parametrize("D", [32, 64])
+def test_weights_of_a_few_bf16_rows(gpu, rows, D):
+    """Steps of up to 32 rows of a KV head round nothing to bf16 but the result: weights are fp32, or two bf16
+    numbers (the first cut off, which leaves less than 2^-7 of the weight, that rounded by 2^-8 of itself, and
+    2^-20 added), and what fp32 arithmetic leaves is the bound of the fp32 step."""
+    st = S.Step([2000 + rows, rows, 300 + rows], [rows] * 3, 1, 1, D, 16, BF, seed=34)
+    out = _attend(st).cpu().double()
+    st.dtype = F32
+    want, bound = st.attention(D ** -0.5)
+    st.v_pages = st.v_pages.abs()
+    bound = bound + (2.0 ** -15 + 2.0 ** -20) * st.attention(D ** -0.5)[0]
+    err = (out - want).abs() - (bound + 2.0 ** -8 * (want.abs() + bound))
+    assert (err <= 0).all(), float(err.max())
