@@ -27,7 +27,12 @@
 //
 // fp32: the same walk with the products of x3.hpp (six bf16 products for an fp32 one), tiles loaded
 // into registers and split into three bf16 planes as they are stored, maxima in natural-log units. 8 prompts'
-// chunks as above over up to 4096 tokens: 136 us (12 GFLOP, 89 TFLOP/s of the 154 of a library product).
+// chunks as above over up to 4096 tokens: 124 to 136 us (12 GFLOP, 89 to 97 TFLOP/s of the 154 of a library
+// product).
+//
+// Which kernel and how a tile's keys are cut follow from the step (the rows of a sequence at most, all tiles'
+// keys): a sequence's results have the same bits in every equal step, and in another one, alone for instance,
+// the same within their roundings.
 #include "common.hpp"
 #include "decode.hpp"
 #include "lanes.hpp"

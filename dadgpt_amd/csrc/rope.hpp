@@ -90,7 +90,7 @@ __device__ __forceinline__ Chunk chunk_of(int c, int rot_dim) {
   return Chunk{{2 * c * VEC, 2 * c * VEC + VEC}, rotated};
 }
 
-// Turns the pairs of two pieces, each result rounded once.
+// Turns the pairs of two pieces in fp32, each result rounded once to T.
 template <typename T, int VEC, bool INTER>
 __device__ __forceinline__ void turn_pieces(Piece<T, VEC>& a, Piece<T, VEC>& b,
                                             const Turn<VEC>& t) {

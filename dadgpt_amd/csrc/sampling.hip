@@ -23,8 +23,8 @@
 //
 // Bound by one CU's operations on a row: two or three an element and pass, about 20 for a weight, and
 // between passes by barriers and chains in LDS. The row (200 KB of fp32 for 50257 logits) comes from L2
-// after the first pass. 50257 logits, us: one row, top-k of 40, 18; 32 rows of all kinds 73; 512 rows of bf16
-// with top-p 153. 32 rows of one kind: no filter 25, top-k of 40 20, of 5000 40, top-p of 0.9 44 (spread of
+// after the first pass. 50257 logits, us: one row, top-k of 40, 18 to 19; 32 rows of all kinds 70 to 84; 512
+// rows of bf16 with top-p 151 to 159, of fp32 143. 32 rows of one kind: no filter 25, top-k of 40 20, of 5000 40, top-p of 0.9 44 (spread of
 // 4) to 95 (of 0.5: 40000 tokens stay), and 320 with all logits equal.
 #include "common.hpp"
 #include "kernels.hpp"
@@ -40,7 +40,10 @@ constexpr int kBuckets = kThreads;          // of a search's: one for each threa
 constexpr int kFew = kThreads;              // elements of a bucket that are compared each with each
 constexpr int kPerThread = 16, kList = kPerThread * kThreads;  // candidates
 constexpr int kOne = 44;                    // weights are multiples of 2^-44
-constexpr float kFaintest = 31.0f;          // e^-31 < 2^-44.7: weighs nothing
+// Where the last bucket by weight begins, in temperatures below the largest logit. e^-31 is 0.61 units of
+// 2^-44, which rounds to 1: every logit in a bucket above the last weighs at least a unit, so that counts (of
+// those that weigh something) and lists (of all in a bucket) agree. From e^-31.19 on weights round to 0.
+constexpr float kFaintest = 31.0f;
 
 typedef unsigned long long u64;
 
@@ -876,7 +879,18 @@ hipError_t launch_sample_t(int* tokens, float* probs, const T* logits, long long
     sample_kernel<T, np()><<<rows, kThreads, 0, stream>>>(tokens, probs, logits, ld, vocab, set);
     return hipGetLastError();
   };
-  // Pieces of 256 elements for each of the 8 waves; up to 25 of them stay in registers (100 for fp32).
+  // Pieces of 256 elements for each of the 8 waves; up to 25 of them stay in registers (100 for fp32), as many
+  // as the others leave room for: larger vocabularies are read again. A row with fewer pieces than its kernel
+  // walks empty ones, so up to 8 have a kernel of their own. 32 rows in fp32, top-k of 40 / top-p of 0.9 / no
+  // filter, us (bf16 within 1.5 of it):
+  //   vocabulary   8 pieces           25                 read again
+  //         4000   20.4  26.7   7.6   23.4  29.3  14.6   20.3  26.6   6.7
+  //        16000   13.0  55.7  10.0   18.2  62.1  17.0   16.0  56.8  11.6
+  //        25000                      19.5  74.1  19.8   22.2  72.9  19.2
+  //        32000                      19.0  71.8  20.7   21.1  70.2  19.9
+  //        40000                      19.8  68.0  22.6   24.0  68.6  24.1
+  //        50257                      20.1  73.4  24.9   28.6  78.1  30.8
+  //       131072                                         48.5   178  64.6
   // With more rows than CUs, two workgroups on a CU, in 128 registers each and with the row from L2, hide
   // more than that saves (512 rows of 50257 in bf16: 153 us, 203 with the rows in registers).
   const int pieces = (vocab + 3 + 256 * kWaves - 1) / (256 * kWaves);

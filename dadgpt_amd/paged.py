@@ -106,7 +106,7 @@ def paged_append(k_pages, v_pages, q_out, q, k, v, block_table, row_start, lens,
                  stream=None) -> None:
     """Writes the rows of k and v [rows, n_kv_heads, d_head] into the pages, and q [rows, n_heads,
     d_head] into q_out (may be q; both None: k and v alone), views whose rows hold their heads side by
-    side, as slices of a fused projection's output do. Sequence s owns rows row_start[s] ..
+    side, as slices of a fused projection's output do; those of k and v lie equally far apart. Sequence s owns rows row_start[s] ..
     row_start[s + 1] - 1, max_rows at most; lens counts its tokens with them, so they are its last;
     token j goes to slot j % page of page block_table[s, j // page]. freqs (rope.rope_frequencies):
     rotate q and k by their token numbers as rope.rope does."""
@@ -156,7 +156,8 @@ def paged_attention(out, q, k_pages, v_pages, block_table, row_start, lens, max_
                     scale: float, workspace, stream=None) -> None:
     """out = softmax(scale q k^T) v for the new tokens q [rows, n_heads, d_head] (rows as in
     paged_append, out may be q), each over its sequence's tokens up to itself. Query head h reads KV head
-    h // (n_heads // n_kv_heads). Rows behind the last sequence are left as they were."""
+    h // (n_heads // n_kv_heads). Rows behind the last sequence are left as they were. Equal steps give
+    equal bits; in a step with other sequences a sequence's may differ by roundings."""
     dtype = q.dtype
     fn = _by_dtype("dadgpt_paged_attention", dtype)
     pk, pv, pt, pr, pl, n_seq, max_pages = _step(k_pages, v_pages, block_table, row_start, lens, dtype)

@@ -59,6 +59,10 @@ int dadgpt_paged_append_f32(float* k_pages, float* v_pages, float* q_out, int64_
                             void* stream);
 
 /* out = softmax(scale q k^T) v for every new row, over its sequence's tokens up to and with its own.
+ * Equal steps give equal bits. The order of the sums, and for bf16 whether the weights are rounded to it for
+ * the product with v (above 32 rows of max_rows * n_heads / n_kv_heads, as dadgpt_flash_attention_* does),
+ * depend on the step's shape and all its lengths, so a sequence in a step with others may differ from
+ * the same sequence alone by those roundings.
  * Row r of q (out) holds n_heads * d_head elements from r * ld_q (ld_out) on; out may be q (ld_out =
  * ld_q). A row none of whose keys weighs anything (it lies before token 0, all its pages are missing,
  * all its scores are -inf) gets zeros. A NaN key or value makes the rows that see it NaN, an infinite value

@@ -46,8 +46,8 @@ int dadgpt_rope_frequencies(double* freqs, int rot_dim, double base, int scaling
  *   freqs      DEVICE double [rot_dim / 2], 8-byte aligned
  *   positions  DEVICE int32 [B, S], 4-byte aligned, any values; NULL: row s is at position s
  * rot_dim is a multiple of 8 of at most d_head (32 or 64). k and k_out may be NULL (Hkv 0): q alone.
- * Angles are reduced in double, so that far positions keep fp32 accuracy; each result is rounded
- * once. In place: q_out = q (k_out = k) with the same strides. No other overlap of an output with
+ * Angles are reduced in double, so that far positions keep fp32 accuracy; results are computed in
+ * fp32, two products and a sum, and bf16's rounded once. In place: q_out = q (k_out = k) with the same strides. No other overlap of an output with
  * another tensor is accepted, but tensors of the same strides may lie in each other's gaps. */
 int dadgpt_rope_bf16(uint16_t* q_out, uint16_t* k_out, const uint16_t* q, const uint16_t* k,
                      const dadgpt_head_strides* strides, int B, int H, int Hkv, int S, int d_head,
