@@ -34,7 +34,8 @@ extern "C" {
  *      is outside (NaN) counts as the nearest end (0).
  * Logits of NaN and -inf are never picked; where there are +inf logits, they alone are, with equal
  * weights. A row that has nothing else gets token -1 and probability 0. Weights are computed in
- * double and summed as multiples of 2^-44, in integers: the result does not depend on the order.
+ * double and summed as multiples of 2^-44, in integers: the result does not depend on the order, and a
+ * token of less than 2^-45 of the largest weight is not drawn, by a uniform number of 0 either.
  * temperature, top_p, min_p (float) and top_k (int32) are DEVICE arrays [rows], 4-byte aligned, each
  * may be NULL: 1, all, 0, all. Outputs overlap nothing else. */
 int dadgpt_sample_bf16(int32_t* tokens, float* probs, const uint16_t* logits, int64_t ld, int rows,
