@@ -24,8 +24,8 @@
 // Bound by one CU's operations on a row: two or three an element and pass, about 20 for a weight, and
 // between passes by barriers and chains in LDS. The row (200 KB of fp32 for 50257 logits) comes from L2
 // after the first pass. 50257 logits, us: one row, top-k of 40, 18 to 19; 32 rows of all kinds 70 to 84; 512
-// rows of bf16 with top-p 151 to 159, of fp32 143. 32 rows of one kind: no filter 25, top-k of 40 20, of 5000 40, top-p of 0.9 44 (spread of
-// 4) to 95 (of 0.5: 40000 tokens stay), and 320 with all logits equal.
+// rows of bf16 with top-p 151 to 159, of fp32 143. 32 rows of one kind: no filter 25, top-k of 40 20, of 5000
+// 43, top-p of 0.9 44 (spread of 4) to 95 (of 0.5: 40000 tokens stay), and 320 with all logits equal.
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
@@ -882,7 +882,7 @@ hipError_t launch_sample_t(int* tokens, float* probs, const T* logits, long long
   // Pieces of 256 elements for each of the 8 waves; up to 25 of them stay in registers (100 for fp32), as many
   // as the others leave room for: larger vocabularies are read again. A row with fewer pieces than its kernel
   // walks empty ones, so up to 8 have a kernel of their own. 32 rows in fp32, top-k of 40 / top-p of 0.9 / no
-  // filter, us (bf16 within 1.5 of it):
+  // filter, us (bf16 within 3.5 of it):
   //   vocabulary   8 pieces           25                 read again
   //         4000   20.4  26.7   7.6   23.4  29.3  14.6   20.3  26.6   6.7
   //        16000   13.0  55.7  10.0   18.2  62.1  17.0   16.0  56.8  11.6
